@@ -291,6 +291,113 @@ at::Tensor ln_modulate(const at::Tensor& x, c10::optional<at::Tensor> out,
   return y;
 }
 
+int dtype_code(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kDtypeF32;
+    case at::kBFloat16: return kDtypeBf16;
+    case at::kHalf: return kDtypeF16;
+    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+
+const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+
+// Rows [M, D] -> {y or q, s or empty, scales or empty}.  Shapes and types are checked by the caller
+// (ops.fused.add_rms_norm); what a kernel reads through these pointers is checked here again.
+std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at::Tensor>& resid,
+                                     const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& scale,
+                                     const c10::optional<at::Tensor>& shift, int64_t rows_per_batch,
+                                     const c10::optional<at::Tensor>& row_map, double eps, int64_t quant, bool blocked,
+                                     const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& s_out) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  check_rowmajor(x, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), D = x.size(1);
+  TORCH_CHECK(M < (1ll << 31) && D >= 1 && D <= 16384, "add_rms_norm: 1 <= D <= 16384, got ", D);
+  AddNormArgs a{};
+  a.dtype = dtype_code(x, "x");
+  auto same = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.dim() == 2 && t.size(0) == M &&
+                    t.size(1) == D && t.stride(1) == 1, name, " must be like x: [M, D], unit inner stride");
+  };
+  a.x = x.data_ptr();
+  a.ldx = x.stride(0);
+  at::Tensor s;
+  if (const at::Tensor* r = given(resid)) {
+    same(*r, "resid");
+    a.resid = r->data_ptr();
+    a.ldr = r->stride(0);
+    s = given(s_out) ? *s_out : at::empty({M, D}, x.options());
+    same(s, "resid_out");
+    a.s_out = s.data_ptr();
+    a.lds = s.stride(0);
+  }
+  if (const at::Tensor* t = given(w)) {
+    TORCH_CHECK(t->device() == x.device() && t->dim() == 1 && t->numel() == D && t->is_contiguous() &&
+                    (t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat),
+                "weight must be contiguous [D] of x's type or float32");
+    a.w = t->data_ptr();
+    a.w_f32 = t->scalar_type() == at::kFloat;
+  }
+  a.rows_per_batch = (int)(rows_per_batch > 0 ? rows_per_batch : M);
+  const at::Tensor* rm = given(row_map);
+  if (rm) {
+    TORCH_CHECK(rm->device() == x.device() && rm->scalar_type() == at::kInt && rm->is_contiguous() && rm->numel() == M,
+                "row_map must be int32 [M]");
+    a.row_map = rm->data_ptr<int>();
+  }
+  auto mod = [&](const c10::optional<at::Tensor>& o, const char* name, const float*& p, long long& bs) {
+    const at::Tensor* t = given(o);
+    if (!t) return;
+    TORCH_CHECK(t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) == D &&
+                    t->stride(1) == 1, name, " must be float32 [batch, D]");
+    TORCH_CHECK(rm || M == 0 || t->size(0) * (int64_t)a.rows_per_batch >= M, name, " has ", t->size(0),
+                " rows: too few for ", M, " rows of ", a.rows_per_batch, " per batch");
+    TORCH_CHECK(a.n_mod == 0 || a.n_mod == t->size(0), "scale and shift differ in their batch rows");
+    TORCH_CHECK(t->size(0) > 0, name, " has no rows");
+    a.n_mod = (int)t->size(0);
+    p = t->data_ptr<float>();
+    bs = t->stride(0);
+  };
+  mod(scale, "scale", a.scale, a.scale_bs);
+  mod(shift, "shift", a.shift, a.shift_bs);
+  a.M = (int)M;
+  a.D = (int)D;
+  a.eps = (float)eps;
+  a.quant = (int)quant;
+  a.blocked = blocked ? 1 : 0;
+  a.err = err_ptr();
+  at::Tensor y, sf;
+  if (quant) {
+    TORCH_CHECK(D % (blocked ? 128 : 32) == 0, "the MX output needs D to be a multiple of ", blocked ? 128 : 32);
+    y = at::empty({M, D}, x.options().dtype(quant == 2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn));
+    sf = blocked ? at::empty({(M + 255) / 256 * 256 * (D / 32)}, x.options().dtype(at::kByte))
+                 : at::empty({M, D / 32}, x.options().dtype(at::kByte));
+    a.sf = sf.data_ptr<uint8_t>();
+  } else {
+    y = given(out) ? *out : at::empty({M, D}, x.options());
+    same(y, "out");
+  }
+  a.y = y.data_ptr();
+  a.ldy = y.stride(0);
+  const int rc = dfl_add_rms_norm(&a, cur_stream());
+  TORCH_CHECK(rc != -3, "the MX output needs 16-byte aligned rows of x, resid, weight, scale and shift");
+  DFL_CHECK_RC(rc, "add_rms_norm");
+  return {y, s, sf};
+}
+
+at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarType dtype) {
+  TORCH_CHECK(q.is_cuda() && q.is_contiguous() && sf.is_contiguous() && sf.device() == q.device(),
+              "mx_dequantize: contiguous CUDA tensors on one device");
+  TORCH_CHECK(q.scalar_type() == at::kFloat8_e4m3fn || q.scalar_type() == at::kFloat8_e5m2, "q must be float8");
+  TORCH_CHECK(sf.scalar_type() == at::kByte && q.numel() == sf.numel() * 32, "one uint8 scale per 32 elements");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options().dtype(dtype));
+  DFL_CHECK_RC(dfl_mx_dequantize(q.data_ptr(), sf.data_ptr(), out.data_ptr(), q.numel(), dtype_code(out, "output"),
+                                 q.scalar_type() == at::kFloat8_e5m2, cur_stream()), "mx_dequantize");
+  return out;
+}
+
 // Head-scatter description shared by the standalone qkv_scatter kernel and the GEMM
 // qkv epilogue (source fields qkv / ld / rows are filled by the caller).
 QkvScatterArgs make_qkv_args(int64_t q_off, int64_t k_off, int64_t v_off, int64_t S_src, int64_t H, int64_t dh,
@@ -902,6 +1009,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale") = py::none(), py::arg("rows_per_batch") = 0, py::arg("eps") = 1e-6,
         py::arg("rms") = false, py::arg("row_map") = py::none(), py::arg("y_peer") = std::vector<int64_t>{},
         py::arg("row0") = 0, py::arg("rows") = -1);
+  m.def("add_rms_norm", &add_rms_norm, py::arg("x"), py::arg("resid"), py::arg("w"), py::arg("scale"), py::arg("shift"),
+        py::arg("rows_per_batch"), py::arg("row_map"), py::arg("eps"), py::arg("quant"), py::arg("blocked"),
+        py::arg("out"), py::arg("s_out"));
+  m.def("mx_dequantize", &mx_dequantize, py::arg("q"), py::arg("scales"), py::arg("dtype"));
   m.def("qkv_scatter", &qkv_scatter);
   m.def("qkv_plan", &qkv_plan);
   m.def("row_sumsq", &row_sumsq);

@@ -106,6 +106,37 @@ typedef struct LnModArgs {
 } LnModArgs;
 int dfl_ln_modulate(const LnModArgs* a, cudaStream_t stream);
 
+enum { kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2 };
+
+// Residual RMSNorm (add_norm.cu): s = x + resid; y = rms(s) [* w] [* (1 + scale[b])] [+ shift[b]].
+// x, resid, s_out, w and (quant = 0) y share one type; D <= 16384, any width and strides
+// (16-byte aligned rows take the vector path).  quant 1 / 2: y holds FP8 E4M3 / E5M2 elements (row
+// stride ldy bytes) and sf one E8M0 scale per 32 columns, plain [M, D/32] or blocked as in
+// dfl_mx_quantize with rows up to the next multiple of 256 zeroed.
+typedef struct AddNormArgs {
+  const void* x; long long ldx;
+  const void* resid; long long ldr;  // or NULL (s = x)
+  void* s_out; long long lds;        // or NULL
+  void* y; long long ldy;
+  const void* w; int w_f32;          // [D] or NULL; w_f32: f32 weights beside 16-bit tensors
+  const float* scale; long long scale_bs;  // f32 [batch, D] or NULL
+  const float* shift; long long shift_bs;
+  const int* row_map;                // optional: modulation row of every row
+  int rows_per_batch;
+  int n_mod;                         // rows of scale / shift: a row_map entry outside [0, n_mod) is an error
+  int* err;                          // (its row is left unmodulated and the error word set)
+  int M, D, M_pad;                   // M_pad is set by the launcher
+  float eps;
+  int dtype;                         // kDtype*
+  int quant, blocked;
+  uint8_t* sf;
+} AddNormArgs;
+int dfl_add_rms_norm(const AddNormArgs* a, cudaStream_t stream);
+
+// Plain-scale MX data -> values: n FP8 elements (a multiple of 32), scales [n / 32], out of type dtype.
+int dfl_mx_dequantize(const void* q, const void* scales, void* out, long long n, int dtype, int e5m2,
+                      cudaStream_t stream);
+
 // q/k RMSNorm + RoPE + scatter to head-major [B, H_local, S_dst, dh] buffers.
 // Source rows are tokens; destination tables hold one pointer per rank so the
 // same pass performs the Ulysses sequence->head all-to-all over NVLink stores.

@@ -29,6 +29,7 @@ CUDA_SOURCES = [
     "gemm.cu",
     "gemm2.cu",
     "norm.cu",
+    "add_norm.cu",
     "attention.cu",
     "comm.cu",
     "mx.cu",

@@ -13,6 +13,7 @@ _EXPORTS = {
     "RMSNorm": "norm",
     "CustomRMSNorm": "norm",
     "rms_norm_fp32": "norm",
+    "add_rms_norm": "norm",
     "attention": "attn",
     "cross_attention": "attn",
     "ring_attention": "attn",

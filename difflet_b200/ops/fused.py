@@ -10,6 +10,7 @@ Ops:
   linear        y = epi(x W^T + b): epi in {none, gelu (column window), silu,
                 gate_resid (resid + gate[b] * y)}; strided outputs allowed
   ln_modulate   LayerNorm / RMSNorm (+affine) (* (1 + scale) + shift)
+  add_rms_norm  residual add + RMSNorm (+ weight, modulation), bf16 / fp16 / fp32 or MXFP8 output
   qkv_scatter   per-head / across-heads q,k RMSNorm + RoPE + scatter to
                 head-major (or token-major) destinations, one per rank
   linear_qkv    linear whose q/k/v column blocks go through qkv_scatter inside the
@@ -211,6 +212,100 @@ def ln_modulate(x, *, shift=None, scale=None, w=None, b=None, eps=1e-6, rms=Fals
         out.copy_(y)
         return out
     return y
+
+
+def _no_grad(name: str, *tensors) -> None:
+    """The kernels record no backward pass: refuse inputs whose gradient would be lost silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
+
+
+# MX element type -> (code of the native kernels, emax of the format, largest finite value)
+MX_CODES = {"float8_e4m3fn": 1, "float8_e5m2": 2, "float8_e4m3fn_x4": 1, "float8_e5m2_x4": 2}
+_NORM_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def add_rms_norm(x, resid=None, w=None, *, eps=1e-6, scale=None, shift=None, rows_per_batch=0, row_map=None,
+                 quantize=None, blocked=False, out=None, resid_out=None):
+    """``s = x + resid``; ``y = s / sqrt(mean(s^2) + eps) * w * (1 + scale[b]) + shift[b]`` -> ``(y, s)``.
+
+    x, resid: [..., D] of one type (bf16, fp16 or fp32; rows with a unit inner stride), D <= 16384.
+    ``resid=None``: s is x itself.  w: [D] of x's type or f32; scale / shift: f32 [B, D] for
+    ``rows_per_batch`` rows each (0: one batch row for all), or by ``row_map`` (int32 [M]).
+    ``quantize`` ("float8_e4m3fn" / "float8_e5m2"): y comes as ``(data, scales)`` in MXFP8, scales plain
+    [..., D/32] or, with ``blocked``, in the layout ``linear_mx`` reads (D a multiple of 128).
+    ``out`` / ``resid_out`` receive y / s and may be x / resid.  The statistics use the unrounded sum.
+    """
+    _no_grad("add_rms_norm", x, resid, w, scale, shift)
+    D = x.shape[-1] if x.dim() else 0
+    if x.dim() < 1 or not 1 <= D <= 16384:
+        raise ValueError(f"add_rms_norm needs [..., D] with 1 <= D <= 16384, got {tuple(x.shape)}")
+    if quantize is not None:
+        if quantize not in MX_CODES:
+            raise NotImplementedError(f"MX element type {quantize!r}: one of {sorted(MX_CODES)}")
+        if D % (128 if blocked else 32):
+            raise ValueError(f"the MX output needs D to be a multiple of {128 if blocked else 32}, got {D}")
+        if out is not None:
+            raise ValueError("out= and quantize= are mutually exclusive")
+    elif blocked:
+        raise ValueError("blocked scales need quantize=")
+    if resid is None:
+        if resid_out is not None:
+            raise ValueError("resid_out needs resid")
+    elif resid.shape != x.shape or resid.dtype != x.dtype or resid.device != x.device:
+        raise ValueError(f"resid {tuple(resid.shape)} {resid.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    for name, t in (("out", out), ("resid_out", resid_out)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    if w is not None and (w.shape != (D,) or w.device != x.device or w.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f"weight must be [{D}] of {x.dtype} or float32 on {x.device}")
+    for name, t in (("scale", scale), ("shift", shift)):
+        if t is not None and (t.dim() != 2 or t.shape[1] != D or t.device != x.device):
+            raise ValueError(f"{name} must be [B, {D}] on {x.device}, got {tuple(t.shape)}")
+    x2 = _rows2d(x)
+    M = x2.shape[0]
+    if row_map is not None and (row_map.dtype != torch.int32 or row_map.numel() != M):
+        raise ValueError(f"row_map must be int32 [{M}]")
+    if x.is_cuda:
+        if x.dtype not in _NORM_DTYPES:
+            raise ValueError(f"add_rms_norm runs in bfloat16, float16 or float32, got {x.dtype}")
+        y2 = s2 = None
+        if out is not None:
+            y2 = out if out.dim() == 2 else out.view(M, D)  # a view: the caller's tensor is written
+        if resid_out is not None:
+            s2 = resid_out if resid_out.dim() == 2 else resid_out.view(M, D)
+        y, s, sf = native().add_rms_norm(x2, None if resid is None else _rows2d(resid), w, scale, shift,
+                                         rows_per_batch, row_map, eps, MX_CODES.get(quantize, 0), blocked, y2, s2)
+        if x.dim() != 2:
+            y = out if out is not None else y.view(x.shape)
+            s = None if resid is None else (resid_out if resid_out is not None else s.view(x.shape))
+            if sf is not None and not blocked:
+                sf = sf.view(*x.shape[:-1], D // 32)
+        s = x if resid is None else s
+        return ((y, sf) if quantize is not None else y), s
+    ct = torch.float64 if x.dtype == torch.float64 else torch.float32
+    s = x2.to(ct) if resid is None else x2.to(ct) + _rows2d(resid).to(ct)
+    y = s * torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + eps)
+    if w is not None:
+        y = y * w.to(ct)
+    if M and (scale is not None or shift is not None):
+        b = row_map.long() if row_map is not None else torch.arange(M) // (rows_per_batch or M)
+        if scale is not None:
+            y = y * (1 + scale.to(ct)[b])
+        if shift is not None:
+            y = y + shift.to(ct)[b]
+    if resid is not None:
+        s = s.to(x.dtype).view(x.shape)
+        s = s if resid_out is None else resid_out.copy_(s)
+    else:
+        s = x
+    if quantize is not None:
+        from difflet_b200.ops.mx import quantize_mx
+
+        q, sf = quantize_mx(y, dtype=quantize)
+        return (q.view(x.shape), block_scales(sf) if blocked else sf.view(*x.shape[:-1], D // 32)), s
+    y = y.to(x.dtype).view(x.shape)
+    return (y if out is None else out.copy_(y)), s
 
 
 def _rope_cpu(x, cos, sin, half):
