@@ -8,6 +8,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <limits>
 #include <string>
 #include <vector>
 
@@ -396,6 +397,108 @@ at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarTy
   DFL_CHECK_RC(dfl_mx_dequantize(q.data_ptr(), sf.data_ptr(), out.data_ptr(), q.numel(), dtype_code(out, "output"),
                                  q.scalar_type() == at::kFloat8_e5m2, cur_stream()), "mx_dequantize");
   return out;
+}
+
+// ---------------------------------------------------------------- cross attention
+// q [B, H, Sq, dh], k / v [B, Hk, Sk, dh]; mask: bool (true = attend) or additive, broadcastable to
+// [B, H, Sq, Sk]; kv_lo / kv_hi int32 [B].
+at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
+                           const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& kv_lo,
+                           const c10::optional<at::Tensor>& kv_hi, const c10::optional<at::Tensor>& out,
+                           const c10::optional<at::Tensor>& lse) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q/k/v must be CUDA tensors [B, H, S, dh]");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "cross attention runs in bfloat16 or float16");
+  const c10::cuda::CUDAGuard guard(q.device());
+  CrossArgs a{};
+  a.B = (int)q.size(0), a.H = (int)q.size(1), a.Sq = (int)q.size(2), a.dh = (int)q.size(3);
+  a.Hk = (int)k.size(1), a.Sk = (int)k.size(2);
+  TORCH_CHECK(a.dh == 64 || a.dh == 128, "head dim must be 64 or 128, got ", a.dh);
+  for (const at::Tensor* t : {&k, &v})
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == q.scalar_type() && t->size(0) == a.B &&
+                    t->size(1) == a.Hk && t->size(2) == a.Sk && t->size(3) == a.dh,
+                "k / v must be [", a.B, ", Hk, Sk, ", a.dh, "] of q's type and device");
+  TORCH_CHECK(a.Hk > 0 && a.H % a.Hk == 0, "query heads must be a multiple of the key heads");
+  at::Tensor o = given(out) ? *out : at::empty_like(q);
+  TORCH_CHECK(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(),
+              "out must be like q");
+  if (o.numel() == 0) return o;
+  // Rows the copies engine can address: unit inner stride, 16-byte multiples elsewhere (an axis of
+  // one element has no stride to speak of, and a repeated axis none at all).
+  auto fits = [](const at::Tensor& t) {
+    bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) == 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0));
+    return ok;
+  };
+  const at::Tensor q_ = fits(q) ? q : q.contiguous();
+  // a head axis that is one head repeated (expand) needs no copy: every query head reads key head 0
+  const bool one = a.Hk > 1 && k.stride(1) == 0 && v.stride(1) == 0;
+  at::Tensor k_ = one ? k.narrow(1, 0, 1) : k, v_ = one ? v.narrow(1, 0, 1) : v;
+  if (one) a.Hk = 1;
+  if (!fits(k_)) k_ = k_.contiguous();
+  if (!fits(v_)) v_ = v_.contiguous();
+  auto stride = [](const at::Tensor& t, int d) { return (long long)(t.size(d) == 1 ? t.size(3) : t.stride(d)); };
+  const bool direct = fits(o);
+  at::Tensor o_ = direct ? o : at::empty(o.sizes(), o.options());
+  a.q = q_.data_ptr(), a.k = k_.data_ptr(), a.v = v_.data_ptr(), a.o = o_.data_ptr();
+  a.q_bs = stride(q_, 0), a.q_hs = stride(q_, 1), a.q_ss = stride(q_, 2);
+  a.k_bs = stride(k_, 0), a.k_hs = stride(k_, 1), a.k_ss = stride(k_, 2);
+  a.v_bs = stride(v_, 0), a.v_hs = stride(v_, 1), a.v_ss = stride(v_, 2);
+  a.o_bs = stride(o_, 0), a.o_hs = stride(o_, 1), a.o_ss = stride(o_, 2);
+  a.f16 = q.scalar_type() == at::kHalf;
+  a.scale = (float)scale;
+  if (const at::Tensor* t = given(lse)) {
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->device() == q.device() &&
+                    t->numel() == (int64_t)a.B * a.H * a.Sq, "lse must be contiguous float32 [B, H, Sq]");
+    a.lse = t->data_ptr<float>();
+  }
+  if (a.Sk == 0) {  // no key at all: every row is empty
+    o.zero_();
+    if (const at::Tensor* t = given(lse)) t->fill_(-std::numeric_limits<float>::infinity());
+    return o;
+  }
+  auto edge = [&](const c10::optional<at::Tensor>& e, const char* name) -> const int* {
+    const at::Tensor* t = given(e);
+    if (!t) return nullptr;
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() == a.B,
+                name, " must be int32 [", a.B, "]");
+    return t->data_ptr<int>();
+  };
+  a.kv_lo = edge(kv_lo, "kv_lo");
+  a.kv_hi = edge(kv_hi, "kv_hi");
+  at::Tensor bits, win;
+  if (const at::Tensor* mt = given(mask)) {
+    TORCH_CHECK(mt->device() == q.device(), "the mask must be on q's device");
+    const at::Tensor m = mt->expand({a.B, a.H, a.Sq, a.Sk});
+    if (m.scalar_type() == at::kBool) {
+      MaskBitsArgs b{};
+      b.mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
+      b.bs = m.stride(0), b.hs = m.stride(1), b.qs = m.stride(2), b.ks = m.stride(3);
+      b.B = b.bs ? a.B : 1, b.H = b.hs ? a.H : 1, b.Q = b.qs ? a.Sq : 1, b.Sk = a.Sk;
+      b.words = (a.Sk + 127) / 128 * 4;
+      bits = at::empty({(int64_t)b.B * b.H * b.Q * b.words}, q.options().dtype(at::kInt));
+      b.bits = reinterpret_cast<uint32_t*>(bits.data_ptr<int>());
+      a.key_bits = b.H == 1 && b.Q == 1;
+      if (a.key_bits && b.B == a.B && !a.kv_lo && !a.kv_hi) {
+        win = at::empty({2, a.B}, q.options().dtype(at::kInt));
+        b.lo = win.data_ptr<int>();
+        b.hi = b.lo + a.B;
+        a.kv_lo = b.lo, a.kv_hi = b.hi;
+      }
+      DFL_CHECK_RC(dfl_cross_mask_bits(&b, cur_stream()), "cross_mask_bits");
+      a.bits = b.bits;
+      a.bits_qs = b.Q > 1 ? b.words : 0;
+      a.bits_hs = b.H > 1 ? (long long)b.Q * b.words : 0;
+      a.bits_bs = b.B > 1 ? (long long)b.H * b.Q * b.words : 0;
+    } else {
+      a.bias_dtype = dtype_code(m, "an additive mask");
+      a.bias = m.data_ptr();
+      a.bias_bs = m.stride(0), a.bias_hs = m.stride(1), a.bias_qs = m.stride(2), a.bias_ks = m.stride(3);
+    }
+  }
+  a.err = err_ptr();
+  DFL_CHECK_RC(dfl_cross_attention(&a, cur_stream()), "cross_attention");
+  if (!direct) o.copy_(o_);
+  return o;
 }
 
 // Head-scatter description shared by the standalone qkv_scatter kernel and the GEMM
@@ -1012,6 +1115,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("add_rms_norm", &add_rms_norm, py::arg("x"), py::arg("resid"), py::arg("w"), py::arg("scale"), py::arg("shift"),
         py::arg("rows_per_batch"), py::arg("row_map"), py::arg("eps"), py::arg("quant"), py::arg("blocked"),
         py::arg("out"), py::arg("s_out"));
+  m.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"),
+        py::arg("mask"), py::arg("kv_lo"), py::arg("kv_hi"), py::arg("out"), py::arg("lse"));
   m.def("mx_dequantize", &mx_dequantize, py::arg("q"), py::arg("scales"), py::arg("dtype"));
   m.def("qkv_scatter", &qkv_scatter);
   m.def("qkv_plan", &qkv_plan);

@@ -36,6 +36,8 @@ enum KernelId : int {
   kKidNorm = 4,
   kKidMx = 5,
   kKidConv = 6,
+  kKidCross = 7,
+  kKidLora = 8,
 };
 
 DFL_DEVICE void record_error(int* err, int code, int kid, int d0, int d1) {

@@ -276,6 +276,37 @@ int dfl_attention(const AttnArgs* a, cudaStream_t stream);
 // Key-range split count that minimises the modelled time of this launch (1 = none).
 int dfl_attention_plan_splits(const AttnArgs* a);
 
+// Cross attention (cross_attn.cuh): q [B, H, Sq, dh], k / v [B, Hk, Sk, dh] (H a multiple of Hk: query
+// head h reads key head h / (H / Hk)), dh 64 or 128, bf16 or fp16, scale > 0.  Element strides, multiples of 8,
+// 16-byte aligned bases.  At most one of bits / bias, beside the key window.
+typedef struct CrossArgs {
+  const void* q; const void* k; const void* v; void* o;
+  long long q_bs, q_hs, q_ss, k_bs, k_hs, k_ss, v_bs, v_hs, v_ss, o_bs, o_hs, o_ss;
+  float* lse;                         // f32 [B, H, Sq] or NULL
+  int B, H, Hk, Sq, Sk, dh, f16;
+  float scale;
+  const int* kv_lo; const int* kv_hi;  // [B] key windows or NULL
+  const uint32_t* bits;                // rows written by dfl_cross_mask_bits; strides in words (0: broadcast)
+  long long bits_bs, bits_hs, bits_qs;
+  int key_bits;                        // the bits are the same for every query and head
+  const void* bias;                    // additive mask, element strides (0: broadcast)
+  long long bias_bs, bias_hs, bias_qs, bias_ks;
+  int bias_dtype;
+  int* err;
+} CrossArgs;
+int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream);
+
+// Boolean mask [B, H, Q, Sk] (1 byte per element, element strides) -> bit rows [B, H, Q, words], words =
+// 4 ceil(Sk / 128); lo / hi (H = Q = 1 only, or NULL): the window of the kept keys of every batch row.
+typedef struct MaskBitsArgs {
+  const uint8_t* mask;
+  long long bs, hs, qs, ks;
+  int B, H, Q, Sk, words;
+  uint32_t* bits;
+  int* lo; int* hi;
+} MaskBitsArgs;
+int dfl_cross_mask_bits(const MaskBitsArgs* a, cudaStream_t stream);
+
 // ---------------------------------------------------------------------------
 // Peer-memory communication runtime (comm.cu)
 // ---------------------------------------------------------------------------

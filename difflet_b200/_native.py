@@ -31,6 +31,8 @@ CUDA_SOURCES = [
     "norm.cu",
     "add_norm.cu",
     "attention.cu",
+    "cross_attn.cu",
+    "cross_attn_f16.cu",
     "comm.cu",
     "mx.cu",
     "conv.cu",
@@ -41,7 +43,7 @@ CUDA_SOURCES = [
     "vae_gn.cu",
 ]
 CPP_SOURCES = ["bindings.cpp"]
-HEADERS = ["common.cuh", "kernels.h", "probe_noalloc.h", "gemm_epilogue.cuh"]
+HEADERS = ["common.cuh", "kernels.h", "probe_noalloc.h", "gemm_epilogue.cuh", "cross_attn.cuh"]
 
 NVCC_FLAGS = [
     "-gencode",

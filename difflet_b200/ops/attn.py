@@ -8,12 +8,14 @@ Contract (difflet/ops/attention.py:4-128, difflet/backends/cuda/ops_impl/attenti
   (both or neither, exclusive with a mask) select the keys ``[bound_min, bound_max)``.
 * ``tp_q`` / ``tp_k`` / ``tp_out`` are layout hints of other hardware: accepted, ignored.
 
-Dispatch: CUDA tensors with head dim 128, no mask, non-causal and bounds that are
+Dispatch: CUDA tensors with head dim 128, bf16, no mask, non-causal and bounds that are
 per batch row (shape ``[B]`` or ``[B, 1, ...]``, the padded-text key windows every
-model here uses) run the tcgen05 kernel (``csrc/attention.cu``).  Anything else on
-CUDA (arbitrary masks, causal, other head dims, per-query windows) is the library
-path: ``torch.nn.functional.scaled_dot_product_attention``.  CPU tensors run the
-fp32 / fp64 oracle of ``ops.fused``.
+model here uses) run the tcgen05 kernel of ``csrc/attention.cu``.  Masks (boolean or
+additive), per-query windows, head dim 64 and fp16 run the tcgen05 kernel of
+``csrc/cross_attn.cuh``, which ``cross_attention`` always takes.  Anything else on CUDA
+(causal, other head dims, fp32) is the library path:
+``torch.nn.functional.scaled_dot_product_attention``.  CPU tensors run the fp32 / fp64
+oracle of ``ops.fused``.
 
 Context-parallel ops (``ring_attention``, ``joint_ring_attention``,
 ``ulysses_attention``, ``joint_ulysses_attention``) run over the cp group of the
@@ -74,6 +76,13 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
             lo = lo.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
             hi = hi.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
         out = F.attention(q4, k4, v4, scale, lse=lse, kv_lo=lo, kv_hi=hi)
+    elif F.cross_kernel_ok(q) and not causal and k4.dtype == v4.dtype == q4.dtype and k4.shape[1] == q4.shape[1]:
+        mask = attention_mask if simple or bound_min is None else _bounds_to_mask(k4, bound_min, bound_max, None)
+        if lo is not None and simple:
+            lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
+        else:
+            lo = hi = None
+        out = F.cross_attention(q4, k4, v4, scale, mask=_mask_on(mask, q), kv_lo=lo, kv_hi=hi, lse=lse)
     else:
         mask = _bounds_to_mask(k4, bound_min, bound_max, attention_mask)
         if lse is not None or not q.is_cuda:  # math path (oracle, or LSE requested off the kernel)
@@ -116,10 +125,84 @@ def _oracle_masked(q, k, v, scale, causal, mask, lse=None):
     return torch.einsum("bhqk,bhkd->bhqd", p, v.to(ct)).to(q.dtype)
 
 
-def cross_attention(q, k, v, *, scale=None, attention_mask=None, **kwargs):
+def _mask_on(mask, q):
+    """A mask on q's device whose type the kernel reads (integers: non-zero = attend, as a boolean)."""
+    if mask is None:
+        return None
+    if not mask.is_floating_point():
+        mask = mask.bool()
+    elif mask.dtype not in (torch.bfloat16, torch.float16, torch.float32) and q.is_cuda:
+        mask = mask.float()
+    return mask.to(q.device)
+
+
+def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, lse=None, out=None, bound_min=None,
+                    bound_max=None, **kwargs):
+    """Attention of ``q [B, H, Sq, D]`` to encoder states ``k, v [B, Hk, Sk, D]`` of another length.
+
+    ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``).  ``attention_mask``: bool (True =
+    attend) or additive, broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
+    each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
+    ``attention``.  A query that no key is left for gives 0.  ``out`` (like q) and ``lse`` (f32 ``[B, H, Sq]``, natural
+    log) are filled when given.  CUDA: bf16 and fp16 with head dim 64 or 128; anything else runs as ``attention``."""
     for key in ("tp_q", "tp_k", "tp_out", "causal"):
         kwargs.pop(key, None)
-    return attention(q, k, v, scale=scale, causal=False, attention_mask=attention_mask, **kwargs)
+    F._no_grad("cross_attention", q, k, v, attention_mask)
+    if q.dim() == 3:
+        if kv_lens is not None or out is not None:
+            raise ValueError("kv_lens and out need q [B, H, S, D]")
+        o = cross_attention(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), scale=scale, attention_mask=attention_mask,
+                            lse=lse, bound_min=bound_min, bound_max=bound_max)
+        return o.squeeze(0)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"q [B, H, Sq, D], k / v [B, Hk, Sk, D]; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, H, Sq, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D or k.shape[1] < 1 or H % k.shape[1]:
+        raise ValueError(f"k / v {tuple(k.shape)} do not match q {tuple(q.shape)} (H must be a multiple of Hk)")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must share type and device")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not match q {tuple(q.shape)} {q.dtype}")
+    if lse is not None and (lse.numel() != B * H * Sq or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous [{B}, {H}, {Sq}]")
+    lo = hi = None
+    if kv_lens is not None:
+        if bound_min is not None or bound_max is not None:
+            raise ValueError("kv_lens and bounds are mutually exclusive")
+        if kv_lens.shape != (B,) or kv_lens.is_floating_point():
+            raise ValueError(f"kv_lens must be integers [{B}]")
+        hi = kv_lens if kv_lens.dtype == torch.int32 and kv_lens.device == q.device else kv_lens.to(q.device, torch.int32)
+        hi = hi.contiguous()
+    elif bound_min is not None or bound_max is not None:
+        if bound_min is None or bound_max is None:
+            raise ValueError("bound_min and bound_max must both be provided")
+        if attention_mask is not None:
+            raise ValueError("attention_mask and bounds are mutually exclusive")
+        lo, hi = _per_batch(bound_min, B), _per_batch(bound_max, B)
+        if lo is None or hi is None:
+            attention_mask, lo, hi = _bounds_to_mask(k, bound_min, bound_max, None), None, None
+        else:
+            lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
+    mask = attention_mask
+    if mask is not None:
+        mask = _mask_on(mask, q)
+        want = (B, H, Sq, k.shape[2])
+        if mask.dim() > 4 or any(m not in (1, w) for m, w in zip(mask.shape[::-1], want[::-1])):
+            raise ValueError(f"attention_mask {tuple(mask.shape)} does not broadcast to {want}")
+    scale = 1.0 if scale is None else float(scale)
+    if not q.is_cuda or F.cross_kernel_ok(q):
+        return F.cross_attention(q, k, v, scale, mask=mask, kv_lo=lo, kv_hi=hi, out=out, lse=lse)
+    if hi is not None:  # off the kernel: the window as a mask
+        idx = torch.arange(k.shape[2], device=q.device)
+        win = (idx < hi[:, None]) if lo is None else (idx < hi[:, None]) & (idx >= lo[:, None])
+        win = win[:, None, None]
+        if mask is None or mask.dtype == torch.bool:
+            mask = win if mask is None else mask & win
+        else:
+            mask = mask.masked_fill(~win, float("-inf"))
+    rep = H // k.shape[1]
+    o = attention(q, k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1), scale=scale, attention_mask=mask, lse=lse)
+    return o if out is None else out.copy_(o)
 
 
 def attention_with_lse(q, k, v, *, scale, bound_min=None, bound_max=None):

@@ -18,6 +18,7 @@ Ops:
   linear_group  two linear / linear_qkv calls with one epilogue kind as one launch
   row_sumsq     per-row sums of squares of q / k column blocks (TP across-heads RMS)
   attention     softmax(scale q k^T) v with key window and LSE
+  cross_attention attention with masks, shared key heads, head dim 64 / 128, bf16 / fp16
   gemv          modulation linears (M <= 8), f32 in/out, optional SiLU
   euler_step    x += dt * (u + s (c - u)) on f32 latents (+ bf16 mirror)
   timestep_embed sinusoidal features
@@ -563,10 +564,17 @@ def kv_split_mode() -> int:
     return -1 if envs.DIFFLET_ATTN_SPLIT != "0" else 1
 
 
+def cross_kernel_ok(q) -> bool:
+    """Whether the masked / head-dim-64 attention kernel takes these queries."""
+    return q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in (torch.bfloat16, torch.float16)
+
+
 def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     """softmax(scale * q k^T) v over [B, H, S, dh]; key window [kv_lo[b], kv_hi[b])."""
     if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128:
         return native().attention(q, k, v, float(scale), out, lse, kv_lo, kv_hi, kv_split=kv_split_mode())
+    if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and cross_kernel_ok(q):
+        return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     if q.is_cuda and lse is None and kv_lo is None:
         o = F.scaled_dot_product_attention(q, k, v, scale=float(scale))
@@ -593,6 +601,42 @@ def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
         out.copy_(o)
         return out
     return o
+
+
+def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=None, lse=None):
+    """softmax(scale q k^T [+ mask]) v with keys of another length than the queries.
+
+    q [B, H, Sq, D]; k, v [B, Hk, Sk, D] with H a multiple of Hk (query head h reads key head
+    ``h // (H // Hk)``); any strides.  ``mask``: bool (True = attend) or additive (bf16, fp16 or f32; -inf or
+    the type's lowest value masks), broadcastable to [B, H, Sq, Sk]; beside it the key window
+    [kv_lo[b], kv_hi[b]) (int32 [B]).  A row without a key is 0 with LSE -inf.  What k and v hold at keys
+    that the window or a key mask (bool, the same for every head and query) excludes is not used.
+    CUDA: bf16 / fp16 with D 64 or 128 run the tcgen05 kernel."""
+    if q.is_cuda:
+        if scale <= 0:  # the kernel scales inside the exponent, where the maximum must commute with it
+            q, scale = (-q, -scale) if scale < 0 else (torch.zeros_like(q), 1.0)
+        return native().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse)
+    ct = torch.float64 if q.dtype == torch.float64 else torch.float32
+    Sk, rep = k.shape[2], q.shape[1] // k.shape[1]
+    idx = torch.arange(Sk)
+    keep = torch.ones(q.shape[0], Sk, dtype=torch.bool)
+    if kv_lo is not None:
+        keep &= idx >= kv_lo.view(-1, 1)
+    if kv_hi is not None:
+        keep &= idx < kv_hi.view(-1, 1)
+    if mask is not None and mask.dtype == torch.bool and mask.dim() == 4 and mask.shape[1] == mask.shape[2] == 1:
+        keep, mask = keep & mask[:, 0, 0], None
+    vz = v.to(ct).masked_fill(~keep[:, None, :, None], 0.0)
+    s = torch.einsum("bhqd,bhkd->bhqk", q.to(ct), k.to(ct).repeat_interleave(rep, 1)) * scale
+    if mask is not None:
+        s = s.masked_fill(~mask, float("-inf")) if mask.dtype == torch.bool else s + mask.to(ct)
+    s = s.masked_fill(~keep[:, None, None], float("-inf"))
+    m = torch.logsumexp(s, -1) if Sk else s.new_full(s.shape[:-1], float("-inf"))
+    p = torch.where(torch.isinf(m)[..., None] & (m < 0)[..., None], torch.zeros_like(s), torch.softmax(s, -1))
+    o = torch.einsum("bhqk,bhkd->bhqd", p, vz.repeat_interleave(rep, 1)).to(q.dtype)
+    if lse is not None:
+        lse.copy_(m.to(lse.dtype).reshape(lse.shape))
+    return o if out is None else out.copy_(o)
 
 
 # --------------------------------------------------------------------------- convolution
