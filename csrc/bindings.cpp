@@ -151,6 +151,77 @@ at::Tensor gemm(const at::Tensor& A, const at::Tensor& B, const c10::optional<at
   return D;
 }
 
+// gemm with low-rank adapters: A_l [n, r, K], B_l [n, N, r], scale [n], ids int32 per row or per
+// rows_per_id rows.
+at::Tensor gemm_lora(const at::Tensor& A, const at::Tensor& B, const c10::optional<at::Tensor>& bias,
+                     c10::optional<at::Tensor> out, int64_t epi, int64_t act_lo, int64_t act_hi,
+                     const c10::optional<at::Tensor>& gate, int64_t rows_per_batch,
+                     const c10::optional<at::Tensor>& resid, bool out_f32, const at::Tensor& A_l, const at::Tensor& B_l,
+                     const at::Tensor& scale, const at::Tensor& ids, int64_t rows_per_id) {
+  check_bf16_cuda(A, "x");
+  check_bf16_cuda(B, "weight");
+  check_rowmajor(A, "x");
+  check_rowmajor(B, "weight");
+  check_bf16_cuda(A_l, "adapter A");
+  check_bf16_cuda(B_l, "adapter B");
+  const int64_t M = A.size(0), K = A.size(1), N = B.size(0);
+  TORCH_CHECK(B.size(1) == K, "K mismatch: x ", A.sizes(), " weight ", B.sizes());
+  TORCH_CHECK(A_l.dim() == 3 && A_l.is_contiguous() && B_l.dim() == 3 && B_l.is_contiguous() && A_l.size(2) == K &&
+                  B_l.size(1) == N && A_l.size(0) == B_l.size(0) && A_l.size(1) == B_l.size(2),
+              "adapters must be contiguous [n, r, K] and [n, N, r]");
+  TORCH_CHECK(scale.is_contiguous() && scale.scalar_type() == at::kFloat && scale.numel() == A_l.size(0),
+              "adapter scale must be float32 [n]");
+  TORCH_CHECK(ids.scalar_type() == at::kInt && ids.is_contiguous() && ids.dim() == 1 &&
+                  ids.numel() == (rows_per_id > 0 ? (M + rows_per_id - 1) / rows_per_id : M),
+              "ids must be int32, one per row or per ", rows_per_id, " rows");
+  for (const at::Tensor* t : {&B, &A_l, &B_l, &scale, &ids})
+    TORCH_CHECK(t->device() == A.device(), "all tensors on one device");
+  TORCH_CHECK(K % 8 == 0, "linear_lora needs K to be a multiple of 8, got ", K);
+  const c10::cuda::CUDAGuard guard(A.device());
+  GemmArgs a{};
+  at::Tensor D = gemm_epilogue_args(a, A, M, N, bias, out, epi, act_lo, act_hi, gate, rows_per_batch, resid, 1.0,
+                                    out_f32, {}, 0, 0, 0, c10::nullopt, "");
+  TORCH_CHECK(epi != kEpiGateResid || gate->size(0) * (int64_t)a.rows_per_batch >= M, "gate has too few rows");
+  a.A = A.data_ptr();
+  a.B = B.data_ptr();
+  a.lda = A.stride(0);
+  a.ldb = B.stride(0);
+  a.K = (int)K;
+  LoraArgs l{};
+  a.lora = &l;
+  l.a = A_l.data_ptr();
+  l.b = B_l.data_ptr();
+  l.scale = scale.data_ptr<float>();
+  l.ids = ids.data_ptr<int>();
+  l.rows_per_id = (int)std::min<int64_t>(rows_per_id > 0 ? rows_per_id : 0, 1 << 30);
+  l.n_adapters = (int)A_l.size(0);
+  l.rank = (int)A_l.size(1);
+  // split-K partial tiles of this call: only launches that leave SMs idle split (one 128 x 256 f32 tile
+  // per CTA tile and at most 96 of them)
+  const auto i32 = A.options().dtype(at::kInt);
+  at::Tensor ws, sem;
+  if ((M + 127) / 128 * ((N + 255) / 256) <= 96) {
+    l.split_ws_floats = 96ll * 128 * 256;
+    l.split_sem_count = 256;
+    ws = at::empty({l.split_ws_floats}, A.options().dtype(at::kFloat));
+    sem = at::empty({l.split_sem_count}, i32);
+    l.split_ws = ws.data_ptr<float>();
+    l.split_sem = sem.data_ptr<int>();
+  }
+  l.tile_rows = dfl_gemm_tile_rows(&a);
+  const int64_t tiles = (M + l.tile_rows - 1) / l.tile_rows;
+  int64_t cap = std::min<int64_t>(l.n_adapters, l.tile_rows);
+  if (rows_per_id > 0) cap = std::min<int64_t>(cap, (l.tile_rows - 1 + rows_per_id - 1) / rows_per_id + 1);
+  l.cap = (int)cap;
+  const at::Tensor t = at::empty({tiles * cap * l.tile_rows, l.rank}, A.options());
+  const at::Tensor list = at::empty({tiles * (1 + cap)}, i32);
+  l.t = t.data_ptr();
+  l.list = list.data_ptr<int>();
+  a.cta_mode = l.tile_rows == 256 ? 2 : 1;  // the tile shape the lists are built for
+  DFL_CHECK_RC(dfl_gemm_lora(&a, cur_stream()), "gemm_lora");
+  return D;
+}
+
 // ---------------------------------------------------------------- MXFP8
 std::vector<at::Tensor> mx_quantize(const at::Tensor& x, bool blocked) {
   check_bf16_cuda(x, "x");
@@ -1099,6 +1170,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_group", &gemm_group, "grouped tcgen05 GEMMs (one launch)", py::arg("A"), py::arg("B"),
         py::arg("bias"), py::arg("out"), py::arg("epi"), py::arg("act_lo"), py::arg("act_hi"), py::arg("gate"),
         py::arg("rows_per_batch"), py::arg("resid"), py::arg("qkv_plan"), py::arg("cta_mode") = 0);
+  m.def("gemm_lora", &gemm_lora, "tcgen05 GEMM with low-rank adapters accumulated beside the weight", py::arg("A"),
+        py::arg("B"), py::arg("bias"), py::arg("out"), py::arg("epi"), py::arg("act_lo"), py::arg("act_hi"),
+        py::arg("gate"), py::arg("rows_per_batch"), py::arg("resid"), py::arg("out_f32"), py::arg("A_l"),
+        py::arg("B_l"), py::arg("scale"), py::arg("ids"), py::arg("rows_per_id"));
   m.def("mx_quantize", &mx_quantize, py::arg("x"), py::arg("blocked") = false);
   m.def("gemm_mx", &gemm_mx, "block-scaled MXFP8 tcgen05 GEMM", py::arg("A"), py::arg("sfa"), py::arg("B"),
         py::arg("sfb"), py::arg("bias") = py::none(), py::arg("out") = py::none(), py::arg("epi") = 0,

@@ -106,7 +106,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int lora_kc = (P.lora_rank + BK - 1) / BK;
+        const int kb_end = kb1 + lora_count(P, mb, lt % P.splits) * lora_kc;
+        for (int kb = kb0; kb < kb_end; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 10 + stage, abort_flag)) {
             ok = false;
             break;
@@ -114,8 +116,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* sa = smem + stage * S::kStageBytes;
           uint8_t* sb = sa + S::kABytes;
           mbar_arrive_expect_tx(&full_bar[stage], S::kStageBytes);
-          tma_load_2d(sa, &P.ta, &full_bar[stage], kb * BK, mb * BM);
-          tma_load_2d(sb, &P.tb, &full_bar[stage], kb * BK, nb * BN);
+          if (kb < kb1) {
+            tma_load_2d(sa, &P.ta, &full_bar[stage], kb * BK, mb * BM);
+            tma_load_2d(sb, &P.tb, &full_bar[stage], kb * BK, nb * BN);
+          } else {
+            const int j = (kb - kb1) / lora_kc, c = (kb - kb1) % lora_kc;
+            tma_load_2d(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * BM);
+            tma_load_2d(sb, &P.tl, &full_bar[stage], c * BK, lora_id(P, mb, j) * P.lora_n + nb * BN);
+          }
           issued[stage] = true;
           issued_parity[stage] = phase;
           if (++stage == STAGES) {
@@ -145,10 +153,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        int lt, kb0, kb1;
+        int lt, mb, nb, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
+        tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int kb_end = kb1 + lora_count(P, mb, lt % P.splits) * ((P.lora_rank + BK - 1) / BK);
+        for (int kb = kb0; kb < kb_end; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 30 + stage, abort_flag)) {
             ok = false;
             break;
@@ -325,9 +335,22 @@ static double split_model(long long tiles, int ctas, int kb_max, int sms, double
 static int g_split_force = 0;
 extern "C" void dfl_gemm_set_split_force(int s) { g_split_force = (s >= 0 && s <= 4) ? s : 0; }
 
-static void plan_split_k(GemmGroup& g, int epi, int bn, int sms, int dev, int ctas) {
+// Split-K workspace of one launch: the call's own (adapter projections, which may run on several
+// streams at once) or the device's.
+struct SplitWs {
+  float* ws;
+  long long floats;
+  int* sem;
+  int sem_count;
+};
+static SplitWs split_ws_of(const GemmArgs* a, int dev) {
+  if (a->lora) return {a->lora->split_ws, a->lora->split_ws_floats, a->lora->split_sem, a->lora->split_sem_count};
   const int d = dev & 15;
-  if (!g_split_ws[d] || epi == kEpiSwiGLU || epi == kEpiQkv) return;
+  return {g_split_ws[d], g_split_ws_floats[d], g_split_sem[d], g_split_sem_count[d]};
+}
+
+static void plan_split_k(GemmGroup& g, int epi, int bn, int sms, const SplitWs& w, int ctas) {
+  if (!w.ws || epi == kEpiSwiGLU || epi == kEpiQkv) return;
   int kb_max = 0;
   for (int i = 0; i < g.count; ++i) kb_max = std::max(kb_max, (g.p[i].K + BK - 1) / BK);
   int best = 1;
@@ -344,10 +367,10 @@ static void plan_split_k(GemmGroup& g, int epi, int bn, int sms, int dev, int ct
     const int per = (kb + best - 1) / best;
     if (per < 4 || (best - 1) * per >= kb) continue;  // every range must hold K blocks
     const long long need = (long long)base_tiles * ctas * BM * bn;  // one partial per CTA tile
-    if (ws_off + need > g_split_ws_floats[d] || sem_off + base_tiles * ctas > g_split_sem_count[d]) continue;
+    if (ws_off + need > w.floats || sem_off + base_tiles * ctas > w.sem_count) continue;
     P.splits = best;
-    P.ws = g_split_ws[d] + ws_off;
-    P.sem = g_split_sem[d] + sem_off;
+    P.ws = w.ws + ws_off;
+    P.sem = w.sem + sem_off;
     ws_off += need;
     sem_off += base_tiles * ctas;
     g.total_tiles += base_tiles * (best - 1);  // one more item per tile and extra range
@@ -357,24 +380,13 @@ static void plan_split_k(GemmGroup& g, int epi, int bn, int sms, int dev, int ct
 
 extern "C" int dfl_gemm_pair_can_split(int epi);
 
-// One launch for `count` GEMMs that share the epilogue kind and output type.  The tile
-// shape (CTA pairs with 256 x 256 tiles, or one CTA with 128 x 256 / 128 x 128 tiles)
-// follows the first problem; the others are tiled the same way.
-extern "C" int dfl_gemm_bf16_group(const GemmArgs* const* args, int count, cudaStream_t stream) {
-  if (count < 1 || count > kMaxGroup) return -12;
+// Tile shape of a launch: CTA pairs (256-row tiles) or single CTAs, wide (256) or narrow columns.
+static bool use_pair(const GemmArgs* const* args, int count, bool has_ws, int sms, bool* wide_out) {
   const GemmArgs* a0 = args[0];
-  for (int i = 0; i < count; ++i) {
-    const int rc = check_args(args[i]);
-    if (rc) return rc;
-    if (args[i]->epi != a0->epi || args[i]->out_f32 != a0->out_f32 || args[i]->err != a0->err) return -12;
-  }
-  int dev = 0;
-  cudaGetDevice(&dev);
   bool wide = a0->cta_mode != 3;  // cta_mode 3: one CTA per tile, 128-column tiles (6 stages)
   for (int i = 0; i < count; ++i) wide = wide && args[i]->N >= 1024;
   bool pair = a0->cta_mode == 2 || (a0->cta_mode == 0 && g_pair_auto && wide && a0->M >= 1024);
-  const int sms = dfl_host::num_sms(dev);
-  if (!pair && a0->cta_mode == 0 && g_pair_auto && wide && g_split_ws[dev & 15] && dfl_gemm_pair_can_split(a0->epi)) {
+  if (!pair && a0->cta_mode == 0 && g_pair_auto && wide && has_ws && dfl_gemm_pair_can_split(a0->epi)) {
     // small M: CTA pairs (with split-K) against single CTAs (with split-K), by the model above
     long long t1 = 0, t2 = 0;
     int kb_max = 0;
@@ -387,6 +399,36 @@ extern "C" int dfl_gemm_bf16_group(const GemmArgs* const* args, int count, cudaS
     pair = split_model(t2, 2, kb_max, sms, kPairKbCost, kFixup256, nullptr) <
            split_model(t1, 1, kb_max, sms, 1.0, kFixup256, nullptr);
   }
+  *wide_out = wide;
+  return pair;
+}
+
+// Rows of an M tile of the launch `a` would get (the adapter lists are built per M tile).
+extern "C" int dfl_gemm_tile_rows(const GemmArgs* a) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  bool wide;
+  return use_pair(&a, 1, split_ws_of(a, dev).ws != nullptr, dfl_host::num_sms(dev), &wide) ? 2 * BM : BM;
+}
+
+// One launch for `count` GEMMs that share the epilogue kind and output type.  The tile
+// shape (CTA pairs with 256 x 256 tiles, or one CTA with 128 x 256 / 128 x 128 tiles)
+// follows the first problem; the others are tiled the same way.
+extern "C" int dfl_gemm_bf16_group(const GemmArgs* const* args, int count, cudaStream_t stream) {
+  if (count < 1 || count > kMaxGroup) return -12;
+  const GemmArgs* a0 = args[0];
+  if (count > 1 && (a0->lora || args[1]->lora)) return -12;
+  for (int i = 0; i < count; ++i) {
+    const int rc = check_args(args[i]);
+    if (rc) return rc;
+    if (args[i]->epi != a0->epi || args[i]->out_f32 != a0->out_f32 || args[i]->err != a0->err) return -12;
+  }
+  int dev = 0;
+  cudaGetDevice(&dev);
+  bool wide;
+  const int sms = dfl_host::num_sms(dev);
+  const SplitWs ws = split_ws_of(a0, dev);
+  const bool pair = use_pair(args, count, ws.ws != nullptr, sms, &wide);
   const int bm = pair ? 2 * BM : BM;
   const int bn = (pair || wide) ? 256 : 128;
   GemmGroup g;
@@ -408,13 +450,25 @@ extern "C" int dfl_gemm_bf16_group(const GemmArgs* const* args, int count, cudaS
     P.num_n = (a->N + bn - 1) / bn;
     P.tiles = P.num_m * P.num_n;
     P.splits = 1;
+    if (const LoraArgs* l = a->lora) {
+      if (l->tile_rows != bm) return -13;
+      rc = dfl_host::make_tmap_2d_bf16(&P.tt, l->t, l->rank, (uint64_t)P.num_m * l->cap * bm, l->rank, BK, BM, true);
+      if (rc) return 4000 + rc;
+      rc = dfl_host::make_tmap_2d_bf16(&P.tl, l->b, l->rank, (uint64_t)l->n_adapters * a->N, l->rank, BK,
+                                       pair ? 128 : bn, true);
+      if (rc) return 5000 + rc;
+      P.lora_list = l->list;
+      P.lora_cap = l->cap;
+      P.lora_rank = l->rank;
+      P.lora_n = a->N;
+    }
     g.total_tiles += P.tiles;
   }
   if (pair) {
-    if (dfl_gemm_pair_can_split(a0->epi)) plan_split_k(g, a0->epi, 256, sms, dev, 2);
+    if (dfl_gemm_pair_can_split(a0->epi)) plan_split_k(g, a0->epi, 256, sms, ws, 2);
     return dfl_gemm_pair_launch(&g, a0->epi, a0->out_f32, a0->err, stream, dev);
   }
-  plan_split_k(g, a0->epi, bn, sms, dev, 1);
+  plan_split_k(g, a0->epi, bn, sms, ws, 1);
   if (wide) return dispatch_epi<256, 4>(a0->epi, a0->out_f32, g, a0->err, stream, dev);
   return dispatch_epi<128, 6>(a0->epi, a0->out_f32, g, a0->err, stream, dev);
 }

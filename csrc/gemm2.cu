@@ -158,15 +158,24 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int lora_kc = (P.lora_rank + BK - 1) / BK;
+        const int kb_end = kb1 + lora_count(P, mb, lt % P.splits) * lora_kc;
+        for (int kb = kb0; kb < kb_end; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
             ok = false;
             break;
           }
           uint8_t* sa = smem + stage * kStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
-          tma_load_2d_pair(sa, &P.ta, &full_bar[stage], kb * BK, mb * 2 * BM + (int)rank * BM);
-          tma_load_2d_pair(sa + kABytes, &P.tb, &full_bar[stage], kb * BK, nb * BN + (int)rank * (BN / 2));
+          if (kb < kb1) {
+            tma_load_2d_pair(sa, &P.ta, &full_bar[stage], kb * BK, mb * 2 * BM + (int)rank * BM);
+            tma_load_2d_pair(sa + kABytes, &P.tb, &full_bar[stage], kb * BK, nb * BN + (int)rank * (BN / 2));
+          } else {
+            const int j = (kb - kb1) / lora_kc, c = (kb - kb1) % lora_kc;
+            tma_load_2d_pair(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * 2 * BM + (int)rank * BM);
+            tma_load_2d_pair(sa + kABytes, &P.tl, &full_bar[stage], c * BK,
+                             lora_id(P, mb, j) * P.lora_n + nb * BN + (int)rank * (BN / 2));
+          }
           issued[stage] = true;
           issued_parity[stage] = phase;
           if (++stage == STAGES) {
@@ -194,10 +203,12 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        int lt, kb0, kb1;
+        int lt, mb, nb, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
+        tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int kb_end = kb1 + lora_count(P, mb, lt % P.splits) * ((P.lora_rank + BK - 1) / BK);
+        for (int kb = kb0; kb < kb_end; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
             ok = false;
             break;

@@ -57,7 +57,22 @@ struct alignas(64) GemmProblem {
   int splits;
   float* ws;  // f32 [num_m * num_n][128][BN] partial tiles
   int* sem;   // [num_m * num_n] split counters, 0 between launches
+  // Low-rank adapters: the K loop of M tile mb goes on over the adapters its rows use (lora_list,
+  // [num_m][1 + lora_cap]: count, adapter ids; NULL: none), accumulating T_j B_j^T onto X W^T.  Block j of
+  // tile mb holds T of adapter j (zero in the rows of other adapters) in rows (mb * lora_cap + j) *
+  // tile rows of tt; tl holds the adapters' B, lora_n rows each.  The last K range of a tile takes them.
+  CUtensorMap tt, tl;
+  const int* lora_list;
+  int lora_cap, lora_rank, lora_n;
 };
+
+// Adapters the K range `split` of M tile mb goes on with.
+DFL_DEVICE int lora_count(const GemmProblem& P, int mb, int split) {
+  return P.lora_list != nullptr && split == P.splits - 1 ? __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap)) : 0;
+}
+DFL_DEVICE int lora_id(const GemmProblem& P, int mb, int j) {
+  return __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap) + 1 + j);
+}
 
 struct alignas(64) GemmGroup {
   GemmProblem p[kMaxGroup];

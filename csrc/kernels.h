@@ -53,7 +53,31 @@ typedef struct GemmArgs {
   // the source rows are the GEMM rows).  Per-head RMS (norm_mode 0 / 1), full-width RoPE,
   // dh 64 or 128, column offsets multiples of dh.
   const struct QkvScatterArgs* qkv;
+  // Low-rank adapters beside the product (dfl_gemm_lora), or NULL.
+  const struct LoraArgs* lora;
 } GemmArgs;
+
+// Adapters of many requests beside one projection (lora.cu, gemm.cu):
+//   D = epi(X W^T + bias + s_i (X A_i^T) B_i^T),  i = adapter of the row (-1: none).
+// A first kernel computes T = s_i X A_i^T per M tile for the adapters its rows use and lists them;
+// the GEMM's K loop then goes on over T_j B_j^T into the same f32 accumulator.
+typedef struct LoraArgs {
+  const void* a;         // bf16 [n_adapters, rank, K] contiguous
+  const void* b;         // bf16 [n_adapters, N, rank] contiguous
+  const float* scale;    // f32 [n_adapters]
+  const int* ids;        // adapter of row r: ids[rows_per_id > 0 ? r / rows_per_id : r]
+  int rows_per_id;
+  int n_adapters, rank;  // rank (padded with zeros): 16, 32, 48, 64 or 128; at most 1024 adapters
+  int cap;               // adapters an M tile can hold: min(n_adapters, what its rows allow)
+  int tile_rows;         // dfl_gemm_tile_rows
+  void* t;               // bf16 [M tiles][cap][tile_rows][rank]
+  int* list;             // [M tiles][1 + cap]
+  // this call's own split-K workspace (no size: none); the counters are zeroed by the first kernel
+  float* split_ws; long long split_ws_floats;
+  int* split_sem; int split_sem_count;
+} LoraArgs;
+int dfl_gemm_tile_rows(const GemmArgs* a);
+int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream);  // a->lora set
 
 int dfl_gemm_bf16(const GemmArgs* a, cudaStream_t stream);
 // Split-K workspace of `device` (f32 partial tiles + int counters that must start at 0 and

@@ -1,0 +1,297 @@
+// Low-rank adapters of many requests beside a shared projection (sm_100a).
+//
+//   y = epi(x W^T + b + s_i (x A_i^T) B_i^T),   i = adapter of the row, -1 for none
+//
+// Two launches.  lora_shrink_kernel reads x once: for each 128-row tile it finds the adapters
+// its rows use, computes x A_j^T for all of them on the tensor cores (up to 128 accumulator columns a
+// pass), and stores T_j = s_j x A_j^T rounded to bf16, zero in the rows of other adapters.  The GEMM (gemm.cu,
+// gemm2.cu) then runs x W^T and goes on over the tile's list with T_j B_j^T in the same f32 accumulator, so
+// the adapters cost it ceil(rank / 64) K blocks per adapter a tile holds, and its epilogue is unchanged.
+//
+// The shrink is bound by reading x (2 M K bytes): a cluster of up to eight CTAs shares a tile, each
+// taking a range of K, so that few tiles still occupy many SMs; the f32 partial sums are added through
+// distributed shared memory in a fixed order.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace {
+using namespace dfl;
+
+constexpr int kBM = 128, kBK = 64, kStages = 3;
+constexpr int kCols = 128;                     // accumulator columns per pass
+constexpr int kXBytes = kBM * kBK * 2;         // 16 KB
+constexpr int kABytes = kCols * kBK * 2;       // 16 KB
+constexpr int kStageBytes = kXBytes + kABytes;
+constexpr int kPartLd = kBM + 1;               // f32 partial [column][row + 1]: conflict-free both ways
+constexpr int kBar = kStages * kStageBytes;
+constexpr int kThreads = 192;
+constexpr int kMaxAdapters = 1024;
+// after the barriers: TMEM slot, abort flag, adapter bitmap, list, row slots
+constexpr int kMisc = kBar + (2 * kStages + 1) * 8;
+constexpr int kBitmap = (kMisc + 8 + 15) / 16 * 16;
+constexpr int kList = kBitmap + kMaxAdapters / 8;       // count, ids (at most 256)
+constexpr int kSlot = kList + 257 * 4;                  // int16 list position of every row (-1: none)
+constexpr int kTotal = (kSlot + kBM * 2 + 15) / 16 * 16 + 1024;
+static_assert(kCols * kPartLd * 4 <= kBar, "partial sums reuse the stages");
+static_assert(kTotal <= 113 * 1024, "two CTAs per SM");
+
+struct ShrinkParams {
+  const int* ids;
+  int rows_per_id;
+  const float* scale;
+  int n_adapters, rank, cap, tile_rows;
+  __nv_bfloat16* t;
+  int* list;
+  int* sem;
+  int sem_count;
+  int M, K;
+};
+
+DFL_DEVICE uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+DFL_DEVICE uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+DFL_DEVICE void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+DFL_DEVICE float ld_cluster(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+
+__global__ void __launch_bounds__(kThreads, 2)
+    lora_shrink_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ta, ShrinkParams p,
+                       int* err) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kBar);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* done_bar = empty_bar + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + kBitmap);
+  int* list = reinterpret_cast<int*>(smem + kList);
+  int16_t* slot = reinterpret_cast<int16_t*>(smem + kSlot);
+  float* part = reinterpret_cast<float*>(smem);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int tile = blockIdx.x / ranks;            // 128-row tile
+  const int per_group = p.tile_rows / kBM;        // 128-row tiles per M tile of the GEMM
+  const int group = tile / per_group;
+  const long long row0 = (long long)tile * kBM, grow0 = (long long)group * p.tile_rows;
+
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.sem_count; i += kThreads) p.sem[i] = 0;
+  if (threadIdx.x < kMaxAdapters / 32) bitmap[threadIdx.x] = 0u;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_shared();
+    prefetch_tmap(&tx);
+    prefetch_tmap(&ta);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // the adapters used by the rows of the GEMM's M tile, ascending
+  auto id_of = [&](long long r) { return __ldg(p.ids + (p.rows_per_id > 0 ? r / p.rows_per_id : r)); };
+  for (int r = threadIdx.x; r < p.tile_rows; r += kThreads) {
+    if (grow0 + r >= p.M) continue;
+    const int id = id_of(grow0 + r);
+    if (id >= 0 && id < p.n_adapters) atomicOr(&bitmap[id / 32], 1u << (id % 32));
+    else if (id != -1) record_error(err, kErrBounds, kKidLora, 10, (int)(grow0 + r));
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t w = bitmap[lane];
+    int at = __popc(w);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
+    }
+    if (lane == 31) list[0] = at;
+    at -= __popc(w);
+    for (uint32_t v = w; v; v &= v - 1) list[1 + at++] = lane * 32 + __ffs(v) - 1;
+  }
+  __syncthreads();
+  const int count = min(list[0], p.cap);  // (cap holds whatever the rows of a tile can name)
+  for (int r = threadIdx.x; r < kBM; r += kThreads) {
+    int s = -1;
+    if (row0 + r < p.M) {
+      const int id = id_of(row0 + r);
+      for (int j = 0; j < count; ++j)
+        if (list[1 + j] == id) s = j;
+    }
+    slot[r] = (int16_t)s;
+  }
+  if (rank == 0 && tile % per_group == 0)
+    for (int i = threadIdx.x; i <= count; i += kThreads) p.list[(long long)group * (1 + p.cap) + i] = i == 0 ? count : list[i];
+  __syncthreads();
+
+  // this CTA's K blocks
+  const int num_k = (p.K + kBK - 1) / kBK, per = (num_k + (int)ranks - 1) / (int)ranks;
+  const int kb0 = min(num_k, (int)rank * per), kb1 = min(num_k, kb0 + per);
+  const int per_pass = kCols / p.rank;  // adapters per pass
+
+  int it = 0;  // stages used so far (all roles count alike)
+  for (int j0 = 0, pass = 0; j0 < count; j0 += per_pass, ++pass) {
+    const int nj = min(per_pass, count - j0);
+    if (warp == 0) {
+      if (lane == 0) {
+        bool ok = true;
+        int i = it;
+        for (int kb = kb0; kb < kb1; ++kb, ++i) {
+          const int s = i % kStages;
+          if (!mbar_wait(&empty_bar[s], ((i / kStages) & 1) ^ 1u, err, kKidLora, 20 + s, abort_flag)) { ok = false; break; }
+          uint8_t* sx = smem + s * kStageBytes;
+          mbar_arrive_expect_tx(&full_bar[s], kXBytes + nj * p.rank * kBK * 2);
+          tma_load_2d(sx, &tx, &full_bar[s], kb * kBK, (int)row0);
+          for (int j = 0; j < nj; ++j)
+            tma_load_2d(sx + kXBytes + j * p.rank * kBK * 2, &ta, &full_bar[s], kb * kBK, list[1 + j0 + j] * p.rank);
+        }
+        if (!ok)  // our own copies must land before the CTA exits
+          for (int k = max(it, i - kStages); k < i; ++k)
+            mbar_wait(&full_bar[k % kStages], (k / kStages) & 1, nullptr, 0, 0, nullptr, 200000000LL);
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const uint32_t idesc = make_idesc_bf16_f32(kBM, nj * p.rank);
+        bool ok = true;
+        int i = it;
+        for (int kb = kb0; kb < kb1; ++kb, ++i) {
+          const int s = i % kStages;
+          if (!mbar_wait(&full_bar[s], (i / kStages) & 1, err, kKidLora, 30 + s, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t xa = smem_u32(smem + s * kStageBytes), aa = xa + kXBytes;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            umma_f16_ss(tmem, make_sdesc_sw128(xa + k * 32, 16, 1024), make_sdesc_sw128(aa + k * 32, 16, 1024), idesc,
+                        (kb > kb0 || k > 0) ? 1u : 0u);
+          umma_commit(&empty_bar[s]);
+        }
+        if (ok) umma_commit(done_bar);
+      }
+    } else {  // one row per thread: accumulator to the partial sums
+      const int row = (warp & 3) * 32 + lane;
+      const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      const bool have = kb1 > kb0 && mbar_wait(done_bar, pass & 1, err, kKidLora, 40, abort_flag);
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < nj * p.rank; c += 16) {
+        uint32_t v[16];
+        if (have) {
+          tmem_ld_32x32b_x16(t_row + c, v);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[(c + e) * kPartLd + row] = have ? __uint_as_float(v[e]) : 0.f;
+      }
+      tc_fence_before();
+    }
+    it += kb1 - kb0;
+    __syncwarp();
+    __syncthreads();
+    cluster_sync();  // every CTA's partial sums are in place
+    // rows [r0, r1) of this CTA: sums over the cluster in rank order, scaled, masked, stored
+    const int rows = kBM / (int)ranks, r0 = (int)rank * rows, n = nj * p.rank;
+    for (int e = threadIdx.x; e < rows * n; e += kThreads) {
+      const int row = r0 + e / n, c = e % n;
+      const int j = j0 + c / p.rank;
+      float v = 0.f;
+      if (slot[row] == j) {
+        for (uint32_t k = 0; k < ranks; ++k) v += ld_cluster(&part[c * kPartLd + row], k);
+        v *= __ldg(p.scale + list[1 + j]);
+      }
+      const long long trow = ((long long)group * p.cap + j) * p.tile_rows + (row0 - grow0) + row;
+      p.t[trow * p.rank + c % p.rank] = __float2bfloat16_rn(v);
+    }
+    cluster_sync();  // the partial sums have been read: the stages may be written again
+    fence_proxy_async_shared();  // generic accesses to the stages before the next pass's copies
+    __syncthreads();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kCols);
+}
+
+}  // namespace
+
+extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
+  const LoraArgs* l = a->lora;
+  if (!l || !l->a || !l->b || !l->scale || !l->ids || !l->t || !l->list) return -20;
+  if (l->n_adapters < 1 || l->n_adapters > kMaxAdapters) return -21;
+  if (l->rank % 16 || l->rank < 16 || l->rank > 128 || (l->rank > 64 && l->rank != 128)) return -22;
+  if (a->epi == kEpiSwiGLU || a->epi == kEpiQkv || a->out_world > 0) return -23;
+  if (l->cap < 1 || l->cap > l->tile_rows || (l->tile_rows != 128 && l->tile_rows != 256)) return -24;
+  if (a->M <= 0 || a->K % 8 || (a->lda * 2) % 16 || (reinterpret_cast<uintptr_t>(a->A) & 15)) return -25;
+  if ((reinterpret_cast<uintptr_t>(l->a) | reinterpret_cast<uintptr_t>(l->b) | reinterpret_cast<uintptr_t>(l->t)) & 15)
+    return -26;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static bool attr[16] = {false};
+  if (!attr[dev & 15]) {
+    cudaError_t e = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTotal);
+    if (e != cudaSuccess) return (int)e;
+    attr[dev & 15] = true;
+  }
+  CUtensorMap tx, ta;
+  int rc = dfl_host::make_tmap_2d_bf16(&tx, a->A, a->K, a->M, a->lda, kBK, kBM, true);
+  if (rc) return 1000 + rc;
+  rc = dfl_host::make_tmap_2d_bf16(&ta, l->a, a->K, (uint64_t)l->n_adapters * l->rank, a->K, kBK, l->rank, true);
+  if (rc) return 2000 + rc;
+  ShrinkParams p{};
+  p.ids = l->ids;
+  p.rows_per_id = l->rows_per_id;
+  p.scale = l->scale;
+  p.n_adapters = l->n_adapters;
+  p.rank = l->rank;
+  p.cap = l->cap;
+  p.tile_rows = l->tile_rows;
+  p.t = reinterpret_cast<__nv_bfloat16*>(l->t);
+  p.list = l->list;
+  p.sem = l->split_sem;
+  p.sem_count = l->split_sem ? l->split_sem_count : 0;
+  p.M = a->M;
+  p.K = a->K;
+  // every 128-row tile of every M tile (the last M tile's second half may lie behind M: zeros)
+  const long long tiles = ((long long)a->M + l->tile_rows - 1) / l->tile_rows * (l->tile_rows / kBM);
+  const int num_k = (a->K + kBK - 1) / kBK, room = 2 * dfl_host::num_sms(dev);
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= room && num_k >= ranks * 2 * 4) ranks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * ranks), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kTotal;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, lora_shrink_kernel, tx, ta, p, a->err);
+  if (e != cudaSuccess) return (int)e;
+  return dfl_gemm_bf16(a, stream);
+}

@@ -28,6 +28,7 @@ EXT_NAME = "_difflet_C"
 CUDA_SOURCES = [
     "gemm.cu",
     "gemm2.cu",
+    "lora.cu",
     "norm.cu",
     "add_norm.cu",
     "attention.cu",

@@ -9,6 +9,8 @@ _EXPORTS = {
     "ColumnParallelLinear": "linear",
     "RowParallelLinear": "linear",
     "ParallelEmbedding": "linear",
+    "LoraBank": "lora",
+    "linear_lora": "lora",
     "LayerNorm": "norm",
     "RMSNorm": "norm",
     "CustomRMSNorm": "norm",

@@ -15,6 +15,7 @@ Ops:
                 head-major (or token-major) destinations, one per rank
   linear_qkv    linear whose q/k/v column blocks go through qkv_scatter inside the
                 GEMM epilogue (no round trip of the qkv rows through HBM)
+  linear_lora   linear with low-rank adapters of many requests accumulated beside the weight
   linear_group  two linear / linear_qkv calls with one epilogue kind as one launch
   row_sumsq     per-row sums of squares of q / k column blocks (TP across-heads RMS)
   attention     softmax(scale q k^T) v with key window and LSE
@@ -213,6 +214,46 @@ def ln_modulate(x, *, shift=None, scale=None, w=None, b=None, eps=1e-6, rms=Fals
         out.copy_(y)
         return out
     return y
+
+
+def linear_lora(x, w, b, bank, ids, rows_per_id=0, *, act=None, act_lo=0, act_hi=None, gate=None, resid=None,
+                gate_rows_per_batch=0, out=None, out_f32=False):
+    """``linear`` with the adapters of ``bank`` (``ops.lora.LoraBank``) beside the weight: rows [M, K], ``ids``
+    per row or per ``rows_per_id`` rows.  Arguments are checked by ``ops.linear_lora``."""
+    N = w.shape[0]
+    act_hi = N if act_hi is None else act_hi
+    M = x.shape[0]
+    if x.is_cuda:
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"linear_lora runs in bfloat16 on CUDA, got {x.dtype}")
+        if M == 0:
+            return x.new_empty(0, N, dtype=torch.float32 if out_f32 else x.dtype) if out is None else out
+        if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+            x = x.contiguous()
+        epi = EPI_GATE_RESID if gate is not None else _ACT[act]
+        if ids.dtype != torch.int32:
+            ids = ids.clamp(-2, 1 << 30).to(torch.int32)  # what no adapter has stays without one
+        return native().gemm_lora(x, w, b, out, epi, act_lo, act_hi, gate, gate_rows_per_batch, resid, out_f32, bank.A,
+                                  bank.B, bank.scale, ids.contiguous(), rows_per_id)
+    ct = torch.float64 if x.dtype == torch.float64 else torch.float32
+    rows = ids.long() if rows_per_id <= 0 else ids.long().repeat_interleave(rows_per_id)[:M]
+    xc = x.to(ct)
+    y = xc @ w.to(ct).t()
+    for i in rows.unique().tolist():
+        if 0 <= i < bank.n:
+            at = rows == i
+            t = (xc[at] @ bank.A[i].to(ct).t() * bank.scale[i].to(ct)).to(x.dtype)
+            y[at] += t.to(ct) @ bank.B[i].to(ct).t()
+    if b is not None:
+        y = y + b.to(ct)
+    if act in ("gelu", "gelu_tanh"):
+        y[:, act_lo:act_hi] = F.gelu(y[:, act_lo:act_hi], approximate="tanh")
+    elif act == "silu":
+        y[:, act_lo:act_hi] = F.silu(y[:, act_lo:act_hi])
+    if gate is not None:
+        y = resid.to(ct) + gate[:, :N].to(ct).repeat_interleave(gate_rows_per_batch or M, 0)[:M] * y
+    y = y.to(torch.float32 if out_f32 else x.dtype)
+    return y if out is None else out.copy_(y)
 
 
 def _no_grad(name: str, *tensors) -> None:
