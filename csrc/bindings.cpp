@@ -536,35 +536,69 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   };
   a.kv_lo = edge(kv_lo, "kv_lo");
   a.kv_hi = edge(kv_hi, "kv_hi");
-  at::Tensor bits, win;
+  at::Tensor m, aux, win;
+  int mdt = 0;  // -1: boolean, else the type of an additive mask
   if (const at::Tensor* mt = given(mask)) {
     TORCH_CHECK(mt->device() == q.device(), "the mask must be on q's device");
-    const at::Tensor m = mt->expand({a.B, a.H, a.Sq, a.Sk});
-    if (m.scalar_type() == at::kBool) {
-      MaskBitsArgs b{};
-      b.mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
-      b.bs = m.stride(0), b.hs = m.stride(1), b.qs = m.stride(2), b.ks = m.stride(3);
-      b.B = b.bs ? a.B : 1, b.H = b.hs ? a.H : 1, b.Q = b.qs ? a.Sq : 1, b.Sk = a.Sk;
-      b.words = (a.Sk + 127) / 128 * 4;
-      bits = at::empty({(int64_t)b.B * b.H * b.Q * b.words}, q.options().dtype(at::kInt));
-      b.bits = reinterpret_cast<uint32_t*>(bits.data_ptr<int>());
-      a.key_bits = b.H == 1 && b.Q == 1;
-      if (a.key_bits && b.B == a.B && !a.kv_lo && !a.kv_hi) {
-        win = at::empty({2, a.B}, q.options().dtype(at::kInt));
-        b.lo = win.data_ptr<int>();
-        b.hi = b.lo + a.B;
-        a.kv_lo = b.lo, a.kv_hi = b.hi;
-      }
-      DFL_CHECK_RC(dfl_cross_mask_bits(&b, cur_stream()), "cross_mask_bits");
-      a.bits = b.bits;
-      a.bits_qs = b.Q > 1 ? b.words : 0;
-      a.bits_hs = b.H > 1 ? (long long)b.Q * b.words : 0;
-      a.bits_bs = b.B > 1 ? (long long)b.H * b.Q * b.words : 0;
-    } else {
-      a.bias_dtype = dtype_code(m, "an additive mask");
-      a.bias = m.data_ptr();
-      a.bias_bs = m.stride(0), a.bias_hs = m.stride(1), a.bias_qs = m.stride(2), a.bias_ks = m.stride(3);
+    m = mt->expand({a.B, a.H, a.Sq, a.Sk});
+    mdt = m.scalar_type() == at::kBool ? -1 : dtype_code(m, "an additive mask");
+  }
+  if (a.H / a.Hk * a.Sq <= 16) {  // too few rows to fill a tile: the keys are split instead
+    DecodeArgs d{};
+    d.q = a.q, d.k = a.k, d.v = a.v, d.o = a.o;
+    d.q_bs = a.q_bs, d.q_hs = a.q_hs, d.q_ss = a.q_ss, d.k_bs = a.k_bs, d.k_hs = a.k_hs, d.k_ss = a.k_ss;
+    d.v_bs = a.v_bs, d.v_hs = a.v_hs, d.v_ss = a.v_ss, d.o_bs = a.o_bs, d.o_hs = a.o_hs, d.o_ss = a.o_ss;
+    d.lse = a.lse;
+    d.B = a.B, d.H = a.H, d.Hk = a.Hk, d.Sq = a.Sq, d.Sk = a.Sk, d.dh = a.dh, d.f16 = a.f16;
+    d.scale = a.scale;
+    d.kv_lo = a.kv_lo, d.kv_hi = a.kv_hi;
+    if (m.defined()) {
+      d.mask = m.data_ptr();
+      d.mask_dtype = mdt;
+      d.m_bs = m.stride(0), d.m_hs = m.stride(1), d.m_qs = m.stride(2), d.m_ks = m.stride(3);
     }
+    DFL_CHECK_RC(dfl_cross_decode(&d, cur_stream()), "cross_attention (few queries)");
+    if (!direct) o.copy_(o_);
+    return o;
+  }
+  if (m.defined() && mdt < 0) {
+    MaskBitsArgs b{};
+    b.mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
+    b.bs = m.stride(0), b.hs = m.stride(1), b.qs = m.stride(2), b.ks = m.stride(3);
+    b.B = b.bs ? a.B : 1, b.H = b.hs ? a.H : 1, b.Q = b.qs ? a.Sq : 1, b.Sk = a.Sk;
+    b.words = (a.Sk + 127) / 128 * 4;
+    aux = at::empty({(int64_t)b.B * b.H * b.Q * b.words}, q.options().dtype(at::kInt));
+    b.bits = reinterpret_cast<uint32_t*>(aux.data_ptr<int>());
+    a.key_bits = b.H == 1 && b.Q == 1;
+    if (a.key_bits && b.B == a.B && !a.kv_lo && !a.kv_hi) {
+      win = at::empty({2, a.B}, q.options().dtype(at::kInt));
+      b.lo = win.data_ptr<int>();
+      b.hi = b.lo + a.B;
+      a.kv_lo = b.lo, a.kv_hi = b.hi;
+    }
+    DFL_CHECK_RC(dfl_cross_mask_bits(&b, cur_stream()), "cross_mask_bits");
+    a.bits = b.bits;
+    a.bits_qs = b.Q > 1 ? b.words : 0;
+    a.bits_hs = b.H > 1 ? (long long)b.Q * b.words : 0;
+    a.bits_bs = b.B > 1 ? (long long)b.H * b.Q * b.words : 0;
+  } else if (m.defined()) {
+    BiasTileArgs t{};
+    t.mask = m.data_ptr();
+    t.dtype = mdt;
+    t.bs = m.stride(0), t.hs = m.stride(1), t.qs = m.stride(2), t.ks = m.stride(3);
+    t.B = t.bs ? a.B : 1, t.H = t.hs ? a.H : 1, t.Q = t.qs ? a.Sq : 1, t.Sk = a.Sk;
+    t.out_f32 = m.scalar_type() != q.scalar_type();
+    const int64_t nq = (t.Q + 31) / 32, nt = (t.Sk + 127) / 128, rows = t.Q > 1 ? 32 : 1, vec = t.out_f32 ? 32 : 16;
+    aux = at::empty({t.B * t.H * nq * nt * vec * rows * 4}, q.options().dtype(at::kInt));
+    t.tiles = aux.data_ptr();
+    DFL_CHECK_RC(dfl_cross_bias_tiles(&t, cur_stream()), "cross_bias_tiles");
+    a.bias_tiles = t.tiles;
+    a.bias_f32 = t.out_f32;
+    a.bias_rows = (int)rows;
+    a.bias_ts = vec * rows;
+    a.bias_qs = t.Q > 1 ? nt * a.bias_ts : 0;
+    a.bias_hs = t.H > 1 ? nq * nt * a.bias_ts : 0;
+    a.bias_bs = t.B > 1 ? t.H * nq * nt * a.bias_ts : 0;
   }
   a.err = err_ptr();
   DFL_CHECK_RC(dfl_cross_attention(&a, cur_stream()), "cross_attention");

@@ -22,7 +22,7 @@
 // item before, so neither P nor O needs a barrier of its own.
 //
 // Masks: a key window [lo, hi) per batch row (tiles outside it are skipped), bits (kBits: packed
-// by cross_mask_bits, per query or shared by all queries) or an additive bias (kBias).
+// by cross_mask_bits, per query or shared by all queries) or an additive bias (kBias16 / kBias32).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -39,7 +39,8 @@ constexpr int kBN = 128;      // keys per tile
 constexpr int kChunk = 16384;  // 128 rows x 64 values: one swizzle chunk
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-enum { kWindow = 0, kBits = 1, kBias = 2 };
+enum { kWindow = 0, kBits = 1, kBias16 = 2, kBias32 = 3 };  // kBias16: of the inputs' type, kBias32: f32
+constexpr bool is_bias(int mask) { return mask >= kBias16; }
 
 struct CrossParams {
   void* o;
@@ -53,9 +54,11 @@ struct CrossParams {
   const uint32_t* bits;   // kBits: rows of `words` words, bit k of a row: key k is kept
   long long bits_bs, bits_hs, bits_qs;  // row strides (in words) by batch, head, query
   int key_bits;           // the bits do not vary over queries (V rows of masked keys are cleaned)
-  const void* bias;       // kBias
-  long long bias_bs, bias_hs, bias_qs, bias_ks;  // element strides
-  int bias_dtype, bias_vec;  // bias_vec: rows start 16-byte aligned, unit key stride
+  // kBias16 / kBias32: blocks of 32 queries x 128 keys written by dfl_cross_bias_tiles (16-byte vectors,
+  // [vector of keys][query], so a warp's loads are contiguous); strides in vectors (0: broadcast)
+  const uint4* bias;
+  long long bias_bs, bias_hs, bias_qs, bias_ts;  // batch, head, 32-query block, key tile
+  int bias_rows;                                 // queries per block: 32, or 1 (one row for all)
 };
 
 template <int DH, int QT>
@@ -165,43 +168,16 @@ DFL_DEVICE bool cross_dirty(const CrossParams& p, const CrossItem& it, int k0) {
   return false;
 }
 
-// 32 bias values of one row from key k on (0 past the last key; those scores are masked anyway).
-DFL_DEVICE void cross_bias32(const CrossParams& p, long long row, int k, float (&v)[32]) {
-  if (p.bias_vec && k + 32 <= p.Sk) {
-    if (p.bias_dtype == kDtypeF32) {
-      const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.bias) + row + k);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 f = __ldg(s + i);
-        v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-      }
-    } else {
-      const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.bias) + row + k);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 w = __ldg(s + i);
-        uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = p.bias_dtype == kDtypeBf16 ? unpack_bf16x2(ws[j])
-                                                      : __half22float2(*reinterpret_cast<__half2*>(&ws[j]));
-          v[8 * i + 2 * j] = f.x, v[8 * i + 2 * j + 1] = f.y;
-        }
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    float f = 0.f;
-    if (k + i < p.Sk) {
-      const long long at = row + (k + i) * p.bias_ks;
-      if (p.bias_dtype == kDtypeF32) f = reinterpret_cast<const float*>(p.bias)[at];
-      else if (p.bias_dtype == kDtypeBf16) f = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[at]);
-      else f = __half2float(reinterpret_cast<const __half*>(p.bias)[at]);
-    }
-    v[i] = f;
-  }
+// Packed pairs of two 16-bit values (bf16 or fp16) as f32.
+template <bool F16>
+DFL_DEVICE float2 unpack2(uint32_t v) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<__half2*>(&v));
+  else return unpack_bf16x2(v);
+}
+DFL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 template <int DH, bool F16, int QT, int MASK>
@@ -420,8 +396,8 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     const uint32_t s_t = tmem + lane_base + 128u * g;
     const uint32_t o_t = tmem + lane_base + C::kOCol + (uint32_t)(DH * g);
     // window / bits: scores are scaled inside the exponent (scale > 0); bias: z is formed first
-    const float sc = MASK == kBias ? kLog2e : p.scale * kLog2e;
-    const float grow = MASK == kBias ? 8.f * kLn2 : 8.f;
+    const float sc = is_bias(MASK) ? kLog2e : p.scale * kLog2e;
+    const float grow = is_bias(MASK) ? 8.f * kLn2 : 8.f;
     bool ok = true;
     int s = 0, used = 0;
     for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
@@ -433,21 +409,53 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         const int k0 = (it.t0 + j) * kBN;
         uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
         if (MASK == kBits && live) keep = cross_bits(p, it, qrow, k0);
+        // bias: 64 registers of it are on their way while the scores are awaited (16 bit: the whole
+        // tile; f32: its first half, the second half follows as the first is used up)
+        uint4 bv[is_bias(MASK) ? 16 : 1];
+        const uint4* bp = nullptr;
+        if constexpr (is_bias(MASK)) {
+          const int qc = min(qrow, p.Sq - 1);  // (rows behind the last query read a valid one)
+          bp = p.bias + it.b * p.bias_bs + it.h * p.bias_hs + (qc / 32) * p.bias_qs + (it.t0 + j) * p.bias_ts +
+               (p.bias_rows > 1 ? qc % 32 : 0);
+#pragma unroll
+          for (int v = 0; v < 16; ++v) bv[v] = __ldg(bp + v * p.bias_rows);
+        }
         if (!mbar_wait(&s_full[g], s & 1, err, kKidCross, 120 + g, abort_flag)) { ok = false; break; }
         tc_fence_after();
         float z[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_t + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[c * 32]));
-        tmem_wait_ld();
-        if constexpr (MASK == kBias) {
-          const long long at = it.b * p.bias_bs + it.h * p.bias_hs + (live ? qrow : 0) * p.bias_qs;
+        if constexpr (is_bias(MASK)) {
+          const uint64_t scale2 = f2_pack(p.scale, p.scale);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            float bv[32];
-            cross_bias32(p, at, k0 + 32 * c, bv);
+            tmem_ld_32x32b_x32(s_t + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[c * 32]));
+            tmem_wait_ld();
+            float* zc = z + 32 * c;
+            if constexpr (MASK == kBias16) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) z[32 * c + e] = fmaf(z[32 * c + e], p.scale, bv[e]);
+              for (int v = 0; v < 4; ++v) {
+                const uint32_t ws[4] = {bv[4 * c + v].x, bv[4 * c + v].y, bv[4 * c + v].z, bv[4 * c + v].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = unpack2<F16>(ws[e]);
+                  float* zp = zc + 8 * v + 2 * e;
+                  f2_unpack(f2_fma(f2_pack(zp[0], zp[1]), scale2, f2_pack(f.x, f.y)), zp[0], zp[1]);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int v = 0; v < 8; ++v) {
+                uint4& b = bv[8 * (c & 1) + v];
+                float* zp = zc + 4 * v;
+                f2_unpack(f2_fma(f2_pack(zp[0], zp[1]), scale2, f2_pack(__uint_as_float(b.x), __uint_as_float(b.y))), zp[0], zp[1]);
+                f2_unpack(f2_fma(f2_pack(zp[2], zp[3]), scale2, f2_pack(__uint_as_float(b.z), __uint_as_float(b.w))), zp[2], zp[3]);
+                if (c < 2) b = __ldg(bp + (16 + 8 * c + v) * p.bias_rows);
+              }
+            }
           }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_t + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[c * 32]));
+          tmem_wait_ld();
         }
         if constexpr (MASK == kBits) {
           if ((keep.x & keep.y & keep.z & keep.w) != ~0u) {
@@ -471,14 +479,14 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
           for (int t = 0; t < 8; ++t) mxa[t] = max3(mxa[t], z[c + t], z[c + 8 + t]);
         }
         const float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), fmaxf(max3(mxa[3], mxa[4], mxa[5]), fmaxf(mxa[6], mxa[7])));
-        const float m_new = fmaxf(m, MASK == kBias ? mx : mx * sc);
+        const float m_new = fmaxf(m, is_bias(MASK) ? mx : mx * sc);
         // warp-uniform decision: tcgen05.ld / st are warp-collective
         const bool need = j > 0 && __any_sync(0xffffffffu, m_new > m + grow);
         const float m_old = m;
         if (j == 0 || need) m = m_new;
         const float m_use = m == -INFINITY ? 0.f : m;
         if (need) {  // O_g is stable: P V_g(s-1) completed before S_g(s)
-          const float f = m_old == -INFINITY ? 0.f : exp2_sfu(MASK == kBias ? (m_old - m) * kLog2e : m_old - m);
+          const float f = m_old == -INFINITY ? 0.f : exp2_sfu(is_bias(MASK) ? (m_old - m) * kLog2e : m_old - m);
 #pragma unroll 1
           for (int c = 0; c < DH / 16; ++c) {
             uint32_t o_raw[16];
@@ -499,9 +507,8 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
           for (int c = 0; c < 16; ++c) {
             const uint64_t zz = f2_pack(z[qtr * 32 + 2 * c], z[qtr * 32 + 2 * c + 1]);
             float x0, x1;
-            if constexpr (MASK == kBias) {  // the difference first: a bias near the type's lowest value times log2(e) is -inf
-              f2_unpack(f2_add(zz, nm2), x0, x1);
-              x0 *= kLog2e, x1 *= kLog2e;
+            if constexpr (is_bias(MASK)) {  // the difference first: a bias near the type's lowest value times log2(e) is -inf
+              f2_unpack(f2_mul(f2_add(zz, nm2), sc2), x0, x1);
             } else {
               f2_unpack(f2_fma(zz, sc2, nm2), x0, x1);
             }
@@ -554,7 +561,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       }
       if (p.lse && live)
         p.lse[((long long)it.b * p.H + it.h) * p.Sq + qrow] =
-            l == 0.f ? -INFINITY : (MASK == kBias ? m + logf(l) : (m + log2f(l)) * kLn2);
+            l == 0.f ? -INFINITY : (is_bias(MASK) ? m + logf(l) : (m + log2f(l)) * kLn2);
     }
   }
 
@@ -617,7 +624,9 @@ int launch_cross_qt(const CrossArgs* a, const CrossParams& p, cudaStream_t strea
 
 template <int DH, bool F16>
 int launch_cross_mask(const CrossArgs* a, const CrossParams& p, cudaStream_t stream, int dev) {
-  if (a->bias) return launch_cross_qt<DH, F16, kBias>(a, p, stream, dev);
+  if (a->bias_tiles)
+    return a->bias_f32 ? launch_cross_qt<DH, F16, kBias32>(a, p, stream, dev)
+                       : launch_cross_qt<DH, F16, kBias16>(a, p, stream, dev);
   if (a->bits) return launch_cross_qt<DH, F16, kBits>(a, p, stream, dev);
   return launch_cross_qt<DH, F16, kWindow>(a, p, stream, dev);
 }
@@ -635,12 +644,9 @@ int cross_entry(const CrossArgs* a, cudaStream_t stream) {
   p.bits = a->bits;
   p.bits_bs = a->bits_bs, p.bits_hs = a->bits_hs, p.bits_qs = a->bits_qs;
   p.key_bits = a->key_bits;
-  p.bias = a->bias;
-  p.bias_bs = a->bias_bs, p.bias_hs = a->bias_hs, p.bias_qs = a->bias_qs, p.bias_ks = a->bias_ks;
-  p.bias_dtype = a->bias_dtype;
-  const int be = a->bias_dtype == kDtypeF32 ? 4 : 8;  // values per 16 bytes
-  p.bias_vec = a->bias && a->bias_ks == 1 && (reinterpret_cast<uintptr_t>(a->bias) & 15) == 0 &&
-               (a->bias_bs | a->bias_hs | a->bias_qs) % be == 0;
+  p.bias = reinterpret_cast<const uint4*>(a->bias_tiles);
+  p.bias_bs = a->bias_bs, p.bias_hs = a->bias_hs, p.bias_qs = a->bias_qs, p.bias_ts = a->bias_ts;
+  p.bias_rows = a->bias_rows;
   int dev = 0;
   cudaGetDevice(&dev);
   return a->dh == 64 ? launch_cross_mask<64, F16>(a, p, stream, dev) : launch_cross_mask<128, F16>(a, p, stream, dev);

@@ -313,12 +313,40 @@ typedef struct CrossArgs {
   const uint32_t* bits;                // rows written by dfl_cross_mask_bits; strides in words (0: broadcast)
   long long bits_bs, bits_hs, bits_qs;
   int key_bits;                        // the bits are the same for every query and head
-  const void* bias;                    // additive mask, element strides (0: broadcast)
-  long long bias_bs, bias_hs, bias_qs, bias_ks;
-  int bias_dtype;
+  // additive mask: blocks written by dfl_cross_bias_tiles, strides in 16-byte vectors (0: broadcast)
+  const void* bias_tiles;
+  long long bias_bs, bias_hs, bias_qs, bias_ts;
+  int bias_rows, bias_f32;
   int* err;
 } CrossArgs;
 int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream);
+
+// Additive mask [B, H, Q, Sk] (its unbroadcast extents, element strides) -> 32-query x 128-key blocks
+// [B][H][ceil(Q / 32)][ceil(Sk / 128)][vector of keys][query], 16-byte vectors of the mask's own 16-bit type
+// or (out_f32) of f32; Q = 1 keeps one query per block.  Positions past Q and Sk hold 0.
+typedef struct BiasTileArgs {
+  const void* mask;
+  int dtype;
+  long long bs, hs, qs, ks;
+  int B, H, Q, Sk, out_f32;
+  void* tiles;
+} BiasTileArgs;
+int dfl_cross_bias_tiles(const BiasTileArgs* a, cudaStream_t stream);
+
+// Attention of a few queries (H / Hk * Sq <= 16 rows share a key head): the same mathematics on the
+// masks as they are (element strides, 0: broadcast); no tile needs filling, so the keys are split instead.
+typedef struct DecodeArgs {
+  const void* q; const void* k; const void* v; void* o;
+  long long q_bs, q_hs, q_ss, k_bs, k_hs, k_ss, v_bs, v_hs, v_ss, o_bs, o_hs, o_ss;
+  float* lse;
+  int B, H, Hk, Sq, Sk, dh, f16;
+  float scale;
+  const int* kv_lo; const int* kv_hi;
+  const void* mask;                    // NULL, bool bytes (mask_dtype -1) or an additive mask
+  int mask_dtype;
+  long long m_bs, m_hs, m_qs, m_ks;
+} DecodeArgs;
+int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream);
 
 // Boolean mask [B, H, Q, Sk] (1 byte per element, element strides) -> bit rows [B, H, Q, words], words =
 // 4 ceil(Sk / 128); lo / hi (H = Q = 1 only, or NULL): the window of the kept keys of every batch row.

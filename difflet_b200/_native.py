@@ -34,6 +34,7 @@ CUDA_SOURCES = [
     "attention.cu",
     "cross_attn.cu",
     "cross_attn_f16.cu",
+    "cross_decode.cu",
     "comm.cu",
     "mx.cu",
     "conv.cu",

@@ -65,7 +65,9 @@ def __getattr__(name: str):
         raise AttributeError(f"module 'difflet_b200.ops' has no attribute {name!r}")
     import importlib
 
-    return getattr(importlib.import_module(f"difflet_b200.ops.{mod}"), name)
+    value = getattr(importlib.import_module(f"difflet_b200.ops.{mod}"), name)
+    globals()[name] = value  # the next access is a plain module attribute
+    return value
 
 
 def __dir__():

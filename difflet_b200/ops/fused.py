@@ -88,6 +88,12 @@ def native():
     return _lib()
 
 
+def _kernels():
+    """The native module for operators that bring their own workspaces (counts a launch)."""
+    LAUNCHES[0] += 1
+    return _nat if _nat is not None else _lib()
+
+
 def _rows2d(x: torch.Tensor) -> torch.Tensor:
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
@@ -233,7 +239,7 @@ def linear_lora(x, w, b, bank, ids, rows_per_id=0, *, act=None, act_lo=0, act_hi
         epi = EPI_GATE_RESID if gate is not None else _ACT[act]
         if ids.dtype != torch.int32:
             ids = ids.clamp(-2, 1 << 30).to(torch.int32)  # what no adapter has stays without one
-        return native().gemm_lora(x, w, b, out, epi, act_lo, act_hi, gate, gate_rows_per_batch, resid, out_f32, bank.A,
+        return _kernels().gemm_lora(x, w, b, out, epi, act_lo, act_hi, gate, gate_rows_per_batch, resid, out_f32, bank.A,
                                   bank.B, bank.scale, ids.contiguous(), rows_per_id)
     ct = torch.float64 if x.dtype == torch.float64 else torch.float32
     rows = ids.long() if rows_per_id <= 0 else ids.long().repeat_interleave(rows_per_id)[:M]
@@ -267,18 +273,18 @@ MX_CODES = {"float8_e4m3fn": 1, "float8_e5m2": 2, "float8_e4m3fn_x4": 1, "float8
 _NORM_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def add_rms_norm(x, resid=None, w=None, *, eps=1e-6, scale=None, shift=None, rows_per_batch=0, row_map=None,
+def add_rms_norm(x, resid=None, weight=None, *, eps=1e-6, scale=None, shift=None, rows_per_batch=0, row_map=None,
                  quantize=None, blocked=False, out=None, resid_out=None):
-    """``s = x + resid``; ``y = s / sqrt(mean(s^2) + eps) * w * (1 + scale[b]) + shift[b]`` -> ``(y, s)``.
+    """``s = x + resid``; ``y = s / sqrt(mean(s^2) + eps) * weight * (1 + scale[b]) + shift[b]`` -> ``(y, s)``.
 
     x, resid: [..., D] of one type (bf16, fp16 or fp32; rows with a unit inner stride), D <= 16384.
-    ``resid=None``: s is x itself.  w: [D] of x's type or f32; scale / shift: f32 [B, D] for
+    ``resid=None``: s is x itself.  weight: [D] of x's type or f32; scale / shift: f32 [B, D] for
     ``rows_per_batch`` rows each (0: one batch row for all), or by ``row_map`` (int32 [M]).
     ``quantize`` ("float8_e4m3fn" / "float8_e5m2"): y comes as ``(data, scales)`` in MXFP8, scales plain
     [..., D/32] or, with ``blocked``, in the layout ``linear_mx`` reads (D a multiple of 128).
     ``out`` / ``resid_out`` receive y / s and may be x / resid.  The statistics use the unrounded sum.
     """
-    _no_grad("add_rms_norm", x, resid, w, scale, shift)
+    _no_grad("add_rms_norm", x, resid, weight, scale, shift)
     D = x.shape[-1] if x.dim() else 0
     if x.dim() < 1 or not 1 <= D <= 16384:
         raise ValueError(f"add_rms_norm needs [..., D] with 1 <= D <= 16384, got {tuple(x.shape)}")
@@ -299,7 +305,7 @@ def add_rms_norm(x, resid=None, w=None, *, eps=1e-6, scale=None, shift=None, row
     for name, t in (("out", out), ("resid_out", resid_out)):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
             raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    if w is not None and (w.shape != (D,) or w.device != x.device or w.dtype not in (x.dtype, torch.float32)):
+    if weight is not None and (weight.shape != (D,) or weight.device != x.device or weight.dtype not in (x.dtype, torch.float32)):
         raise ValueError(f"weight must be [{D}] of {x.dtype} or float32 on {x.device}")
     for name, t in (("scale", scale), ("shift", shift)):
         if t is not None and (t.dim() != 2 or t.shape[1] != D or t.device != x.device):
@@ -316,7 +322,7 @@ def add_rms_norm(x, resid=None, w=None, *, eps=1e-6, scale=None, shift=None, row
             y2 = out if out.dim() == 2 else out.view(M, D)  # a view: the caller's tensor is written
         if resid_out is not None:
             s2 = resid_out if resid_out.dim() == 2 else resid_out.view(M, D)
-        y, s, sf = native().add_rms_norm(x2, None if resid is None else _rows2d(resid), w, scale, shift,
+        y, s, sf = _kernels().add_rms_norm(x2, None if resid is None else _rows2d(resid), weight, scale, shift,
                                          rows_per_batch, row_map, eps, MX_CODES.get(quantize, 0), blocked, y2, s2)
         if x.dim() != 2:
             y = out if out is not None else y.view(x.shape)
@@ -328,8 +334,8 @@ def add_rms_norm(x, resid=None, w=None, *, eps=1e-6, scale=None, shift=None, row
     ct = torch.float64 if x.dtype == torch.float64 else torch.float32
     s = x2.to(ct) if resid is None else x2.to(ct) + _rows2d(resid).to(ct)
     y = s * torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + eps)
-    if w is not None:
-        y = y * w.to(ct)
+    if weight is not None:
+        y = y * weight.to(ct)
     if M and (scale is not None or shift is not None):
         b = row_map.long() if row_map is not None else torch.arange(M) // (rows_per_batch or M)
         if scale is not None:
@@ -656,7 +662,7 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
     if q.is_cuda:
         if scale <= 0:  # the kernel scales inside the exponent, where the maximum must commute with it
             q, scale = (-q, -scale) if scale < 0 else (torch.zeros_like(q), 1.0)
-        return native().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse)
+        return _kernels().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     Sk, rep = k.shape[2], q.shape[1] // k.shape[1]
     idx = torch.arange(Sk)

@@ -89,7 +89,7 @@ def dequantize_mx(data, scale, *, dtype: str = "float8_e4m3fn", output_dtype=tor
             and output_dtype in (torch.bfloat16, torch.float16, torch.float32)):
         from difflet_b200.ops import fused as F
 
-        return F.native().mx_dequantize(data, scale, output_dtype)
+        return F._kernels().mx_dequantize(data, scale, output_dtype)
     s = torch.pow(2.0, scale.to(torch.float32) - BIAS)
     v = data.to(torch.float32).reshape(*data.shape[:-1], K // GROUP, GROUP) * s[..., None]
     return v.reshape(data.shape).to(output_dtype)

@@ -55,13 +55,8 @@ class LayerNorm(nn.LayerNorm):
         return super().forward(x)
 
 
-def add_rms_norm(x, resid=None, weight=None, *, eps: float = 1e-6, scale=None, shift=None, rows_per_batch: int = 0,
-                 row_map=None, quantize: str | None = None, blocked: bool = False, out=None, resid_out=None):
-    """Residual addition + RMSNorm in one pass: ``(y, s)`` with ``s = x + resid`` and ``y`` the
-    normalised (weighted, adaLN-modulated) sum, in x's type or as MXFP8 ``(data, scales)`` for
-    ``matmul_mx`` (``blocked=True``: for ``ops.fused.linear_mx``).  See ``ops.fused.add_rms_norm``."""
-    return F.add_rms_norm(x, resid, weight, eps=eps, scale=scale, shift=shift, rows_per_batch=rows_per_batch,
-                          row_map=row_map, quantize=quantize, blocked=blocked, out=out, resid_out=resid_out)
-
+# Residual addition + RMSNorm in one pass, in the input's type or into MXFP8 (``matmul_mx`` reads the plain
+# scales, ``ops.fused.linear_mx`` the blocked ones).
+add_rms_norm = F.add_rms_norm
 
 __all__ = ["CustomRMSNorm", "LayerNorm", "RMSNorm", "add_rms_norm", "rms_norm_fp32"]
