@@ -67,9 +67,10 @@ struct CrossCfg {
   static constexpr int kProducerWarp = 4 * QT, kMmaWarp = 4 * QT + 1, kCleanWarp = 4 * QT + 2;
   static constexpr int kTile = 128 * DH * 2;
   static constexpr int kChunks = DH / 64;
-  static constexpr int kRing = DH == 64 ? 8 : (QT == 2 ? 5 : 6);
+  static constexpr int kRing = DH == 64 ? 8 : (QT == 2 ? 4 : 5);
   static constexpr int kQ = 0, kKV = QT * kTile;
-  static constexpr int kBar = kKV + kRing * kTile;
+  static constexpr int kOut = kKV + kRing * kTile;  // 4 KB per softmax warp: 32 rows x 64 columns on their way out
+  static constexpr int kBar = kOut + 4 * QT * 4096;
   // q_full[2], q_empty[2], kv_full[R], kv_empty[R], s_full[2], p_full[2][2], o_full[2], v_clean[R]
   static constexpr int kNumBars = 4 + 3 * kRing + 2 + 4 + 2;
   static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
@@ -133,6 +134,16 @@ DFL_DEVICE void tma_load_4d(uint8_t* dst, const CUtensorMap* map, uint64_t* bar,
       : "memory");
 }
 
+DFL_DEVICE void tma_store_4d(const CUtensorMap* map, const uint8_t* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+DFL_DEVICE void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+DFL_DEVICE void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+DFL_DEVICE void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // One work item: its query block, head, batch row, key window and key tiles.
 struct CrossItem {
   int q0, h, b, lo, hi, t0, n;
@@ -183,7 +194,8 @@ DFL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
 template <int DH, bool F16, int QT, int MASK>
 __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     cross_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                      const __grid_constant__ CUtensorMap tv, const CrossParams p, int* err) {
+                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
+                      const CrossParams p, int* err) {
   using C = CrossCfg<DH, QT>;
   constexpr int R = C::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -541,20 +553,33 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum stays NaN)
         const bool none = l == 0.f;
+        // 64 columns at a time through shared memory (the store's swizzle: 16-byte piece i of row r at
+        // i ^ (r % 8)): a thread's own row would cost a line per lane and store
+        uint8_t* stage = smem + C::kOut + warp * 4096;
 #pragma unroll 1
-        for (int c = 0; c < DH / 32; ++c) {
-          uint32_t o_raw[32];
-          tmem_ld_32x32b_x32(o_t + c * 32, o_raw);
-          tmem_wait_ld();
-          if (live) {
+        for (int ch = 0; ch < C::kChunks; ++ch) {
+          if (lane == 0) bulk_wait_read();  // what left this buffer last has been read
+          __syncwarp();
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t o_raw[32];
+            tmem_ld_32x32b_x32(o_t + ch * 64 + hf * 32, o_raw);
+            tmem_wait_ld();
             float o[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : __uint_as_float(o_raw[e]) * inv;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              reinterpret_cast<uint4*>(op + c * 32)[q] =
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((hf * 4 + q) ^ (lane & 7)) * 16)) =
                   make_uint4(pack2<F16>(o[8 * q], o[8 * q + 1]), pack2<F16>(o[8 * q + 2], o[8 * q + 3]),
                              pack2<F16>(o[8 * q + 4], o[8 * q + 5]), pack2<F16>(o[8 * q + 6], o[8 * q + 7]));
+          }
+          fence_proxy_async_shared();
+          __syncwarp();
+          const int r0 = it.q0 + g * kBM + (warp & 3) * 32;
+          if (lane == 0 && r0 < p.Sq) {  // (rows past the last query are clipped)
+            tma_store_4d(&to, stage, ch * 64, r0, it.h, it.b);
+            bulk_commit();
           }
         }
         tc_fence_before();  // O_g has been read before this thread's next P_g signal
@@ -563,6 +588,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         p.lse[((long long)it.b * p.H + it.h) * p.Sq + qrow] =
             l == 0.f ? -INFINITY : (is_bias(MASK) ? m + logf(l) : (m + log2f(l)) * kLn2);
     }
+    if (lane == 0) bulk_wait_all();  // this warp's stores have left shared memory
   }
 
   tc_fence_before();
@@ -572,12 +598,12 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
 }
 
 inline int cross_tmap(CUtensorMap* map, const void* base, int D, long long S, int H, int B, long long ss, long long hs,
-                      long long bs, bool f16) {
+                      long long bs, bool f16, int box_rows = 128) {
   dfl_host::EncodeTiledFn fn = dfl_host::get_encode_tiled();
   if (!fn) return 999;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)hs * 2, (cuuint64_t)bs * 2};
-  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return (int)fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -600,17 +626,19 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
     }
     attr[dev & 15] = true;
   }
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   int rc = cross_tmap(&tq, a->q, DH, a->Sq, a->H, a->B, a->q_ss, a->q_hs, a->q_bs, F16);
   if (rc) return 1000 + rc;
   rc = cross_tmap(&tk, a->k, DH, a->Sk, a->Hk, a->B, a->k_ss, a->k_hs, a->k_bs, F16);
   if (rc) return 2000 + rc;
   rc = cross_tmap(&tv, a->v, DH, a->Sk, a->Hk, a->B, a->v_ss, a->v_hs, a->v_bs, F16);
   if (rc) return 3000 + rc;
+  rc = cross_tmap(&to, a->o, DH, a->Sq, a->H, a->B, a->o_ss, a->o_hs, a->o_bs, F16, 32);
+  if (rc) return 4000 + rc;
   p.n_qb = (a->Sq + QT * kBM - 1) / (QT * kBM);
   const long long items = (long long)p.n_qb * a->H * a->B;
   const int sms = dfl_host::num_sms(dev);
-  kern<<<(unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream>>>(tq, tk, tv, p, a->err);
+  kern<<<(unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream>>>(tq, tk, tv, to, p, a->err);
   return (int)cudaGetLastError();
 }
 

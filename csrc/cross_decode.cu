@@ -3,7 +3,7 @@
 //
 // Bound by reading K and V once: a 128-row tensor-memory tile would be nearly empty, so the keys are
 // split over up to eight CTAs (one cluster per key head and batch row) of four warps, and each warp walks
-// its own 32-key blocks with a running maximum and sum.  Q K^T runs on the warp-level m16n8k16 matrix
+// its own 16-key blocks with a running maximum and sum.  Q K^T runs on the warp-level m16n8k16 matrix
 // instruction straight from registers: both operands take the head dimension in the same permuted
 // order (lane t of a quad holds 8 contiguous values of every 32), so every load is 16 contiguous bytes and nothing is
 // staged.  P V is f32 multiply-adds, a lane holding dh / 32 columns of every row, with P unrounded.  The partial
@@ -17,6 +17,7 @@ namespace {
 using namespace dfl;
 
 constexpr int kWarps = 4;
+constexpr int kKeys = 16;  // per warp and step: its K and V (8 KB at dh 128) are in flight together
 constexpr float kLog2e = 1.4426950408889634f;
 
 DFL_DEVICE float exp2_sfu(float x) {
@@ -74,13 +75,13 @@ DFL_DEVICE float masked_score(const DecodeArgs& a, float s, int b, int h, int q,
 
 // NR: rows held by the P V accumulators (4, 8 or 16).
 template <int DH, bool F16, int NR>
-__global__ void __launch_bounds__(32 * kWarps) cross_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cross_decode_kernel(const DecodeArgs a) {
   constexpr int KC = DH / 32;  // 16-byte pieces of a key row per lane
   constexpr int DL = DH / 32;  // output columns per lane
   // P of the block a warp is at; later this CTA's joined rows, read by the cluster
-  constexpr int kBuf = kWarps * NR * 32 > NR * DH ? kWarps * NR * 32 : NR * DH;
-  __shared__ __align__(16) float s_buf[kBuf];
-  float(*s_p)[NR][32] = reinterpret_cast<float(*)[NR][32]>(s_buf);
+  static_assert(kWarps * kKeys <= DH, "shared buffer");
+  __shared__ __align__(16) float s_buf[NR * DH];
+  float(*s_p)[NR][kKeys] = reinterpret_cast<float(*)[NR][kKeys]>(s_buf);
   float(*c_o)[DH] = reinterpret_cast<float(*)[DH]>(s_buf);
   __shared__ float s_f[kWarps][16];               // rescaling of the rows, then their maxima
   __shared__ float s_l[kWarps][16];
@@ -113,13 +114,13 @@ __global__ void __launch_bounds__(32 * kWarps) cross_decode_kernel(const DecodeA
 #pragma unroll
     for (int d = 0; d < DL; ++d) o[r][d] = 0.f;
 
-  // 32-key blocks of the window, dealt to the warps of all splits in turn
-  const int nb = hi > lo ? (hi - lo + 31) / 32 : 0;
+  // blocks of the window, dealt to the warps of all splits in turn
+  const int nb = hi > lo ? (hi - lo + kKeys - 1) / kKeys : 0;
   for (int blk = split * kWarps + warp; blk < nb; blk += splits * kWarps) {
-    const int k0 = lo + blk * 32;
-    uint4 kf[4][KC];
+    const int k0 = lo + blk * kKeys;
+    uint4 kf[kKeys / 8][KC];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < kKeys / 8; ++n) {
       const int key = k0 + 8 * n + quad;
 #pragma unroll
       for (int c = 0; c < KC; ++c)
@@ -134,12 +135,12 @@ __global__ void __launch_bounds__(32 * kWarps) cross_decode_kernel(const DecodeA
         w[0] = k0 + key < hi ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
       }
     };
-    uint32_t vf[16][DL / 2];  // the block's first half is on its way during the scores
+    uint32_t vf[kKeys][DL / 2];  // on its way during the scores
 #pragma unroll
-    for (int k = 0; k < 16; ++k) load_v(k, vf[k]);
-    float s[4][4];
+    for (int k = 0; k < kKeys; ++k) load_v(k, vf[k]);
+    float s[kKeys / 8][4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < kKeys / 8; ++n) {
       s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_decode_kernel(const DecodeA
       const int h = head_of(r), q = query_of(r);
       float mx = m[i];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int key = k0 + 8 * n + 2 * t + e;
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(32 * kWarps) cross_decode_kernel(const DecodeA
       m[i] = mx;
       l[i] *= f;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int n = 0; n < kKeys / 8; ++n) {
         const float p0 = exp2_sfu((s[n][2 * i] - mu) * kLog2e), p1 = exp2_sfu((s[n][2 * i + 1] - mu) * kLog2e);
         l[i] += p0 + p1;
         if (r < NR) *reinterpret_cast<float2*>(&s_p[warp][r][8 * n + 2 * t]) = make_float2(p0, p1);
@@ -185,35 +186,29 @@ __global__ void __launch_bounds__(32 * kWarps) cross_decode_kernel(const DecodeA
       for (int d = 0; d < DL; ++d) o[r][d] *= f;
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half)
+    for (int k4 = 0; k4 < kKeys; k4 += 4) {
+      float4 p[NR];
+      float4 any = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) load_v(16 + k, vf[k]);
+      for (int r = 0; r < NR; ++r) {
+        p[r] = r < R ? *reinterpret_cast<const float4*>(&s_p[warp][r][k4]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        any.x += p[r].x, any.y += p[r].y, any.z += p[r].z, any.w += p[r].w;
+      }
+      const float anys[4] = {any.x, any.y, any.z, any.w};
 #pragma unroll
-      for (int k4 = 0; k4 < 16; k4 += 4) {
-        float4 p[NR];
-        float4 any = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < 4; ++k) {
+        float v[DL];
+#pragma unroll
+        for (int d = 0; d < DL / 2; ++d) {
+          const float2 x = unpack2<F16>(vf[k4 + k][d]);
+          // a key that no row keeps adds nothing, whatever V holds there
+          v[2 * d] = anys[k] == 0.f ? 0.f : x.x, v[2 * d + 1] = anys[k] == 0.f ? 0.f : x.y;
+        }
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          p[r] = r < R ? *reinterpret_cast<const float4*>(&s_p[warp][r][16 * half + k4]) : make_float4(0.f, 0.f, 0.f, 0.f);
-          any.x += p[r].x, any.y += p[r].y, any.z += p[r].z, any.w += p[r].w;
-        }
-        const float anys[4] = {any.x, any.y, any.z, any.w};
+          const float pk = k == 0 ? p[r].x : k == 1 ? p[r].y : k == 2 ? p[r].z : p[r].w;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float v[DL];
-#pragma unroll
-          for (int d = 0; d < DL / 2; ++d) {
-            const float2 x = unpack2<F16>(vf[k4 + k][d]);
-            // a key that no row keeps adds nothing, whatever V holds there
-            v[2 * d] = anys[k] == 0.f ? 0.f : x.x, v[2 * d + 1] = anys[k] == 0.f ? 0.f : x.y;
-          }
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const float pk = k == 0 ? p[r].x : k == 1 ? p[r].y : k == 2 ? p[r].z : p[r].w;
-#pragma unroll
-            for (int d = 0; d < DL; ++d) o[r][d] = fmaf(pk, v[d], o[r][d]);
-          }
+          for (int d = 0; d < DL; ++d) o[r][d] = fmaf(pk, v[d], o[r][d]);
         }
       }
     }
@@ -309,10 +304,10 @@ extern "C" int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream) {
   if ((a->q_ss | a->q_hs | a->q_bs | a->k_ss | a->k_hs | a->k_bs | a->v_ss | a->v_hs | a->v_bs) % 8) return -5;
   int dev = 0;
   cudaGetDevice(&dev);
-  // CTAs per key head: as many as fill the SMs a few times over, each warp keeping a 32-key block or more
+  // CTAs per key head: as many as fill the SMs a few times over, each warp keeping a block or more
   const long long heads = (long long)a->B * a->Hk, room = 4ll * dfl_host::num_sms(dev);
   int splits = 1;
-  while (splits < 8 && heads * splits * 2 <= room && a->Sk >= splits * 2 * kWarps * 32) splits *= 2;
+  while (splits < 8 && heads * splits * 2 <= room && a->Sk >= splits * 2 * kWarps * kKeys) splits *= 2;
   if (a->dh == 64) return a->f16 ? decode_rows<64, true>(a, splits, stream) : decode_rows<64, false>(a, splits, stream);
   return a->f16 ? decode_rows<128, true>(a, splits, stream) : decode_rows<128, false>(a, splits, stream);
 }
