@@ -196,6 +196,12 @@ at::Tensor gemm_lora(const at::Tensor& A, const at::Tensor& B, const c10::option
   l.rows_per_id = (int)std::min<int64_t>(rows_per_id > 0 ? rows_per_id : 0, 1 << 30);
   l.n_adapters = (int)A_l.size(0);
   l.rank = (int)A_l.size(1);
+  if (dfl_lora_rows((int)M)) {
+    const at::Tensor t = at::empty({M, l.rank}, A.options().dtype(at::kFloat));
+    l.t = t.data_ptr();
+    DFL_CHECK_RC(dfl_gemm_lora(&a, cur_stream()), "gemm_lora");
+    return D;
+  }
   // split-K partial tiles of this call: only launches that leave SMs idle split (one 128 x 256 f32 tile
   // per CTA tile and at most 96 of them)
   const auto i32 = A.options().dtype(at::kInt);

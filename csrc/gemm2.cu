@@ -158,24 +158,35 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        const int lora_kc = (P.lora_rank + BK - 1) / BK;
-        const int kb_end = kb1 + lora_count(P, mb, lt % P.splits) * lora_kc;
-        for (int kb = kb0; kb < kb_end; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
             ok = false;
             break;
           }
           uint8_t* sa = smem + stage * kStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
-          if (kb < kb1) {
-            tma_load_2d_pair(sa, &P.ta, &full_bar[stage], kb * BK, mb * 2 * BM + (int)rank * BM);
-            tma_load_2d_pair(sa + kABytes, &P.tb, &full_bar[stage], kb * BK, nb * BN + (int)rank * (BN / 2));
-          } else {
-            const int j = (kb - kb1) / lora_kc, c = (kb - kb1) % lora_kc;
-            tma_load_2d_pair(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * 2 * BM + (int)rank * BM);
-            tma_load_2d_pair(sa + kABytes, &P.tl, &full_bar[stage], c * BK,
-                             lora_id(P, mb, j) * P.lora_n + nb * BN + (int)rank * (BN / 2));
+          tma_load_2d_pair(sa, &P.ta, &full_bar[stage], kb * BK, mb * 2 * BM + (int)rank * BM);
+          tma_load_2d_pair(sa + kABytes, &P.tb, &full_bar[stage], kb * BK, nb * BN + (int)rank * (BN / 2));
+          issued[stage] = true;
+          issued_parity[stage] = phase;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
           }
+        }
+        if (P.lora_list == nullptr || !ok) continue;
+        const int lora_kc = (P.lora_rank + BK - 1) / BK, extra = lora_count(P, mb, lt % P.splits) * lora_kc;
+        for (int e = 0; e < extra; ++e) {  // T_j, B_j of the tile's adapters
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const int j = e / lora_kc, c = e % lora_kc;
+          uint8_t* sa = smem + stage * kStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
+          tma_load_2d_pair(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * 2 * BM + (int)rank * BM);
+          tma_load_2d_pair(sa + kABytes, &P.tl, &full_bar[stage], c * BK,
+                           lora_id(P, mb, j) * P.lora_n + nb * BN + (int)rank * (BN / 2));
           issued[stage] = true;
           issued_parity[stage] = phase;
           if (++stage == STAGES) {
@@ -203,12 +214,10 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        int lt, mb, nb, kb0, kb1;
+        int lt, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
-        tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        const int kb_end = kb1 + lora_count(P, mb, lt % P.splits) * ((P.lora_rank + BK - 1) / BK);
-        for (int kb = kb0; kb < kb_end; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
             ok = false;
             break;
@@ -224,6 +233,28 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
+          }
+        }
+        if (P.lora_list != nullptr && ok) {
+          int mb, nb;
+          tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
+          const int extra = lora_count(P, mb, lt % P.splits) * ((P.lora_rank + BK - 1) / BK);
+          for (int e = 0; e < extra; ++e) {
+            if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(smem + stage * kStageBytes), b_addr = a_addr + kABytes;
+            const int ks = lora_ksteps(P, e, BK);
+            for (int k = 0; k < ks; ++k)
+              umma_f16_pair(d_tmem, make_sdesc_sw128(a_addr + k * 32, 16, 1024),
+                            make_sdesc_sw128(b_addr + k * 32, 16, 1024), idesc, 1u);
+            umma_commit_pair(&empty_bar[stage]);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
         if (!ok) break;

@@ -70,6 +70,11 @@ struct alignas(64) GemmProblem {
 DFL_DEVICE int lora_count(const GemmProblem& P, int mb, int split) {
   return P.lora_list != nullptr && split == P.splits - 1 ? __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap)) : 0;
 }
+// 16-wide K steps of extra block e that hold adapter columns (the rest of its 64 columns is zero).
+DFL_DEVICE int lora_ksteps(const GemmProblem& P, int e, int BK) {
+  const int c = P.lora_rank > BK ? e % (P.lora_rank / BK) : 0;
+  return min(BK, P.lora_rank - c * BK) / 16;
+}
 DFL_DEVICE int lora_id(const GemmProblem& P, int mb, int j) {
   return __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap) + 1 + j);
 }

@@ -8,6 +8,9 @@
 // gemm2.cu) then runs x W^T and goes on over the tile's list with T_j B_j^T in the same f32 accumulator, so
 // the adapters cost it ceil(rank / 64) K blocks per adapter a tile holds, and its epilogue is unchanged.
 //
+// Up to 32 rows (single tokens of a batch) take two kernels of their own, lora_rows_t_kernel and
+// lora_rows_kernel below: there the weight's bytes are all that counts.
+//
 // The shrink is bound by reading x (2 M K bytes): a cluster of up to eight CTAs shares a tile, each
 // taking a range of K, so that few tiles still occupy many SMs; the f32 partial sums are added through
 // distributed shared memory in a fixed order.
@@ -235,16 +238,232 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 1) tmem_dealloc(tmem, kCols);
 }
 
+// ---------------------------------------------------------------------------
+// Few rows (M <= 32): bound by reading W once (2 N K bytes).
+//   lora_rows_t_kernel  T[m, r] = s_i x[m] . A_i[r] in f32, one warp per (m, r)
+//   lora_rows_kernel    a CTA of 8 warps owns 16 output columns; its warps take 128-wide pieces of K in turn and
+//                       multiply on the warp-level m16n8k16 instruction, W as the 16-row operand straight
+//                       from global memory (both operands in the same permuted K order, so that a lane
+//                       loads 16 contiguous bytes); partial sums are added in warp order, then T B^T and the epilogue.
+// The second kernel is launched with programmatic serialisation: it streams W while T is computed and waits
+// for T only before it is used.
+// ---------------------------------------------------------------------------
+constexpr int kRowsMax = 32;
+
+struct RowsParams {
+  const __nv_bfloat16* x; long long ldx;
+  const __nv_bfloat16* w; long long ldw;
+  const __nv_bfloat16* a;
+  const __nv_bfloat16* b;
+  const float* scale;
+  const int* ids;
+  int rows_per_id, n_adapters, rank;
+  float* t;  // [M, rank]
+  const __nv_bfloat16* bias;
+  void* y; long long ldy;
+  int out_f32, epi, act_lo, act_hi;
+  const float* gate; long long gate_bs; int gate_rows;
+  const __nv_bfloat16* resid; long long ldr;
+  int M, N, K;
+};
+
+DFL_DEVICE int rows_id(const RowsParams& p, int m) {
+  const int id = __ldg(p.ids + (p.rows_per_id > 0 ? m / p.rows_per_id : m));
+  return id >= 0 && id < p.n_adapters ? id : -1;
+}
+
+DFL_DEVICE float dot8(const uint4& a, const uint4& b, float acc) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = unpack_bf16x2(x[i]), v = unpack_bf16x2(y[i]);
+    acc = fmaf(u.x, v.x, acc);
+    acc = fmaf(u.y, v.y, acc);
+  }
+  return acc;
+}
+
+__global__ void __launch_bounds__(256) lora_rows_t_kernel(RowsParams p, int* err) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int m = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int raw = __ldg(p.ids + (p.rows_per_id > 0 ? m / p.rows_per_id : m)), id = rows_id(p, m);
+  if (id < 0) {
+    if (raw != -1 && blockIdx.y == 0 && threadIdx.x == 0) record_error(err, kErrBounds, kKidLora, 11, m);
+    return;  // (its T is not read)
+  }
+  if (r >= p.rank) return;
+  const uint4* x = reinterpret_cast<const uint4*>(p.x + m * p.ldx);
+  const uint4* a = reinterpret_cast<const uint4*>(p.a + ((long long)id * p.rank + r) * p.K);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int nv = p.K / 8;
+  int v = lane;
+  for (; v + 96 < nv; v += 128) {
+    uint4 xa[4], aa[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) xa[u] = __ldg(x + v + 32 * u), aa[u] = __ldg(a + v + 32 * u);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[u] = dot8(xa[u], aa[u], acc[u]);
+  }
+  for (; v < nv; v += 32) acc[0] = dot8(__ldg(x + v), __ldg(a + v), acc[0]);
+  const float sum = warp_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+  if (lane == 0) p.t[m * p.rank + r] = sum * __ldg(p.scale + id);
+}
+
+DFL_DEVICE void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+DFL_DEVICE uint4 ld_stream16(const uint4* p) {  // read once: no L1 allocation
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// NB: groups of 8 rows.
+template <int NB>
+__global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
+  __shared__ float red[8][16][8 * NB + 1];
+  __shared__ float lora[16][8 * NB + 1];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
+  const int n0 = blockIdx.x * 16;
+  const __nv_bfloat16* w0 = p.w + (long long)min(n0 + quad, p.N - 1) * p.ldw + 8 * t;
+  const __nv_bfloat16* w1 = p.w + (long long)min(n0 + quad + 8, p.N - 1) * p.ldw + 8 * t;
+  float c[NB][4];
+#pragma unroll
+  for (int g = 0; g < NB; ++g) c[g][0] = c[g][1] = c[g][2] = c[g][3] = 0.f;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 2
+  for (int k0 = warp * 128; k0 < p.K; k0 += 8 * 128) {
+    uint4 a[4][2], b[4][NB];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + 32 * u;
+      const bool in = k + 8 * t < p.K;  // K is a multiple of 8: a lane's piece is inside or outside
+      a[u][0] = in ? ld_stream16(reinterpret_cast<const uint4*>(w0 + k)) : zero;
+      a[u][1] = in ? ld_stream16(reinterpret_cast<const uint4*>(w1 + k)) : zero;
+#pragma unroll
+      for (int g = 0; g < NB; ++g)
+        b[u][g] = in && 8 * g + quad < p.M
+                      ? __ldg(reinterpret_cast<const uint4*>(p.x + (8 * g + quad) * p.ldx + k + 8 * t)) : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int g = 0; g < NB; ++g) {
+        mma_bf16(c[g], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][g].x, b[u][g].y);
+        mma_bf16(c[g], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][g].z, b[u][g].w);
+      }
+  }
+  // c[g][2 i + e]: column quad + 8 i, row 8 g + 2 t + e
+#pragma unroll
+  for (int g = 0; g < NB; ++g)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) red[warp][quad + 8 * i][8 * g + 2 * t + e] = c[g][2 * i + e];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // T is complete
+  {  // T B^T: 16 lanes share a column, 8 values of the rank each
+    const int n = threadIdx.x / 16, r0 = (threadIdx.x % 16) * 8;
+    for (int m = 0; m < p.M; ++m) {
+      const int id = rows_id(p, m);
+      float v = 0.f;
+      if (id >= 0 && r0 < p.rank && n0 + n < p.N) {
+        const uint4 bw = __ldg(reinterpret_cast<const uint4*>(p.b + ((long long)id * p.N + n0 + n) * p.rank + r0));
+        const float4 t0 = *reinterpret_cast<const float4*>(p.t + m * p.rank + r0);
+        const float4 t1 = *reinterpret_cast<const float4*>(p.t + m * p.rank + r0 + 4);
+        const float2 b0 = unpack_bf16x2(bw.x), b1 = unpack_bf16x2(bw.y), b2 = unpack_bf16x2(bw.z), b3 = unpack_bf16x2(bw.w);
+        v = ((b0.x * t0.x + b0.y * t0.y) + (b1.x * t0.z + b1.y * t0.w)) +
+            ((b2.x * t1.x + b2.y * t1.y) + (b3.x * t1.z + b3.y * t1.w));
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (threadIdx.x % 16 == 0) lora[n][m] = v;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * p.M; i += 256) {
+    const int n = i % 16, m = i / 16, col = n0 + n;
+    if (col >= p.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += red[k][n][m];
+    v += lora[n][m];
+    if (p.bias) v += __bfloat162float(p.bias[col]);
+    if (col >= p.act_lo && col < p.act_hi) {
+      if (p.epi == kEpiGelu) v = gelu_tanh(v);
+      else if (p.epi == kEpiSilu) v = silu(v);
+    }
+    if (p.epi == kEpiGateResid)
+      v = fmaf(p.gate[(long long)(m / p.gate_rows) * p.gate_bs + col], v, __bfloat162float(p.resid[m * p.ldr + col]));
+    if (p.out_f32) reinterpret_cast<float*>(p.y)[m * p.ldy + col] = v;
+    else reinterpret_cast<__nv_bfloat16*>(p.y)[m * p.ldy + col] = __float2bfloat16_rn(v);
+  }
+}
+
+template <int NB>
+int launch_rows(const RowsParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.N + 15) / 16, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, lora_rows_kernel<NB>, p);
+}
+
+int lora_rows(const GemmArgs* a, cudaStream_t stream) {
+  const LoraArgs* l = a->lora;
+  if (a->gate_row_map || a->alpha != 1.f) return -27;
+  if ((reinterpret_cast<uintptr_t>(a->B) & 15) || a->ldb % 8) return -4;
+  RowsParams p{};
+  p.x = reinterpret_cast<const __nv_bfloat16*>(a->A), p.ldx = a->lda;
+  p.w = reinterpret_cast<const __nv_bfloat16*>(a->B), p.ldw = a->ldb;
+  p.a = reinterpret_cast<const __nv_bfloat16*>(l->a);
+  p.b = reinterpret_cast<const __nv_bfloat16*>(l->b);
+  p.scale = l->scale;
+  p.ids = l->ids;
+  p.rows_per_id = l->rows_per_id, p.n_adapters = l->n_adapters, p.rank = l->rank;
+  p.t = reinterpret_cast<float*>(l->t);
+  p.bias = reinterpret_cast<const __nv_bfloat16*>(a->bias);
+  p.y = a->D, p.ldy = a->ldd;
+  p.out_f32 = a->out_f32, p.epi = a->epi, p.act_lo = a->act_lo, p.act_hi = a->act_hi;
+  p.gate = a->gate, p.gate_bs = a->gate_bstride, p.gate_rows = a->rows_per_batch > 0 ? a->rows_per_batch : a->M;
+  p.resid = reinterpret_cast<const __nv_bfloat16*>(a->resid), p.ldr = a->ldr;
+  p.M = a->M, p.N = a->N, p.K = a->K;
+  if (p.epi == kEpiGateResid && (!p.gate || !p.resid)) return -8;
+  lora_rows_t_kernel<<<dim3(p.M, (p.rank + 7) / 8), 256, 0, stream>>>(p, a->err);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  if (p.M <= 8) return launch_rows<1>(p, stream);
+  if (p.M <= 16) return launch_rows<2>(p, stream);
+  return launch_rows<4>(p, stream);
+}
+
 }  // namespace
+
+extern "C" int dfl_lora_rows(int M) { return M <= kRowsMax; }
 
 extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
   const LoraArgs* l = a->lora;
-  if (!l || !l->a || !l->b || !l->scale || !l->ids || !l->t || !l->list) return -20;
+  if (!l || !l->a || !l->b || !l->scale || !l->ids || !l->t) return -20;
   if (l->n_adapters < 1 || l->n_adapters > kMaxAdapters) return -21;
   if (l->rank % 16 || l->rank < 16 || l->rank > 128 || (l->rank > 64 && l->rank != 128)) return -22;
   if (a->epi == kEpiSwiGLU || a->epi == kEpiQkv || a->out_world > 0) return -23;
+  if (a->M > 0 && a->M <= kRowsMax) {
+    if (a->K % 8 || (a->lda % 8) || ((reinterpret_cast<uintptr_t>(a->A) | reinterpret_cast<uintptr_t>(l->a) |
+                                      reinterpret_cast<uintptr_t>(l->b) | reinterpret_cast<uintptr_t>(l->t)) & 15))
+      return -25;
+    return lora_rows(a, stream);
+  }
   if (l->cap < 1 || l->cap > l->tile_rows || (l->tile_rows != 128 && l->tile_rows != 256)) return -24;
-  if (a->M <= 0 || a->K % 8 || (a->lda * 2) % 16 || (reinterpret_cast<uintptr_t>(a->A) & 15)) return -25;
+  if (!l->list || a->M <= 0 || a->K % 8 || (a->lda * 2) % 16 || (reinterpret_cast<uintptr_t>(a->A) & 15)) return -25;
   if ((reinterpret_cast<uintptr_t>(l->a) | reinterpret_cast<uintptr_t>(l->b) | reinterpret_cast<uintptr_t>(l->t)) & 15)
     return -26;
   int dev = 0;
