@@ -77,6 +77,15 @@ struct Io<__half> {
   }
 };
 
+// Rows are read once: no L1 allocation, so that the weight and modulation rows stay there.
+DFL_DEVICE uint4 ld_stream16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
 DFL_DEVICE uint32_t fp8x4(const float* v, float inv, int e5m2) {
   const __nv_fp8_interpretation_t k = e5m2 ? __NV_E5M2 : __NV_E4M3;
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, k);
@@ -88,7 +97,7 @@ DFL_DEVICE uint32_t fp8x4(const float* v, float inv, int e5m2) {
 // contiguous bytes (D a multiple of E, 16-byte aligned rows); otherwise the group's values lie NT
 // apart, which keeps single-value accesses coalesced for odd widths, strides and addresses.
 template <typename T, int NT, int VPT, bool VEC>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(AddNormArgs a) {
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT == 128 && VEC ? 6 : 1) add_rms_norm_kernel(AddNormArgs a) {
   constexpr int E = Io<T>::E;
   constexpr int kRows = NT < 128 ? 128 / NT : 1;  // rows per block
   constexpr int kWarps = NT / 32;
@@ -114,8 +123,8 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(AddNo
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const bool in = col(i, 0) < a.D;
-      px[i] = in ? *reinterpret_cast<const uint4*>(x + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
-      pr[i] = in && rs ? *reinterpret_cast<const uint4*>(rs + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
+      px[i] = in ? ld_stream16(x + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
+      pr[i] = in && rs ? ld_stream16(rs + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -280,28 +289,38 @@ int dispatch_norm(const AddNormArgs& a, bool vec, cudaStream_t stream) {
   }
 }
 
-// MX -> values: one thread per 16 FP8 elements.
+// MX -> values, 8 elements per thread and step (lanes contiguous on both sides), four steps in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) mx_dequant_kernel(const uint4* __restrict__ q, const uint8_t* __restrict__ sf,
-                                                         T* __restrict__ out, long long n16, int e5m2) {
-  constexpr int E = Io<T>::E;
+__global__ void __launch_bounds__(256) mx_dequant_kernel(const uint2* __restrict__ q, const uint8_t* __restrict__ sf,
+                                                         T* __restrict__ out, long long n8, int e5m2) {
+  constexpr int E = Io<T>::E, U = 4;
   const __nv_fp8_interpretation_t k = e5m2 ? __NV_E5M2 : __NV_E4M3;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n16; i += (long long)gridDim.x * blockDim.x) {
-    const uint4 w = q[i];
-    const uint32_t s = sf[i / 2];
-    // 2^(s - 127): the biased exponent is the f32 exponent field (s = 0: the subnormal 2^-127)
-    const float f = s ? __uint_as_float(s << 23) : __uint_as_float(0x00400000u);
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    float v[16];
+  const long long i0 = (long long)blockIdx.x * (256 * U) + threadIdx.x;
+  uint2 w[U];
+  uint32_t s[U];
 #pragma unroll
-    for (int h = 0; h < 8; ++h) {
+  for (int u = 0; u < U; ++u) {
+    const long long i = i0 + 256 * u;
+    w[u] = i < n8 ? __ldg(q + i) : make_uint2(0u, 0u);
+    s[u] = i < n8 ? __ldg(sf + i / 4) : 0u;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long i = i0 + 256 * u;
+    if (i >= n8) break;
+    // 2^(s - 127): the biased exponent is the f32 exponent field (s = 0: the subnormal 2^-127)
+    const float f = s[u] ? __uint_as_float(s[u] << 23) : __uint_as_float(0x00400000u);
+    const uint32_t ws[2] = {w[u].x, w[u].y};
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
       const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(ws[h / 2] >> (16 * (h & 1))), k);
       const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&r));
       v[2 * h] = p.x * f, v[2 * h + 1] = p.y * f;
     }
-    uint4* o = reinterpret_cast<uint4*>(out + i * 16);
+    uint4* o = reinterpret_cast<uint4*>(out + i * 8);
 #pragma unroll
-    for (int h = 0; h < 16 / E; ++h) o[h] = Io<T>::pack(*reinterpret_cast<float(*)[E]>(&v[h * E]));
+    for (int h = 0; h < 8 / E; ++h) o[h] = Io<T>::pack(*reinterpret_cast<float(*)[E]>(&v[h * E]));
   }
 }
 
@@ -333,17 +352,17 @@ extern "C" int dfl_mx_dequantize(const void* q, const void* scales, void* out, l
                                  cudaStream_t stream) {
   if (n <= 0) return 0;
   if (n % 32 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)) return -2;
-  const long long n16 = n / 16;
-  const long long blocks = (n16 + 255) / 256;
-  const int grid = (int)(blocks < 148 * 64 ? blocks : 148 * 64);
-  const uint4* qp = reinterpret_cast<const uint4*>(q);
+  const long long n8 = n / 8, blocks = (n8 + 1023) / 1024;
+  if (blocks >= (1ll << 31)) return -3;
+  const unsigned grid = (unsigned)blocks;
+  const uint2* qp = reinterpret_cast<const uint2*>(q);
   const uint8_t* sp = reinterpret_cast<const uint8_t*>(scales);
   switch (dtype) {
-    case kDtypeF32: mx_dequant_kernel<<<grid, 256, 0, stream>>>(qp, sp, reinterpret_cast<float*>(out), n16, e5m2); break;
+    case kDtypeF32: mx_dequant_kernel<<<grid, 256, 0, stream>>>(qp, sp, reinterpret_cast<float*>(out), n8, e5m2); break;
     case kDtypeBf16:
-      mx_dequant_kernel<<<grid, 256, 0, stream>>>(qp, sp, reinterpret_cast<__nv_bfloat16*>(out), n16, e5m2);
+      mx_dequant_kernel<<<grid, 256, 0, stream>>>(qp, sp, reinterpret_cast<__nv_bfloat16*>(out), n8, e5m2);
       break;
-    case kDtypeF16: mx_dequant_kernel<<<grid, 256, 0, stream>>>(qp, sp, reinterpret_cast<__half*>(out), n16, e5m2); break;
+    case kDtypeF16: mx_dequant_kernel<<<grid, 256, 0, stream>>>(qp, sp, reinterpret_cast<__half*>(out), n8, e5m2); break;
     default: return -1;
   }
   return (int)cudaGetLastError();

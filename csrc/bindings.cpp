@@ -4,6 +4,7 @@
 // in kernels.h; this file only validates tensors, picks strides and streams,
 // and forwards.  Every entry point raises on a non-zero launcher status.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -48,6 +49,22 @@ cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 const void* opt_ptr(const c10::optional<at::Tensor>& t) {
   return (t.has_value() && t->defined()) ? t->data_ptr() : nullptr;
 }
+
+// at::empty on t's device without the dispatcher (a microsecond of a small call).
+at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt);
+}
+
+int dtype_code(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kDtypeF32;
+    case at::kBFloat16: return kDtypeBf16;
+    case at::kHalf: return kDtypeF16;
+    default: TORCH_CHECK_VALUE(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+
+const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 
 // ---------------------------------------------------------------------------
 // Output + epilogue fields shared by the bf16 and MXFP8 GEMMs.  With out_peer
@@ -151,37 +168,78 @@ at::Tensor gemm(const at::Tensor& A, const at::Tensor& B, const c10::optional<at
   return D;
 }
 
-// gemm with low-rank adapters: A_l [n, r, K], B_l [n, N, r], scale [n], ids int32 per row or per
-// rows_per_id rows.
-at::Tensor gemm_lora(const at::Tensor& A, const at::Tensor& B, const c10::optional<at::Tensor>& bias,
-                     c10::optional<at::Tensor> out, int64_t epi, int64_t act_lo, int64_t act_hi,
+// x [..., K] with low-rank adapters: A_l [n, r, K], B_l [n, N, r], scale [n], ids per row or per rows_per_id
+// rows.  Refused arguments raise ValueError.
+at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::optional<at::Tensor>& bias,
+                     const c10::optional<at::Tensor>& y, int64_t epi, int64_t act_lo, int64_t act_hi,
                      const c10::optional<at::Tensor>& gate, int64_t rows_per_batch,
-                     const c10::optional<at::Tensor>& resid, bool out_f32, const at::Tensor& A_l, const at::Tensor& B_l,
-                     const at::Tensor& scale, const at::Tensor& ids, int64_t rows_per_id) {
-  check_bf16_cuda(A, "x");
-  check_bf16_cuda(B, "weight");
-  check_rowmajor(A, "x");
-  check_rowmajor(B, "weight");
-  check_bf16_cuda(A_l, "adapter A");
-  check_bf16_cuda(B_l, "adapter B");
-  const int64_t M = A.size(0), K = A.size(1), N = B.size(0);
-  TORCH_CHECK(B.size(1) == K, "K mismatch: x ", A.sizes(), " weight ", B.sizes());
-  TORCH_CHECK(A_l.dim() == 3 && A_l.is_contiguous() && B_l.dim() == 3 && B_l.is_contiguous() && A_l.size(2) == K &&
-                  B_l.size(1) == N && A_l.size(0) == B_l.size(0) && A_l.size(1) == B_l.size(2),
-              "adapters must be contiguous [n, r, K] and [n, N, r]");
-  TORCH_CHECK(scale.is_contiguous() && scale.scalar_type() == at::kFloat && scale.numel() == A_l.size(0),
-              "adapter scale must be float32 [n]");
-  TORCH_CHECK(ids.scalar_type() == at::kInt && ids.is_contiguous() && ids.dim() == 1 &&
-                  ids.numel() == (rows_per_id > 0 ? (M + rows_per_id - 1) / rows_per_id : M),
-              "ids must be int32, one per row or per ", rows_per_id, " rows");
-  for (const at::Tensor* t : {&B, &A_l, &B_l, &scale, &ids})
-    TORCH_CHECK(t->device() == A.device(), "all tensors on one device");
-  TORCH_CHECK(K % 8 == 0, "linear_lora needs K to be a multiple of 8, got ", K);
-  const c10::cuda::CUDAGuard guard(A.device());
+                     const c10::optional<at::Tensor>& resid_in, bool out_f32, const at::Tensor& A_l, const at::Tensor& B_l,
+                     const at::Tensor& scale, const at::Tensor& ids_in, int64_t rows_per_id) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && B.dim() == 2, "x [..., K] and weight [N, K] must be CUDA tensors");
+  for (const at::Tensor* t : {&x, &B, &A_l, &B_l})
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16, "linear_lora runs in bfloat16 on CUDA: x ", x.scalar_type(),
+                      ", weight ", B.scalar_type(), ", bank ", A_l.scalar_type());
+  for (const at::Tensor* t : {&B, &A_l, &B_l, &scale, &ids_in})
+    TORCH_CHECK_VALUE(t->device() == x.device(), "x, weight, bank and ids must be on one device");
+  const int64_t K = x.size(-1), N = B.size(0);
+  TORCH_CHECK_VALUE(A_l.dim() == 3 && A_l.is_contiguous() && B_l.dim() == 3 && B_l.is_contiguous() &&
+                        A_l.size(0) == B_l.size(0) && A_l.size(1) == B_l.size(2),
+                    "adapters must be contiguous [n, r, K] and [n, N, r]");
+  TORCH_CHECK_VALUE(A_l.size(2) == K, "x ", x.sizes(), " does not end in the bank's ", A_l.size(2), " inputs");
+  TORCH_CHECK_VALUE(B.size(1) == K && B_l.size(1) == N, "weight ", B.sizes(), " is not [", B_l.size(1), ", ", K, "]");
+  TORCH_CHECK_VALUE(B.stride(1) == 1 && B.stride(0) % 8 == 0 && K % 8 == 0 && N % (out_f32 ? 4 : 8) == 0,
+                    "linear_lora needs rows of whole 16-byte pieces: K ", K, ", N ", N);
+  TORCH_CHECK_VALUE(scale.is_contiguous() && scale.scalar_type() == at::kFloat && scale.numel() == A_l.size(0),
+                    "adapter scale must be float32 [n]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor A = x.dim() == 2 ? x : x.reshape({-1, K});
+  const int64_t M = A.size(0);
+  TORCH_CHECK_VALUE(M < (1ll << 30), "too many rows");
+  if (A.stride(1) != 1 || (M > 1 && (A.stride(0) % 8 || A.stride(0) < K)) || reinterpret_cast<uintptr_t>(A.data_ptr()) % 16)
+    A = A.contiguous();
+  if (reinterpret_cast<uintptr_t>(A.data_ptr()) % 16) A = A.clone();  // contiguous, but from an odd start
+  TORCH_CHECK_VALUE(at::isIntegralType(ids_in.scalar_type(), false) && ids_in.dim() == 1, "ids must be a vector of integers");
+  TORCH_CHECK_VALUE(ids_in.numel() == (rows_per_id > 0 ? (M + rows_per_id - 1) / rows_per_id : M),
+                    rows_per_id > 0 ? (M + rows_per_id - 1) / rows_per_id : M, " ids expected for ", M, " rows, got ",
+                    ids_in.numel());
+  // what does not fit 32 bits names no adapter either
+  const at::Tensor ids = ids_in.scalar_type() == at::kInt && ids_in.is_contiguous()
+                             ? ids_in
+                             : (ids_in.scalar_type() == at::kLong ? ids_in.clamp(-2, 1 << 30) : ids_in).to(at::kInt).contiguous();
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = N;
+  const auto ydt = out_f32 ? at::kFloat : at::kBFloat16;
+  at::Tensor res;
+  if (given(y)) {
+    res = *y;
+    TORCH_CHECK_VALUE(res.sizes() == at::IntArrayRef(shape) && res.scalar_type() == ydt && res.device() == x.device(), "out ",
+                      res.sizes(), " ", res.scalar_type(), " must be ", at::IntArrayRef(shape), " ", ydt);
+  } else {
+    res = new_like(x, shape, ydt);
+  }
+  if (M == 0) return res;
+  c10::optional<at::Tensor> out = res.dim() == 2 ? res : res.view({M, N}), resid;
+  TORCH_CHECK_VALUE(out->stride(1) == 1 && out->stride(0) % (out_f32 ? 4 : 8) == 0 &&
+                        reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, "out needs 16-byte aligned rows");
+  if (const at::Tensor* t = given(bias))
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 && t->dim() == 1 && t->numel() == N && t->is_contiguous() &&
+                          t->device() == x.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                      "bias must be contiguous bfloat16 [", N, "], 16-byte aligned");
+  TORCH_CHECK_VALUE(bool(given(gate)) == bool(given(resid_in)) && bool(given(gate)) == (epi == kEpiGateResid),
+                    "gate and resid come together, without act");
+  if (const at::Tensor* t = given(resid_in)) {
+    TORCH_CHECK_VALUE(t->sizes() == at::IntArrayRef(shape) && t->scalar_type() == at::kBFloat16 && t->device() == x.device(),
+                      "resid must be bfloat16 ", at::IntArrayRef(shape));
+    TORCH_CHECK_VALUE(!out_f32, "the gated residual is stored in bfloat16");
+    resid = t->dim() == 2 ? *t : t->reshape({M, N});
+    const int64_t rpb = rows_per_batch > 0 ? rows_per_batch : M;
+    TORCH_CHECK_VALUE(gate->scalar_type() == at::kFloat && gate->dim() == 2 && gate->stride(1) == 1 && gate->size(1) >= N &&
+                          gate->device() == x.device() && gate->size(0) * rpb >= M,
+                      "gate must be float32 [B, ", N, "] with a row for every ", rpb, " rows");
+  }
   GemmArgs a{};
-  at::Tensor D = gemm_epilogue_args(a, A, M, N, bias, out, epi, act_lo, act_hi, gate, rows_per_batch, resid, 1.0,
+  gemm_epilogue_args(a, A, M, N, bias, out, epi, act_lo, act_hi, gate, rows_per_batch, resid, 1.0,
                                     out_f32, {}, 0, 0, 0, c10::nullopt, "");
-  TORCH_CHECK(epi != kEpiGateResid || gate->size(0) * (int64_t)a.rows_per_batch >= M, "gate has too few rows");
   a.A = A.data_ptr();
   a.B = B.data_ptr();
   a.lda = A.stride(0);
@@ -197,35 +255,34 @@ at::Tensor gemm_lora(const at::Tensor& A, const at::Tensor& B, const c10::option
   l.n_adapters = (int)A_l.size(0);
   l.rank = (int)A_l.size(1);
   if (dfl_lora_rows((int)M)) {
-    const at::Tensor t = at::empty({M, l.rank}, A.options().dtype(at::kFloat));
+    const at::Tensor t = new_like(A, {M, l.rank}, at::kFloat);
     l.t = t.data_ptr();
     DFL_CHECK_RC(dfl_gemm_lora(&a, cur_stream()), "gemm_lora");
-    return D;
+    return res;
   }
-  // split-K partial tiles of this call: only launches that leave SMs idle split (one 128 x 256 f32 tile
-  // per CTA tile and at most 96 of them)
-  const auto i32 = A.options().dtype(at::kInt);
-  at::Tensor ws, sem;
-  if ((M + 127) / 128 * ((N + 255) / 256) <= 96) {
-    l.split_ws_floats = 96ll * 128 * 256;
-    l.split_sem_count = 256;
-    ws = at::empty({l.split_ws_floats}, A.options().dtype(at::kFloat));
-    sem = at::empty({l.split_sem_count}, i32);
-    l.split_ws = ws.data_ptr<float>();
-    l.split_sem = sem.data_ptr<int>();
-  }
+  // one buffer: T | tile lists | split-K counters | split-K partial tiles (of this call alone; only launches
+  // that leave SMs idle split, one 128 x 256 f32 tile per CTA tile and at most 96 of them)
+  l.split_ws_floats = (M + 127) / 128 * ((N + 255) / 256) <= 96 ? 96ll * 128 * 256 : 0;
+  l.split_sem_count = l.split_ws_floats ? 256 : 0;
   l.tile_rows = dfl_gemm_tile_rows(&a);
   const int64_t tiles = (M + l.tile_rows - 1) / l.tile_rows;
   int64_t cap = std::min<int64_t>(l.n_adapters, l.tile_rows);
   if (rows_per_id > 0) cap = std::min<int64_t>(cap, (l.tile_rows - 1 + rows_per_id - 1) / rows_per_id + 1);
   l.cap = (int)cap;
-  const at::Tensor t = at::empty({tiles * cap * l.tile_rows, l.rank}, A.options());
-  const at::Tensor list = at::empty({tiles * (1 + cap)}, i32);
-  l.t = t.data_ptr();
-  l.list = list.data_ptr<int>();
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  const int64_t t_bytes = up(tiles * cap * l.tile_rows * l.rank * 2), list_bytes = up(tiles * (1 + cap) * 4),
+                sem_bytes = up(l.split_sem_count * 4);
+  const at::Tensor buf = new_like(A, {t_bytes + list_bytes + sem_bytes + l.split_ws_floats * 4}, at::kByte);
+  uint8_t* base = buf.data_ptr<uint8_t>();
+  l.t = base;
+  l.list = reinterpret_cast<int*>(base + t_bytes);
+  if (l.split_ws_floats) {
+    l.split_sem = reinterpret_cast<int*>(base + t_bytes + list_bytes);
+    l.split_ws = reinterpret_cast<float*>(base + t_bytes + list_bytes + sem_bytes);
+  }
   a.cta_mode = l.tile_rows == 256 ? 2 : 1;  // the tile shape the lists are built for
   DFL_CHECK_RC(dfl_gemm_lora(&a, cur_stream()), "gemm_lora");
-  return D;
+  return res;
 }
 
 // ---------------------------------------------------------------- MXFP8
@@ -369,70 +426,73 @@ at::Tensor ln_modulate(const at::Tensor& x, c10::optional<at::Tensor> out,
   return y;
 }
 
-int dtype_code(const at::Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return kDtypeF32;
-    case at::kBFloat16: return kDtypeBf16;
-    case at::kHalf: return kDtypeF16;
-    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
-  }
-}
 
-const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
-
-// Rows [M, D] -> {y or q, s or empty, scales or empty}.  Shapes and types are checked by the caller
-// (ops.fused.add_rms_norm); what a kernel reads through these pointers is checked here again.
+// x [..., D] -> {y or q, s or undefined, scales or undefined}.  Refused arguments raise ValueError.
 std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at::Tensor>& resid,
                                      const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& scale,
                                      const c10::optional<at::Tensor>& shift, int64_t rows_per_batch,
                                      const c10::optional<at::Tensor>& row_map, double eps, int64_t quant, bool blocked,
                                      const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& s_out) {
-  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
-  check_rowmajor(x, "x");
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1, "x must be a CUDA tensor [..., D]");
+  const int64_t D = x.size(-1);
+  TORCH_CHECK_VALUE(D >= 1 && D <= 16384, "add_rms_norm needs [..., D] with 1 <= D <= 16384, got ", x.sizes());
   const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t M = x.size(0), D = x.size(1);
-  TORCH_CHECK(M < (1ll << 31) && D >= 1 && D <= 16384, "add_rms_norm: 1 <= D <= 16384, got ", D);
   AddNormArgs a{};
   a.dtype = dtype_code(x, "x");
-  auto same = [&](const at::Tensor& t, const char* name) {
-    TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.dim() == 2 && t.size(0) == M &&
-                    t.size(1) == D && t.stride(1) == 1, name, " must be like x: [M, D], unit inner stride");
+  auto like_x = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(), name, " ",
+                      t.sizes(), " ", t.scalar_type(), " does not match x ", x.sizes(), " ", x.scalar_type());
   };
-  a.x = x.data_ptr();
-  a.ldx = x.stride(0);
-  at::Tensor s;
+  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, D});
+  const int64_t M = x2.size(0);
+  TORCH_CHECK_VALUE(M < (1ll << 31), "too many rows");
+  TORCH_CHECK_VALUE(x2.stride(1) == 1 || D == 1, "x needs a unit inner stride");
+  // a view, not a copy: results go into the caller's tensor
+  auto rows = [&](const at::Tensor& t, const char* name) {
+    const at::Tensor v = t.dim() == 2 ? t : t.view({M, D});
+    TORCH_CHECK_VALUE(v.stride(1) == 1 || D == 1, name, " needs a unit inner stride");
+    return v;
+  };
+  a.x = x2.data_ptr();
+  a.ldx = x2.stride(0);
+  at::Tensor s, s2, r2;
   if (const at::Tensor* r = given(resid)) {
-    same(*r, "resid");
-    a.resid = r->data_ptr();
-    a.ldr = r->stride(0);
-    s = given(s_out) ? *s_out : at::empty({M, D}, x.options());
-    same(s, "resid_out");
-    a.s_out = s.data_ptr();
-    a.lds = s.stride(0);
+    like_x(*r, "resid");
+    r2 = r->dim() == 2 ? *r : r->reshape({-1, D});
+    TORCH_CHECK_VALUE(r2.stride(1) == 1 || D == 1, "resid needs a unit inner stride");
+    a.resid = r2.data_ptr();
+    a.ldr = r2.stride(0);
+    if (given(s_out)) like_x(*s_out, "resid_out");
+    s = given(s_out) ? *s_out : new_like(x, x.sizes(), x.scalar_type());
+    s2 = rows(s, "resid_out");
+    a.s_out = s2.data_ptr();
+    a.lds = s2.stride(0);
+  } else {
+    TORCH_CHECK_VALUE(!given(s_out), "resid_out needs resid");
   }
   if (const at::Tensor* t = given(w)) {
-    TORCH_CHECK(t->device() == x.device() && t->dim() == 1 && t->numel() == D && t->is_contiguous() &&
-                    (t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat),
-                "weight must be contiguous [D] of x's type or float32");
+    TORCH_CHECK_VALUE(t->device() == x.device() && t->dim() == 1 && t->size(0) == D && (t->stride(0) == 1 || D == 1) &&
+                          (t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat),
+                      "weight must be contiguous [", D, "] of ", x.scalar_type(), " or float32 on x's device");
     a.w = t->data_ptr();
     a.w_f32 = t->scalar_type() == at::kFloat;
   }
-  a.rows_per_batch = (int)(rows_per_batch > 0 ? rows_per_batch : M);
+  a.rows_per_batch = (int)std::max<int64_t>(1, rows_per_batch > 0 ? std::min(rows_per_batch, M) : M);
   const at::Tensor* rm = given(row_map);
   if (rm) {
-    TORCH_CHECK(rm->device() == x.device() && rm->scalar_type() == at::kInt && rm->is_contiguous() && rm->numel() == M,
-                "row_map must be int32 [M]");
+    TORCH_CHECK_VALUE(rm->device() == x.device() && rm->scalar_type() == at::kInt && rm->is_contiguous() && rm->numel() == M,
+                      "row_map must be int32 [", M, "]");
     a.row_map = rm->data_ptr<int>();
   }
   auto mod = [&](const c10::optional<at::Tensor>& o, const char* name, const float*& p, long long& bs) {
     const at::Tensor* t = given(o);
     if (!t) return;
-    TORCH_CHECK(t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) == D &&
-                    t->stride(1) == 1, name, " must be float32 [batch, D]");
-    TORCH_CHECK(rm || M == 0 || t->size(0) * (int64_t)a.rows_per_batch >= M, name, " has ", t->size(0),
-                " rows: too few for ", M, " rows of ", a.rows_per_batch, " per batch");
-    TORCH_CHECK(a.n_mod == 0 || a.n_mod == t->size(0), "scale and shift differ in their batch rows");
-    TORCH_CHECK(t->size(0) > 0, name, " has no rows");
+    TORCH_CHECK_VALUE(t->device() == x.device() && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) > 0 &&
+                          t->size(1) == D && (t->stride(1) == 1 || D == 1),
+                      name, " must be float32 [B, ", D, "] with a unit inner stride on x's device");
+    TORCH_CHECK_VALUE(rm || t->size(0) * (int64_t)a.rows_per_batch >= M, name, " has ", t->size(0), " rows: too few for ",
+                      M, " rows of ", a.rows_per_batch, " per batch");
+    TORCH_CHECK_VALUE(a.n_mod == 0 || a.n_mod == t->size(0), "scale and shift differ in their batch rows");
     a.n_mod = (int)t->size(0);
     p = t->data_ptr<float>();
     bs = t->stride(0);
@@ -445,21 +505,32 @@ std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at
   a.quant = (int)quant;
   a.blocked = blocked ? 1 : 0;
   a.err = err_ptr();
-  at::Tensor y, sf;
+  at::Tensor y, y2, sf;
   if (quant) {
-    TORCH_CHECK(D % (blocked ? 128 : 32) == 0, "the MX output needs D to be a multiple of ", blocked ? 128 : 32);
-    y = at::empty({M, D}, x.options().dtype(quant == 2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn));
-    sf = blocked ? at::empty({(M + 255) / 256 * 256 * (D / 32)}, x.options().dtype(at::kByte))
-                 : at::empty({M, D / 32}, x.options().dtype(at::kByte));
+    TORCH_CHECK_VALUE(!given(out), "out= and quantize= are mutually exclusive");
+    TORCH_CHECK_VALUE(D % (blocked ? 128 : 32) == 0, "the MX output needs D to be a multiple of ", blocked ? 128 : 32,
+                      ", got ", D);
+    y = new_like(x, x.sizes(), quant == 2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn);
+    if (blocked) {
+      sf = new_like(x, {(M + 255) / 256 * 256 * (D / 32)}, at::kByte);
+    } else {
+      std::vector<int64_t> shape = x.sizes().vec();
+      shape.back() = D / 32;
+      sf = new_like(x, shape, at::kByte);
+    }
     a.sf = sf.data_ptr<uint8_t>();
+    a.y = y.data_ptr();
+    a.ldy = D;
   } else {
-    y = given(out) ? *out : at::empty({M, D}, x.options());
-    same(y, "out");
+    TORCH_CHECK_VALUE(!blocked, "blocked scales need quantize=");
+    if (given(out)) like_x(*out, "out");
+    y = given(out) ? *out : new_like(x, x.sizes(), x.scalar_type());
+    y2 = rows(y, "out");
+    a.y = y2.data_ptr();
+    a.ldy = y2.stride(0);
   }
-  a.y = y.data_ptr();
-  a.ldy = y.stride(0);
   const int rc = dfl_add_rms_norm(&a, cur_stream());
-  TORCH_CHECK(rc != -3, "the MX output needs 16-byte aligned rows of x, resid, weight, scale and shift");
+  TORCH_CHECK_VALUE(rc != -3, "the MX output needs 16-byte aligned rows of x, resid, weight, scale and shift");
   DFL_CHECK_RC(rc, "add_rms_norm");
   return {y, s, sf};
 }
@@ -470,7 +541,7 @@ at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarTy
   TORCH_CHECK(q.scalar_type() == at::kFloat8_e4m3fn || q.scalar_type() == at::kFloat8_e5m2, "q must be float8");
   TORCH_CHECK(sf.scalar_type() == at::kByte && q.numel() == sf.numel() * 32, "one uint8 scale per 32 elements");
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options().dtype(dtype));
+  at::Tensor out = new_like(q, q.sizes(), dtype);
   DFL_CHECK_RC(dfl_mx_dequantize(q.data_ptr(), sf.data_ptr(), out.data_ptr(), q.numel(), dtype_code(out, "output"),
                                  q.scalar_type() == at::kFloat8_e5m2, cur_stream()), "mx_dequantize");
   return out;
@@ -483,21 +554,24 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
                            const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& kv_lo,
                            const c10::optional<at::Tensor>& kv_hi, const c10::optional<at::Tensor>& out,
                            const c10::optional<at::Tensor>& lse) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q/k/v must be CUDA tensors [B, H, S, dh]");
-  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "cross attention runs in bfloat16 or float16");
+  TORCH_CHECK_VALUE(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q/k/v must be CUDA tensors [B, H, S, D]");
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
+                    "cross attention runs in bfloat16 or float16, got ", q.scalar_type());
   const c10::cuda::CUDAGuard guard(q.device());
+  for (const at::Tensor* t : {&q, &k})
+    TORCH_CHECK_VALUE(t->size(0) < (1 << 30) && t->size(1) < (1 << 30) && t->size(2) < (1 << 30), "a length is too large");
   CrossArgs a{};
   a.B = (int)q.size(0), a.H = (int)q.size(1), a.Sq = (int)q.size(2), a.dh = (int)q.size(3);
   a.Hk = (int)k.size(1), a.Sk = (int)k.size(2);
-  TORCH_CHECK(a.dh == 64 || a.dh == 128, "head dim must be 64 or 128, got ", a.dh);
+  TORCH_CHECK_VALUE(a.dh == 64 || a.dh == 128, "head dim must be 64 or 128, got ", a.dh);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(0) == a.B && k.size(3) == a.dh, "k ", k.sizes(), " and v ", v.sizes(),
+                    " must be [", a.B, ", Hk, Sk, ", a.dh, "]");
   for (const at::Tensor* t : {&k, &v})
-    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == q.scalar_type() && t->size(0) == a.B &&
-                    t->size(1) == a.Hk && t->size(2) == a.Sk && t->size(3) == a.dh,
-                "k / v must be [", a.B, ", Hk, Sk, ", a.dh, "] of q's type and device");
-  TORCH_CHECK(a.Hk > 0 && a.H % a.Hk == 0, "query heads must be a multiple of the key heads");
+    TORCH_CHECK_VALUE(t->device() == q.device() && t->scalar_type() == q.scalar_type(), "q, k and v must share type and device");
+  TORCH_CHECK_VALUE(a.Hk > 0 && a.H % a.Hk == 0, "the query heads (", a.H, ") must be a multiple of the key heads (", a.Hk, ")");
   at::Tensor o = given(out) ? *out : at::empty_like(q);
-  TORCH_CHECK(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(),
-              "out must be like q");
+  TORCH_CHECK_VALUE(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.device() == q.device(), "out ", o.sizes(),
+                    " ", o.scalar_type(), " does not match q ", q.sizes(), " ", q.scalar_type());
   if (o.numel() == 0) return o;
   // Rows the copies engine can address: unit inner stride, 16-byte multiples elsewhere (an axis of
   // one element has no stride to speak of, and a repeated axis none at all).
@@ -524,8 +598,8 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   a.f16 = q.scalar_type() == at::kHalf;
   a.scale = (float)scale;
   if (const at::Tensor* t = given(lse)) {
-    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->device() == q.device() &&
-                    t->numel() == (int64_t)a.B * a.H * a.Sq, "lse must be contiguous float32 [B, H, Sq]");
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->is_contiguous() && t->device() == q.device() &&
+                          t->numel() == (int64_t)a.B * a.H * a.Sq, "lse must be contiguous float32 [B, H, Sq]");
     a.lse = t->data_ptr<float>();
   }
   if (a.Sk == 0) {  // no key at all: every row is empty
@@ -533,19 +607,25 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     if (const at::Tensor* t = given(lse)) t->fill_(-std::numeric_limits<float>::infinity());
     return o;
   }
-  auto edge = [&](const c10::optional<at::Tensor>& e, const char* name) -> const int* {
+  at::Tensor edges[2];
+  auto edge = [&](const c10::optional<at::Tensor>& e, const char* name, at::Tensor& keep) -> const int* {
     const at::Tensor* t = given(e);
     if (!t) return nullptr;
-    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() == a.B,
-                name, " must be int32 [", a.B, "]");
-    return t->data_ptr<int>();
+    TORCH_CHECK_VALUE(at::isIntegralType(t->scalar_type(), false) && t->dim() == 1 && t->size(0) == a.B, name,
+                      " must be integers [", a.B, "]");
+    keep = t->to(at::TensorOptions().device(q.device()).dtype(at::kInt)).contiguous();
+    return keep.data_ptr<int>();
   };
-  a.kv_lo = edge(kv_lo, "kv_lo");
-  a.kv_hi = edge(kv_hi, "kv_hi");
-  at::Tensor m, aux, win;
+  a.kv_lo = edge(kv_lo, "kv_lo", edges[0]);
+  a.kv_hi = edge(kv_hi, "kv_lens", edges[1]);
+  at::Tensor m, aux;
   int mdt = 0;  // -1: boolean, else the type of an additive mask
   if (const at::Tensor* mt = given(mask)) {
-    TORCH_CHECK(mt->device() == q.device(), "the mask must be on q's device");
+    TORCH_CHECK_VALUE(mt->device() == q.device(), "the mask must be on q's device");
+    const int64_t want[4] = {a.B, a.H, a.Sq, a.Sk};
+    bool fit = mt->dim() <= 4;
+    for (int64_t d = 0; fit && d < mt->dim(); ++d) fit = mt->size(-1 - d) == 1 || mt->size(-1 - d) == want[3 - d];
+    TORCH_CHECK_VALUE(fit, "attention_mask ", mt->sizes(), " does not broadcast to [", a.B, ", ", a.H, ", ", a.Sq, ", ", a.Sk, "]");
     m = mt->expand({a.B, a.H, a.Sq, a.Sk});
     mdt = m.scalar_type() == at::kBool ? -1 : dtype_code(m, "an additive mask");
   }
@@ -573,12 +653,12 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     b.bs = m.stride(0), b.hs = m.stride(1), b.qs = m.stride(2), b.ks = m.stride(3);
     b.B = b.bs ? a.B : 1, b.H = b.hs ? a.H : 1, b.Q = b.qs ? a.Sq : 1, b.Sk = a.Sk;
     b.words = (a.Sk + 127) / 128 * 4;
-    aux = at::empty({(int64_t)b.B * b.H * b.Q * b.words}, q.options().dtype(at::kInt));
+    const int64_t n_bits = (int64_t)b.B * b.H * b.Q * b.words;
+    aux = new_like(q, {n_bits + 2 * a.B}, at::kInt);  // bit rows, then a window per batch row
     b.bits = reinterpret_cast<uint32_t*>(aux.data_ptr<int>());
     a.key_bits = b.H == 1 && b.Q == 1;
     if (a.key_bits && b.B == a.B && !a.kv_lo && !a.kv_hi) {
-      win = at::empty({2, a.B}, q.options().dtype(at::kInt));
-      b.lo = win.data_ptr<int>();
+      b.lo = aux.data_ptr<int>() + n_bits;
       b.hi = b.lo + a.B;
       a.kv_lo = b.lo, a.kv_hi = b.hi;
     }
@@ -595,7 +675,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     t.B = t.bs ? a.B : 1, t.H = t.hs ? a.H : 1, t.Q = t.qs ? a.Sq : 1, t.Sk = a.Sk;
     t.out_f32 = m.scalar_type() != q.scalar_type();
     const int64_t nq = (t.Q + 31) / 32, nt = (t.Sk + 127) / 128, rows = t.Q > 1 ? 32 : 1, vec = t.out_f32 ? 32 : 16;
-    aux = at::empty({t.B * t.H * nq * nt * vec * rows * 4}, q.options().dtype(at::kInt));
+    aux = new_like(q, {t.B * t.H * nq * nt * vec * rows * 4}, at::kInt);
     t.tiles = aux.data_ptr();
     DFL_CHECK_RC(dfl_cross_bias_tiles(&t, cur_stream()), "cross_bias_tiles");
     a.bias_tiles = t.tiles;
@@ -1210,8 +1290,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_group", &gemm_group, "grouped tcgen05 GEMMs (one launch)", py::arg("A"), py::arg("B"),
         py::arg("bias"), py::arg("out"), py::arg("epi"), py::arg("act_lo"), py::arg("act_hi"), py::arg("gate"),
         py::arg("rows_per_batch"), py::arg("resid"), py::arg("qkv_plan"), py::arg("cta_mode") = 0);
-  m.def("gemm_lora", &gemm_lora, "tcgen05 GEMM with low-rank adapters accumulated beside the weight", py::arg("A"),
-        py::arg("B"), py::arg("bias"), py::arg("out"), py::arg("epi"), py::arg("act_lo"), py::arg("act_hi"),
+  m.def("gemm_lora", &gemm_lora, "tcgen05 GEMM with low-rank adapters accumulated beside the weight", py::arg("x"),
+        py::arg("w"), py::arg("bias"), py::arg("out"), py::arg("epi"), py::arg("act_lo"), py::arg("act_hi"),
         py::arg("gate"), py::arg("rows_per_batch"), py::arg("resid"), py::arg("out_f32"), py::arg("A_l"),
         py::arg("B_l"), py::arg("scale"), py::arg("ids"), py::arg("rows_per_id"));
   m.def("mx_quantize", &mx_quantize, py::arg("x"), py::arg("blocked") = false);

@@ -16,7 +16,7 @@
 namespace {
 using namespace dfl;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kMaxSplits = 8;
 constexpr int kKeys = 16;  // per warp and step: its K and V (8 KB at dh 128) are in flight together
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -36,7 +36,7 @@ DFL_DEVICE void cluster_sync() {
 DFL_DEVICE float ld_cluster(const float* p, uint32_t rank) {
   uint32_t a;
   float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
   return v;
 }
@@ -248,16 +248,26 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cr
   if (splits > 1) cluster_sync();
   for (int i = threadIdx.x + 32 * kWarps * split; i < R * DH; i += 32 * kWarps * splits) {
     const int r = i / DH, d = i % DH;
+    // all remote reads first: they are independent, and each takes most of a microsecond
+    float mc[kMaxSplits], lc[kMaxSplits], oc[kMaxSplits];
     float mx = -INFINITY;
-    for (int c = 0; c < splits; ++c) mx = fmaxf(mx, splits > 1 ? ld_cluster(&c_m[r], c) : c_m[r]);
+#pragma unroll
+    for (int c = 0; c < kMaxSplits; ++c) {
+      const bool in = c < splits;
+      mc[c] = in ? (splits > 1 ? ld_cluster(&c_m[r], c) : c_m[r]) : -INFINITY;
+      lc[c] = in ? (splits > 1 ? ld_cluster(&c_l[r], c) : c_l[r]) : 0.f;
+      oc[c] = in ? (splits > 1 ? ld_cluster(&c_o[r][d], c) : c_o[r][d]) : 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < kMaxSplits; ++c) mx = fmaxf(mx, mc[c]);
     const float mu = mx == -INFINITY ? 0.f : mx;
     float ov = 0.f, lv = 0.f;
-    for (int c = 0; c < splits; ++c) {
-      const float mc = splits > 1 ? ld_cluster(&c_m[r], c) : c_m[r], lc = splits > 1 ? ld_cluster(&c_l[r], c) : c_l[r];
-      if (mc == -INFINITY && lc == 0.f) continue;
-      const float f = exp2_sfu((mc - mu) * kLog2e);
-      ov += f * (splits > 1 ? ld_cluster(&c_o[r][d], c) : c_o[r][d]);
-      lv += f * lc;
+#pragma unroll
+    for (int c = 0; c < kMaxSplits; ++c) {
+      if (mc[c] == -INFINITY && lc[c] == 0.f) continue;
+      const float f = exp2_sfu((mc[c] - mu) * kLog2e);
+      ov += f * oc[c];
+      lv += f * lc[c];
     }
     const float y = lv == 0.f ? 0.f : ov / lv;
     const long long at = b * a.o_bs + (long long)head_of(r) * a.o_hs + (long long)query_of(r) * a.o_ss + d;
@@ -307,7 +317,7 @@ extern "C" int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream) {
   // CTAs per key head: as many as fill the SMs a few times over, each warp keeping a block or more
   const long long heads = (long long)a->B * a->Hk, room = 4ll * dfl_host::num_sms(dev);
   int splits = 1;
-  while (splits < 8 && heads * splits * 2 <= room && a->Sk >= splits * 2 * kWarps * kKeys) splits *= 2;
+  while (splits < kMaxSplits && heads * splits * 2 <= room && a->Sk >= splits * 2 * kWarps * kKeys) splits *= 2;
   if (a->dh == 64) return a->f16 ? decode_rows<64, true>(a, splits, stream) : decode_rows<64, false>(a, splits, stream);
   return a->f16 ? decode_rows<128, true>(a, splits, stream) : decode_rows<128, false>(a, splits, stream);
 }

@@ -46,7 +46,8 @@ struct Smem {
   static_assert(kTotal <= 232448, "shared memory budget");
 };
 
-template <int BN, int STAGES, int EPI, bool OUT_F32>
+// LORA: the K loop goes on over the adapters of the tile (a variant of its own: the plain one is untouched).
+template <int BN, int STAGES, int EPI, bool OUT_F32, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_tcgen05_kernel(const __grid_constant__ GemmGroup grp, int* err) {
   using S = Smem<BN, STAGES>;
@@ -106,6 +107,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
+        // (read here: its latency passes behind the K loop)
+        const int extra = LORA ? lora_blocks(P, mb, lt % P.splits, BK) : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 10 + stage, abort_flag)) {
             ok = false;
@@ -123,23 +126,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             phase ^= 1u;
           }
         }
-        if (P.lora_list == nullptr || !ok) continue;
-        const int lora_kc = (P.lora_rank + BK - 1) / BK, extra = lora_count(P, mb, lt % P.splits) * lora_kc;
-        for (int e = 0; e < extra; ++e) {  // T_j, B_j of the tile's adapters
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 10 + stage, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const int j = e / lora_kc, c = e % lora_kc;
-          uint8_t* sa = smem + stage * S::kStageBytes;
-          mbar_arrive_expect_tx(&full_bar[stage], S::kStageBytes);
-          tma_load_2d(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * BM);
-          tma_load_2d(sa + S::kABytes, &P.tl, &full_bar[stage], c * BK, lora_id(P, mb, j) * P.lora_n + nb * BN);
-          issued[stage] = true;
-          issued_parity[stage] = phase;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+        if constexpr (LORA) {
+          int id = lora_id(P, mb, 0, extra), j = 0, c = 0;
+          for (int e = 0; ok && e < extra; ++e) {  // T_j, B_j of the tile's adapters
+            if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 10 + stage, abort_flag)) {
+              ok = false;
+              break;
+            }
+            uint8_t* sa = smem + stage * S::kStageBytes;
+            mbar_arrive_expect_tx(&full_bar[stage], S::kStageBytes);
+            tma_load_2d(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * BM);
+            tma_load_2d(sa + S::kABytes, &P.tl, &full_bar[stage], c * BK, id * P.lora_n + nb * BN);
+            if (++c * BK >= P.lora_rank) c = 0, id = lora_id(P, mb, ++j, extra - e - 1);
+            issued[stage] = true;
+            issued_parity[stage] = phase;
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
       }
@@ -167,6 +171,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         int lt, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
+        int extra = 0;
+        if constexpr (LORA) {
+          int mb, nb;
+          tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
+          extra = lora_blocks(P, mb, lt % P.splits, BK);
+        }
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 30 + stage, abort_flag)) {
             ok = false;
@@ -187,11 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             phase ^= 1u;
           }
         }
-        if (P.lora_list != nullptr && ok) {
-          int mb, nb;
-          tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
-          const int extra = lora_count(P, mb, lt % P.splits) * ((P.lora_rank + BK - 1) / BK);
-          for (int e = 0; e < extra; ++e) {
+        if constexpr (LORA) {
+          for (int e = 0; ok && e < extra; ++e) {
             if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 30 + stage, abort_flag)) {
               ok = false;
               break;
@@ -255,10 +262,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem_base, kTmemCols);
 }
 
-template <int BN, int STAGES, int EPI, bool OUT_F32>
+template <int BN, int STAGES, int EPI, bool OUT_F32, bool LORA>
 int launch_variant(const GemmGroup& g, int* err, cudaStream_t stream, int device) {
   using S = Smem<BN, STAGES>;
-  auto kern = gemm_tcgen05_kernel<BN, STAGES, EPI, OUT_F32>;
+  auto kern = gemm_tcgen05_kernel<BN, STAGES, EPI, OUT_F32, LORA>;
   static bool attr_set[16] = {false};
   if (!attr_set[device & 15]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
@@ -271,22 +278,28 @@ int launch_variant(const GemmGroup& g, int* err, cudaStream_t stream, int device
   return (int)cudaGetLastError();
 }
 
+template <int BN, int STAGES, int EPI, bool OUT_F32>
+int launch_lora(const GemmGroup& g, int* err, cudaStream_t s, int dev) {
+  return g.p[0].lora_list ? launch_variant<BN, STAGES, EPI, OUT_F32, true>(g, err, s, dev)
+                          : launch_variant<BN, STAGES, EPI, OUT_F32, false>(g, err, s, dev);
+}
+
 template <int BN, int STAGES>
 int dispatch_epi(int epi, bool out_f32, const GemmGroup& g, int* err, cudaStream_t s, int dev) {
   switch (epi) {
     case kEpiNone:
-      return out_f32 ? launch_variant<BN, STAGES, kEpiNone, true>(g, err, s, dev)
-                     : launch_variant<BN, STAGES, kEpiNone, false>(g, err, s, dev);
+      return out_f32 ? launch_lora<BN, STAGES, kEpiNone, true>(g, err, s, dev)
+                     : launch_lora<BN, STAGES, kEpiNone, false>(g, err, s, dev);
     case kEpiGelu:
-      return launch_variant<BN, STAGES, kEpiGelu, false>(g, err, s, dev);
+      return launch_lora<BN, STAGES, kEpiGelu, false>(g, err, s, dev);
     case kEpiSilu:
-      return launch_variant<BN, STAGES, kEpiSilu, false>(g, err, s, dev);
+      return launch_lora<BN, STAGES, kEpiSilu, false>(g, err, s, dev);
     case kEpiGateResid:
-      return launch_variant<BN, STAGES, kEpiGateResid, false>(g, err, s, dev);
-    case kEpiSwiGLU:
-      return launch_variant<BN, STAGES, kEpiSwiGLU, false>(g, err, s, dev);
+      return launch_lora<BN, STAGES, kEpiGateResid, false>(g, err, s, dev);
+    case kEpiSwiGLU:  // (no adapters: dfl_gemm_lora refuses them)
+      return launch_variant<BN, STAGES, kEpiSwiGLU, false, false>(g, err, s, dev);
     case kEpiQkv:
-      return launch_variant<BN, STAGES, kEpiQkv, false>(g, err, s, dev);
+      return launch_variant<BN, STAGES, kEpiQkv, false, false>(g, err, s, dev);
     default:
       return -1;
   }
@@ -439,7 +452,7 @@ extern "C" int dfl_gemm_tile_rows(const GemmArgs* a) {
   int dev = 0;
   cudaGetDevice(&dev);
   bool wide;
-  return use_pair(&a, 1, split_ws_of(a, dev).ws != nullptr, dfl_host::num_sms(dev), &wide) ? 2 * BM : BM;
+  return use_pair(&a, 1, split_ws_of(a, dev).floats > 0, dfl_host::num_sms(dev), &wide) ? 2 * BM : BM;
 }
 
 // One launch for `count` GEMMs that share the epilogue kind and output type.  The tile
@@ -459,7 +472,7 @@ extern "C" int dfl_gemm_bf16_group(const GemmArgs* const* args, int count, cudaS
   bool wide;
   const int sms = dfl_host::num_sms(dev);
   const SplitWs ws = split_ws_of(a0, dev);
-  const bool pair = use_pair(args, count, ws.ws != nullptr, sms, &wide);
+  const bool pair = use_pair(args, count, ws.floats > 0, sms, &wide);
   const int bm = pair ? 2 * BM : BM;
   const int bn = (pair || wide) ? 256 : 128;
   GemmGroup g;

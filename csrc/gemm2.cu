@@ -95,7 +95,8 @@ DFL_DEVICE void mbar_arrive_cta0(uint64_t* bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
 
-template <int EPI, bool OUT_F32, int EW>
+// LORA: the K loop goes on over the adapters of the tile (a variant of its own: the plain one is untouched).
+template <int EPI, bool OUT_F32, int EW, bool LORA>
 __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
     gemm_pair_kernel(const __grid_constant__ GemmGroup grp, int* err) {
   using C = PairCfg<EPI, EW>;
@@ -158,6 +159,8 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
+        // (read here: its latency passes behind the K loop)
+        const int extra = LORA ? lora_blocks(P, mb, lt % P.splits, BK) : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
             ok = false;
@@ -174,24 +177,25 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
             phase ^= 1u;
           }
         }
-        if (P.lora_list == nullptr || !ok) continue;
-        const int lora_kc = (P.lora_rank + BK - 1) / BK, extra = lora_count(P, mb, lt % P.splits) * lora_kc;
-        for (int e = 0; e < extra; ++e) {  // T_j, B_j of the tile's adapters
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const int j = e / lora_kc, c = e % lora_kc;
-          uint8_t* sa = smem + stage * kStageBytes;
-          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
-          tma_load_2d_pair(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * 2 * BM + (int)rank * BM);
-          tma_load_2d_pair(sa + kABytes, &P.tl, &full_bar[stage], c * BK,
-                           lora_id(P, mb, j) * P.lora_n + nb * BN + (int)rank * (BN / 2));
-          issued[stage] = true;
-          issued_parity[stage] = phase;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+        if constexpr (LORA) {
+          int id = lora_id(P, mb, 0, extra), j = 0, c = 0;
+          for (int e = 0; ok && e < extra; ++e) {  // T_j, B_j of the tile's adapters
+            if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
+              ok = false;
+              break;
+            }
+            uint8_t* sa = smem + stage * kStageBytes;
+            if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
+            tma_load_2d_pair(sa, &P.tt, &full_bar[stage], c * BK, (mb * P.lora_cap + j) * 2 * BM + (int)rank * BM);
+            tma_load_2d_pair(sa + kABytes, &P.tl, &full_bar[stage], c * BK,
+                             id * P.lora_n + nb * BN + (int)rank * (BN / 2));
+            if (++c * BK >= P.lora_rank) c = 0, id = lora_id(P, mb, ++j, extra - e - 1);
+            issued[stage] = true;
+            issued_parity[stage] = phase;
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
       }
@@ -217,6 +221,12 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         int lt, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
+        int extra = 0;
+        if constexpr (LORA) {
+          int mb, nb;
+          tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
+          extra = lora_blocks(P, mb, lt % P.splits, BK);
+        }
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
             ok = false;
@@ -235,11 +245,8 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
             phase ^= 1u;
           }
         }
-        if (P.lora_list != nullptr && ok) {
-          int mb, nb;
-          tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
-          const int extra = lora_count(P, mb, lt % P.splits) * ((P.lora_rank + BK - 1) / BK);
-          for (int e = 0; e < extra; ++e) {
+        if constexpr (LORA) {
+          for (int e = 0; ok && e < extra; ++e) {
             if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
               ok = false;
               break;
@@ -315,10 +322,10 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
 // the rest; 4 or 8 = that count for every epilogue.
 int g_epi_warps = 0;
 
-template <int EPI, bool OUT_F32, int EW>
+template <int EPI, bool OUT_F32, int EW, bool LORA>
 int launch_pair_ew(const GemmGroup& g, int* err, cudaStream_t stream, int dev) {
   using C = PairCfg<EPI, EW>;
-  auto kern = gemm_pair_kernel<EPI, OUT_F32, EW>;
+  auto kern = gemm_pair_kernel<EPI, OUT_F32, EW, LORA>;
   static bool attr[16] = {false};
   if (!attr[dev & 15]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemTotal);
@@ -352,8 +359,13 @@ int launch_pair_ew(const GemmGroup& g, int* err, cudaStream_t stream, int dev) {
 template <int EPI, bool OUT_F32>
 int launch_pair(const GemmGroup& g, int* err, cudaStream_t stream, int dev) {
   const int ew = g_epi_warps ? g_epi_warps : (EPI == kEpiQkv ? 8 : 4);
-  return ew == 8 ? launch_pair_ew<EPI, OUT_F32, 8>(g, err, stream, dev)
-                 : launch_pair_ew<EPI, OUT_F32, 4>(g, err, stream, dev);
+  if constexpr (EPI != kEpiSwiGLU && EPI != kEpiQkv) {
+    if (g.p[0].lora_list)
+      return ew == 8 ? launch_pair_ew<EPI, OUT_F32, 8, true>(g, err, stream, dev)
+                     : launch_pair_ew<EPI, OUT_F32, 4, true>(g, err, stream, dev);
+  }
+  return ew == 8 ? launch_pair_ew<EPI, OUT_F32, 8, false>(g, err, stream, dev)
+                 : launch_pair_ew<EPI, OUT_F32, 4, false>(g, err, stream, dev);
 }
 
 }  // namespace

@@ -66,17 +66,19 @@ struct alignas(64) GemmProblem {
   int lora_cap, lora_rank, lora_n;
 };
 
-// Adapters the K range `split` of M tile mb goes on with.
-DFL_DEVICE int lora_count(const GemmProblem& P, int mb, int split) {
-  return P.lora_list != nullptr && split == P.splits - 1 ? __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap)) : 0;
+// Extra K blocks (adapters x 64-column pieces of the rank) of M tile mb in K range `split`.
+DFL_DEVICE int lora_blocks(const GemmProblem& P, int mb, int split, int BK) {
+  if (P.lora_list == nullptr || split != P.splits - 1) return 0;
+  return __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap)) * ((P.lora_rank + BK - 1) / BK);
 }
 // 16-wide K steps of extra block e that hold adapter columns (the rest of its 64 columns is zero).
 DFL_DEVICE int lora_ksteps(const GemmProblem& P, int e, int BK) {
   const int c = P.lora_rank > BK ? e % (P.lora_rank / BK) : 0;
   return min(BK, P.lora_rank - c * BK) / 16;
 }
-DFL_DEVICE int lora_id(const GemmProblem& P, int mb, int j) {
-  return __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap) + 1 + j);
+// Adapter j of M tile mb (`left` blocks to go: none is read behind the list).
+DFL_DEVICE int lora_id(const GemmProblem& P, int mb, int j, int left) {
+  return left <= 0 ? 0 : __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap) + 1 + j);
 }
 
 struct alignas(64) GemmGroup {

@@ -14,35 +14,39 @@
 // The shrink is bound by reading x (2 M K bytes): a cluster of up to eight CTAs shares a tile, each
 // taking a range of K, so that few tiles still occupy many SMs; the f32 partial sums are added through
 // distributed shared memory in a fixed order.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace {
 using namespace dfl;
 
-constexpr int kBM = 128, kBK = 64, kStages = 3;
-constexpr int kCols = 128;                     // accumulator columns per pass
+constexpr int kBM = 128, kBK = 64, kMaxStages = 12;
 constexpr int kXBytes = kBM * kBK * 2;         // 16 KB
-constexpr int kABytes = kCols * kBK * 2;       // 16 KB
-constexpr int kStageBytes = kXBytes + kABytes;
-constexpr int kPartLd = kBM + 1;               // f32 partial [column][row + 1]: conflict-free both ways
-constexpr int kBar = kStages * kStageBytes;
 constexpr int kThreads = 192;
 constexpr int kMaxAdapters = 1024;
-// after the barriers: TMEM slot, abort flag, adapter bitmap, list, row slots
-constexpr int kMisc = kBar + (2 * kStages + 1) * 8;
+// Shared memory: a region for the stages (x tile, adapter rows), later for the partial sums; then
+// barriers, TMEM slot, abort flag, adapter bitmap, list (count, ids: at most 256) and the list position of every row.
+// With no more tiles than SMs one CTA per SM takes a large region (a K block arrives about 1.4 us after it was
+// asked for, so the depth sets the rate: 5120 x 4096 rank 32 takes 15 us with 64 KB in flight); else two share an SM.
+constexpr int kRegionTwo = 96 * 1024, kRegionOne = 208 * 1024;
+constexpr int kMisc = (2 * kMaxStages + 1) * 8;
 constexpr int kBitmap = (kMisc + 8 + 15) / 16 * 16;
-constexpr int kList = kBitmap + kMaxAdapters / 8;       // count, ids (at most 256)
-constexpr int kSlot = kList + 257 * 4;                  // int16 list position of every row (-1: none)
-constexpr int kTotal = (kSlot + kBM * 2 + 15) / 16 * 16 + 1024;
-static_assert(kCols * kPartLd * 4 <= kBar, "partial sums reuse the stages");
-static_assert(kTotal <= 113 * 1024, "two CTAs per SM");
+constexpr int kList = kBitmap + kMaxAdapters / 8;
+constexpr int kSlot = kList + 257 * 4;
+constexpr int kTail = (kSlot + kBM * 2 + 15) / 16 * 16 + 1024;
+static_assert(kRegionTwo + kTail <= 113 * 1024, "two CTAs per SM");
+static_assert(kRegionOne + kTail <= 232448, "one CTA per SM");
+static_assert((kBM + 7) * (128 + 4) * 4 <= kRegionTwo, "partial sums reuse the stages");
 
 struct ShrinkParams {
   const int* ids;
   int rows_per_id;
   const float* scale;
   int n_adapters, rank, cap, tile_rows;
+  int per_pass;  // adapters per pass: at most 128 accumulator columns
+  int region, stages;  // stages of kXBytes + per_pass * rank * 128 bytes
   __nv_bfloat16* t;
   int* list;
   int* sem;
@@ -63,12 +67,14 @@ DFL_DEVICE uint32_t cluster_size() {
 DFL_DEVICE void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-DFL_DEVICE float ld_cluster(const float* p, uint32_t rank) {
+DFL_DEVICE void st_cluster4(float* p, uint32_t rank, const uint32_t* v) {  // 16 bytes into CTA `rank` of the cluster
   uint32_t a;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+DFL_DEVICE void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 __global__ void __launch_bounds__(kThreads, 2)
@@ -76,14 +82,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                        int* err) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kBar);
-  uint64_t* empty_bar = full_bar + kStages;
-  uint64_t* done_bar = empty_bar + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kMisc);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + p.region);
+  uint64_t* empty_bar = full_bar + kMaxStages;
+  uint64_t* done_bar = empty_bar + kMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.region + kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + kBitmap);
-  int* list = reinterpret_cast<int*>(smem + kList);
-  int16_t* slot = reinterpret_cast<int16_t*>(smem + kSlot);
+  uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + p.region + kBitmap);
+  int* list = reinterpret_cast<int*>(smem + p.region + kList);
+  int16_t* slot = reinterpret_cast<int16_t*>(smem + p.region + kSlot);
   float* part = reinterpret_cast<float*>(smem);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -97,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int i = threadIdx.x; i < p.sem_count; i += kThreads) p.sem[i] = 0;
   if (threadIdx.x < kMaxAdapters / 32) bitmap[threadIdx.x] = 0u;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+    for (int s = 0; s < kMaxStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -106,13 +112,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     prefetch_tmap(&ta);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, kCols);
+    tmem_alloc(tmem_slot, 128);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+
+  // this CTA's K blocks; the first x tiles are on their way while the adapters are looked up
+  const int stages = p.stages, stage_bytes = kXBytes + p.per_pass * p.rank * kBK * 2;
+  const int num_k = (p.K + kBK - 1) / kBK, per = (num_k + (int)ranks - 1) / (int)ranks;
+  const int kb0 = min(num_k, (int)rank * per), kb1 = min(num_k, kb0 + per);
+  const int early = min(stages, kb1 - kb0);
+  if (warp == 0 && lane == 0)
+    for (int i = 0; i < early; ++i) {
+      mbar_expect_tx(&full_bar[i], kXBytes);
+      tma_load_2d(smem + i * stage_bytes, &tx, &full_bar[i], (kb0 + i) * kBK, (int)row0);
+    }
 
   // the adapters used by the rows of the GEMM's M tile, ascending
   auto id_of = [&](long long r) { return __ldg(p.ids + (p.rows_per_id > 0 ? r / p.rows_per_id : r)); };
@@ -150,41 +167,46 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int i = threadIdx.x; i <= count; i += kThreads) p.list[(long long)group * (1 + p.cap) + i] = i == 0 ? count : list[i];
   __syncthreads();
 
-  // this CTA's K blocks
-  const int num_k = (p.K + kBK - 1) / kBK, per = (num_k + (int)ranks - 1) / (int)ranks;
-  const int kb0 = min(num_k, (int)rank * per), kb1 = min(num_k, kb0 + per);
-  const int per_pass = kCols / p.rank;  // adapters per pass
+  if (count == 0 && warp == 0 && lane == 0)  // no adapter: the early copies must land before the CTA exits
+    for (int i = 0; i < early; ++i) {
+      mbar_arrive(&full_bar[i]);
+      mbar_wait(&full_bar[i], 0, err, kKidLora, 50 + i, abort_flag);
+    }
 
   int it = 0;  // stages used so far (all roles count alike)
-  for (int j0 = 0, pass = 0; j0 < count; j0 += per_pass, ++pass) {
-    const int nj = min(per_pass, count - j0);
+  for (int j0 = 0, pass = 0; j0 < count; j0 += p.per_pass, ++pass) {
+    const int nj = min(p.per_pass, count - j0), n = nj * p.rank;
+    const int rows_per = (kBM + (int)ranks - 1) / (int)ranks, pitch = n + 4;
     if (warp == 0) {
       if (lane == 0) {
         bool ok = true;
         int i = it;
         for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = i % kStages;
-          if (!mbar_wait(&empty_bar[s], ((i / kStages) & 1) ^ 1u, err, kKidLora, 20 + s, abort_flag)) { ok = false; break; }
-          uint8_t* sx = smem + s * kStageBytes;
-          mbar_arrive_expect_tx(&full_bar[s], kXBytes + nj * p.rank * kBK * 2);
-          tma_load_2d(sx, &tx, &full_bar[s], kb * kBK, (int)row0);
+          const int s = i % stages;
+          uint8_t* sx = smem + s * stage_bytes;
+          if (i >= early) {
+            if (!mbar_wait(&empty_bar[s], ((i / stages) & 1) ^ 1u, err, kKidLora, 20 + s, abort_flag)) { ok = false; break; }
+            mbar_expect_tx(&full_bar[s], kXBytes);
+            tma_load_2d(sx, &tx, &full_bar[s], kb * kBK, (int)row0);
+          }
+          mbar_arrive_expect_tx(&full_bar[s], n * kBK * 2);
           for (int j = 0; j < nj; ++j)
             tma_load_2d(sx + kXBytes + j * p.rank * kBK * 2, &ta, &full_bar[s], kb * kBK, list[1 + j0 + j] * p.rank);
         }
         if (!ok)  // our own copies must land before the CTA exits
-          for (int k = max(it, i - kStages); k < i; ++k)
-            mbar_wait(&full_bar[k % kStages], (k / kStages) & 1, nullptr, 0, 0, nullptr, 200000000LL);
+          for (int k = max(0, i - stages); k < i; ++k)
+            mbar_wait(&full_bar[k % stages], (k / stages) & 1, nullptr, 0, 0, nullptr, 200000000LL);
       }
     } else if (warp == 1) {
       if (lane == 0) {
-        const uint32_t idesc = make_idesc_bf16_f32(kBM, nj * p.rank);
+        const uint32_t idesc = make_idesc_bf16_f32(kBM, n);
         bool ok = true;
         int i = it;
         for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = i % kStages;
-          if (!mbar_wait(&full_bar[s], (i / kStages) & 1, err, kKidLora, 30 + s, abort_flag)) { ok = false; break; }
+          const int s = i % stages;
+          if (!mbar_wait(&full_bar[s], (i / stages) & 1, err, kKidLora, 30 + s, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t xa = smem_u32(smem + s * kStageBytes), aa = xa + kXBytes;
+          const uint32_t xa = smem_u32(smem + s * stage_bytes), aa = xa + kXBytes;
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k)
             umma_f16_ss(tmem, make_sdesc_sw128(xa + k * 32, 16, 1024), make_sdesc_sw128(aa + k * 32, 16, 1024), idesc,
@@ -193,49 +215,85 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (ok) umma_commit(done_bar);
       }
-    } else {  // one row per thread: accumulator to the partial sums
-      const int row = (warp & 3) * 32 + lane;
-      const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const bool have = kb1 > kb0 && mbar_wait(done_bar, pass & 1, err, kKidLora, 40, abort_flag);
+    }
+    // one row per thread of warps 2..5
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const long long trow0 = (long long)group * p.cap * p.tile_rows + (row0 - grow0);  // + j * tile_rows + row
+    bool have = false;
+    if (warp >= 2) {
+      have = kb1 > kb0 && mbar_wait(done_bar, pass & 1, err, kKidLora, 40, abort_flag);
       tc_fence_after();
+    }
+    __syncwarp();
+    if (ranks == 1) {
+      if (warp >= 2) {
 #pragma unroll 1
-      for (int c = 0; c < nj * p.rank; c += 16) {
-        uint32_t v[16];
-        if (have) {
+        for (int c = 0; c < n; c += 16) {
+          const int j = j0 + c / p.rank;
+          uint32_t v[16];
           tmem_ld_32x32b_x16(t_row + c, v);
           tmem_wait_ld();
-        }
+          const float f = __ldg(p.scale + list[1 + j]);
+          const bool mine = have && slot[row] == j;
+          uint32_t w[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) part[(c + e) * kPartLd + row] = have ? __uint_as_float(v[e]) : 0.f;
+          for (int e = 0; e < 8; ++e)
+            w[e] = mine ? pack_bf16x2(f * __uint_as_float(v[2 * e]), f * __uint_as_float(v[2 * e + 1])) : 0u;
+          uint4* dst = reinterpret_cast<uint4*>(p.t + (trow0 + (long long)j * p.tile_rows + row) * p.rank + c % p.rank);
+          dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+        tc_fence_before();
       }
-      tc_fence_before();
+    } else {
+      __syncthreads();
+      cluster_sync();  // every CTA is through with its stages: they take the partial sums
+      if (warp >= 2) {
+        // row -> the CTA that joins it: [source rank][row of the owner][column]
+        const uint32_t owner = row / rows_per;
+        float* dst = part + ((int)rank * rows_per + row % rows_per) * pitch;
+#pragma unroll 1
+        for (int c = 0; c < n; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(t_row + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = have ? v[e] : 0u;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) st_cluster4(dst + c + 4 * q, owner, v + 4 * q);
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      cluster_sync();  // the partial sums of this CTA's rows have arrived
+      const int r0 = (int)rank * rows_per, rows = min(rows_per, kBM - r0), half = n / 2;
+      for (int e = threadIdx.x; e < rows * half; e += kThreads) {
+        const int rl = e / half, c = 2 * (e % half), j = j0 + c / p.rank;
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < (int)ranks) {  // in rank order
+            const float2 f = *reinterpret_cast<const float2*>(part + (k * rows_per + rl) * pitch + c);
+            x += f.x, y += f.y;
+          }
+        const bool mine = slot[r0 + rl] == j;
+        const float f = __ldg(p.scale + list[1 + j]);
+        *reinterpret_cast<uint32_t*>(p.t + (trow0 + (long long)j * p.tile_rows + r0 + rl) * p.rank + c % p.rank) =
+            mine ? pack_bf16x2(f * x, f * y) : 0u;
+      }
     }
     it += kb1 - kb0;
-    __syncwarp();
-    __syncthreads();
-    cluster_sync();  // every CTA's partial sums are in place
-    // rows [r0, r1) of this CTA: sums over the cluster in rank order, scaled, masked, stored
-    const int rows = kBM / (int)ranks, r0 = (int)rank * rows, n = nj * p.rank;
-    for (int e = threadIdx.x; e < rows * n; e += kThreads) {
-      const int row = r0 + e / n, c = e % n;
-      const int j = j0 + c / p.rank;
-      float v = 0.f;
-      if (slot[row] == j) {
-        for (uint32_t k = 0; k < ranks; ++k) v += ld_cluster(&part[c * kPartLd + row], k);
-        v *= __ldg(p.scale + list[1 + j]);
-      }
-      const long long trow = ((long long)group * p.cap + j) * p.tile_rows + (row0 - grow0) + row;
-      p.t[trow * p.rank + c % p.rank] = __float2bfloat16_rn(v);
-    }
-    cluster_sync();  // the partial sums have been read: the stages may be written again
     fence_proxy_async_shared();  // generic accesses to the stages before the next pass's copies
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, kCols);
+  if (warp == 1) tmem_dealloc(tmem, 128);
 }
 
 // ---------------------------------------------------------------------------
@@ -468,11 +526,31 @@ extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
     return -26;
   int dev = 0;
   cudaGetDevice(&dev);
-  static bool attr[16] = {false};
-  if (!attr[dev & 15]) {
-    cudaError_t e = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTotal);
+  // clusters of 1..8 CTAs, one CTA per SM, that are resident at once (a cluster stays inside one GPC)
+  static int resident[16][9] = {{0}};
+  int* fit = resident[dev & 15];
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (!fit[1]) {
+    cudaError_t e = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRegionOne + kTail);
     if (e != cudaSuccess) return (int)e;
-    attr[dev & 15] = true;
+    int found[9] = {0};
+    for (int c = 2; c <= 8; ++c) {
+      at[0].val.clusterDim.x = c;
+      cfg.gridDim = dim3((unsigned)(c * 1024), 1, 1);
+      cfg.dynamicSmemBytes = kRegionOne + kTail;
+      e = cudaOccupancyMaxActiveClusters(&found[c], lora_shrink_kernel, &cfg);
+      if (e != cudaSuccess) return (int)e;
+    }
+    for (int c = 2; c <= 8; ++c) fit[c] = found[c];
+    fit[1] = dfl_host::num_sms(dev);
   }
   CUtensorMap tx, ta;
   int rc = dfl_host::make_tmap_2d_bf16(&tx, a->A, a->K, a->M, a->lda, kBK, kBM, true);
@@ -493,23 +571,18 @@ extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
   p.sem_count = l->split_sem ? l->split_sem_count : 0;
   p.M = a->M;
   p.K = a->K;
+  p.per_pass = std::max(1, std::min(l->cap, 128 / l->rank));
   // every 128-row tile of every M tile (the last M tile's second half may lie behind M: zeros)
   const long long tiles = ((long long)a->M + l->tile_rows - 1) / l->tile_rows * (l->tile_rows / kBM);
-  const int num_k = (a->K + kBK - 1) / kBK, room = 2 * dfl_host::num_sms(dev);
-  int ranks = 1;
-  while (ranks < 8 && tiles * ranks * 2 <= room && num_k >= ranks * 2 * 4) ranks *= 2;
-  cudaLaunchConfig_t cfg = {};
+  const int num_k = (a->K + kBK - 1) / kBK;
+  int ranks = 1;  // the most CTAs a tile that are all resident, each with four K blocks or more
+  for (int c = 2; c <= 8; ++c)
+    if (tiles <= fit[c] && num_k >= 4 * c) ranks = c;
+  p.region = tiles * ranks <= fit[1] ? kRegionOne : kRegionTwo;
+  p.stages = std::min(kMaxStages, p.region / (kXBytes + p.per_pass * l->rank * kBK * 2));
   cfg.gridDim = dim3((unsigned)(tiles * ranks), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = kTotal;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
+  cfg.dynamicSmemBytes = p.region + kTail;
   at[0].val.clusterDim.x = ranks;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, lora_shrink_kernel, tx, ta, p, a->err);
   if (e != cudaSuccess) return (int)e;
   return dfl_gemm_bf16(a, stream);

@@ -125,13 +125,16 @@ def _oracle_masked(q, k, v, scale, causal, mask, lse=None):
     return torch.einsum("bhqk,bhkd->bhqd", p, v.to(ct)).to(q.dtype)
 
 
+_MASK_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
 def _mask_on(mask, q):
     """A mask on q's device whose type the kernel reads (integers: non-zero = attend, as a boolean)."""
     if mask is None:
         return None
     if not mask.is_floating_point():
         mask = mask.bool()
-    elif mask.dtype not in (torch.bfloat16, torch.float16, torch.float32) and q.is_cuda:
+    elif mask.dtype not in _MASK_DTYPES and q.is_cuda:
         mask = mask.float()
     return mask.to(q.device)
 
@@ -145,9 +148,14 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
     ``attention``.  A query that no key is left for gives 0.  ``out`` (like q) and ``lse`` (f32 ``[B, H, Sq]``, natural
     log) are filled when given.  CUDA: bf16 and fp16 with head dim 64 or 128; anything else runs as ``attention``."""
+    F._no_grad("cross_attention", q, k, v, attention_mask)
+    if (q.dim() == 4 and bound_min is None and bound_max is None and F.cross_kernel_ok(q)
+            and (attention_mask is None or attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)):
+        # the binding checks shapes, types and devices (ValueError)
+        return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
+                                 out=out, lse=lse)
     for key in ("tp_q", "tp_k", "tp_out", "causal"):
         kwargs.pop(key, None)
-    F._no_grad("cross_attention", q, k, v, attention_mask)
     if q.dim() == 3:
         if kv_lens is not None or out is not None:
             raise ValueError("kv_lens and out need q [B, H, S, D]")

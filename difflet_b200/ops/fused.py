@@ -224,23 +224,15 @@ def ln_modulate(x, *, shift=None, scale=None, w=None, b=None, eps=1e-6, rms=Fals
 
 def linear_lora(x, w, b, bank, ids, rows_per_id=0, *, act=None, act_lo=0, act_hi=None, gate=None, resid=None,
                 gate_rows_per_batch=0, out=None, out_f32=False):
-    """``linear`` with the adapters of ``bank`` (``ops.lora.LoraBank``) beside the weight: rows [M, K], ``ids``
-    per row or per ``rows_per_id`` rows.  Arguments are checked by ``ops.linear_lora``."""
+    """``linear`` with the adapters of ``bank`` (``ops.lora.LoraBank``) beside the weight: x [..., K] (CPU: rows [M, K],
+    checked by ``ops.linear_lora``), ``ids`` per row or per ``rows_per_id`` rows."""
     N = w.shape[0]
+    if x.is_cuda:
+        epi = EPI_GATE_RESID if gate is not None else _ACT[act]
+        return _kernels().gemm_lora(x, w, b, out, epi, act_lo, N if act_hi is None else act_hi, gate, gate_rows_per_batch,
+                                    resid, out_f32, bank.A, bank.B, bank.scale, ids, rows_per_id)
     act_hi = N if act_hi is None else act_hi
     M = x.shape[0]
-    if x.is_cuda:
-        if x.dtype != torch.bfloat16:
-            raise ValueError(f"linear_lora runs in bfloat16 on CUDA, got {x.dtype}")
-        if M == 0:
-            return x.new_empty(0, N, dtype=torch.float32 if out_f32 else x.dtype) if out is None else out
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-            x = x.contiguous()
-        epi = EPI_GATE_RESID if gate is not None else _ACT[act]
-        if ids.dtype != torch.int32:
-            ids = ids.clamp(-2, 1 << 30).to(torch.int32)  # what no adapter has stays without one
-        return _kernels().gemm_lora(x, w, b, out, epi, act_lo, act_hi, gate, gate_rows_per_batch, resid, out_f32, bank.A,
-                                  bank.B, bank.scale, ids.contiguous(), rows_per_id)
     ct = torch.float64 if x.dtype == torch.float64 else torch.float32
     rows = ids.long() if rows_per_id <= 0 else ids.long().repeat_interleave(rows_per_id)[:M]
     xc = x.to(ct)
@@ -264,13 +256,14 @@ def linear_lora(x, w, b, bank, ids, rows_per_id=0, *, act=None, act_lo=0, act_hi
 
 def _no_grad(name: str, *tensors) -> None:
     """The kernels record no backward pass: refuse inputs whose gradient would be lost silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
 
 
 # MX element type -> (code of the native kernels, emax of the format, largest finite value)
 MX_CODES = {"float8_e4m3fn": 1, "float8_e5m2": 2, "float8_e4m3fn_x4": 1, "float8_e5m2_x4": 2}
-_NORM_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def add_rms_norm(x, resid=None, weight=None, *, eps=1e-6, scale=None, shift=None, rows_per_batch=0, row_map=None,
@@ -285,52 +278,44 @@ def add_rms_norm(x, resid=None, weight=None, *, eps=1e-6, scale=None, shift=None
     ``out`` / ``resid_out`` receive y / s and may be x / resid.  The statistics use the unrounded sum.
     """
     _no_grad("add_rms_norm", x, resid, weight, scale, shift)
-    D = x.shape[-1] if x.dim() else 0
-    if x.dim() < 1 or not 1 <= D <= 16384:
-        raise ValueError(f"add_rms_norm needs [..., D] with 1 <= D <= 16384, got {tuple(x.shape)}")
+    code = 0
     if quantize is not None:
-        if quantize not in MX_CODES:
+        code = MX_CODES.get(quantize, 0)
+        if not code:
             raise NotImplementedError(f"MX element type {quantize!r}: one of {sorted(MX_CODES)}")
+    if x.is_cuda:  # the binding checks shapes, types and strides (ValueError)
+        y, s, sf = _kernels().add_rms_norm(x, resid, weight, scale, shift, rows_per_batch, row_map, eps, code, blocked, out,
+                                           resid_out)
+        return ((y, sf) if code else y), (x if resid is None else s)
+    D = x.shape[-1] if x.dim() else 0
+    if not 1 <= D <= 16384:
+        raise ValueError(f"add_rms_norm needs [..., D] with 1 <= D <= 16384, got {tuple(x.shape)}")
+    if code:
         if D % (128 if blocked else 32):
             raise ValueError(f"the MX output needs D to be a multiple of {128 if blocked else 32}, got {D}")
         if out is not None:
             raise ValueError("out= and quantize= are mutually exclusive")
     elif blocked:
         raise ValueError("blocked scales need quantize=")
-    if resid is None:
-        if resid_out is not None:
-            raise ValueError("resid_out needs resid")
-    elif resid.shape != x.shape or resid.dtype != x.dtype or resid.device != x.device:
-        raise ValueError(f"resid {tuple(resid.shape)} {resid.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    for name, t in (("out", out), ("resid_out", resid_out)):
+    if resid is None and resid_out is not None:
+        raise ValueError("resid_out needs resid")
+    for name, t in (("resid", resid), ("out", out), ("resid_out", resid_out)):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
             raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    if weight is not None and (weight.shape != (D,) or weight.device != x.device or weight.dtype not in (x.dtype, torch.float32)):
+    if weight is not None and (weight.shape != (D,) or weight.device != x.device
+                               or weight.dtype not in (x.dtype, torch.float32)):
         raise ValueError(f"weight must be [{D}] of {x.dtype} or float32 on {x.device}")
-    for name, t in (("scale", scale), ("shift", shift)):
-        if t is not None and (t.dim() != 2 or t.shape[1] != D or t.device != x.device):
-            raise ValueError(f"{name} must be [B, {D}] on {x.device}, got {tuple(t.shape)}")
     x2 = _rows2d(x)
     M = x2.shape[0]
+    for name, t in (("scale", scale), ("shift", shift)):
+        if t is not None and (t.dim() != 2 or t.shape[1] != D or t.device != x.device or t.shape[0] < 1):
+            raise ValueError(f"{name} must be [B, {D}] on {x.device}, got {tuple(t.shape)}")
+        if t is not None and row_map is None and t.shape[0] * (rows_per_batch or M) < M:
+            raise ValueError(f"{name} has {t.shape[0]} rows: too few for {M} rows of {rows_per_batch} per batch")
+    if scale is not None and shift is not None and scale.shape[0] != shift.shape[0]:
+        raise ValueError("scale and shift differ in their batch rows")
     if row_map is not None and (row_map.dtype != torch.int32 or row_map.numel() != M):
         raise ValueError(f"row_map must be int32 [{M}]")
-    if x.is_cuda:
-        if x.dtype not in _NORM_DTYPES:
-            raise ValueError(f"add_rms_norm runs in bfloat16, float16 or float32, got {x.dtype}")
-        y2 = s2 = None
-        if out is not None:
-            y2 = out if out.dim() == 2 else out.view(M, D)  # a view: the caller's tensor is written
-        if resid_out is not None:
-            s2 = resid_out if resid_out.dim() == 2 else resid_out.view(M, D)
-        y, s, sf = _kernels().add_rms_norm(x2, None if resid is None else _rows2d(resid), weight, scale, shift,
-                                         rows_per_batch, row_map, eps, MX_CODES.get(quantize, 0), blocked, y2, s2)
-        if x.dim() != 2:
-            y = out if out is not None else y.view(x.shape)
-            s = None if resid is None else (resid_out if resid_out is not None else s.view(x.shape))
-            if sf is not None and not blocked:
-                sf = sf.view(*x.shape[:-1], D // 32)
-        s = x if resid is None else s
-        return ((y, sf) if quantize is not None else y), s
     ct = torch.float64 if x.dtype == torch.float64 else torch.float32
     s = x2.to(ct) if resid is None else x2.to(ct) + _rows2d(resid).to(ct)
     y = s * torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + eps)

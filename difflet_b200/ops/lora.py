@@ -94,19 +94,23 @@ def linear_lora(x, w, b=None, *, bank: LoraBank, ids, rows_per_batch: int = 0, a
     number outside the bank, which also sets the device error word) means none.  ``gate`` f32 [B, N] with
     ``gate_rows_per_batch`` rows each (0: ``rows_per_batch``, else all).  The rank-r
     intermediate is rounded to x's type once; everything is accumulated in f32 and rounded at the end."""
-    F._no_grad("linear_lora", x, b, bank.A, bank.B, gate, resid)
+    F._no_grad("linear_lora", x, b, gate, resid)
+    if act not in (None, "none", "gelu", "gelu_tanh", "silu"):
+        raise ValueError(f"act {act!r}: linear_lora has none, gelu and silu")
+    if gate is not None and act not in (None, "none"):
+        raise ValueError("act and gate are mutually exclusive")
+    rpb = gate_rows_per_batch or rows_per_batch
+    if x.is_cuda and not isinstance(w, F.MXWeight):  # the binding checks shapes, types and devices (ValueError)
+        return F.linear_lora(x, w, b, bank, ids, rows_per_batch, act=act, act_lo=act_lo, act_hi=act_hi, gate=gate,
+                             resid=resid, gate_rows_per_batch=rpb, out=out, out_f32=out_f32)
     if x.dim() < 1 or x.shape[-1] != bank.in_features:
         raise ValueError(f"x {tuple(x.shape)} does not end in the bank's {bank.in_features} inputs")
     if tuple(w.shape) != (bank.out_features, bank.in_features):
         raise ValueError(f"weight {tuple(w.shape)} is not [{bank.out_features}, {bank.in_features}]")
     if bank.device != x.device or w.device != x.device or ids.device != x.device:
         raise ValueError("x, weight, bank and ids must be on one device")
-    if act not in (None, "none", "gelu", "gelu_tanh", "silu"):
-        raise ValueError(f"act {act!r}: linear_lora has none, gelu and silu")
     if (gate is None) != (resid is None):
         raise ValueError("gate and resid come together")
-    if gate is not None and act not in (None, "none"):
-        raise ValueError("act and gate are mutually exclusive")
     x2 = F._rows2d(x)
     M, N = x2.shape[0], bank.out_features
     if ids.is_floating_point() or ids.dim() != 1:
@@ -127,7 +131,6 @@ def linear_lora(x, w, b=None, *, bank: LoraBank, ids, rows_per_batch: int = 0, a
         if out.shape != (*x.shape[:-1], N):
             raise ValueError(f"out must be {(*x.shape[:-1], N)}, got {tuple(out.shape)}")
         out2 = out if out.dim() == 2 else out.view(M, N)
-    rpb = gate_rows_per_batch or rows_per_batch
     y = F.linear_lora(x2, w, b, bank, ids, rows_per_batch, act=act, act_lo=act_lo, act_hi=act_hi, gate=gate, resid=res2,
                       gate_rows_per_batch=rpb, out=out2, out_f32=out_f32)
     return out if out is not None else (y if x.dim() == 2 else y.view(*x.shape[:-1], N))

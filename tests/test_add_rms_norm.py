@@ -99,6 +99,29 @@ def test_kernel(native, M, D, batch, dtype):
 
 
 @pytest.mark.gpu
+def test_kernel_refusals(native):
+    x = torch.randn(4, 96, device="cuda")
+    c = lambda *s, **kw: torch.zeros(*s, device="cuda", **kw)  # noqa: E731
+    for kw in (dict(resid=c(4, 95)), dict(resid=c(4, 96).half()), dict(resid=torch.zeros(4, 96)), dict(weight=c(95)), dict(weight=c(96).half()),
+               dict(scale=c(96)), dict(shift=c(2, 95)), dict(shift=c(2, 96).half()), dict(scale=c(2, 96), rows_per_batch=1),
+               dict(scale=c(2, 96), shift=c(1, 96)), dict(resid_out=c(4, 96)), dict(out=c(4, 95)), dict(blocked=True),
+               dict(quantize="float8_e4m3fn", blocked=True), dict(quantize="float8_e4m3fn", out=c(4, 96)),
+               dict(row_map=c(3, dtype=torch.int32)), dict(row_map=c(4, dtype=torch.int64)), dict(weight=c(192)[::2])):
+        with pytest.raises(ValueError):
+            ops.add_rms_norm(x, **kw)
+    for bad in (c(2, 16385), x.t(), x.double(), x.int()):
+        with pytest.raises(ValueError):
+            ops.add_rms_norm(bad)
+    for bad in (c(2, 33), c(2, 65)[:, 1:]):
+        with pytest.raises(ValueError):
+            ops.add_rms_norm(bad, quantize="float8_e4m3fn")
+    with pytest.raises(NotImplementedError):
+        ops.add_rms_norm(x, quantize="int8")
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.add_rms_norm(x.clone().requires_grad_())
+
+
+@pytest.mark.gpu
 def test_kernel_strided_aliased_mapped(native):
     big = torch.randn(40, 2, 1032, device="cuda").bfloat16()
     for off in (0, 8, 3):  # aligned and odd starts of strided rows

@@ -173,6 +173,22 @@ def test_kernel_ignores_masked_contents(native, kind, D):
 
 
 @pytest.mark.gpu
+def test_kernel_refusals(native):
+    q, k, v = _inputs(2, 4, 2, 3, 5, 64, torch.bfloat16, "cuda")
+    lens = torch.tensor([5, 2], device="cuda")
+    ones = lambda *s: torch.ones(*s, device="cuda", dtype=torch.bool)  # noqa: E731
+    for args, kw in (((q, k, v[:, :, :4]), {}), ((q[:, :3], k, v), {}), ((q, k[:1], v[:1]), {}), ((q, k.half(), v.half()), {}),
+                     ((q, k.cpu(), v.cpu()), {}), ((q, k, v), dict(kv_lens=lens.float())), ((q, k, v), dict(kv_lens=lens[:1])),
+                     ((q, k, v), dict(kv_lens=lens, bound_min=lens, bound_max=lens)), ((q, k, v), dict(bound_min=lens)),
+                     ((q, k, v), dict(attention_mask=ones(2, 4, 3, 4))), ((q, k, v), dict(attention_mask=ones(3, 1, 1, 5))),
+                     ((q, k, v), dict(attention_mask=ones(1, 2, 4, 3, 5))), ((q, k, v), dict(attention_mask=ones(5).cpu())),
+                     ((q, k, v), dict(out=q[:1])), ((q, k, v), dict(out=q.half())),
+                     ((q, k, v), dict(lse=torch.empty(2, 4, 2, device="cuda"))), ((q[0], k[0], v[0]), dict(kv_lens=lens))):
+        with pytest.raises(ValueError):
+            ops.cross_attention(*args, **kw)
+
+
+@pytest.mark.gpu
 def test_kernel_layouts(native):
     B, H, Sq, Sk, D = 2, 6, 200, 300, 64
     q, k, v = _inputs(B, H, H, Sq, Sk, D, torch.bfloat16, "cuda")

@@ -172,6 +172,26 @@ def test_kernel_gated_residual_layouts(native):
 
 
 @pytest.mark.gpu
+def test_kernel_refusals(native):
+    x, w, b, A, B, scale = _make(6, 24, 32, [4, 4], "cuda")
+    bank = ops.LoraBank(A, B, scale)
+    ids = torch.zeros(6, dtype=torch.long, device="cuda")
+    c = lambda *s, **kw: torch.ones(*s, device="cuda", **kw)  # noqa: E731
+    for a, kw in (((x[:, :16], w, b), {}), ((x, w[:16], b), {}), ((x.float(), w, b), {}), ((x, w.float(), b), {}), ((x, w.cpu(), b), {}),
+                  ((x, w, b[:16]), {}), ((x, w, b.float()), {}), ((x, w, b), dict(ids=ids[:5])), ((x, w, b), dict(ids=ids.float())),
+                  ((x, w, b), dict(ids=ids.cpu())), ((x, w, b), dict(ids=ids[:1], rows_per_batch=4)), ((x, w, b), dict(act="swiglu")),
+                  ((x, w, b), dict(gate=c(1, 24))), ((x, w, b), dict(resid=c(6, 24, dtype=BF))),
+                  ((x, w, b), dict(gate=c(1, 24), resid=c(6, 24, dtype=BF), gate_rows_per_batch=2)),
+                  ((x, w, b), dict(gate=c(1, 24), resid=c(6, 24))), ((x, w, b), dict(act="gelu", gate=c(1, 24), resid=c(6, 24, dtype=BF))),
+                  ((x, w, b), dict(out=c(6, 23, dtype=BF))), ((x, w, b), dict(out=c(6, 24))), ((x, w, b), dict(out=c(6, 25, dtype=BF)[:, 1:]))):
+        with pytest.raises(ValueError):
+            ops.linear_lora(*a, bank=bank, **{"ids": ids, **kw})
+    odd = ops.LoraBank([a[:, :30] for a in A], B, scale)  # rows that are no whole 16-byte pieces
+    with pytest.raises(ValueError):
+        ops.linear_lora(x[:, :30], w[:, :30], b, bank=odd, ids=ids)
+
+
+@pytest.mark.gpu
 def test_kernel_rows_do_not_see_each_other(native):
     """A row's result does not depend on which adapters its neighbours use."""
     M, N, K = 512, 1024, 256
