@@ -9,7 +9,10 @@
 // registers.  The norm uses the unrounded sum, and y is rounded once: to the output type, or
 // (MX) straight from f32 to FP8.
 //
-// Bound by HBM: 8 bytes per value in bf16 (x, resid, s, y), 7.03 with the FP8 output.
+// Bound by HBM: 8 bytes per value in bf16 (x, resid, s, y), 7.03 with the FP8 output.  At 32760 x 5120 bf16 takes
+// 200 us (6.7 TB/s; a plain copy reaches 6.5), with adaLN modulation into MXFP8 206 us (5.7 TB/s: two words of
+// scales per 128 columns and 40 KB of modulation a row through L1).  Measured and slower: a register cap for six
+// or more blocks per SM, no-allocate loads, a persistent form fed by bulk copies.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -77,15 +80,6 @@ struct Io<__half> {
   }
 };
 
-// Rows are read once: no L1 allocation, so that the weight and modulation rows stay there.
-DFL_DEVICE uint4 ld_stream16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-
 DFL_DEVICE uint32_t fp8x4(const float* v, float inv, int e5m2) {
   const __nv_fp8_interpretation_t k = e5m2 ? __NV_E5M2 : __NV_E4M3;
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, k);
@@ -97,7 +91,7 @@ DFL_DEVICE uint32_t fp8x4(const float* v, float inv, int e5m2) {
 // contiguous bytes (D a multiple of E, 16-byte aligned rows); otherwise the group's values lie NT
 // apart, which keeps single-value accesses coalesced for odd widths, strides and addresses.
 template <typename T, int NT, int VPT, bool VEC>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT == 128 && VEC ? 6 : 1) add_rms_norm_kernel(AddNormArgs a) {
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(AddNormArgs a) {
   constexpr int E = Io<T>::E;
   constexpr int kRows = NT < 128 ? 128 / NT : 1;  // rows per block
   constexpr int kWarps = NT / 32;
@@ -123,8 +117,8 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT == 128 && VEC ? 6 : 1)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const bool in = col(i, 0) < a.D;
-      px[i] = in ? ld_stream16(x + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
-      pr[i] = in && rs ? ld_stream16(rs + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
+      px[i] = in ? *reinterpret_cast<const uint4*>(x + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
+      pr[i] = in && rs ? *reinterpret_cast<const uint4*>(rs + col(i, 0)) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {

@@ -225,12 +225,12 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
     TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 && t->dim() == 1 && t->numel() == N && t->is_contiguous() &&
                           t->device() == x.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                       "bias must be contiguous bfloat16 [", N, "], 16-byte aligned");
+  TORCH_CHECK_VALUE(!out_f32 || epi == kEpiNone, "out_f32 comes without act and gate");
   TORCH_CHECK_VALUE(bool(given(gate)) == bool(given(resid_in)) && bool(given(gate)) == (epi == kEpiGateResid),
                     "gate and resid come together, without act");
   if (const at::Tensor* t = given(resid_in)) {
     TORCH_CHECK_VALUE(t->sizes() == at::IntArrayRef(shape) && t->scalar_type() == at::kBFloat16 && t->device() == x.device(),
                       "resid must be bfloat16 ", at::IntArrayRef(shape));
-    TORCH_CHECK_VALUE(!out_f32, "the gated residual is stored in bfloat16");
     resid = t->dim() == 2 ? *t : t->reshape({M, N});
     const int64_t rpb = rows_per_batch > 0 ? rows_per_batch : M;
     TORCH_CHECK_VALUE(gate->scalar_type() == at::kFloat && gate->dim() == 2 && gate->stride(1) == 1 && gate->size(1) >= N &&

@@ -280,7 +280,8 @@ int launch_variant(const GemmGroup& g, int* err, cudaStream_t stream, int device
 
 template <int BN, int STAGES, int EPI, bool OUT_F32>
 int launch_lora(const GemmGroup& g, int* err, cudaStream_t s, int dev) {
-  return g.p[0].lora_list ? launch_variant<BN, STAGES, EPI, OUT_F32, true>(g, err, s, dev)
+  constexpr int LEPI = EPI == kEpiSilu ? kEpiSiluQuick : EPI;
+  return g.p[0].lora_list ? launch_variant<BN, STAGES, LEPI, OUT_F32, true>(g, err, s, dev)
                           : launch_variant<BN, STAGES, EPI, OUT_F32, false>(g, err, s, dev);
 }
 

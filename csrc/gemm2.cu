@@ -360,9 +360,13 @@ template <int EPI, bool OUT_F32>
 int launch_pair(const GemmGroup& g, int* err, cudaStream_t stream, int dev) {
   const int ew = g_epi_warps ? g_epi_warps : (EPI == kEpiQkv ? 8 : 4);
   if constexpr (EPI != kEpiSwiGLU && EPI != kEpiQkv) {
+    // Adapters: eight epilogue warps where the K loop is too short to hide four (4372 x 7296, GELU: K 576 77 -> 59 us,
+    // 1024 83 -> 68, 1536 92 -> 87, 2304 118 -> 119) and no K range is split (its fixup wants four).
+    constexpr int LEPI = EPI == kEpiSilu ? kEpiSiluQuick : EPI;
     if (g.p[0].lora_list)
-      return ew == 8 ? launch_pair_ew<EPI, OUT_F32, 8, true>(g, err, stream, dev)
-                     : launch_pair_ew<EPI, OUT_F32, 4, true>(g, err, stream, dev);
+      return ew == 8 || (g_epi_warps == 0 && g.p[0].splits == 1 && g.p[0].K <= 1536)
+                 ? launch_pair_ew<LEPI, OUT_F32, 8, true>(g, err, stream, dev)
+                 : launch_pair_ew<LEPI, OUT_F32, 4, true>(g, err, stream, dev);
   }
   return ew == 8 ? launch_pair_ew<EPI, OUT_F32, 8, false>(g, err, stream, dev)
                  : launch_pair_ew<EPI, OUT_F32, 4, false>(g, err, stream, dev);

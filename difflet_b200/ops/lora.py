@@ -99,6 +99,8 @@ def linear_lora(x, w, b=None, *, bank: LoraBank, ids, rows_per_batch: int = 0, a
         raise ValueError(f"act {act!r}: linear_lora has none, gelu and silu")
     if gate is not None and act not in (None, "none"):
         raise ValueError("act and gate are mutually exclusive")
+    if out_f32 and (gate is not None or act not in (None, "none")):
+        raise ValueError("out_f32 comes without act and gate")
     rpb = gate_rows_per_batch or rows_per_batch
     if x.is_cuda and not isinstance(w, F.MXWeight):  # the binding checks shapes, types and devices (ValueError)
         return F.linear_lora(x, w, b, bank, ids, rows_per_batch, act=act, act_lo=act_lo, act_hi=act_hi, gate=gate,

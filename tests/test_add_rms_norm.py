@@ -99,6 +99,29 @@ def test_kernel(native, M, D, batch, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,D,batch,dtype,fmt", [(9601, 1032, 3, torch.bfloat16, None), (2501, 4096, 2, torch.float32, None),
+                                                 (2400, 8192, 0, torch.float16, None), (9700, 1024, 1, torch.bfloat16, "float8_e4m3fn"),
+                                                 (2431, 5120, 7, torch.bfloat16, "float8_e5m2"), (5000, 2048, 2, torch.float32, "float8_e4m3fn")])
+def test_kernel_many_rows(native, M, D, batch, dtype, fmt):
+    x, resid, w, scale, shift = _inputs(M, D, dtype, "cuda", M, max(batch, 1))
+    m = torch.randint(0, max(batch, 1), (M,), device="cuda", dtype=torch.int32)
+    kw = dict(eps=1e-5, scale=scale, shift=shift, row_map=m) if batch else dict(eps=1e-5)
+    rs, ry, size = _ref(x, resid, w, 1e-5, scale if batch else None, shift if batch else None, m.long())
+    y, s = ops.add_rms_norm(x, resid, w, quantize=fmt, **kw)
+    _check(s, rs, x.double().abs() + resid.double().abs(), dtype)
+    if fmt is None:
+        _check(y, ry, size, dtype)
+        _check(ops.add_rms_norm(x, None, w, eps=1e-5)[0], *_ref(x, None, w, 1e-5, None, None, None)[1:], dtype)
+        a, b = x.clone(), resid.clone()
+        ops.add_rms_norm(a, b, w, out=a, resid_out=b, **kw)
+        assert torch.equal(a, y) and torch.equal(b, s)
+    else:
+        _check_mx(*y, ry, size, *((8, 448.0, 3, -6) if fmt == "float8_e4m3fn" else (15, 57344.0, 2, -14)))
+        (qb, sb), _ = ops.add_rms_norm(x, resid, w, quantize=fmt, blocked=True, **kw)
+        assert torch.equal(qb.view(torch.uint8), y[0].view(torch.uint8)) and torch.equal(sb, F.block_scales(y[1]))
+
+
+@pytest.mark.gpu
 def test_kernel_refusals(native):
     x = torch.randn(4, 96, device="cuda")
     c = lambda *s, **kw: torch.zeros(*s, device="cuda", **kw)  # noqa: E731

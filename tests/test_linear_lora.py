@@ -96,7 +96,7 @@ def test_refusals():
                   ((x, w, b), dict(ids=ids[:1], rows_per_batch=4)), ((x, w, b), dict(act="swiglu")),
                   ((x, w, b), dict(gate=torch.ones(1, 24))), ((x, w, b), dict(resid=torch.ones(6, 24))),
                   ((x, w, b), dict(act="gelu", gate=torch.ones(1, 24), resid=torch.ones(6, 24))),
-                  ((x, w, b), dict(out=torch.empty(6, 23))), ((x.double(), w.double(), b.double()), {})):
+                  ((x, w, b), dict(act="gelu", out_f32=True)), ((x, w, b), dict(out=torch.empty(6, 23))), ((x.double(), w.double(), b.double()), {})):
         with pytest.raises(ValueError):
             ops.linear_lora(*a, bank=bank, **{"ids": ids, **kw})
     with pytest.raises(RuntimeError, match="no backward"):
