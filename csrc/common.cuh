@@ -180,6 +180,11 @@ DFL_DEVICE void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// Programmatic launch: let the next kernel of the stream start / wait until the previous one is complete (nothing
+// to wait for in a launch without the attribute).
+DFL_DEVICE void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+DFL_DEVICE void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // D[tmem] (+)= A[smem] * B[smem]^T, kind::f16 (bf16 or f16 inputs, same type for A and B).
 DFL_DEVICE void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                             uint32_t accumulate) {

@@ -101,14 +101,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t issued_parity[STAGES];
       bool issued[STAGES];
       for (int s = 0; s < STAGES; ++s) issued[s] = false, issued_parity[s] = 0;
-      bool ok = true;
+      bool ok = true, listed = false;  // listed: the adapter lists are complete
       for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
         int lt, mb, nb, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        // (read here: its latency passes behind the K loop)
-        const int extra = LORA ? lora_blocks(P, mb, lt % P.splits, BK) : 0;
+        // the tile's list is read here, its latency passes behind the K loop; before the first one is complete, after it
+        int extra = LORA && listed ? lora_blocks(P, mb, lt % P.splits, BK) : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 10 + stage, abort_flag)) {
             ok = false;
@@ -127,6 +127,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if constexpr (LORA) {
+          if (!listed) {
+            griddep_wait();
+            listed = true;
+            extra = lora_blocks(P, mb, lt % P.splits, BK);
+          }
           int id = lora_id(P, mb, 0, extra), j = 0, c = 0;
           for (int e = 0; ok && e < extra; ++e) {  // T_j, B_j of the tile's adapters
             if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 10 + stage, abort_flag)) {
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
-      bool ok = true;
+      bool ok = true, listed = false;  // listed: the adapter lists are complete
       for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, err, kKidGemm, 20 + acc, abort_flag)) {
           ok = false;
@@ -171,11 +176,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         int lt, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        int extra = 0;
+        int extra = 0, mb = 0;
         if constexpr (LORA) {
-          int mb, nb;
+          int nb;
           tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
-          extra = lora_blocks(P, mb, lt % P.splits, BK);
+          if (listed) extra = lora_blocks(P, mb, lt % P.splits, BK);
         }
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 30 + stage, abort_flag)) {
@@ -198,6 +203,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if constexpr (LORA) {
+          if (!listed) {
+            griddep_wait();
+            listed = true;
+            extra = lora_blocks(P, mb, lt % P.splits, BK);
+          }
           for (int e = 0; ok && e < extra; ++e) {
             if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 30 + stage, abort_flag)) {
               ok = false;
@@ -225,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // Epilogue warps 2..5 -> TMEM lane quarter (warp % 4)
     const int sub = warp & 3;
+    if constexpr (LORA) griddep_wait();  // (the split-K counters are zeroed by the kernel before)
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
@@ -274,6 +285,19 @@ int launch_variant(const GemmGroup& g, int* err, cudaStream_t stream, int device
   }
   const int sms = dfl_host::num_sms(device);
   const int grid = g.total_tiles < sms ? g.total_tiles : sms;
+  if constexpr (LORA) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = S::kTotal;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kern, g, err);
+  }
   kern<<<grid, kThreads, S::kTotal, stream>>>(g, err);
   return (int)cudaGetLastError();
 }

@@ -153,14 +153,14 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
       bool issued[STAGES];
       uint32_t issued_parity[STAGES];
       for (int s = 0; s < STAGES; ++s) issued[s] = false, issued_parity[s] = 0;
-      bool ok = true;
+      bool ok = true, listed = false;  // listed: the adapter lists are complete
       for (int t = pair; t < num_tiles && ok; t += num_pairs) {
         int lt, mb, nb, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
         tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        // (read here: its latency passes behind the K loop)
-        const int extra = LORA ? lora_blocks(P, mb, lt % P.splits, BK) : 0;
+        // the tile's list is read here, its latency passes behind the K loop; before the first one is complete, after it
+        int extra = LORA && listed ? lora_blocks(P, mb, lt % P.splits, BK) : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
             ok = false;
@@ -178,6 +178,11 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
           }
         }
         if constexpr (LORA) {
+          if (!listed) {
+            griddep_wait();
+            listed = true;
+            extra = lora_blocks(P, mb, lt % P.splits, BK);
+          }
           int id = lora_id(P, mb, 0, extra), j = 0, c = 0;
           for (int e = 0; ok && e < extra; ++e) {  // T_j, B_j of the tile's adapters
             if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kKidGemm, 310 + stage, abort_flag)) {
@@ -210,7 +215,7 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
       constexpr uint32_t idesc = make_idesc_bf16_f32(2 * BM, BN);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
+      bool ok = true, listed = false;  // listed: the adapter lists are complete
       for (int t = pair; t < num_tiles && ok; t += num_pairs) {
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, err, kKidGemm, 320 + acc, abort_flag)) {
           ok = false;
@@ -221,11 +226,11 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
         int lt, kb0, kb1;
         const GemmProblem& P = group_tile(grp, t, lt);
         split_k_range(P, lt % P.splits, BK, kb0, kb1);
-        int extra = 0;
+        int extra = 0, mb = 0;
         if constexpr (LORA) {
-          int mb, nb;
+          int nb;
           tile_coords(lt / P.splits, P.num_m, P.num_n, mb, nb);
-          extra = lora_blocks(P, mb, lt % P.splits, BK);
+          if (listed) extra = lora_blocks(P, mb, lt % P.splits, BK);
         }
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
@@ -246,6 +251,11 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
           }
         }
         if constexpr (LORA) {
+          if (!listed) {
+            griddep_wait();
+            listed = true;
+            extra = lora_blocks(P, mb, lt % P.splits, BK);
+          }
           for (int e = 0; ok && e < extra; ++e) {
             if (!mbar_wait(&full_bar[stage], phase, err, kKidGemm, 330 + stage, abort_flag)) {
               ok = false;
@@ -274,6 +284,7 @@ __global__ void __launch_bounds__(PairCfg<EPI, EW>::kThreads, 1)
     if constexpr (EW == 8) regs_dec();  // the idle warps of warpgroup 0
   } else {
     if constexpr (EW == 8) regs_inc();
+    if constexpr (LORA) griddep_wait();  // (the split-K counters are zeroed by the kernel before)
     const int ew = warp - C::kFirstEpiWarp;  // epilogue warp 0 .. EW-1
     const int sub = warp & 3;  // the TMEM lane quarter this warp may access
     const int slice = ew >> 2;  // which kCols columns of the tile (EW == 8: two slices)
@@ -345,13 +356,15 @@ int launch_pair_ew(const GemmGroup& g, int* err, cudaStream_t stream, int dev) {
   cfg.blockDim = dim3(C::kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemTotal;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = 2;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = LORA ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, g, err);
   return (int)e;
 }
@@ -361,10 +374,11 @@ int launch_pair(const GemmGroup& g, int* err, cudaStream_t stream, int dev) {
   const int ew = g_epi_warps ? g_epi_warps : (EPI == kEpiQkv ? 8 : 4);
   if constexpr (EPI != kEpiSwiGLU && EPI != kEpiQkv) {
     // Adapters: eight epilogue warps where the K loop is too short to hide four (4372 x 7296, GELU: K 576 77 -> 59 us,
-    // 1024 83 -> 68, 1536 92 -> 87, 2304 118 -> 119) and no K range is split (its fixup wants four).
+    // 1024 83 -> 68, 1536 92 -> 87, 2304 118 -> 119) or a single round of tiles leaves the epilogue exposed, and no K range is split (its fixup wants four).
     constexpr int LEPI = EPI == kEpiSilu ? kEpiSiluQuick : EPI;
     if (g.p[0].lora_list)
-      return ew == 8 || (g_epi_warps == 0 && g.p[0].splits == 1 && g.p[0].K <= 1536)
+      return ew == 8 || (g_epi_warps == 0 && g.p[0].splits == 1 &&
+                        (g.p[0].K <= 1536 || g.total_tiles <= dfl_host::num_sms(dev) / 2))
                  ? launch_pair_ew<LEPI, OUT_F32, 8, true>(g, err, stream, dev)
                  : launch_pair_ew<LEPI, OUT_F32, 4, true>(g, err, stream, dev);
   }

@@ -77,10 +77,11 @@ struct alignas(64) GemmProblem {
   int lora_cap, lora_rank, lora_n;
 };
 
+// (The lists are written while this kernel may already run: read past L1, after griddep_wait.)
 // Extra K blocks (adapters x 64-column pieces of the rank) of M tile mb in K range `split`.
 DFL_DEVICE int lora_blocks(const GemmProblem& P, int mb, int split, int BK) {
   if (P.lora_list == nullptr || split != P.splits - 1) return 0;
-  return __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap)) * ((P.lora_rank + BK - 1) / BK);
+  return __ldcg(P.lora_list + (long long)mb * (1 + P.lora_cap)) * ((P.lora_rank + BK - 1) / BK);
 }
 // 16-wide K steps of extra block e that hold adapter columns (the rest of its 64 columns is zero).
 DFL_DEVICE int lora_ksteps(const GemmProblem& P, int e, int BK) {
@@ -89,7 +90,7 @@ DFL_DEVICE int lora_ksteps(const GemmProblem& P, int e, int BK) {
 }
 // Adapter j of M tile mb (`left` blocks to go: none is read behind the list).
 DFL_DEVICE int lora_id(const GemmProblem& P, int mb, int j, int left) {
-  return left <= 0 ? 0 : __ldg(P.lora_list + (long long)mb * (1 + P.lora_cap) + 1 + j);
+  return left <= 0 ? 0 : __ldcg(P.lora_list + (long long)mb * (1 + P.lora_cap) + 1 + j);
 }
 
 struct alignas(64) GemmGroup {

@@ -80,6 +80,7 @@ DFL_DEVICE void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __global__ void __launch_bounds__(kThreads, 2)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ta, ShrinkParams p,
                        int* err) {
+  griddep_launch();  // the GEMM may start on x W^T; it waits for this kernel before its first adapter block
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + p.region);
@@ -342,7 +343,7 @@ DFL_DEVICE float dot8(const uint4& a, const uint4& b, float acc) {
 }
 
 __global__ void __launch_bounds__(256) lora_rows_t_kernel(RowsParams p, int* err) {
-  asm volatile("griddepcontrol.launch_dependents;");
+  griddep_launch();
   const int m = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   const int raw = __ldg(p.ids + (p.rows_per_id > 0 ? m / p.rows_per_id : m)), id = rows_id(p, m);
   if (id < 0) {
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) red[warp][quad + 8 * i][8 * g + 2 * t + e] = c[g][2 * i + e];
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // T is complete
+  griddep_wait();  // T is complete
   {  // T B^T: 16 lanes share a column, 8 values of the rank each
     const int n = threadIdx.x / 16, r0 = (threadIdx.x % 16) * 8;
     for (int m = 0; m < p.M; ++m) {
@@ -431,8 +432,8 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
       float v = 0.f;
       if (id >= 0 && r0 < p.rank && n0 + n < p.N) {
         const uint4 bw = __ldg(reinterpret_cast<const uint4*>(p.b + ((long long)id * p.N + n0 + n) * p.rank + r0));
-        const float4 t0 = *reinterpret_cast<const float4*>(p.t + m * p.rank + r0);
-        const float4 t1 = *reinterpret_cast<const float4*>(p.t + m * p.rank + r0 + 4);
+        const float4 t0 = __ldcg(reinterpret_cast<const float4*>(p.t + m * p.rank + r0));
+        const float4 t1 = __ldcg(reinterpret_cast<const float4*>(p.t + m * p.rank + r0 + 4));
         const float2 b0 = unpack_bf16x2(bw.x), b1 = unpack_bf16x2(bw.y), b2 = unpack_bf16x2(bw.z), b3 = unpack_bf16x2(bw.w);
         v = ((b0.x * t0.x + b0.y * t0.y) + (b1.x * t0.z + b1.y * t0.w)) +
             ((b2.x * t1.x + b2.y * t1.y) + (b3.x * t1.z + b3.y * t1.w));
