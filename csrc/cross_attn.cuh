@@ -10,16 +10,24 @@
 // Persistent, one CTA per SM; a work item is a block of QT * 128 queries of one head:
 //   TMA warp     Q tiles of the next item as soon as the last Q K^T of this one has read them;
 //                K_j, V_j through a ring of shared-memory slots
-//   MMA warp     steps (item, tile) as one sequence, PV0(s-1) QK0(s) PV1(s-1) QK1(s), so the
-//                scores of the next item are computed while this item's rows are stored
+//   MMA warp     steps s = (item, tile) as one sequence, PV0(s-1) QK0(s) PV1(s-1) QK1(s), so the scores of
+//                the next item are computed while this item's rows are stored.  The fixed order also
+//                keeps the two tiles out of step, one in its exponentials while the other multiplies (with a
+//                warp per tile they fall into step and share the SFU: 402 us where this takes 349)
 //   clean warp   zeroes the V rows of masked keys (what lies behind a sequence's length may be
 //                anything; 0 * NaN would reach the sums), in the tiles that hold some
 //   softmax      one warpgroup per Q tile, one query row per thread; P goes back to tensor memory
 //                over S and is the A operand of P V; O is rescaled only when the maximum grew by
 //                more than 2^8
-// tcgen05 operations of the issuing thread complete in order: when S_g(s) is ready, P V_g(s-1) has
+// tcgen05 operations of an issuing thread complete in order: when S_g(s) is ready, P V_g(s-1) has
 // finished, and P_g(first tile of an item) is signalled only after its warpgroup has read O_g of the
 // item before, so neither P nor O needs a barrier of its own.
+//
+// 40 heads x 32760 queries x 512 keys x 128: 349 us (984 TFLOP/s; the products alone take 205 at the library's rate, the
+// exponentials 180 at the SFU's).  What is left is the round trip of a Q tile (scores, exponentials, P, next
+// scores: 3650 cycles for 2 x 1024 of products), which two tiles do not fill, and the turn of the items.  Measured
+// and slower or equal: part of the exponentials on the FMA pipe (387 us), an MMA warp per Q tile (402), three K / V slots
+// with a larger output buffer (388), the second half of a row kept in registers past the first P (348).
 //
 // Masks: a key window [lo, hi) per batch row (tiles outside it are skipped), bits (kBits: packed
 // by cross_mask_bits, per query or shared by all queries) or an additive bias (kBias16 / kBias32).
@@ -67,7 +75,7 @@ struct CrossCfg {
   static constexpr int kProducerWarp = 4 * QT, kMmaWarp = 4 * QT + 1, kCleanWarp = 4 * QT + 2;
   static constexpr int kTile = 128 * DH * 2;
   static constexpr int kChunks = DH / 64;
-  static constexpr int kRing = DH == 64 ? 8 : (QT == 2 ? 4 : 5);
+  static constexpr int kRing = DH == 64 ? 8 : (QT == 2 ? 4 : 5);  // (three slots: 360 -> 388 us at 512 keys)
   static constexpr int kQ = 0, kKV = QT * kTile;
   static constexpr int kOut = kKV + kRing * kTile;  // 4 KB per softmax warp: 32 rows x 64 columns on their way out
   static constexpr int kBar = kOut + 4 * QT * 4096;
@@ -144,33 +152,46 @@ DFL_DEVICE void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "
 DFL_DEVICE void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 DFL_DEVICE void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// One work item: its query block, head, batch row, key window and key tiles.
-struct CrossItem {
+// The work items of one CTA: its query block, head, batch row, key window and key tiles, advanced by
+// gridDim.x items without divisions (this stands on the issuing warps' critical path).
+template <int QT>
+struct CrossItems {
   int q0, h, b, lo, hi, t0, n;
+  int qb, dq, dh, db;
+  DFL_DEVICE explicit CrossItems(const CrossParams& p) {
+    const int i = blockIdx.x, g = gridDim.x;
+    qb = i % p.n_qb, h = (i / p.n_qb) % p.H, b = i / p.n_qb / p.H;
+    dq = g % p.n_qb, dh = (g / p.n_qb) % p.H, db = g / p.n_qb / p.H;
+    window(p);
+  }
+  DFL_DEVICE bool more(const CrossParams& p) const { return b < p.B; }
+  DFL_DEVICE void next(const CrossParams& p) {
+    const int was = b;
+    qb += dq, h += dh, b += db;
+    if (qb >= p.n_qb) qb -= p.n_qb, ++h;
+    if (h >= p.H) h -= p.H, ++b;
+    q0 = qb * (QT * kBM);
+    if (b != was) window(p);
+  }
+  DFL_DEVICE void window(const CrossParams& p) {
+    q0 = qb * (QT * kBM);
+    if (b >= p.B) return;
+    lo = p.kv_lo ? max(0, __ldg(p.kv_lo + b)) : 0;
+    hi = p.kv_hi ? min(p.Sk, __ldg(p.kv_hi + b)) : p.Sk;
+    t0 = lo / kBN;
+    n = hi > lo ? (hi + kBN - 1) / kBN - t0 : 0;
+  }
 };
 
-template <int QT>
-DFL_DEVICE CrossItem cross_item(const CrossParams& p, int i) {
-  CrossItem it;
-  it.q0 = (i % p.n_qb) * (QT * kBM);
-  const int hb = i / p.n_qb;
-  it.h = hb % p.H;
-  it.b = hb / p.H;
-  it.lo = p.kv_lo ? max(0, __ldg(p.kv_lo + it.b)) : 0;
-  it.hi = p.kv_hi ? min(p.Sk, __ldg(p.kv_hi + it.b)) : p.Sk;
-  it.t0 = it.lo / kBN;
-  it.n = it.hi > it.lo ? (it.hi + kBN - 1) / kBN - it.t0 : 0;
-  return it;
-}
-
 // The words of key tile k0 for one row of a bit mask (whole 128-key groups are stored).
-DFL_DEVICE uint4 cross_bits(const CrossParams& p, const CrossItem& it, int q, int k0) {
+template <class Item>
+DFL_DEVICE uint4 cross_bits(const CrossParams& p, const Item& it, int q, int k0) {
   return __ldg(reinterpret_cast<const uint4*>(p.bits + it.b * p.bits_bs + it.h * p.bits_hs + q * p.bits_qs + k0 / 32));
 }
 
 // Whether tile k0 holds V rows of keys that no query of this batch row may see.
-template <int MASK>
-DFL_DEVICE bool cross_dirty(const CrossParams& p, const CrossItem& it, int k0) {
+template <int MASK, class Item>
+DFL_DEVICE bool cross_dirty(const CrossParams& p, const Item& it, int k0) {
   if (it.lo > k0 || it.hi < min(k0 + kBN, p.Sk)) return true;
   if (MASK == kBits && p.key_bits) {
     const uint4 w = cross_bits(p, it, 0, k0);
@@ -213,7 +234,6 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int n_items = p.n_qb * p.H * p.B;
   const bool cleaning = p.kv_lo || p.kv_hi || (MASK == kBits && p.key_bits);  // masked keys may hold anything
 
   if (threadIdx.x == 0) {
@@ -248,8 +268,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       for (int i = 0; i < R; ++i) issued[i] = false, issued_par[i] = 0;
       bool ok = true;
       int L = 0, used = 0;  // used: items with key tiles so far
-      for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-        const CrossItem it = cross_item<QT>(p, i);
+      for (CrossItems<QT> it(p); it.more(p) && ok; it.next(p)) {
         if (it.n == 0) continue;
         const int hk = it.h / p.rep;
         for (int j = 0; j < it.n && ok; ++j) {
@@ -334,8 +353,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         clean_par ^= 1u << slot;
         return mbar_wait(&v_clean[slot], par, err, kKidCross, 116, abort_flag);
       };
-      for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-        const CrossItem it = cross_item<QT>(p, i);
+      for (CrossItems<QT> it(p); it.more(p) && ok; it.next(p)) {
         if (it.n == 0) continue;
         for (int j = 0; j < it.n && ok; ++j, ++s) {
           if (!wait_load(2 * s, 113)) { ok = false; break; }
@@ -370,8 +388,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     int s = 0;
     // every V tile passes here in order (its phase of v_clean[slot] completes once), so neither this
     // warp nor the MMA warp can be a phase of a slot ahead of the other
-    for (int i = blockIdx.x; cleaning && i < n_items && ok; i += gridDim.x) {
-      const CrossItem it = cross_item<QT>(p, i);
+    for (CrossItems<QT> it(p); cleaning && it.more(p) && ok; it.next(p)) {
       for (int j = 0; j < it.n && ok; ++j, ++s) {
         const int k0 = (it.t0 + j) * kBN, L = 2 * s + 1;
         const bool dirty = cross_dirty<MASK>(p, it, k0);
@@ -412,8 +429,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     const float grow = is_bias(MASK) ? 8.f * kLn2 : 8.f;
     bool ok = true;
     int s = 0, used = 0;
-    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-      const CrossItem it = cross_item<QT>(p, i);
+    for (CrossItems<QT> it(p); it.more(p) && ok; it.next(p)) {
       const int qrow = it.q0 + g * kBM + row;
       const bool live = qrow < p.Sq;
       float m = -INFINITY, l = 0.f;  // running maximum (log2 units; bias: natural units) and sum
@@ -553,9 +569,10 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum stays NaN)
         const bool none = l == 0.f;
-        // 64 columns at a time through shared memory (the store's swizzle: 16-byte piece i of row r at
-        // i ^ (r % 8)): a thread's own row would cost a line per lane and store
+        // through shared memory (the store's swizzle: 16-byte piece i of row r at i ^ (r % 8)): a thread's own
+        // row would cost a line per lane and store
         uint8_t* stage = smem + C::kOut + warp * 4096;
+        const int r0 = it.q0 + g * kBM + (warp & 3) * 32;
 #pragma unroll 1
         for (int ch = 0; ch < C::kChunks; ++ch) {
           if (lane == 0) bulk_wait_read();  // what left this buffer last has been read
@@ -565,18 +582,17 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
             uint32_t o_raw[32];
             tmem_ld_32x32b_x32(o_t + ch * 64 + hf * 32, o_raw);
             tmem_wait_ld();
-            float o[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : __uint_as_float(o_raw[e]) * inv;
+            for (int i = 0; i < 4; ++i) {
+              float o[8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((hf * 4 + q) ^ (lane & 7)) * 16)) =
-                  make_uint4(pack2<F16>(o[8 * q], o[8 * q + 1]), pack2<F16>(o[8 * q + 2], o[8 * q + 3]),
-                             pack2<F16>(o[8 * q + 4], o[8 * q + 5]), pack2<F16>(o[8 * q + 6], o[8 * q + 7]));
+              for (int e = 0; e < 8; ++e) o[e] = none ? 0.f : __uint_as_float(o_raw[8 * i + e]) * inv;
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((hf * 4 + i) ^ (lane & 7)) * 16)) =
+                  make_uint4(pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3]), pack2<F16>(o[4], o[5]), pack2<F16>(o[6], o[7]));
+            }
           }
           fence_proxy_async_shared();
           __syncwarp();
-          const int r0 = it.q0 + g * kBM + (warp & 3) * 32;
           if (lane == 0 && r0 < p.Sq) {  // (rows past the last query are clipped)
             tma_store_4d(&to, stage, ch * 64, r0, it.h, it.b);
             bulk_commit();
@@ -598,12 +614,12 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
 }
 
 inline int cross_tmap(CUtensorMap* map, const void* base, int D, long long S, int H, int B, long long ss, long long hs,
-                      long long bs, bool f16, int box_rows = 128) {
+                      long long bs, bool f16, bool out = false) {
   dfl_host::EncodeTiledFn fn = dfl_host::get_encode_tiled();
   if (!fn) return 999;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)hs * 2, (cuuint64_t)bs * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t box[4] = {64, out ? 32u : 128u, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return (int)fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -633,7 +649,7 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
   if (rc) return 2000 + rc;
   rc = cross_tmap(&tv, a->v, DH, a->Sk, a->Hk, a->B, a->v_ss, a->v_hs, a->v_bs, F16);
   if (rc) return 3000 + rc;
-  rc = cross_tmap(&to, a->o, DH, a->Sq, a->H, a->B, a->o_ss, a->o_hs, a->o_bs, F16, 32);
+  rc = cross_tmap(&to, a->o, DH, a->Sq, a->H, a->B, a->o_ss, a->o_hs, a->o_bs, F16, true);
   if (rc) return 4000 + rc;
   p.n_qb = (a->Sq + QT * kBM - 1) / (QT * kBM);
   const long long items = (long long)p.n_qb * a->H * a->B;
