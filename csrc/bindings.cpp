@@ -269,6 +269,8 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
   int64_t cap = std::min<int64_t>(l.n_adapters, l.tile_rows);
   if (rows_per_id > 0) cap = std::min<int64_t>(cap, (l.tile_rows - 1 + rows_per_id - 1) / rows_per_id + 1);
   l.cap = (int)cap;
+  TORCH_CHECK_VALUE(tiles * cap * l.tile_rows < (1ll << 31) && l.n_adapters * N < (1ll << 31),
+                    "linear_lora: ", M, " rows that may mix ", cap, " adapters a tile are too many for one call");
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   const int64_t t_bytes = up(tiles * cap * l.tile_rows * l.rank * 2), list_bytes = up(tiles * (1 + cap) * 4),
                 sem_bytes = up(l.split_sem_count * 4);
@@ -613,7 +615,9 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     if (!t) return nullptr;
     TORCH_CHECK_VALUE(at::isIntegralType(t->scalar_type(), false) && t->dim() == 1 && t->size(0) == a.B, name,
                       " must be integers [", a.B, "]");
-    keep = t->to(at::TensorOptions().device(q.device()).dtype(at::kInt)).contiguous();
+    // (a count that does not fit 32 bits is more than every key)
+    keep = (t->scalar_type() == at::kLong ? t->clamp(-1, 1 << 30) : *t)
+               .to(at::TensorOptions().device(q.device()).dtype(at::kInt)).contiguous();
     return keep.data_ptr<int>();
   };
   a.kv_lo = edge(kv_lo, "kv_lo", edges[0]);
@@ -629,7 +633,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     m = mt->expand({a.B, a.H, a.Sq, a.Sk});
     mdt = m.scalar_type() == at::kBool ? -1 : dtype_code(m, "an additive mask");
   }
-  if (a.H / a.Hk * a.Sq <= 16) {  // too few rows to fill a tile: the keys are split instead
+  if (a.H / a.Hk * (int64_t)a.Sq <= 16 && a.B <= 65535 && a.Hk <= 65535) {  // too few rows to fill a tile: the keys are split instead
     DecodeArgs d{};
     d.q = a.q, d.k = a.k, d.v = a.v, d.o = a.o;
     d.q_bs = a.q_bs, d.q_hs = a.q_hs, d.q_ss = a.q_ss, d.k_bs = a.k_bs, d.k_hs = a.k_hs, d.k_ss = a.k_ss;

@@ -76,7 +76,7 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
             lo = lo.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
             hi = hi.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
         out = F.attention(q4, k4, v4, scale, lse=lse, kv_lo=lo, kv_hi=hi)
-    elif F.cross_kernel_ok(q) and not causal and k4.dtype == v4.dtype == q4.dtype and k4.shape[1] == q4.shape[1]:
+    elif F.cross_kernel_ok(q, k, v, attention_mask) and not causal and k4.dtype == v4.dtype == q4.dtype and k4.shape[1] == q4.shape[1]:
         mask = attention_mask if simple or bound_min is None else _bounds_to_mask(k4, bound_min, bound_max, None)
         if lo is not None and simple:
             lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
@@ -134,8 +134,9 @@ def _mask_on(mask, q):
         return None
     if not mask.is_floating_point():
         mask = mask.bool()
-    elif mask.dtype not in _MASK_DTYPES and q.is_cuda:
-        mask = mask.float()
+    elif mask.dtype not in _MASK_DTYPES and q.is_cuda:  # finite values stay finite (the type's lowest masks softly)
+        low = torch.finfo(torch.float32)
+        mask = torch.where(mask.isfinite(), mask.clamp(low.min, low.max), mask).float()
     return mask.to(q.device)
 
 
@@ -147,9 +148,10 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     attend) or additive, broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
     ``attention``.  A query that no key is left for gives 0.  ``out`` (like q) and ``lse`` (f32 ``[B, H, Sq]``, natural
-    log) are filled when given.  CUDA: bf16 and fp16 with head dim 64 or 128; anything else runs as ``attention``."""
-    F._no_grad("cross_attention", q, k, v, attention_mask)
-    if (q.dim() == 4 and bound_min is None and bound_max is None and F.cross_kernel_ok(q)
+    log) are filled when given.  CUDA: bf16 and fp16 with head dim 64 or 128; anything else, and what asks for
+    gradients, runs as ``attention``."""
+    kernel = F.cross_kernel_ok(q, k, v, attention_mask)
+    if (kernel and q.dim() == 4 and bound_min is None and bound_max is None
             and (attention_mask is None or attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)):
         # the binding checks shapes, types and devices (ValueError)
         return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
@@ -198,7 +200,7 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         if mask.dim() > 4 or any(m not in (1, w) for m, w in zip(mask.shape[::-1], want[::-1])):
             raise ValueError(f"attention_mask {tuple(mask.shape)} does not broadcast to {want}")
     scale = 1.0 if scale is None else float(scale)
-    if not q.is_cuda or F.cross_kernel_ok(q):
+    if not q.is_cuda or kernel:
         return F.cross_attention(q, k, v, scale, mask=mask, kv_lo=lo, kv_hi=hi, out=out, lse=lse)
     if hi is not None:  # off the kernel: the window as a mask
         idx = torch.arange(k.shape[2], device=q.device)

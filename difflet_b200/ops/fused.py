@@ -256,10 +256,8 @@ def linear_lora(x, w, b, bank, ids, rows_per_id=0, *, act=None, act_lo=0, act_hi
 
 def _no_grad(name: str, *tensors) -> None:
     """The kernels record no backward pass: refuse inputs whose gradient would be lost silently."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
+    if wants_grad(*tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
 
 
 # MX element type -> (code of the native kernels, emax of the format, largest finite value)
@@ -596,16 +594,27 @@ def kv_split_mode() -> int:
     return -1 if envs.DIFFLET_ATTN_SPLIT != "0" else 1
 
 
-def cross_kernel_ok(q) -> bool:
-    """Whether the masked / head-dim-64 attention kernel takes these queries."""
-    return q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in (torch.bfloat16, torch.float16)
+def wants_grad(*tensors) -> bool:
+    """Whether autograd would record an operation on these (None allowed)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def cross_kernel_ok(q, k, v, mask=None) -> bool:
+    """Whether the masked / head-dim-64 attention kernel takes these inputs (it records no backward pass: what asks
+    for gradients stays on the torch path)."""
+    return (q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in (torch.bfloat16, torch.float16)
+            and not wants_grad(q, k, v, mask))
 
 
 def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     """softmax(scale * q k^T) v over [B, H, S, dh]; key window [kv_lo[b], kv_hi[b])."""
     if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128:
         return native().attention(q, k, v, float(scale), out, lse, kv_lo, kv_hi, kv_split=kv_split_mode())
-    if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and cross_kernel_ok(q):
+    if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and cross_kernel_ok(q, k, v):
         return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     if q.is_cuda and lse is None and kv_lo is None:

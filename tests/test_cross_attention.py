@@ -121,8 +121,6 @@ def test_refusals():
                      ((q, k, v), dict(lse=torch.empty(2, 4, 2))), ((q[0], k[0], v[0]), dict(kv_lens=lens))):
         with pytest.raises(ValueError):
             ops.cross_attention(*args, **kw)
-    with pytest.raises(RuntimeError, match="no backward"):
-        ops.cross_attention(q.clone().requires_grad_(), k, v)
 
 
 # ----------------------------------------------------------------------------- B200
@@ -234,6 +232,53 @@ def test_attention_takes_the_kernel(native):
     _check(F.attention(q, k, v, 0.1, kv_lo=torch.zeros_like(hi), kv_hi=hi), _ref(q, k, v, 0.1, lens=hi), q.dtype, 64, Sk,
            v.abs().max().item())
     _check(ops.attention(q, k, v, scale=0.1), _ref(q, k, v, 0.1), q.dtype, 64, Sk, v.abs().max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_stay_on_the_torch_path(native, D):
+    """Inputs that ask for gradients keep the differentiable path, and get the formula's gradients."""
+    q, k, v = (t.detach().requires_grad_() for t in _inputs(2, 2, 2, 20, 33, D, torch.bfloat16, "cuda"))
+    m = torch.rand(2, 1, 20, 33, device="cuda") < 0.7
+    m[..., 0] = True
+    w = torch.randn(2, 2, 20, D, device="cuda")
+    ref = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    z = (ref[0] @ ref[1].transpose(2, 3) * 0.1).masked_fill(~m, -math.inf)
+    want = torch.autograd.grad(((z.softmax(-1) @ ref[2]) * w.double()).sum(), ref)
+    for fn in (ops.cross_attention, ops.attention):
+        got = torch.autograd.grad((fn(q, k, v, scale=0.1, attention_mask=m) * w).sum(), (q, k, v))
+        for a, b in zip(got, want):  # the library's bf16 products: a few roundings (2^-8) of the largest value
+            assert (a.double() - b).abs().max() <= 2.0 ** -5 * b.abs().max()
+    with torch.no_grad():
+        o = ops.cross_attention(q, k, v, scale=0.1, attention_mask=m)
+    _check(o, _ref(q.detach(), k.detach(), v.detach(), 0.1, m), q.dtype, D, 33, v.abs().max().item())
+
+
+@pytest.mark.gpu
+def test_kernel_unusual_masks_and_lengths(native):
+    B, H, Sq, Sk, D = 2, 2, 40, 50, 64
+    q, k, v = _inputs(B, H, H, Sq, Sk, D, torch.bfloat16, "cuda")
+    all_keys = ops.cross_attention(q, k, v, scale=0.1)
+    for lens in (torch.tensor([1 << 40, 50]), torch.tensor([50, 99], dtype=torch.int16)):  # any integers, any device
+        assert torch.equal(ops.cross_attention(q, k, v, scale=0.1, kv_lens=lens), all_keys)
+    assert bool((ops.cross_attention(q, k, v, scale=0.1, kv_lens=torch.tensor([-3, 0])) == 0).all())
+    m = torch.rand(B, 1, Sq, Sk, device="cuda") < 0.5
+    want = ops.cross_attention(q, k, v, scale=0.1, attention_mask=m)
+    assert torch.equal(ops.cross_attention(q, k, v, scale=0.1, attention_mask=m.int()), want)
+    low = torch.zeros(m.shape, device="cuda", dtype=torch.float64).masked_fill(~m, torch.finfo(torch.float64).min)
+    low[:, :, 3] = torch.finfo(torch.float64).min  # a row at the lowest value everywhere: the mean of the values
+    o = ops.cross_attention(q, k, v, scale=0.1, attention_mask=low)
+    mean = v.double().mean(2)
+    assert bool(((o[:, :, 3].double() - mean).abs() <= 2.0 ** -7 * (mean.abs() + v.double().abs().mean(2))).all())
+    keep = torch.arange(Sq, device="cuda") != 3
+    assert torch.allclose(o[:, :, keep].float(), want[:, :, keep].float(), atol=2.0 ** -6)
+    assert torch.equal(ops.cross_attention(q, k, v, scale=0.1, attention_mask=torch.tensor(True, device="cuda")), all_keys)
+    big = _inputs(70000, 1, 1, 1, 3, 64, torch.bfloat16, "cuda")  # more batch rows than a grid axis holds
+    o = ops.cross_attention(*big, scale=0.1)
+    _check(o, _ref(*big, 0.1), q.dtype, 64, 3, big[2].abs().max().item())
+    same = q.contiguous()
+    got = ops.cross_attention(same, k, v, scale=0.1, out=same)  # in place of the queries
+    assert got is same and torch.equal(got, all_keys)
 
 
 @pytest.mark.gpu

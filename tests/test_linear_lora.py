@@ -192,6 +192,20 @@ def test_kernel_refusals(native):
 
 
 @pytest.mark.gpu
+def test_kernel_beside_a_weight_kept_in_eight_bits(native):
+    x, w, b, A, B, scale = _make(70, 256, 512, [8, 8], "cuda")
+    bank, ids = ops.LoraBank(A, B, scale), torch.randint(-1, 2, (70,), device="cuda")
+    q = F.MXWeight.quantize(w, compute="dequant")
+    got = ops.linear_lora(x.view(7, 10, 512), q, b, bank=bank, ids=ids, act="gelu")
+    assert got.shape == (7, 10, 256)
+    assert torch.equal(got.view(70, 256), ops.linear_lora(x, q.dequantize(), b, bank=bank, ids=ids, act="gelu"))
+    with pytest.raises(NotImplementedError):
+        ops.linear_lora(x, F.MXWeight.quantize(w), b, bank=bank, ids=ids)
+    row = ops.linear_lora(x[0], w, b, bank=bank, ids=ids[:1])  # a single row as a vector
+    assert row.shape == (256,) and torch.equal(row, ops.linear_lora(x[:1], w, b, bank=bank, ids=ids[:1])[0])
+
+
+@pytest.mark.gpu
 def test_kernel_rows_do_not_see_each_other(native):
     """A row's result does not depend on which adapters its neighbours use."""
     M, N, K = 512, 1024, 256
