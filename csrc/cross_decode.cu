@@ -41,6 +41,23 @@ DFL_DEVICE float ld_cluster(const float* p, uint32_t rank) {
   return v;
 }
 
+// Packed f32 pairs.
+DFL_DEVICE uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+DFL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+DFL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 template <bool F16>
 DFL_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (F16)
@@ -78,14 +95,15 @@ template <int DH, bool F16, int NR>
 __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cross_decode_kernel(const DecodeArgs a) {
   constexpr int KC = DH / 32;  // 16-byte pieces of a key row per lane
   constexpr int DL = DH / 32;  // output columns per lane
-  // P of the block a warp is at; later this CTA's joined rows, read by the cluster
-  static_assert(kWarps * kKeys <= DH, "shared buffer");
-  __shared__ __align__(16) float s_buf[NR * DH];
-  float(*s_p)[NR][kKeys] = reinterpret_cast<float(*)[NR][kKeys]>(s_buf);
+  // P of the block a warp is at, every value twice (the packed multiply-add takes pairs); later this CTA's joined
+  // rows, read by the cluster
+  constexpr int kBuf = kWarps * NR * kKeys * 2 > NR * DH ? kWarps * NR * kKeys * 2 : NR * DH;
+  __shared__ __align__(16) float s_buf[kBuf];
+  float(*s_p)[NR][kKeys * 2] = reinterpret_cast<float(*)[NR][kKeys * 2]>(s_buf);
   float(*c_o)[DH] = reinterpret_cast<float(*)[DH]>(s_buf);
   __shared__ float s_f[kWarps][16];               // rescaling of the rows, then their maxima
   __shared__ float s_l[kWarps][16];
-  __shared__ float s_o[kWarps][NR][DH];
+  __shared__ __align__(16) float s_o[kWarps][NR][DH];
   __shared__ float c_m[16], c_l[16];
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
@@ -108,36 +126,34 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cr
       qf[c][i] = r < R ? *reinterpret_cast<const uint4*>(qp + 32 * c + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
   }
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[NR][DL];
+  uint64_t o[NR][DL / 2];  // pairs of columns
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int d = 0; d < DL; ++d) o[r][d] = 0.f;
+    for (int d = 0; d < DL / 2; ++d) o[r][d] = 0ull;
 
   // blocks of the window, dealt to the warps of all splits in turn
   const int nb = hi > lo ? (hi - lo + kKeys - 1) / kKeys : 0;
   for (int blk = split * kWarps + warp; blk < nb; blk += splits * kWarps) {
-    const int k0 = lo + blk * kKeys;
+    const int k0 = lo + blk * kKeys, left = hi - k0;  // keys of this block (kKeys or more: all)
     uint4 kf[kKeys / 8][KC];
+    const uint16_t* kb = kp + (long long)(k0 + quad) * a.k_ss + 8 * t;
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n) {
-      const int key = k0 + 8 * n + quad;
+    for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
       for (int c = 0; c < KC; ++c)
-        kf[n][c] = key < hi ? __ldg(reinterpret_cast<const uint4*>(kp + key * a.k_ss + 32 * c + 8 * t)) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    auto load_v = [&](int key, uint32_t (&w)[DL / 2]) {
-      const uint16_t* p = vp + (k0 + key) * a.v_ss + lane * DL;
-      if constexpr (DL == 4) {
-        const uint2 x = k0 + key < hi ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
-        w[0] = x.x, w[1] = x.y;
-      } else {
-        w[0] = k0 + key < hi ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
-      }
-    };
+        kf[n][c] = 8 * n + quad < left ? __ldg(reinterpret_cast<const uint4*>(kb + 8 * n * a.k_ss + 32 * c)) : make_uint4(0u, 0u, 0u, 0u);
     uint32_t vf[kKeys][DL / 2];  // on its way during the scores
+    const uint16_t* vb = vp + (long long)k0 * a.v_ss + lane * DL;
 #pragma unroll
-    for (int k = 0; k < kKeys; ++k) load_v(k, vf[k]);
+    for (int k = 0; k < kKeys; ++k) {
+      if constexpr (DL == 4) {
+        const uint2 x = k < left ? __ldg(reinterpret_cast<const uint2*>(vb + k * a.v_ss)) : make_uint2(0u, 0u);
+        vf[k][0] = x.x, vf[k][1] = x.y;
+      } else {
+        vf[k][0] = k < left ? __ldg(reinterpret_cast<const uint32_t*>(vb + k * a.v_ss)) : 0u;
+      }
+    }
     float s[kKeys / 8][4];
 #pragma unroll
     for (int n = 0; n < kKeys / 8; ++n) {
@@ -150,7 +166,7 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cr
     }
     // s[n][2 i + e]: row quad + 8 i, key 8 n + 2 t + e
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < (NR + 7) / 8; ++i) {
       const int r = quad + 8 * i;
       if (8 * i >= R) continue;  // (uniform: no row of this half exists)
       const int h = head_of(r), q = query_of(r);
@@ -159,9 +175,9 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cr
       for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int key = k0 + 8 * n + 2 * t + e;
+          const int key = 8 * n + 2 * t + e;
           float& z = s[n][2 * i + e];
-          z = r < R && key < hi ? masked_score(a, z, b, h, q, key) : -INFINITY;
+          z = r < R && key < left ? masked_score(a, z, b, h, q, k0 + key) : -INFINITY;
           mx = fmaxf(mx, z);
         }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -174,42 +190,44 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cr
       for (int n = 0; n < kKeys / 8; ++n) {
         const float p0 = exp2_sfu((s[n][2 * i] - mu) * kLog2e), p1 = exp2_sfu((s[n][2 * i + 1] - mu) * kLog2e);
         l[i] += p0 + p1;
-        if (r < NR) *reinterpret_cast<float2*>(&s_p[warp][r][8 * n + 2 * t]) = make_float2(p0, p1);
+        if (r < NR) *reinterpret_cast<float4*>(&s_p[warp][r][2 * (8 * n + 2 * t)]) = make_float4(p0, p0, p1, p1);
       }
       if (t == 0) s_f[warp][r] = f;
     }
     __syncwarp();
+    if (a.mask != nullptr && a.mask_dtype < 0) {
+      // a key that no row keeps adds nothing, whatever V holds there
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      const float f = r < R ? s_f[warp][r] : 0.f;
+      for (int k = 0; k < kKeys; ++k) {
+        float any = 0.f;
 #pragma unroll
-      for (int d = 0; d < DL; ++d) o[r][d] *= f;
+        for (int r = 0; r < NR; ++r)
+          if (r < R) any += s_p[warp][r][2 * k];
+#pragma unroll
+        for (int d = 0; d < DL / 2; ++d) vf[k][d] = any == 0.f ? 0u : vf[k][d];
+      }
     }
 #pragma unroll
-    for (int k4 = 0; k4 < kKeys; k4 += 4) {
-      float4 p[NR];
-      float4 any = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < NR; ++r) {
+      if (r >= R) continue;
+      const float f = s_f[warp][r];
+#pragma unroll
+      for (int d = 0; d < DL / 2; ++d) o[r][d] = f2_mul(o[r][d], f2_pack(f, f));
+    }
+#pragma unroll
+    for (int k = 0; k < kKeys; k += 2) {
+      uint64_t v0[DL / 2], v1[DL / 2];
+#pragma unroll
+      for (int d = 0; d < DL / 2; ++d) {
+        const float2 x = unpack2<F16>(vf[k][d]), y = unpack2<F16>(vf[k + 1][d]);
+        v0[d] = f2_pack(x.x, x.y), v1[d] = f2_pack(y.x, y.y);
+      }
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        p[r] = r < R ? *reinterpret_cast<const float4*>(&s_p[warp][r][k4]) : make_float4(0.f, 0.f, 0.f, 0.f);
-        any.x += p[r].x, any.y += p[r].y, any.z += p[r].z, any.w += p[r].w;
-      }
-      const float anys[4] = {any.x, any.y, any.z, any.w};
+        if (r >= R) continue;
+        const ulonglong2 p = *reinterpret_cast<const ulonglong2*>(&s_p[warp][r][2 * k]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v[DL];
-#pragma unroll
-        for (int d = 0; d < DL / 2; ++d) {
-          const float2 x = unpack2<F16>(vf[k4 + k][d]);
-          // a key that no row keeps adds nothing, whatever V holds there
-          v[2 * d] = anys[k] == 0.f ? 0.f : x.x, v[2 * d + 1] = anys[k] == 0.f ? 0.f : x.y;
-        }
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float pk = k == 0 ? p[r].x : k == 1 ? p[r].y : k == 2 ? p[r].z : p[r].w;
-#pragma unroll
-          for (int d = 0; d < DL; ++d) o[r][d] = fmaf(pk, v[d], o[r][d]);
-        }
+        for (int d = 0; d < DL / 2; ++d) o[r][d] = f2_fma(p.y, v1[d], f2_fma(p.x, v0[d], o[r][d]));
       }
     }
     __syncwarp();
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cr
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int d = 0; d < DL; ++d) s_o[warp][r][lane * DL + d] = o[r][d];
+    for (int d = 0; d < DL / 2; ++d) *reinterpret_cast<uint64_t*>(&s_o[warp][r][lane * DL + 2 * d]) = o[r][d];
   __syncthreads();
   for (int i = threadIdx.x; i < R * DH; i += 32 * kWarps) {
     const int r = i / DH, d = i % DH;
