@@ -8,6 +8,11 @@
 // order (lane t of a quad holds 8 contiguous values of every 32), so every load is 16 contiguous bytes and nothing is
 // staged.  P V is f32 multiply-adds, a lane holding dh / 32 columns of every row, with P unrounded.  The partial
 // results are joined by log-sum-exp through distributed shared memory, in a fixed order.
+//
+// 8 x 8 key heads of up to 3276 keys x 128, four query heads each: 25 us (84 MB, 3.4 TB/s; 13 us at the copy rate).
+// About 6 us of it are the launch and the joins; the rest runs at 4.4 TB/s, four CTAs of 128 registers per SM being
+// what the loads in flight allow.  Measured and slower: 32-key blocks with fewer CTAs (31 us), the next block's
+// loads issued into the registers as they come free (35 us).
 #include <cuda_fp16.h>
 
 #include "common.cuh"

@@ -12,7 +12,8 @@ propagation, and all are functional (outputs are new tensors).
 Ops: ``attention``, ``linear`` (bias + optional GELU / SiLU on a column window),
 ``linear_gate_resid`` (``resid + gate * (x W^T + b)``), ``ln_modulate`` (LayerNorm / RMSNorm
 with affine and per-batch shift / scale), ``rms_norm``, ``quantize_mx`` (OCP-MX E4M3 +
-E8M0 per 32), ``linear_mx`` (block-scaled GEMM on quantized operands), ``gemv``.
+E8M0 per 32), ``linear_mx`` (block-scaled GEMM on quantized operands), ``gemv``,
+``add_rms_norm`` (residual addition + RMSNorm), ``cross_attention`` (masks, key counts, shared key heads).
 """
 
 from __future__ import annotations
@@ -148,6 +149,35 @@ def _(W, x, bias=None, silu_in=False, silu_out=False):
     return x.new_empty((x.shape[0], W.shape[0]), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32)
 
 
-OPS = ("attention", "linear", "linear_gate_resid", "ln_modulate", "rms_norm", "quantize_mx", "linear_mx", "gemv")
+@torch.library.custom_op(f"{_NS}::add_rms_norm", mutates_args=())
+def add_rms_norm(x: torch.Tensor, resid: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
+                 rows_per_batch: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(RMSNorm(x + resid) * weight * (1 + scale[batch]) + shift[batch], x + resid)."""
+    return F.add_rms_norm(x, resid, weight, eps=eps, scale=scale, shift=shift, rows_per_batch=rows_per_batch)
+
+
+@add_rms_norm.register_fake
+def _(x, resid, weight=None, eps=1e-6, scale=None, shift=None, rows_per_batch=0):
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{_NS}::cross_attention", mutates_args=())
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
+                    attention_mask: Optional[torch.Tensor] = None,
+                    kv_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T + mask) v with encoder states [B, Hk, Sk, D] of another length, masks and key counts."""
+    from difflet_b200.ops.attn import cross_attention as _cross
+
+    return _cross(q, k, v, scale=scale, attention_mask=attention_mask, kv_lens=kv_lens)
+
+
+@cross_attention.register_fake
+def _(q, k, v, scale, attention_mask=None, kv_lens=None):
+    return torch.empty_like(q)
+
+
+OPS = ("attention", "linear", "linear_gate_resid", "ln_modulate", "rms_norm", "quantize_mx", "linear_mx", "gemv",
+       "add_rms_norm", "cross_attention")
 
 __all__ = list(OPS)

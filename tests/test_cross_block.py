@@ -94,6 +94,21 @@ def test_layer_kernels_and_graph(native):
     assert torch.equal(cap, step())
 
 
+def test_dispatcher_ops():
+    from difflet_b200.ops import library  # noqa: F401  (registers the ops)
+
+    g = torch.Generator().manual_seed(0)
+    x, r, w = torch.randn(5, 32, generator=g), torch.randn(5, 32, generator=g), torch.randn(32, generator=g)
+    y, s = torch.ops.difflet.add_rms_norm(x, r, w)
+    want = ops.add_rms_norm(x, r, w)
+    assert torch.equal(y, want[0]) and torch.equal(s, want[1])
+    q, k = torch.randn(2, 4, 3, 16, generator=g), torch.randn(2, 2, 7, 16, generator=g)
+    lens = torch.tensor([7, 2])
+    assert torch.equal(torch.ops.difflet.cross_attention(q, k, k, 0.25, None, lens), ops.cross_attention(q, k, k, scale=0.25, kv_lens=lens))
+    for op, args in ((torch.ops.difflet.add_rms_norm, (x, r, w)), (torch.ops.difflet.cross_attention, (q, k, k, 0.25, None, lens))):
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+
+
 @pytest.mark.gpu
 def test_norm_feeds_both_projections(native):
     """One residual norm in bf16 for the adapters and one in MXFP8 for the block-scaled projection agree."""
