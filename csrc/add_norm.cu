@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(AddNo
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) sq += red[w];
   }
-  const float rstd = rsqrtf(sq / (float)a.D + a.eps);
+  const float rstd = __frsqrt_rn(sq / (float)a.D + a.eps);  // one rounding: it scales a whole row
   const float *sc = nullptr, *sh = nullptr;
   if (a.n_mod > 0) {
     const int b = a.row_map ? a.row_map[row] : (int)(row / a.rows_per_batch);

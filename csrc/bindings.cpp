@@ -591,7 +591,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   if (!fits(v_)) v_ = v_.contiguous();
   auto stride = [](const at::Tensor& t, int d) { return (long long)(t.size(d) == 1 ? t.size(3) : t.stride(d)); };
   const bool direct = fits(o);
-  at::Tensor o_ = direct ? o : at::empty(o.sizes(), o.options());
+  at::Tensor o_ = direct ? o : new_like(o, o.sizes(), o.scalar_type());
   a.q = q_.data_ptr(), a.k = k_.data_ptr(), a.v = v_.data_ptr(), a.o = o_.data_ptr();
   a.q_bs = stride(q_, 0), a.q_hs = stride(q_, 1), a.q_ss = stride(q_, 2);
   a.k_bs = stride(k_, 0), a.k_hs = stride(k_, 1), a.k_ss = stride(k_, 2);
@@ -624,13 +624,16 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   a.kv_hi = edge(kv_hi, "kv_lens", edges[1]);
   at::Tensor m, aux;
   int mdt = 0;  // -1: boolean, else the type of an additive mask
+  long long ms[4] = {0, 0, 0, 0};
   if (const at::Tensor* mt = given(mask)) {
     TORCH_CHECK_VALUE(mt->device() == q.device(), "the mask must be on q's device");
     const int64_t want[4] = {a.B, a.H, a.Sq, a.Sk};
     bool fit = mt->dim() <= 4;
     for (int64_t d = 0; fit && d < mt->dim(); ++d) fit = mt->size(-1 - d) == 1 || mt->size(-1 - d) == want[3 - d];
     TORCH_CHECK_VALUE(fit, "attention_mask ", mt->sizes(), " does not broadcast to [", a.B, ", ", a.H, ", ", a.Sq, ", ", a.Sk, "]");
-    m = mt->expand({a.B, a.H, a.Sq, a.Sk});
+    m = *mt;
+    for (int64_t d = 0; d < m.dim(); ++d)  // strides of the mask as [B, H, Sq, Sk], 0 where it is broadcast
+      ms[3 - d] = m.size(-1 - d) == 1 ? 0 : m.stride(-1 - d);
     mdt = m.scalar_type() == at::kBool ? -1 : dtype_code(m, "an additive mask");
   }
   if (a.H / a.Hk * (int64_t)a.Sq <= 16 && a.B <= 65535 && a.Hk <= 65535) {  // too few rows to fill a tile: the keys are split instead
@@ -645,7 +648,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     if (m.defined()) {
       d.mask = m.data_ptr();
       d.mask_dtype = mdt;
-      d.m_bs = m.stride(0), d.m_hs = m.stride(1), d.m_qs = m.stride(2), d.m_ks = m.stride(3);
+      d.m_bs = ms[0], d.m_hs = ms[1], d.m_qs = ms[2], d.m_ks = ms[3];
     }
     DFL_CHECK_RC(dfl_cross_decode(&d, cur_stream()), "cross_attention (few queries)");
     if (!direct) o.copy_(o_);
@@ -654,7 +657,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   if (m.defined() && mdt < 0) {
     MaskBitsArgs b{};
     b.mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
-    b.bs = m.stride(0), b.hs = m.stride(1), b.qs = m.stride(2), b.ks = m.stride(3);
+    b.bs = ms[0], b.hs = ms[1], b.qs = ms[2], b.ks = ms[3];
     b.B = b.bs ? a.B : 1, b.H = b.hs ? a.H : 1, b.Q = b.qs ? a.Sq : 1, b.Sk = a.Sk;
     b.words = (a.Sk + 127) / 128 * 4;
     const int64_t n_bits = (int64_t)b.B * b.H * b.Q * b.words;
@@ -675,7 +678,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     BiasTileArgs t{};
     t.mask = m.data_ptr();
     t.dtype = mdt;
-    t.bs = m.stride(0), t.hs = m.stride(1), t.qs = m.stride(2), t.ks = m.stride(3);
+    t.bs = ms[0], t.hs = ms[1], t.qs = ms[2], t.ks = ms[3];
     t.B = t.bs ? a.B : 1, t.H = t.hs ? a.H : 1, t.Q = t.qs ? a.Sq : 1, t.Sk = a.Sk;
     t.out_f32 = m.scalar_type() != q.scalar_type();
     const int64_t nq = (t.Q + 31) / 32, nt = (t.Sk + 127) / 128, rows = t.Q > 1 ? 32 : 1, vec = t.out_f32 ? 32 : 16;
