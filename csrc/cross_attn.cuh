@@ -27,7 +27,9 @@
 // exponentials 180 at the SFU's).  What is left is the round trip of a Q tile (scores, exponentials, P, next
 // scores: 3650 cycles for 2 x 1024 of products), which two tiles do not fill, and the turn of the items.  Measured
 // and slower or equal: part of the exponentials on the FMA pipe (387 us), an MMA warp per Q tile (402), three K / V slots
-// with a larger output buffer (388), the second half of a row kept in registers past the first P (348).
+// with a larger output buffer (388), the second half of a row kept in registers past the first P (348), the first
+// quarter's exponentials under the old maximum while the new one is found (362), both P V before the new scores at
+// the turn of an item (366).
 //
 // Masks: a key window [lo, hi) per batch row (tiles outside it are skipped), bits (kBits: packed
 // by cross_mask_bits, per query or shared by all queries) or an additive bias (kBias16 / kBias32).
