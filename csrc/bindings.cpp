@@ -650,6 +650,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
       d.mask_dtype = mdt;
       d.m_bs = ms[0], d.m_hs = ms[1], d.m_qs = ms[2], d.m_ks = ms[3];
     }
+    d.err = err_ptr();
     DFL_CHECK_RC(dfl_cross_decode(&d, cur_stream()), "cross_attention (few queries)");
     if (!direct) o.copy_(o_);
     return o;

@@ -1,19 +1,25 @@
 // Attention of a few queries to many keys (single tokens, pooling queries): at most 16 query rows
 // share a key head.  sm_100a.
 //
-// Bound by reading K and V once: a 128-row tensor-memory tile would be nearly empty, so the keys are
-// split over up to eight CTAs (one cluster per key head and batch row) of four warps, and each warp walks
-// its own 16-key blocks with a running maximum and sum.  Q K^T runs on the warp-level m16n8k16 matrix
-// instruction straight from registers: both operands take the head dimension in the same permuted
-// order (lane t of a quad holds 8 contiguous values of every 32), so every load is 16 contiguous bytes and nothing is
-// staged.  P V is f32 multiply-adds, a lane holding dh / 32 columns of every row, with P unrounded.  The partial
-// results are joined by log-sum-exp through distributed shared memory, in a fixed order.
+// Bound by reading K and V once: a 128-row tensor-memory tile would be nearly empty, so the keys are split over up
+// to sixteen CTAs (one cluster per key head and batch row).  In each, one warp keeps a ring of 32-key stages full with
+// tiled copies (64 KB in flight per CTA at dh 128, two CTAs per SM), and four warps walk 16-key blocks of them with
+// a running maximum and sum on the warp-level m16n8k16 matrix instruction.  S = Q K^T takes Q and K with the head
+// dimension in the same permuted order (lane t of a quad holds 8 contiguous values of every 32), 16 contiguous bytes
+// a load.  O^T += V^T P^T: a lane's P, rounded to the inputs' type as the instruction asks, is its second operand as it
+// stands, V is transposed on the way from shared memory, and eight query rows fill the instruction's narrow side.  The
+// partial results are joined by log-sum-exp through distributed shared memory, in a fixed order.
 //
-// 8 x 8 key heads of up to 3276 keys x 128, four query heads each: 25 us (84 MB, 3.4 TB/s; 13 us at the copy rate).
-// About 6 us of it are the launch and the joins; the rest runs at 4.4 TB/s, four CTAs of 128 registers per SM being
-// what the loads in flight allow.  Measured and slower: 32-key blocks with fewer CTAs (31 us), the next block's
-// loads issued into the registers as they come free (35 us).
+// 8 x 8 key heads of 4096 keys x 128, four query heads each, nothing in L2: 23.8 us (134 MB, 5.6 TB/s; 20.8 us at the copy
+// rate); 16384 keys 78 us (6.9 TB/s).  About 3.5 us are the launch, the first copies and the joins: 256 keys take 5 us.
+// Measured and slower at 4096 keys: K and V loaded straight into registers with P V as f32 multiply-adds (40 us,
+// bound by its instructions: 134 at 16384), the same arithmetic from the ring (41 us), eight such warps and a ring of
+// 128 KB in one CTA per SM (25.5 us, and 11.4 instead of 10.0 at 1024), a ring of six stages (24.4 us; six warps
+// on it 25.6 us), partial results read remotely instead of written (25.4 us; 17.5 instead of 6.3 for 16 rows of 64 keys).
 #include <cuda_fp16.h>
+
+#include <algorithm>
+#include <mutex>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -21,8 +27,11 @@
 namespace {
 using namespace dfl;
 
-constexpr int kWarps = 4, kMaxSplits = 8;
-constexpr int kKeys = 16;  // per warp and step: its K and V (8 KB at dh 128) are in flight together
+constexpr int kMaxSplits = 16;
+constexpr int kKeys = 16;  // per warp and step
+constexpr int kWarps = 4, kGroups = kWarps / 2;  // a pair of warps shares a stage, the pairs take the stages in turn
+constexpr int kStageKeys = 2 * kKeys, kStages = 4;
+static_assert(kStages % kGroups == 0, "a slot always serves the same warps, whose waits then follow every phase of it");
 constexpr float kLog2e = 1.4426950408889634f;
 
 DFL_DEVICE float exp2_sfu(float x) {
@@ -30,37 +39,21 @@ DFL_DEVICE float exp2_sfu(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-DFL_DEVICE uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-DFL_DEVICE void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-DFL_DEVICE float ld_cluster(const float* p, uint32_t rank) {
+DFL_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+DFL_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Stores to the same place in the shared memory of CTA `rank` of the cluster.
+DFL_DEVICE uint32_t cluster_addr(const void* p, uint32_t rank) {
   uint32_t a;
-  float v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
 }
-
-// Packed f32 pairs.
-DFL_DEVICE uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
+DFL_DEVICE void st_cluster(float2* p, uint32_t rank, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr(p, rank)), "f"(v.x), "f"(v.y) : "memory");
 }
-DFL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-DFL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
+DFL_DEVICE void st_cluster(float4* p, uint32_t rank, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr(p, rank)), "f"(v.x), "f"(v.y), "f"(v.z),
+               "f"(v.w)
+               : "memory");
 }
 
 template <bool F16>
@@ -77,12 +70,6 @@ DFL_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool F16>
-DFL_DEVICE float2 unpack2(uint32_t v) {
-  if constexpr (F16) return __half22float2(*reinterpret_cast<__half2*>(&v));
-  else return unpack_bf16x2(v);
-}
-
 // Score of (row, key) after the mask: -inf when excluded.
 DFL_DEVICE float masked_score(const DecodeArgs& a, float s, int b, int h, int q, int k) {
   const float z = s * a.scale;
@@ -95,235 +82,362 @@ DFL_DEVICE float masked_score(const DecodeArgs& a, float s, int b, int h, int q,
   return fmaf(s, a.scale, m);
 }
 
-// NR: rows held by the P V accumulators (4, 8 or 16).
-template <int DH, bool F16, int NR>
-__global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 4 : NR == 8 ? 3 : 2) cross_decode_kernel(const DecodeArgs a) {
-  constexpr int KC = DH / 32;  // 16-byte pieces of a key row per lane
-  constexpr int DL = DH / 32;  // output columns per lane
-  // P of the block a warp is at, every value twice (the packed multiply-add takes pairs); later this CTA's joined
-  // rows, read by the cluster
-  constexpr int kBuf = kWarps * NR * kKeys * 2 > NR * DH ? kWarps * NR * kKeys * 2 : NR * DH;
-  __shared__ __align__(16) float s_buf[kBuf];
-  float(*s_p)[NR][kKeys * 2] = reinterpret_cast<float(*)[NR][kKeys * 2]>(s_buf);
-  float(*c_o)[DH] = reinterpret_cast<float(*)[DH]>(s_buf);
-  __shared__ float s_f[kWarps][16];               // rescaling of the rows, then their maxima
-  __shared__ float s_l[kWarps][16];
-  __shared__ __align__(16) float s_o[kWarps][NR][DH];
-  __shared__ float c_m[16], c_l[16];
+template <bool F16>
+DFL_DEVICE uint32_t pack2(float lo, float hi) {
+  if constexpr (F16) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
 
+// What a part of the keys with maximum m and sum l counts in a whole of maximum mu.
+DFL_DEVICE float part_weight(float m, float l, float mu) { return m == -INFINITY && l == 0.f ? 0.f : exp2_sfu((m - mu) * kLog2e); }
+
+// Joins the warps' results (maxima and sums s_ml, rows s_o) in this CTA, then the CTAs of the cluster, and stores the
+// rows.  Every CTA writes its share of each quarter row into the CTA that stores it (c_o: R dh / splits values
+// from each, c_ml: every CTA's maxima and sums), so one cluster barrier is waited for and nothing is read remotely.
+template <int DH, bool F16, class SO>
+DFL_DEVICE void decode_join(const DecodeArgs& a, int R, const float2 (&s_ml)[kWarps][16], SO s_o, float4* c_o,
+                            float2 (&c_ml)[kMaxSplits][16]) {
+  const int splits = gridDim.x, split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, rep = a.H / a.Hk;
+  const int n4 = R * (DH / 4), share = n4 / splits;  // splits divides dh / 4
+  __syncthreads();
+  if (splits > 1) cluster_wait();  // every CTA of the cluster has started
+  for (int i = threadIdx.x; i < n4; i += blockDim.x) {
+    const int r = i / (DH / 4), d = i % (DH / 4) * 4;
+    float mx = s_ml[0][r].x;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, s_ml[w][r].x);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float4 ov = make_float4(0.f, 0.f, 0.f, 0.f);
+    float lv = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = part_weight(s_ml[w][r].x, s_ml[w][r].y, mu);
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
+      ov.x += f * x.x, ov.y += f * x.y, ov.z += f * x.z, ov.w += f * x.w;
+      lv += f * s_ml[w][r].y;
+    }
+    st_cluster(&c_o[split * share + i % share], i / share, ov);
+    // a row's pieces tell one CTA each of its maximum and sum (there are as many pieces as that or more)
+    if (d / 4 < splits) st_cluster(&c_ml[split][r], d / 4, make_float2(mx, lv));
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < share; i += blockDim.x) {
+    const int r = (split * share + i) / (DH / 4), d = (split * share + i) % (DH / 4) * 4;
+    float mx = -INFINITY;
+    for (int c = 0; c < splits; ++c) mx = fmaxf(mx, c_ml[c][r].x);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float4 ov = make_float4(0.f, 0.f, 0.f, 0.f);
+    float lv = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < splits; ++c) {
+      const float2 ml = c_ml[c][r];
+      const float f = part_weight(ml.x, ml.y, mu);
+      const float4 x = c_o[c * share + i];
+      ov.x += f * x.x, ov.y += f * x.y, ov.z += f * x.z, ov.w += f * x.w;
+      lv += f * ml.y;
+    }
+    const float inv = lv == 0.f ? 0.f : 1.f / lv;
+    const int h = hk * rep + r / a.Sq, q = r % a.Sq;
+    const uint2 y = make_uint2(pack2<F16>(ov.x * inv, ov.y * inv), pack2<F16>(ov.z * inv, ov.w * inv));
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + b * a.o_bs + (long long)h * a.o_hs + (long long)q * a.o_ss + d) = y;
+    if (a.lse && d == 0) a.lse[((long long)b * a.H + h) * a.Sq + q] = lv == 0.f ? -INFINITY : mx + logf(lv);
+  }
+}
+
+DFL_DEVICE void tma_load_4d(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+// Four 8 x 8 matrices of 16-bit values, transposed: lane l names row l % 8 of matrix l / 8.
+DFL_DEVICE void ldmatrix_x4_trans(uint32_t (&r)[4], const uint8_t* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p))
+               : "memory");
+}
+// NB: blocks of eight query rows.  The last warp fills the ring.
+template <int DH, bool F16, int NB>
+__global__ void __launch_bounds__(32 * (kWarps + 1), 2)
+    cross_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const DecodeArgs a) {
+  constexpr int KC = DH / 32, DT = DH / 16;
+  constexpr int kTile = kStageKeys * DH * 2, kChunk = kStageKeys * 128;
+  static_assert(kWarps * 8 * NB * DH * 4 <= kStages * 2 * kTile, "the warps' results take the stages' place");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float(*s_o)[8 * NB][DH] = reinterpret_cast<float(*)[8 * NB][DH]>(smem);
+  __shared__ float2 s_ml[kWarps][16], c_ml[kMaxSplits][16];
+  __shared__ float4 c_o[2 * NB * DH];
+  __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ int aborted;
+  volatile int* abort_flag = &aborted;
+
+  if (gridDim.x > 1) cluster_arrive();  // waited for before the first remote write
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
   const int splits = gridDim.x, split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int rep = a.H / a.Hk, R = rep * a.Sq;
   const int lo = a.kv_lo ? max(0, a.kv_lo[b]) : 0, hi = a.kv_hi ? min(a.Sk, a.kv_hi[b]) : a.Sk;
-  const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k) + b * a.k_bs + hk * a.k_hs;
-  const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + b * a.v_bs + hk * a.v_hs;
-  auto head_of = [&](int r) { return hk * rep + r / a.Sq; };
-  auto query_of = [&](int r) { return r % a.Sq; };
-
-  uint4 qf[KC][2];  // rows quad and quad + 8
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = quad + 8 * i;
-    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_bs + (long long)head_of(r) * a.q_hs +
-                         (long long)query_of(r) * a.q_ss;
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-      qf[c][i] = r < R ? *reinterpret_cast<const uint4*>(qp + 32 * c + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
+  const int nb = hi > lo ? (hi - lo + kStageKeys - 1) / kStageKeys : 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 2);
+    aborted = 0;
+    fence_barrier_init();
+    fence_proxy_async_shared();
   }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  uint64_t o[NR][DL / 2];  // pairs of columns
-#pragma unroll
-  for (int r = 0; r < NR; ++r)
-#pragma unroll
-    for (int d = 0; d < DL / 2; ++d) o[r][d] = 0ull;
+  __syncthreads();
 
-  // blocks of the window, dealt to the warps of all splits in turn
-  const int nb = hi > lo ? (hi - lo + kKeys - 1) / kKeys : 0;
-  for (int blk = split * kWarps + warp; blk < nb; blk += splits * kWarps) {
-    const int k0 = lo + blk * kKeys, left = hi - k0;  // keys of this block (kKeys or more: all)
-    uint4 kf[kKeys / 8][KC];
-    const uint16_t* kb = kp + (long long)(k0 + quad) * a.k_ss + 8 * t;
+  if (warp == kWarps) {
+    if (lane == 0) {
+      int i = 0;
+      for (int blk = split; blk < nb; blk += splits, ++i) {
+        const int slot = i % kStages, k0 = lo + blk * kStageKeys;
+        if (!mbar_wait(&empty[slot], ((i / kStages) & 1) ^ 1u, a.err, kKidCross, 150 + slot, abort_flag)) break;
+        uint8_t* st = smem + slot * 2 * kTile;
+        mbar_arrive_expect_tx(&full[slot], 2 * kTile);
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n)
+        for (int c = 0; c < DH / 64; ++c) tma_load_4d(st + c * kChunk, &tk, &full[slot], 64 * c, k0, hk, b);
+#pragma unroll
+        for (int c = 0; c < DH / 64; ++c) tma_load_4d(st + kTile + c * kChunk, &tv, &full[slot], 64 * c, k0, hk, b);
+      }
+      for (int k = max(0, i - kStages); k < i; ++k)  // every copy has landed before the stages are used otherwise
+        mbar_wait(&full[k % kStages], (k / kStages) & 1, nullptr, 0, 0, nullptr, 200000000LL);
+    }
+    __syncwarp();
+    __syncthreads();
+  } else {
+    uint4 qf[KC][NB];  // rows quad and quad + 8
+    int hrow[NB], qrow[NB];
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+      const int r = quad + 8 * h;
+      hrow[h] = hk * rep + r / a.Sq, qrow[h] = r % a.Sq;
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_bs + (long long)hrow[h] * a.q_hs +
+                           (long long)qrow[h] * a.q_ss;
 #pragma unroll
       for (int c = 0; c < KC; ++c)
-        kf[n][c] = 8 * n + quad < left ? __ldg(reinterpret_cast<const uint4*>(kb + 8 * n * a.k_ss + 32 * c)) : make_uint4(0u, 0u, 0u, 0u);
-    uint32_t vf[kKeys][DL / 2];  // on its way during the scores
-    const uint16_t* vb = vp + (long long)k0 * a.v_ss + lane * DL;
-#pragma unroll
-    for (int k = 0; k < kKeys; ++k) {
-      if constexpr (DL == 4) {
-        const uint2 x = k < left ? __ldg(reinterpret_cast<const uint2*>(vb + k * a.v_ss)) : make_uint2(0u, 0u);
-        vf[k][0] = x.x, vf[k][1] = x.y;
-      } else {
-        vf[k][0] = k < left ? __ldg(reinterpret_cast<const uint32_t*>(vb + k * a.v_ss)) : 0u;
-      }
+        qf[c][h] = r < R ? *reinterpret_cast<const uint4*>(qp + 32 * c + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
     }
-    float s[kKeys / 8][4];
+    float m[NB], l[NB];
+    float o[NB][DT][4];  // [2 j + e]: column 16 dt + quad + 8 j of row 8 h + 2 t + e
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int h = 0; h < NB; ++h) {
+      m[h] = -INFINITY, l[h] = 0.f;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        mma16816<F16>(s[n], qf[c][0].x, qf[c][1].x, qf[c][0].y, qf[c][1].y, kf[n][c].x, kf[n][c].y);
-        mma16816<F16>(s[n], qf[c][0].z, qf[c][1].z, qf[c][0].w, qf[c][1].w, kf[n][c].z, kf[n][c].w);
-      }
+      for (int d = 0; d < DT; ++d) o[h][d][0] = o[h][d][1] = o[h][d][2] = o[h][d][3] = 0.f;
     }
-    // s[n][2 i + e]: row quad + 8 i, key 8 n + 2 t + e
-#pragma unroll
-    for (int i = 0; i < (NR + 7) / 8; ++i) {
-      const int r = quad + 8 * i;
-      if (8 * i >= R) continue;  // (uniform: no row of this half exists)
-      const int h = head_of(r), q = query_of(r);
-      float mx = m[i];
-#pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = 8 * n + 2 * t + e;
-          float& z = s[n][2 * i + e];
-          z = r < R && key < left ? masked_score(a, z, b, h, q, k0 + key) : -INFINITY;
-          mx = fmaxf(mx, z);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mu = mx == -INFINITY ? 0.f : mx;
-      const float f = m[i] == -INFINITY ? 0.f : exp2_sfu((m[i] - mu) * kLog2e);
-      m[i] = mx;
-      l[i] *= f;
-#pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n) {
-        const float p0 = exp2_sfu((s[n][2 * i] - mu) * kLog2e), p1 = exp2_sfu((s[n][2 * i + 1] - mu) * kLog2e);
-        l[i] += p0 + p1;
-        if (r < NR) *reinterpret_cast<float4*>(&s_p[warp][r][2 * (8 * n + 2 * t)]) = make_float4(p0, p0, p1, p1);
-      }
-      if (t == 0) s_f[warp][r] = f;
-    }
-    __syncwarp();
-    if (a.mask != nullptr && a.mask_dtype < 0) {
-      // a key that no row keeps adds nothing, whatever V holds there
-#pragma unroll
-      for (int k = 0; k < kKeys; ++k) {
-        float any = 0.f;
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-          if (r < R) any += s_p[warp][r][2 * k];
-#pragma unroll
-        for (int d = 0; d < DL / 2; ++d) vf[k][d] = any == 0.f ? 0u : vf[k][d];
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      if (r >= R) continue;
-      const float f = s_f[warp][r];
-#pragma unroll
-      for (int d = 0; d < DL / 2; ++d) o[r][d] = f2_mul(o[r][d], f2_pack(f, f));
-    }
-#pragma unroll
-    for (int k = 0; k < kKeys; k += 2) {
-      uint64_t v0[DL / 2], v1[DL / 2];
-#pragma unroll
-      for (int d = 0; d < DL / 2; ++d) {
-        const float2 x = unpack2<F16>(vf[k][d]), y = unpack2<F16>(vf[k + 1][d]);
-        v0[d] = f2_pack(x.x, x.y), v1[d] = f2_pack(y.x, y.y);
-      }
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        if (r >= R) continue;
-        const ulonglong2 p = *reinterpret_cast<const ulonglong2*>(&s_p[warp][r][2 * k]);
-#pragma unroll
-        for (int d = 0; d < DL / 2; ++d) o[r][d] = f2_fma(p.y, v1[d], f2_fma(p.x, v0[d], o[r][d]));
-      }
-    }
-    __syncwarp();
-  }
+    const bool by_bool = a.mask != nullptr && a.mask_dtype < 0;
+    // row and 16-byte piece that this lane names to ldmatrix: columns + 0 | + 8 of keys 0-7, then of keys 8-15
+    const int vrow = (lane / 16) * 8 + lane % 8, vcol = lane / 8 % 2;
 
-  // join the warps of this CTA, then the CTAs of the cluster
+    int i = 0;
+    for (int blk = split; blk < nb; blk += splits, ++i) {
+      if (i % kGroups != warp / 2) continue;
+      const int slot = i % kStages, row0 = 16 * (warp % 2), k0 = lo + blk * kStageKeys + row0, left = hi - k0;
+      if (!mbar_wait(&full[slot], (i / kStages) & 1, a.err, kKidCross, 160 + slot, abort_flag)) break;
+      if (left > 0) {
+        // 128-byte rows in the copies' swizzle: 16-byte piece p of row r lies at p ^ (r % 8)
+        uint8_t* st = smem + slot * 2 * kTile + row0 * 128;
+        float s[2][4], s2[2][4];  // two chains of products each: the instruction's latency is what one alone would show
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (t == 0) s_f[warp][quad + 8 * i] = m[i], s_l[warp][quad + 8 * i] = l[i];
-  }
+        for (int n = 0; n < 2; ++n) {
 #pragma unroll
-  for (int r = 0; r < NR; ++r)
+          for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
-    for (int d = 0; d < DL / 2; ++d) *reinterpret_cast<uint64_t*>(&s_o[warp][r][lane * DL + 2 * d]) = o[r][d];
-  __syncthreads();
-  for (int i = threadIdx.x; i < R * DH; i += 32 * kWarps) {
-    const int r = i / DH, d = i % DH;
-    float mx = s_f[0][r];
+          for (int c = 0; c < KC; ++c) {
+            const uint4 k = *reinterpret_cast<const uint4*>(st + (c / 2) * kChunk + (8 * n + quad) * 128 + ((((c & 1) * 4 + t) ^ quad) * 16));
+            const uint4 q0 = qf[c][0], q1 = NB == 2 ? qf[c][NB - 1] : make_uint4(0u, 0u, 0u, 0u);
+            mma16816<F16>(s[n], q0.x, q1.x, q0.y, q1.y, k.x, k.y);
+            mma16816<F16>(s2[n], q0.z, q1.z, q0.w, q1.w, k.z, k.w);
+          }
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, s_f[w][r]);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float ov = 0.f, lv = 0.f;
+          for (int e = 0; e < 2 * NB; ++e) s[n][e] += s2[n][e];
+        }
+        // s[n][2 h + e]: row quad + 8 h, key 8 n + 2 t + e
+        const bool plain = a.mask == nullptr && left >= kKeys;  // (rows past R are not stored, whatever they hold)
+        float f[NB];
+        bool moved = false;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (s_f[w][r] == -INFINITY && s_l[w][r] == 0.f) continue;
-      const float f = exp2_sfu((s_f[w][r] - mu) * kLog2e);
-      ov += f * s_o[w][r][d];
-      lv += f * s_l[w][r];
+        for (int h = 0; h < NB; ++h) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = 8 * n + 2 * t + e;
+              float& z = s[n][2 * h + e];
+              if (plain) z *= a.scale;
+              else z = quad + 8 * h < R && key < left ? masked_score(a, z, b, hrow[h], qrow[h], k0 + key) : -INFINITY;
+              mx = fmaxf(mx, z);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          // the old maximum serves until it is exceeded by 5 (P stays below 2^8, the sums are exact all the same)
+          f[h] = 1.f;
+          if (mx > m[h] + 5.f) {
+            f[h] = m[h] == -INFINITY ? 0.f : exp2_sfu((m[h] - mx) * kLog2e);
+            m[h] = mx;
+            moved = true;
+          }
+        }
+        uint32_t keep[2][2];
+        if (by_bool) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              keep[n][e] = __ballot_sync(0xffffffffu, s[n][e] != -INFINITY || (NB == 2 && s[n][2 + e] != -INFINITY));
+        }
+        uint32_t p[NB][2];
+#pragma unroll
+        for (int h = 0; h < NB; ++h) {
+          const float mu = m[h] == -INFINITY ? 0.f : m[h];
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float p0 = exp2_sfu((s[n][2 * h] - mu) * kLog2e), p1 = exp2_sfu((s[n][2 * h + 1] - mu) * kLog2e);
+            sum += p0 + p1;
+            p[h][n] = pack2<F16>(p0, p1);
+          }
+          l[h] = l[h] * f[h] + sum;
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int h = 0; h < NB; ++h) {
+            const float f0 = __shfl_sync(0xffffffffu, f[h], 8 * t), f1 = __shfl_sync(0xffffffffu, f[h], 8 * t + 4);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[h][d][0] *= f0, o[h][d][1] *= f1, o[h][d][2] *= f0, o[h][d][3] *= f1;
+          }
+        }
+        uint8_t* sv = st + kTile;
+        if (left < kKeys || by_bool) {
+          // what V holds at keys that no row keeps is not used: those rows become 0 (a product with P = 0 would
+          // pass a NaN on)
+          bool drop = lane < 16 && lane >= left;
+          if (by_bool && lane < 16) {
+            const uint32_t any = lane < 8 ? (lane & 1 ? keep[0][1] : keep[0][0]) : (lane & 1 ? keep[1][1] : keep[1][0]);
+            drop = drop || !(any & (0x11111111u << (lane % 8 / 2)));
+          }
+          if (drop)
+#pragma unroll
+            for (int c = 0; c < DH / 8; ++c)
+              *reinterpret_cast<uint4*>(sv + (c / 8) * kChunk + lane * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_shared();  // before the stage's next copy
+          __syncwarp();
+        }
+        // O^T += V^T P^T: P is laid out as the instruction's second operand already, V is transposed on its way
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          uint32_t v[4];
+          const int piece = 2 * d + vcol;  // of 8 columns
+          ldmatrix_x4_trans(v, sv + (piece / 8) * kChunk + vrow * 128 + (((piece % 8) ^ (vrow & 7)) * 16));
+#pragma unroll
+          for (int h = 0; h < NB; ++h) mma16816<F16>(o[h][d], v[0], v[1], v[2], v[3], p[h][0], p[h][1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    c_o[r][d] = ov;
-    if (d == 0) c_m[r] = mx, c_l[r] = lv;
-  }
-  __syncthreads();
-  if (splits > 1) cluster_sync();
-  for (int i = threadIdx.x + 32 * kWarps * split; i < R * DH; i += 32 * kWarps * splits) {
-    const int r = i / DH, d = i % DH;
-    // all remote reads first: they are independent, and each takes most of a microsecond
-    float mc[kMaxSplits], lc[kMaxSplits], oc[kMaxSplits];
-    float mx = -INFINITY;
+    __syncwarp();
+    __syncthreads();  // every stage has been read: the results take their place
 #pragma unroll
-    for (int c = 0; c < kMaxSplits; ++c) {
-      const bool in = c < splits;
-      mc[c] = in ? (splits > 1 ? ld_cluster(&c_m[r], c) : c_m[r]) : -INFINITY;
-      lc[c] = in ? (splits > 1 ? ld_cluster(&c_l[r], c) : c_l[r]) : 0.f;
-      oc[c] = in ? (splits > 1 ? ld_cluster(&c_o[r][d], c) : c_o[r][d]) : 0.f;
+    for (int h = 0; h < NB; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (t == 0) s_ml[warp][quad + 8 * h] = make_float2(m[h], l[h]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_o[warp][8 * h + 2 * t + j % 2][16 * d + quad + 8 * (j / 2)] = o[h][d][j];
     }
-#pragma unroll
-    for (int c = 0; c < kMaxSplits; ++c) mx = fmaxf(mx, mc[c]);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float ov = 0.f, lv = 0.f;
-#pragma unroll
-    for (int c = 0; c < kMaxSplits; ++c) {
-      if (mc[c] == -INFINITY && lc[c] == 0.f) continue;
-      const float f = exp2_sfu((mc[c] - mu) * kLog2e);
-      ov += f * oc[c];
-      lv += f * lc[c];
-    }
-    const float y = lv == 0.f ? 0.f : ov / lv;
-    const long long at = b * a.o_bs + (long long)head_of(r) * a.o_hs + (long long)query_of(r) * a.o_ss + d;
-    if constexpr (F16) reinterpret_cast<__half*>(a.o)[at] = __float2half_rn(y);
-    else reinterpret_cast<__nv_bfloat16*>(a.o)[at] = __float2bfloat16_rn(y);
-    if (a.lse && d == 0)
-      a.lse[((long long)b * a.H + head_of(r)) * a.Sq + query_of(r)] = lv == 0.f ? -INFINITY : mx + logf(lv);
   }
-  if (splits > 1) cluster_sync();  // no CTA leaves while its results may be read
+  decode_join<DH, F16>(a, R, s_ml, s_o, c_o, c_ml);
 }
 
-template <int DH, bool F16, int NR>
-int launch_decode(const DecodeArgs* a, int splits, cudaStream_t stream) {
+int decode_tmap(CUtensorMap* map, const void* base, const DecodeArgs* a, long long ss, long long hs, long long bs) {
+  dfl_host::EncodeTiledFn fn = dfl_host::get_encode_tiled();
+  if (!fn) return 999;
+  cuuint64_t dims[4] = {(cuuint64_t)a->dh, (cuuint64_t)a->Sk, (cuuint64_t)a->Hk, (cuuint64_t)a->B};
+  cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)hs * 2, (cuuint64_t)bs * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)kStageKeys, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return (int)fn(map, a->f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
+                 dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+// Clusters of 1, 2, 4, 8 or 16 CTAs that are resident together (0: this size cannot be launched), found once per device.
+struct Resident {
+  int clusters[5] = {0, 0, 0, 0, 0};
+  cudaError_t err = cudaSuccess;
+  std::once_flag once;
+};
+
+template <int DH, bool F16, int NB>
+int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
+  static Resident resident[16];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  auto kern = cross_decode_kernel<DH, F16, NB>;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits, a->Hk, a->B);
-  cfg.blockDim = dim3(32 * kWarps, 1, 1);
+  cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
+  cfg.dynamicSmemBytes = kStages * 2 * kStageKeys * DH * 2 + 1024;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = splits;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, cross_decode_kernel<DH, F16, NR>, *a);
+  Resident& res = resident[dev & 15];
+  std::call_once(res.once, [&] {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    for (int i = 0; i < 5 && e == cudaSuccess; ++i) {
+      at[0].val.clusterDim.x = 1 << i;
+      cfg.gridDim = dim3((unsigned)(1 << i), 1024, 1);
+      e = cudaOccupancyMaxActiveClusters(&res.clusters[i], kern, &cfg);
+    }
+    res.err = e;
+  });
+  if (res.err != cudaSuccess) return (int)res.err;
+  // CTAs per key head: each wave of clusters costs its keys per CTA and a launch, ramp and join worth about 300 keys of
+  // 128 values; no CTA gets less than a turn of its warps.  64 heads of 4096 keys take 4 (1, 2, 4, 8, 16: 52, 30, 24, 28,
+  // 42 us), 72 of 512 take 2 (9.0, 6.8, 9.6, 12.8, 25 us), 48 of 4096 x 64 take 8 (45, 25, 16, 12, 22 us), 480 of 1024
+  // take 1 (43, 53, 60, 87, 172 us).
+  const long long heads = (long long)a->B * a->Hk;
+  int splits = 1;
+  long long best = -1;
+  for (int i = 0; i < 5; ++i) {
+    const long long fit = res.clusters[i], keys = (a->Sk + (1 << i) - 1) >> i;
+    if (fit <= 0 || (i > 0 && keys < kGroups * kStageKeys)) continue;
+    const long long cost = (heads + fit - 1) / fit * (keys + 300 * 128 / DH);
+    if (best < 0 || cost < best) best = cost, splits = 1 << i;
+  }
+  CUtensorMap tk, tv;
+  int rc = decode_tmap(&tk, a->k, a, a->k_ss, a->k_hs, a->k_bs);
+  if (rc) return 1000 + rc;
+  rc = decode_tmap(&tv, a->v, a, a->v_ss, a->v_hs, a->v_bs);
+  if (rc) return 2000 + rc;
+  at[0].val.clusterDim.x = splits;
+  cfg.gridDim = dim3(splits, a->Hk, a->B);
+  return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, *a);
 }
 
 template <int DH, bool F16>
-int decode_rows(const DecodeArgs* a, int splits, cudaStream_t stream) {
-  const int R = a->H / a->Hk * a->Sq;
-  if (R <= 4) return launch_decode<DH, F16, 4>(a, splits, stream);
-  if (R <= 8) return launch_decode<DH, F16, 8>(a, splits, stream);
-  return launch_decode<DH, F16, 16>(a, splits, stream);
+int decode_rows(const DecodeArgs* a, cudaStream_t stream) {
+  if (a->H / a->Hk * a->Sq <= 8) return launch_decode<DH, F16, 1>(a, stream);
+  return launch_decode<DH, F16, 2>(a, stream);
 }
 
 }  // namespace
@@ -333,14 +447,10 @@ extern "C" int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream) {
   if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk || a->H / a->Hk * a->Sq > 16) return -3;
   if (a->B > 65535 || a->Hk > 65535) return -8;
   auto al16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
-  if (!al16(a->q) || !al16(a->k) || !al16(a->v)) return -4;
-  if ((a->q_ss | a->q_hs | a->q_bs | a->k_ss | a->k_hs | a->k_bs | a->v_ss | a->v_hs | a->v_bs) % 8) return -5;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  // CTAs per key head: as many as fill the SMs a few times over, each warp keeping a block or more
-  const long long heads = (long long)a->B * a->Hk, room = 4ll * dfl_host::num_sms(dev);
-  int splits = 1;
-  while (splits < kMaxSplits && heads * splits * 2 <= room && a->Sk >= splits * 2 * kWarps * kKeys) splits *= 2;
-  if (a->dh == 64) return a->f16 ? decode_rows<64, true>(a, splits, stream) : decode_rows<64, false>(a, splits, stream);
-  return a->f16 ? decode_rows<128, true>(a, splits, stream) : decode_rows<128, false>(a, splits, stream);
+  if (!al16(a->q) || !al16(a->k) || !al16(a->v) || !al16(a->o)) return -4;
+  if ((a->q_ss | a->q_hs | a->q_bs | a->k_ss | a->k_hs | a->k_bs | a->v_ss | a->v_hs | a->v_bs | a->o_ss | a->o_hs |
+       a->o_bs) % 8)
+    return -5;
+  if (a->dh == 64) return a->f16 ? decode_rows<64, true>(a, stream) : decode_rows<64, false>(a, stream);
+  return a->f16 ? decode_rows<128, true>(a, stream) : decode_rows<128, false>(a, stream);
 }

@@ -346,6 +346,7 @@ typedef struct DecodeArgs {
   const void* mask;                    // NULL, bool bytes (mask_dtype -1) or an additive mask
   int mask_dtype;
   long long m_bs, m_hs, m_qs, m_ks;
+  int* err;
 } DecodeArgs;
 int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream);
 

@@ -170,6 +170,55 @@ def test_kernel_ignores_masked_contents(native, kind, D):
     assert torch.equal(o, clean) and bool((o[3] == 0).all())
 
 
+# Up to 16 rows per key head: every way to share the keys among CTAs (one key to a turn of sixteen CTAs, more heads than
+# fit at once), one and two blocks of eight rows.
+FEW = [  # B, H, Hk, Sq, Sk, D
+    (2, 4, 4, 1, 1, 128), (2, 2, 1, 3, 63, 64), (1, 16, 1, 1, 129, 128), (3, 16, 2, 1, 1023, 64), (2, 8, 2, 2, 2081, 128), (1, 3, 3, 16, 4100, 64),
+    (1, 2, 1, 5, 5000, 128), (7, 64, 64, 1, 100, 128),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", [None, "lens", "keys", "head", "bias"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", FEW)
+def test_few_queries(native, B, H, Hk, Sq, Sk, D, kind, dtype):
+    q, k, v = _inputs(B, H, Hk, Sq, Sk, D, dtype, "cuda", 7 * Sq + Sk)
+    lens = mask = None
+    if kind == "lens":
+        lens = torch.tensor([(Sk, Sk // 3, 1, 0)[b % 4] for b in range(B)], device="cuda", dtype=torch.int32)
+    elif kind:
+        mask = _mask(kind, B, H, Sq, Sk, "cuda", dtype)
+    lse = torch.empty(B, H, Sq, device="cuda")
+    o = ops.cross_attention(q, k, v, scale=D ** -0.5, attention_mask=mask, kv_lens=lens, lse=lse)
+    _check(o, _ref(q, k, v, D ** -0.5, mask, lens), dtype, D, Sk, v.abs().max().item(), lse)
+    if kind == "lens":  # what lies behind a length is not used, whatever it holds
+        behind = (torch.arange(Sk, device="cuda") >= lens[:, None])[:, None, :, None]
+        k, v = k.masked_fill(behind, float("nan")), v.masked_fill(behind, float("inf"))
+    elif kind == "keys":
+        gone = ~mask.expand(B, 1, 1, Sk).transpose(2, 3)
+        k, v = k.masked_fill(gone, float("inf")), v.masked_fill(gone, float("nan"))
+    else:  # repeatable, and the same from other strides
+        k, v = k.contiguous(), v.contiguous()
+    assert torch.equal(o, ops.cross_attention(q, k, v, scale=D ** -0.5, attention_mask=mask, kv_lens=lens))
+    F._lib()
+    from difflet_b200 import _native
+
+    _native.check_device_errors()
+
+
+@pytest.mark.gpu
+def test_few_queries_rise(native):
+    """Scores that rise along the keys (the running maximum moves at almost every block), and rows that differ."""
+    B, H, Hk, Sq, Sk, D = 1, 8, 2, 4, 3000, 128
+    q, k, v = _inputs(B, H, Hk, Sq, Sk, D, torch.bfloat16, "cuda")
+    k[..., 0] = torch.arange(Sk, device="cuda") / 64
+    q[..., 0] = torch.arange(H, device="cuda")[:, None] - 2.0
+    lse = torch.empty(B, H, Sq, device="cuda")
+    o = ops.cross_attention(q, k, v, scale=0.5, lse=lse)
+    _check(o, _ref(q, k, v, 0.5), torch.bfloat16, D, Sk, v.abs().max().item(), lse)
+
+
 @pytest.mark.gpu
 def test_kernel_refusals(native):
     q, k, v = _inputs(2, 4, 2, 3, 5, 64, torch.bfloat16, "cuda")
