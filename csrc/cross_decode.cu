@@ -188,14 +188,15 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
   const int splits = gridDim.x, split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int rep = a.H / a.Hk, R = rep * a.Sq;
-  const int lo = a.kv_lo ? max(0, a.kv_lo[b]) : 0, hi = a.kv_hi ? min(a.Sk, a.kv_hi[b]) : a.Sk;
-  const int nb = hi > lo ? (hi - lo + kStageKeys - 1) / kStageKeys : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 2);
     aborted = 0;
     fence_barrier_init();
     fence_proxy_async_shared();
   }
+  griddep_wait();  // (launched while the kernel before it ends)
+  const int lo = a.kv_lo ? max(0, a.kv_lo[b]) : 0, hi = a.kv_hi ? min(a.Sk, a.kv_hi[b]) : a.Sk;
+  const int nb = hi > lo ? (hi - lo + kStageKeys - 1) / kStageKeys : 0;
   __syncthreads();
 
   if (warp == kWarps) {
@@ -394,9 +395,11 @@ int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
   cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
   cfg.dynamicSmemBytes = kStages * 2 * kStageKeys * DH * 2 + 1024;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   Resident& res = resident[dev & 15];
@@ -431,6 +434,7 @@ int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
   if (rc) return 2000 + rc;
   at[0].val.clusterDim.x = splits;
   cfg.gridDim = dim3(splits, a->Hk, a->B);
+  cfg.numAttrs = 2;
   return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, *a);
 }
 
