@@ -480,6 +480,22 @@ extern "C" int dfl_gemm_tile_rows(const GemmArgs* a) {
   return use_pair(&a, 1, split_ws_of(a, dev).floats > 0, dfl_host::num_sms(dev), &wide) ? 2 * BM : BM;
 }
 
+// CTAs of the launch `a` would get.
+extern "C" int dfl_gemm_ctas(const GemmArgs* a) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  bool wide;
+  const int sms = dfl_host::num_sms(dev);
+  const SplitWs ws = split_ws_of(a, dev);
+  const bool pair = use_pair(&a, 1, ws.floats > 0, sms, &wide);
+  const int bm = pair ? 2 * BM : BM, bn = pair || wide ? 256 : 128, ctas = pair ? 2 : 1;
+  const long long tiles = (long long)((a->M + bm - 1) / bm) * ((a->N + bn - 1) / bn);
+  int splits = 1;
+  if (ws.ws && a->epi != kEpiSwiGLU && a->epi != kEpiQkv && (!pair || dfl_gemm_pair_can_split(a->epi)))
+    split_model(tiles, ctas, (a->K + BK - 1) / BK, sms, pair ? kPairKbCost : 1.0, bn >= 256 ? kFixup256 : kFixup128, &splits);
+  return (int)std::min<long long>(tiles * splits * ctas, sms / ctas * ctas);
+}
+
 // One launch for `count` GEMMs that share the epilogue kind and output type.  The tile
 // shape (CTA pairs with 256 x 256 tiles, or one CTA with 128 x 256 / 128 x 128 tiles)
 // follows the first problem; the others are tiled the same way.

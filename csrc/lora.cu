@@ -80,6 +80,7 @@ DFL_DEVICE void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __global__ void __launch_bounds__(kThreads, 2)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ta, ShrinkParams p,
                        int* err) {
+  griddep_wait();    // (launched while the kernel before it ends)
   griddep_launch();  // the GEMM may start on x W^T; it waits for this kernel before its first adapter block
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -178,26 +179,28 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int j0 = 0, pass = 0; j0 < count; j0 += p.per_pass, ++pass) {
     const int nj = min(p.per_pass, count - j0), n = nj * p.rank;
     const int rows_per = (kBM + (int)ranks - 1) / (int)ranks, pitch = n + 4;
-    if (warp == 0) {
-      if (lane == 0) {
-        bool ok = true;
-        int i = it;
-        for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = i % stages;
-          uint8_t* sx = smem + s * stage_bytes;
+    if (warp == 0) {  // lane 0 copies x, each lane one adapter's rows (one thread alone takes 0.1 us a copy to issue them)
+      bool ok = true;
+      int i = it;
+      for (int kb = kb0; kb < kb1; ++kb, ++i) {
+        const int s = i % stages;
+        uint8_t* sx = smem + s * stage_bytes;
+        if (i >= early) ok = mbar_wait(&empty_bar[s], ((i / stages) & 1) ^ 1u, err, kKidLora, 20 + s, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) {
           if (i >= early) {
-            if (!mbar_wait(&empty_bar[s], ((i / stages) & 1) ^ 1u, err, kKidLora, 20 + s, abort_flag)) { ok = false; break; }
             mbar_expect_tx(&full_bar[s], kXBytes);
             tma_load_2d(sx, &tx, &full_bar[s], kb * kBK, (int)row0);
           }
           mbar_arrive_expect_tx(&full_bar[s], n * kBK * 2);
-          for (int j = 0; j < nj; ++j)
-            tma_load_2d(sx + kXBytes + j * p.rank * kBK * 2, &ta, &full_bar[s], kb * kBK, list[1 + j0 + j] * p.rank);
         }
-        if (!ok)  // our own copies must land before the CTA exits
-          for (int k = max(0, i - stages); k < i; ++k)
-            mbar_wait(&full_bar[k % stages], (k / stages) & 1, nullptr, 0, 0, nullptr, 200000000LL);
+        __syncwarp();
+        for (int j = lane; j < nj; j += 32)
+          tma_load_2d(sx + kXBytes + j * p.rank * kBK * 2, &ta, &full_bar[s], kb * kBK, list[1 + j0 + j] * p.rank);
       }
+      if (lane == 0 && i < it + kb1 - kb0)  // given up: our own copies must land before the CTA exits
+        for (int k = max(0, i - stages); k < i; ++k)
+          mbar_wait(&full_bar[k % stages], (k / stages) & 1, nullptr, 0, 0, nullptr, 200000000LL);
     } else if (warp == 1) {
       if (lane == 0) {
         const uint32_t idesc = make_idesc_bf16_f32(kBM, n);
@@ -303,7 +306,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 //   lora_rows_kernel    a CTA of 8 warps owns 16 output columns; its warps take 128-wide pieces of K in turn and
 //                       multiply on the warp-level m16n8k16 instruction, W as the 16-row operand straight
 //                       from global memory (both operands in the same permuted K order, so that a lane
-//                       loads 16 contiguous bytes); partial sums are added in warp order, then T B^T and the epilogue.
+//                       loads 16 contiguous bytes); partial sums are added in warp order, then T B^T and the epilogue,
+//                       a thread per output (16 lanes to a product and a row at a time: 16 x 2048 x 2048 14.8 us, now 6.7).
 // The second kernel is launched with programmatic serialisation: it streams W while T is computed and waits
 // for T only before it is used.
 // ---------------------------------------------------------------------------
@@ -343,6 +347,7 @@ DFL_DEVICE float dot8(const uint4& a, const uint4& b, float acc) {
 }
 
 __global__ void __launch_bounds__(256) lora_rows_t_kernel(RowsParams p, int* err) {
+  griddep_wait();
   griddep_launch();
   const int m = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   const int raw = __ldg(p.ids + (p.rows_per_id > 0 ? m / p.rows_per_id : m)), id = rows_id(p, m);
@@ -386,7 +391,6 @@ DFL_DEVICE uint4 ld_stream16(const uint4* p) {  // read once: no L1 allocation
 template <int NB>
 __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
   __shared__ float red[8][16][8 * NB + 1];
-  __shared__ float lora[16][8 * NB + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
   const int n0 = blockIdx.x * 16;
   const __nv_bfloat16* w0 = p.w + (long long)min(n0 + quad, p.N - 1) * p.ldw + 8 * t;
@@ -395,6 +399,7 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
 #pragma unroll
   for (int g = 0; g < NB; ++g) c[g][0] = c[g][1] = c[g][2] = c[g][3] = 0.f;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  int id = threadIdx.x / 16 < p.M ? rows_id(p, threadIdx.x / 16) : -1;  // of the row this thread stores
 #pragma unroll 2
   for (int k0 = warp * 128; k0 < p.K; k0 += 8 * 128) {
     uint4 a[4][2], b[4][NB];
@@ -424,33 +429,39 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) red[warp][quad + 8 * i][8 * g + 2 * t + e] = c[g][2 * i + e];
+  // T B^T: a thread takes whole products, of one column and every 16th row
+  const int n = threadIdx.x % 16, col = n0 + n;
+  auto b_row = [&](int id) { return reinterpret_cast<const uint4*>(p.b + ((long long)id * p.N + col) * p.rank); };
+  uint4 first[2];  // the adapter's first 16 values, on their way while the warps' sums are stored and T is waited for
+  if (col >= p.N) id = -1;
+  if (id >= 0) first[0] = __ldg(b_row(id)), first[1] = __ldg(b_row(id) + 1);
   griddep_wait();  // T is complete
-  {  // T B^T: 16 lanes share a column, 8 values of the rank each
-    const int n = threadIdx.x / 16, r0 = (threadIdx.x % 16) * 8;
-    for (int m = 0; m < p.M; ++m) {
-      const int id = rows_id(p, m);
-      float v = 0.f;
-      if (id >= 0 && r0 < p.rank && n0 + n < p.N) {
-        const uint4 bw = __ldg(reinterpret_cast<const uint4*>(p.b + ((long long)id * p.N + n0 + n) * p.rank + r0));
-        const float4 t0 = __ldcg(reinterpret_cast<const float4*>(p.t + m * p.rank + r0));
-        const float4 t1 = __ldcg(reinterpret_cast<const float4*>(p.t + m * p.rank + r0 + 4));
-        const float2 b0 = unpack_bf16x2(bw.x), b1 = unpack_bf16x2(bw.y), b2 = unpack_bf16x2(bw.z), b3 = unpack_bf16x2(bw.w);
-        v = ((b0.x * t0.x + b0.y * t0.y) + (b1.x * t0.z + b1.y * t0.w)) +
-            ((b2.x * t1.x + b2.y * t1.y) + (b3.x * t1.z + b3.y * t1.w));
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (threadIdx.x % 16 == 0) lora[n][m] = v;
-    }
-  }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * p.M; i += 256) {
-    const int n = i % 16, m = i / 16, col = n0 + n;
-    if (col >= p.N) continue;
+  if (col >= p.N) return;
+  for (int m = threadIdx.x / 16; m < p.M; m += 16) {
+    if (m >= 16) {
+      id = rows_id(p, m);
+      if (id >= 0) first[0] = __ldg(b_row(id)), first[1] = __ldg(b_row(id) + 1);
+    }
     float v = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v += red[k][n][m];
-    v += lora[n][m];
+    if (id >= 0) {
+      const uint4* bw = b_row(id);
+      const float4* t4 = reinterpret_cast<const float4*>(p.t + m * p.rank);
+      float acc[2] = {0.f, 0.f};
+#pragma unroll 2
+      for (int r = 0; r < p.rank / 8; r += 2)  // (a multiple of 16)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 w = r == 0 ? first[u] : __ldg(bw + r + u);
+          const float4 t0 = __ldcg(t4 + 2 * (r + u)), t1 = __ldcg(t4 + 2 * (r + u) + 1);
+          const float2 b0 = unpack_bf16x2(w.x), b1 = unpack_bf16x2(w.y), b2 = unpack_bf16x2(w.z), b3 = unpack_bf16x2(w.w);
+          acc[u] += ((b0.x * t0.x + b0.y * t0.y) + (b1.x * t0.z + b1.y * t0.w)) +
+                    ((b2.x * t1.x + b2.y * t1.y) + (b3.x * t1.z + b3.y * t1.w));
+        }
+      v += acc[0] + acc[1];
+    }
     if (p.bias) v += __bfloat162float(p.bias[col]);
     if (col >= p.act_lo && col < p.act_hi) {
       if (p.epi == kEpiGelu) v = gelu_tanh(v);
@@ -463,10 +474,11 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
   }
 }
 
-template <int NB>
-int launch_rows(const RowsParams& p, cudaStream_t stream) {
+// Launches 256-thread blocks that may start while the kernel before them ends (they wait for it themselves).
+template <class... Params, class... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.N + 15) / 16, 1, 1);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(256, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
@@ -474,7 +486,7 @@ int launch_rows(const RowsParams& p, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, lora_rows_kernel<NB>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 int lora_rows(const GemmArgs* a, cudaStream_t stream) {
@@ -497,12 +509,10 @@ int lora_rows(const GemmArgs* a, cudaStream_t stream) {
   p.resid = reinterpret_cast<const __nv_bfloat16*>(a->resid), p.ldr = a->ldr;
   p.M = a->M, p.N = a->N, p.K = a->K;
   if (p.epi == kEpiGateResid && (!p.gate || !p.resid)) return -8;
-  lora_rows_t_kernel<<<dim3(p.M, (p.rank + 7) / 8), 256, 0, stream>>>(p, a->err);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_early(lora_rows_t_kernel, dim3(p.M, (p.rank + 7) / 8), stream, p, a->err);
   if (e != cudaSuccess) return (int)e;
-  if (p.M <= 8) return launch_rows<1>(p, stream);
-  if (p.M <= 16) return launch_rows<2>(p, stream);
-  return launch_rows<4>(p, stream);
+  const auto kern = p.M <= 8 ? lora_rows_kernel<1> : p.M <= 16 ? lora_rows_kernel<2> : lora_rows_kernel<4>;
+  return (int)launch_early(kern, dim3((p.N + 15) / 16), stream, p);
 }
 
 }  // namespace
@@ -531,10 +541,12 @@ extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
   static int resident[16][9] = {{0}};
   int* fit = resident[dev & 15];
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.stream = stream;
   cfg.attrs = at;
@@ -579,11 +591,17 @@ extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
   int ranks = 1;  // the most CTAs a tile that are all resident, each with four K blocks or more
   for (int c = 2; c <= 8; ++c)
     if (tiles <= fit[c] && num_k >= 4 * c) ranks = c;
+  // Fewer where that leaves the GEMM's CTAs SMs of their own, whose loop over x then runs at the same time: a K block takes
+  // 0.8 us here and 0.28 us there, so the longer loop here has to be shorter than the one it hides (12 tiles beside 96
+  // CTAs, K 2048, 7 adapters: 8 CTAs a tile 32.7 us for both kernels, 4 beside the GEMM 25.9, 3 28.2, 2 32.5).
+  const long long beside = (fit[1] - dfl_gemm_ctas(a)) / tiles;
+  if (beside >= 1 && beside < ranks && 20 * (ranks - beside) < 7 * beside * ranks) ranks = (int)beside;
   p.region = tiles * ranks <= fit[1] ? kRegionOne : kRegionTwo;
   p.stages = std::min(kMaxStages, p.region / (kXBytes + p.per_pass * l->rank * kBK * 2));
   cfg.gridDim = dim3((unsigned)(tiles * ranks), 1, 1);
   cfg.dynamicSmemBytes = p.region + kTail;
   at[0].val.clusterDim.x = ranks;
+  cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(&cfg, lora_shrink_kernel, tx, ta, p, a->err);
   if (e != cudaSuccess) return (int)e;
   return dfl_gemm_bf16(a, stream);
