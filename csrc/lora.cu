@@ -13,7 +13,7 @@
 //
 // The shrink is bound by reading x (2 M K bytes): a cluster of up to eight CTAs shares a tile, each
 // taking a range of K, so that few tiles still occupy many SMs; the f32 partial sums are added through
-// distributed shared memory in a fixed order.
+// distributed shared memory in a fixed order.  Where a tile's adapters take several passes, several such clusters share them.
 #include <algorithm>
 
 #include "common.cuh"
@@ -46,6 +46,7 @@ struct ShrinkParams {
   const float* scale;
   int n_adapters, rank, cap, tile_rows;
   int per_pass;  // adapters per pass: at most 128 accumulator columns
+  int tiles, slices;
   int region, stages;  // stages of kXBytes + per_pass * rank * 128 bytes
   __nv_bfloat16* t;
   int* list;
@@ -96,7 +97,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
-  const int tile = blockIdx.x / ranks;            // 128-row tile
+  const int tile = blockIdx.x / ranks % p.tiles;  // 128-row tile
+  const int slice = blockIdx.x / ranks / p.tiles; // of the tile's passes: every p.slices-th
   const int per_group = p.tile_rows / kBM;        // 128-row tiles per M tile of the GEMM
   const int group = tile / per_group;
   const long long row0 = (long long)tile * kBM, grow0 = (long long)group * p.tile_rows;
@@ -165,18 +167,19 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     slot[r] = (int16_t)s;
   }
-  if (rank == 0 && tile % per_group == 0)
+  if (rank == 0 && slice == 0 && tile % per_group == 0)
     for (int i = threadIdx.x; i <= count; i += kThreads) p.list[(long long)group * (1 + p.cap) + i] = i == 0 ? count : list[i];
   __syncthreads();
 
-  if (count == 0 && warp == 0 && lane == 0)  // no adapter: the early copies must land before the CTA exits
+  const int first = slice * p.per_pass;  // of the list
+  if (count <= first && warp == 0 && lane == 0)  // no adapter: the early copies must land before the CTA exits
     for (int i = 0; i < early; ++i) {
       mbar_arrive(&full_bar[i]);
       mbar_wait(&full_bar[i], 0, err, kKidLora, 50 + i, abort_flag);
     }
 
   int it = 0;  // stages used so far (all roles count alike)
-  for (int j0 = 0, pass = 0; j0 < count; j0 += p.per_pass, ++pass) {
+  for (int j0 = first, pass = 0; j0 < count; j0 += p.slices * p.per_pass, ++pass) {
     const int nj = min(p.per_pass, count - j0), n = nj * p.rank;
     const int rows_per = (kBM + (int)ranks - 1) / (int)ranks, pitch = n + 4;
     if (warp == 0) {  // lane 0 copies x, each lane one adapter's rows (one thread alone takes 0.1 us a copy to issue them)
@@ -587,18 +590,32 @@ extern "C" int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream) {
   p.per_pass = std::max(1, std::min(l->cap, 128 / l->rank));
   // every 128-row tile of every M tile (the last M tile's second half may lie behind M: zeros)
   const long long tiles = ((long long)a->M + l->tile_rows - 1) / l->tile_rows * (l->tile_rows / kBM);
-  const int num_k = (a->K + kBK - 1) / kBK;
-  int ranks = 1;  // the most CTAs a tile that are all resident, each with four K blocks or more
-  for (int c = 2; c <= 8; ++c)
-    if (tiles <= fit[c] && num_k >= 4 * c) ranks = c;
-  // Fewer where that leaves the GEMM's CTAs SMs of their own, whose loop over x then runs at the same time: a K block takes
-  // 0.8 us here and 0.28 us there, so the longer loop here has to be shorter than the one it hides (12 tiles beside 96
-  // CTAs, K 2048, 7 adapters: 8 CTAs a tile 32.7 us for both kernels, 4 beside the GEMM 25.9, 3 28.2, 2 32.5).
-  const long long beside = (fit[1] - dfl_gemm_ctas(a)) / tiles;
-  if (beside >= 1 && beside < ranks && 20 * (ranks - beside) < 7 * beside * ranks) ranks = (int)beside;
-  p.region = tiles * ranks <= fit[1] ? kRegionOne : kRegionTwo;
+  // How many CTAs share a tile's K, and how many clusters its passes, all of them resident.  In 0.1 us: a K block takes 8
+  // here and 3 in the GEMM, a join 30, launch and lists 60.  Where the GEMM's CTAs find SMs of their own beside, its loop
+  // over x runs at the same time; else after.  12 tiles beside 96 CTAs, K 2048, 7 adapters: 8 CTAs a tile 32.7 us for both
+  // kernels, 4 (beside) 25.9, 3 28.2, 2 32.5.  6 tiles of 12 passes, K 3648,
+  // rank 128: one cluster of 8 a tile 147 us, six of 4 53 us.
+  const int num_k = (a->K + kBK - 1) / kBK, passes = (l->cap + p.per_pass - 1) / p.per_pass;
+  const long long room = fit[1] - dfl_gemm_ctas(a), gemm = 30 + 3ll * num_k;
+  int ranks = 1;
+  long long slices = 1, best = -1;
+  for (int c = 1; c <= 8; ++c) {
+    if (c > 1 && (tiles > fit[c] || num_k < 4 * c)) continue;
+    auto consider = [&](long long sl, bool beside) {
+      sl = std::max(1ll, std::min<long long>(passes, sl));
+      const long long t = 60 + (passes + sl - 1) / sl * ((num_k + c - 1) / c * 8ll + (c > 1 ? 30 : 0));
+      const long long cost = beside ? std::max(t, gemm) + t / 4 : t + gemm;
+      if (best < 0 || cost < best) best = cost, ranks = c, slices = sl;
+    };
+    consider(fit[c] / tiles, false);
+    if (tiles * c <= room) consider(std::min<long long>(room / (tiles * c), fit[c] / tiles), true);
+  }
+  p.tiles = (int)tiles;
+  p.slices = (int)slices;
+  const long long ctas = tiles * ranks * slices;
+  p.region = ctas <= fit[1] ? kRegionOne : kRegionTwo;
   p.stages = std::min(kMaxStages, p.region / (kXBytes + p.per_pass * l->rank * kBK * 2));
-  cfg.gridDim = dim3((unsigned)(tiles * ranks), 1, 1);
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
   cfg.dynamicSmemBytes = p.region + kTail;
   at[0].val.clusterDim.x = ranks;
   cfg.numAttrs = 2;

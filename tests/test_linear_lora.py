@@ -143,6 +143,16 @@ def test_kernel(native, M, N, K, ranks, how):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["rows", "batch"])
+@pytest.mark.parametrize("M,N,K,ranks", [
+    (200, 384, 1280, [128] * 9), (664, 640, 2000, [128, 100] * 6), (90, 3200, 2880, [64] * 11), (1333, 2048, 2048, [8] * 7),  # passes shared out
+    (17, 24, 72, [48]), (32, 1000, 2056, [128, 3, 64]), (16, 2056, 520, [128, 80]),  # rows and columns at the ends of a thread's share
+])
+def test_kernel_passes_and_few_rows(native, M, N, K, ranks, how):
+    test_kernel(native, M, N, K, ranks, how)
+
+
+@pytest.mark.gpu
 def test_kernel_gated_residual_layouts(native):
     M, N, K = 600, 1024, 512
     x, w, b, A, B, scale = _make(M, N, K, [16, 32], "cuda")
