@@ -337,4 +337,20 @@ int make_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t d0, uint64_t 
                       uint64_t stride1_elems, uint64_t stride2_elems, uint32_t b0, uint32_t b1,
                       uint32_t b2, bool swizzle128);
 int num_sms(int device);
+// A launch that may start while the kernel before it ends (the kernel waits for that itself: griddep_wait).
+template <class... Params, class... Args>
+cudaError_t launch_early(void (*kernel)(Params...), unsigned grid, int threads, size_t smem, cudaStream_t stream,
+                         const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 }  // namespace dfl_host

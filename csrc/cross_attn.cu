@@ -8,6 +8,8 @@ namespace {
 // Bit rows of a boolean mask: one warp per (row, 32-key word), bits past the last key set (the key
 // window excludes those keys).  Rows are [B, H, Q] of the mask's own (unbroadcast) extents.
 __global__ void __launch_bounds__(256) cross_mask_bits_kernel(MaskBitsArgs a) {
+  griddep_wait();
+  griddep_launch();
   const long long n = (long long)a.B * a.H * a.Q * a.words;
   const int lane = threadIdx.x % 32;
   for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / 32; i < n;
@@ -27,6 +29,8 @@ __global__ void __launch_bounds__(256) cross_mask_bits_kernel(MaskBitsArgs a) {
 // A key mask ([B, 1, 1, Sk]): one block per batch row writes its bit row and the key window [first kept
 // key, last kept key + 1); a row that keeps nothing gets [0, 0).
 __global__ void __launch_bounds__(256) cross_key_mask_kernel(MaskBitsArgs a) {
+  griddep_wait();
+  griddep_launch();  // the attention sets itself up meanwhile
   __shared__ int s_lo[8], s_hi[8];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, b = blockIdx.x;
   int lo = a.Sk, hi = 0;
@@ -61,6 +65,8 @@ DFL_DEVICE float mask_value(const void* p, int dtype, long long at) {
 // rows (any stride, any alignment) would cost a line per query and load.
 template <bool F32>
 __global__ void __launch_bounds__(256) cross_bias_tiles_kernel(BiasTileArgs a) {
+  griddep_wait();
+  griddep_launch();
   constexpr int E = F32 ? 4 : 8, V = 128 / E;
   const int rows = a.Q > 1 ? 32 : 1, nq = (a.Q + 31) / 32, nt = (a.Sk + 127) / 128;
   const long long n = (long long)a.B * a.H * nq * nt * V * rows;
@@ -103,9 +109,7 @@ extern "C" int dfl_cross_bias_tiles(const BiasTileArgs* a, cudaStream_t stream) 
                       (a->Q > 1 ? 32 : 1);
   const long long blocks = (n + 255) / 256;
   const unsigned grid = (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32);
-  if (a->out_f32) cross_bias_tiles_kernel<true><<<grid, 256, 0, stream>>>(*a);
-  else cross_bias_tiles_kernel<false><<<grid, 256, 0, stream>>>(*a);
-  return (int)cudaGetLastError();
+  return (int)dfl_host::launch_early(a->out_f32 ? cross_bias_tiles_kernel<true> : cross_bias_tiles_kernel<false>, grid, 256, 0, stream, *a);
 }
 
 extern "C" int dfl_cross_mask_bits(const MaskBitsArgs* a, cudaStream_t stream) {
@@ -113,13 +117,11 @@ extern "C" int dfl_cross_mask_bits(const MaskBitsArgs* a, cudaStream_t stream) {
   if (a->words != (a->Sk + 127) / 128 * 4) return -3;
   if (a->lo) {
     if (a->H != 1 || a->Q != 1 || !a->hi) return -4;
-    cross_key_mask_kernel<<<(unsigned)a->B, 256, 0, stream>>>(*a);
-    return (int)cudaGetLastError();
+    return (int)dfl_host::launch_early(cross_key_mask_kernel, (unsigned)a->B, 256, 0, stream, *a);
   }
   const long long warps = (long long)a->B * a->H * a->Q * a->words;
   const long long blocks = (warps + 7) / 8;
-  cross_mask_bits_kernel<<<(unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, stream>>>(*a);
-  return (int)cudaGetLastError();
+  return (int)dfl_host::launch_early(cross_mask_bits_kernel, (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, stream, *a);
 }
 
 extern "C" int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream) {

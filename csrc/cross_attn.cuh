@@ -178,8 +178,8 @@ struct CrossItems {
   DFL_DEVICE void window(const CrossParams& p) {
     q0 = qb * (QT * kBM);
     if (b >= p.B) return;
-    lo = p.kv_lo ? max(0, __ldg(p.kv_lo + b)) : 0;
-    hi = p.kv_hi ? min(p.Sk, __ldg(p.kv_hi + b)) : p.Sk;
+    lo = p.kv_lo ? max(0, __ldcg(p.kv_lo + b)) : 0;
+    hi = p.kv_hi ? min(p.Sk, __ldcg(p.kv_hi + b)) : p.Sk;
     t0 = lo / kBN;
     n = hi > lo ? (hi + kBN - 1) / kBN - t0 : 0;
   }
@@ -188,7 +188,7 @@ struct CrossItems {
 // The words of key tile k0 for one row of a bit mask (whole 128-key groups are stored).
 template <class Item>
 DFL_DEVICE uint4 cross_bits(const CrossParams& p, const Item& it, int q, int k0) {
-  return __ldg(reinterpret_cast<const uint4*>(p.bits + it.b * p.bits_bs + it.h * p.bits_hs + q * p.bits_qs + k0 / 32));
+  return __ldcg(reinterpret_cast<const uint4*>(p.bits + it.b * p.bits_bs + it.h * p.bits_hs + q * p.bits_qs + k0 / 32));
 }
 
 // Whether tile k0 holds V rows of keys that no query of this batch row may see.
@@ -258,6 +258,8 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // (launched while the kernel before it, the mask's own among them, ends: what that writes is read past L1)
+  griddep_wait();
 
   // Register split for QT = 2: 128 x 64 + 256 x 216 = 63488 <= 384 x 168 at launch (checked by the
   // launcher); every warp of a warpgroup executes its setmaxnreg.
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
           bp = p.bias + it.b * p.bias_bs + it.h * p.bias_hs + (qc / 32) * p.bias_qs + (it.t0 + j) * p.bias_ts +
                (p.bias_rows > 1 ? qc % 32 : 0);
 #pragma unroll
-          for (int v = 0; v < 16; ++v) bv[v] = __ldg(bp + v * p.bias_rows);
+          for (int v = 0; v < 16; ++v) bv[v] = __ldcg(bp + v * p.bias_rows);
         }
         if (!mbar_wait(&s_full[g], s & 1, err, kKidCross, 120 + g, abort_flag)) { ok = false; break; }
         tc_fence_after();
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
                 float* zp = zc + 4 * v;
                 f2_unpack(f2_fma(f2_pack(zp[0], zp[1]), scale2, f2_pack(__uint_as_float(b.x), __uint_as_float(b.y))), zp[0], zp[1]);
                 f2_unpack(f2_fma(f2_pack(zp[2], zp[3]), scale2, f2_pack(__uint_as_float(b.z), __uint_as_float(b.w))), zp[2], zp[3]);
-                if (c < 2) b = __ldg(bp + (16 + 8 * c + v) * p.bias_rows);
+                if (c < 2) b = __ldcg(bp + (16 + 8 * c + v) * p.bias_rows);
               }
             }
           }
@@ -656,8 +658,7 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
   p.n_qb = (a->Sq + QT * kBM - 1) / (QT * kBM);
   const long long items = (long long)p.n_qb * a->H * a->B;
   const int sms = dfl_host::num_sms(dev);
-  kern<<<(unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream>>>(tq, tk, tv, to, p, a->err);
-  return (int)cudaGetLastError();
+  return (int)dfl_host::launch_early(kern, (unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream, tq, tk, tv, to, p, a->err);
 }
 
 // Two ping-pong Q tiles per CTA unless one holds every query, or twice the items still fit the SMs.

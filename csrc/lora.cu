@@ -81,7 +81,8 @@ DFL_DEVICE void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __global__ void __launch_bounds__(kThreads, 2)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ta, ShrinkParams p,
                        int* err) {
-  griddep_wait();    // (launched while the kernel before it ends)
+  // (launched while the kernel before it ends: what that may write is not read through the read-only path)
+  griddep_wait();
   griddep_launch();  // the GEMM may start on x W^T; it waits for this kernel before its first adapter block
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
 
   // the adapters used by the rows of the GEMM's M tile, ascending
-  auto id_of = [&](long long r) { return __ldg(p.ids + (p.rows_per_id > 0 ? r / p.rows_per_id : r)); };
+  auto id_of = [&](long long r) { return p.ids[p.rows_per_id > 0 ? r / p.rows_per_id : r]; };
   for (int r = threadIdx.x; r < p.tile_rows; r += kThreads) {
     if (grow0 + r >= p.M) continue;
     const int id = id_of(grow0 + r);
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           uint32_t v[16];
           tmem_ld_32x32b_x16(t_row + c, v);
           tmem_wait_ld();
-          const float f = __ldg(p.scale + list[1 + j]);
+          const float f = p.scale[list[1 + j]];
           const bool mine = have && slot[row] == j;
           uint32_t w[8];
 #pragma unroll
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             x += f.x, y += f.y;
           }
         const bool mine = slot[r0 + rl] == j;
-        const float f = __ldg(p.scale + list[1 + j]);
+        const float f = p.scale[list[1 + j]];
         *reinterpret_cast<uint32_t*>(p.t + (trow0 + (long long)j * p.tile_rows + r0 + rl) * p.rank + c % p.rank) =
             mine ? pack_bf16x2(f * x, f * y) : 0u;
       }
@@ -334,7 +335,7 @@ struct RowsParams {
 };
 
 DFL_DEVICE int rows_id(const RowsParams& p, int m) {
-  const int id = __ldg(p.ids + (p.rows_per_id > 0 ? m / p.rows_per_id : m));
+  const int id = p.ids[p.rows_per_id > 0 ? m / p.rows_per_id : m];
   return id >= 0 && id < p.n_adapters ? id : -1;
 }
 
@@ -352,10 +353,10 @@ DFL_DEVICE float dot8(const uint4& a, const uint4& b, float acc) {
 __global__ void __launch_bounds__(256) lora_rows_t_kernel(RowsParams p, int* err) {
   griddep_wait();
   griddep_launch();
-  const int m = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int raw = __ldg(p.ids + (p.rows_per_id > 0 ? m / p.rows_per_id : m)), id = rows_id(p, m);
+  const int m = blockIdx.x % p.M, r = blockIdx.x / p.M * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int raw = p.ids[p.rows_per_id > 0 ? m / p.rows_per_id : m], id = rows_id(p, m);
   if (id < 0) {
-    if (raw != -1 && blockIdx.y == 0 && threadIdx.x == 0) record_error(err, kErrBounds, kKidLora, 11, m);
+    if (raw != -1 && r == 0 && lane == 0) record_error(err, kErrBounds, kKidLora, 11, m);
     return;  // (its T is not read)
   }
   if (r >= p.rank) return;
@@ -367,13 +368,13 @@ __global__ void __launch_bounds__(256) lora_rows_t_kernel(RowsParams p, int* err
   for (; v + 96 < nv; v += 128) {
     uint4 xa[4], aa[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) xa[u] = __ldg(x + v + 32 * u), aa[u] = __ldg(a + v + 32 * u);
+    for (int u = 0; u < 4; ++u) xa[u] = __ldcg(x + v + 32 * u), aa[u] = __ldcg(a + v + 32 * u);
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc[u] = dot8(xa[u], aa[u], acc[u]);
   }
-  for (; v < nv; v += 32) acc[0] = dot8(__ldg(x + v), __ldg(a + v), acc[0]);
+  for (; v < nv; v += 32) acc[0] = dot8(__ldcg(x + v), __ldcg(a + v), acc[0]);
   const float sum = warp_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
-  if (lane == 0) p.t[m * p.rank + r] = sum * __ldg(p.scale + id);
+  if (lane == 0) p.t[m * p.rank + r] = sum * __ldcg(p.scale + id);
 }
 
 DFL_DEVICE void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -477,21 +478,6 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(RowsParams p) {
   }
 }
 
-// Launches 256-thread blocks that may start while the kernel before them ends (they wait for it themselves).
-template <class... Params, class... Args>
-cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 int lora_rows(const GemmArgs* a, cudaStream_t stream) {
   const LoraArgs* l = a->lora;
   if (a->gate_row_map || a->alpha != 1.f) return -27;
@@ -512,10 +498,10 @@ int lora_rows(const GemmArgs* a, cudaStream_t stream) {
   p.resid = reinterpret_cast<const __nv_bfloat16*>(a->resid), p.ldr = a->ldr;
   p.M = a->M, p.N = a->N, p.K = a->K;
   if (p.epi == kEpiGateResid && (!p.gate || !p.resid)) return -8;
-  const cudaError_t e = launch_early(lora_rows_t_kernel, dim3(p.M, (p.rank + 7) / 8), stream, p, a->err);
+  const cudaError_t e = dfl_host::launch_early(lora_rows_t_kernel, (unsigned)(p.M * ((p.rank + 7) / 8)), 256, 0, stream, p, a->err);
   if (e != cudaSuccess) return (int)e;
   const auto kern = p.M <= 8 ? lora_rows_kernel<1> : p.M <= 16 ? lora_rows_kernel<2> : lora_rows_kernel<4>;
-  return (int)launch_early(kern, dim3((p.N + 15) / 16), stream, p);
+  return (int)dfl_host::launch_early(kern, (unsigned)((p.N + 15) / 16), 256, 0, stream, p);
 }
 
 }  // namespace
