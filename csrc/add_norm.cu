@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT) add_rms_norm_kernel(AddNo
   __shared__ float red[kWarps > 1 ? kWarps : 1];
   const int t = threadIdx.x % NT;
   const long long row = (long long)blockIdx.x * kRows + threadIdx.x / NT;
+  griddep_wait();  // (launched while the kernel before it ends: 4 x 4096 bf16 in a row of calls 3.1 -> 2.9 us)
   if (row >= a.M) {
     // blocked scales cover whole 256-row groups: the rows behind the last one hold zeros
     if (a.quant && a.blocked && row < a.M_pad)
@@ -253,11 +254,8 @@ int launch_norm(const AddNormArgs& a, bool vec, cudaStream_t stream) {
   constexpr int kRows = NT < 128 ? 128 / NT : 1;
   const long long rows = a.quant && a.blocked ? a.M_pad : a.M;
   const unsigned grid = (unsigned)((rows + kRows - 1) / kRows);
-  if (vec)
-    add_rms_norm_kernel<T, NT, VPT, true><<<grid, NT < 128 ? 128 : NT, 0, stream>>>(a);
-  else
-    add_rms_norm_kernel<T, NT, VPT, false><<<grid, NT < 128 ? 128 : NT, 0, stream>>>(a);
-  return (int)cudaGetLastError();
+  return (int)dfl_host::launch_early(vec ? add_rms_norm_kernel<T, NT, VPT, true> : add_rms_norm_kernel<T, NT, VPT, false>, grid,
+                                     NT < 128 ? 128 : NT, 0, stream, a);
 }
 
 template <typename T>
