@@ -636,21 +636,21 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
       ms[3 - d] = m.size(-1 - d) == 1 ? 0 : m.stride(-1 - d);
     mdt = m.scalar_type() == at::kBool ? -1 : dtype_code(m, "an additive mask");
   }
-  if (a.H / a.Hk * (int64_t)a.Sq <= 16 && a.B <= 65535 && a.Hk <= 65535) {  // too few rows to fill a tile: the keys are split instead
-    DecodeArgs d{};
-    d.q = a.q, d.k = a.k, d.v = a.v, d.o = a.o;
-    d.q_bs = a.q_bs, d.q_hs = a.q_hs, d.q_ss = a.q_ss, d.k_bs = a.k_bs, d.k_hs = a.k_hs, d.k_ss = a.k_ss;
-    d.v_bs = a.v_bs, d.v_hs = a.v_hs, d.v_ss = a.v_ss, d.o_bs = a.o_bs, d.o_hs = a.o_hs, d.o_ss = a.o_ss;
-    d.lse = a.lse;
-    d.B = a.B, d.H = a.H, d.Hk = a.Hk, d.Sq = a.Sq, d.Sk = a.Sk, d.dh = a.dh, d.f16 = a.f16;
-    d.scale = a.scale;
-    d.kv_lo = a.kv_lo, d.kv_hi = a.kv_hi;
-    if (m.defined()) {
-      d.mask = m.data_ptr();
-      d.mask_dtype = mdt;
-      d.m_bs = ms[0], d.m_hs = ms[1], d.m_qs = ms[2], d.m_ks = ms[3];
-    }
-    d.err = err_ptr();
+  DecodeArgs d{};
+  d.q = a.q, d.k = a.k, d.v = a.v, d.o = a.o;
+  d.q_bs = a.q_bs, d.q_hs = a.q_hs, d.q_ss = a.q_ss, d.k_bs = a.k_bs, d.k_hs = a.k_hs, d.k_ss = a.k_ss;
+  d.v_bs = a.v_bs, d.v_hs = a.v_hs, d.v_ss = a.v_ss, d.o_bs = a.o_bs, d.o_hs = a.o_hs, d.o_ss = a.o_ss;
+  d.lse = a.lse;
+  d.B = a.B, d.H = a.H, d.Hk = a.Hk, d.Sq = a.Sq, d.Sk = a.Sk, d.dh = a.dh, d.f16 = a.f16;
+  d.scale = a.scale;
+  d.kv_lo = a.kv_lo, d.kv_hi = a.kv_hi;
+  if (m.defined()) {
+    d.mask = m.data_ptr();
+    d.mask_dtype = mdt;
+    d.m_bs = ms[0], d.m_hs = ms[1], d.m_qs = ms[2], d.m_ks = ms[3];
+  }
+  d.err = err_ptr();
+  if (dfl_cross_decode_takes(&d)) {  // too few rows to fill the other kernel's tiles: the keys are split instead
     DFL_CHECK_RC(dfl_cross_decode(&d, cur_stream()), "cross_attention (few queries)");
     if (!direct) o.copy_(o_);
     return o;

@@ -1,5 +1,5 @@
-// Attention of a few queries to many keys (single tokens, pooling queries): at most 16 query rows
-// share a key head.  sm_100a.
+// Attention of a few queries to many keys (single tokens, pooling queries): up to 16 query rows that share a key head
+// to a CTA; more rows where the kernel of cross_attn.cuh would have too few tiles (dfl_cross_decode_takes).  sm_100a.
 //
 // Bound by reading K and V once: a 128-row tensor-memory tile would be nearly empty, so the keys are split over up
 // to sixteen CTAs (one cluster per key head and batch row).  In each, one warp keeps a ring of 32-key stages full with
@@ -27,7 +27,7 @@
 namespace {
 using namespace dfl;
 
-constexpr int kMaxSplits = 16;
+constexpr int kMaxSplits = 16, kMaxRows = 512;
 constexpr int kKeys = 16;  // per warp and step
 constexpr int kWarps = 4, kGroups = kWarps / 2;  // a pair of warps shares a stage, the pairs take the stages in turn
 constexpr int kStageKeys = 2 * kKeys, kStages = 4;
@@ -99,9 +99,9 @@ DFL_DEVICE float part_weight(float m, float l, float mu) { return m == -INFINITY
 // rows.  Every CTA writes its share of each quarter row into the CTA that stores it (c_o: R dh / splits values
 // from each, c_ml: every CTA's maxima and sums), so one cluster barrier is waited for and nothing is read remotely.
 template <int DH, bool F16, class SO>
-DFL_DEVICE void decode_join(const DecodeArgs& a, int R, const float2 (&s_ml)[kWarps][16], SO s_o, float4* c_o,
+DFL_DEVICE void decode_join(const DecodeArgs& a, int hk, int r0, int R, const float2 (&s_ml)[kWarps][16], SO s_o, float4* c_o,
                             float2 (&c_ml)[kMaxSplits][16]) {
-  const int splits = gridDim.x, split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, rep = a.H / a.Hk;
+  const int splits = gridDim.x, split = blockIdx.x, b = blockIdx.z, rep = a.H / a.Hk;
   const int n4 = R * (DH / 4), share = n4 / splits;  // splits divides dh / 4
   __syncthreads();
   if (splits > 1) cluster_wait();  // every CTA of the cluster has started
@@ -147,7 +147,7 @@ DFL_DEVICE void decode_join(const DecodeArgs& a, int R, const float2 (&s_ml)[kWa
       lv += f * ml.y;
     }
     const float inv = lv == 0.f ? 0.f : 1.f / lv;
-    const int h = hk * rep + r / a.Sq, q = r % a.Sq;
+    const int h = hk * rep + (r0 + r) / a.Sq, q = (r0 + r) % a.Sq;
     const uint2 y = make_uint2(pack2<F16>(ov.x * inv, ov.y * inv), pack2<F16>(ov.z * inv, ov.w * inv));
     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + b * a.o_bs + (long long)h * a.o_hs + (long long)q * a.o_ss + d) = y;
     if (a.lse && d == 0) a.lse[((long long)b * a.H + h) * a.Sq + q] = lv == 0.f ? -INFINITY : mx + logf(lv);
@@ -186,8 +186,9 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
 
   if (gridDim.x > 1) cluster_arrive();  // waited for before the first remote write
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
-  const int splits = gridDim.x, split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  const int rep = a.H / a.Hk, R = rep * a.Sq;
+  const int splits = gridDim.x, split = blockIdx.x, b = blockIdx.z;
+  const int rep = a.H / a.Hk, groups = gridDim.y / a.Hk, hk = blockIdx.y / groups;
+  const int r0 = blockIdx.y % groups * (8 * NB), R = min(8 * NB, rep * a.Sq - r0);  // this CTA's rows of the key head
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 2);
     aborted = 0;
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
       const int r = quad + 8 * h;
-      hrow[h] = hk * rep + r / a.Sq, qrow[h] = r % a.Sq;
+      hrow[h] = hk * rep + (r0 + r) / a.Sq, qrow[h] = (r0 + r) % a.Sq;
       const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_bs + (long long)hrow[h] * a.q_hs +
                            (long long)qrow[h] * a.q_ss;
 #pragma unroll
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
         for (int j = 0; j < 4; ++j) s_o[warp][8 * h + 2 * t + j % 2][16 * d + quad + 8 * (j / 2)] = o[h][d][j];
     }
   }
-  decode_join<DH, F16>(a, R, s_ml, s_o, c_o, c_ml);
+  decode_join<DH, F16>(a, hk, r0, R, s_ml, s_o, c_o, c_ml);
 }
 
 int decode_tmap(CUtensorMap* map, const void* base, const DecodeArgs* a, long long ss, long long hs, long long bs) {
@@ -385,25 +386,32 @@ struct Resident {
   std::once_flag once;
 };
 
+int rows_of(const DecodeArgs* a) { return a->H / a->Hk * a->Sq; }
+int groups_of(const DecodeArgs* a) { return (rows_of(a) + 15) / 16; }
+int smem_bytes(int dh) { return kStages * 2 * kStageKeys * dh * 2 + 1024; }
+
+// How one call is laid out: CTAs per group of rows, and what that is expected to take, in 11 ns.
+struct Plan {
+  int splits;
+  long long cost;
+};
+
 template <int DH, bool F16, int NB>
-int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
+int plan_decode(const DecodeArgs* a, Plan* plan) {
   static Resident resident[16];
   int dev = 0;
   cudaGetDevice(&dev);
-  auto kern = cross_decode_kernel<DH, F16, NB>;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
-  cfg.dynamicSmemBytes = kStages * 2 * kStageKeys * DH * 2 + 1024;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
   Resident& res = resident[dev & 15];
   std::call_once(res.once, [&] {
+    auto kern = cross_decode_kernel<DH, F16, NB>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
+    cfg.dynamicSmemBytes = smem_bytes(DH);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     for (int i = 0; i < 5 && e == cudaSuccess; ++i) {
@@ -418,43 +426,81 @@ int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
   // 128 values; no CTA gets less than a turn of its warps.  64 heads of 4096 keys take 4 (1, 2, 4, 8, 16: 52, 30, 24, 28,
   // 42 us), 72 of 512 take 2 (9.0, 6.8, 9.6, 12.8, 25 us), 48 of 4096 x 64 take 8 (45, 25, 16, 12, 22 us), 480 of 1024
   // take 1 (43, 53, 60, 87, 172 us).
-  const long long heads = (long long)a->B * a->Hk;
-  int splits = 1;
-  long long best = -1;
+  const long long heads = (long long)a->B * a->Hk * groups_of(a);
+  plan->cost = -1;
   for (int i = 0; i < 5; ++i) {
     const long long fit = res.clusters[i], keys = (a->Sk + (1 << i) - 1) >> i;
     if (fit <= 0 || (i > 0 && keys < kGroups * kStageKeys)) continue;
     const long long cost = (heads + fit - 1) / fit * (keys + 300 * 128 / DH);
-    if (best < 0 || cost < best) best = cost, splits = 1 << i;
+    if (plan->cost < 0 || cost < plan->cost) plan->cost = cost, plan->splits = 1 << i;
   }
+  return 0;
+}
+
+template <int DH, bool F16, int NB>
+int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
+  Plan plan;
+  int rc = plan_decode<DH, F16, NB>(a, &plan);
+  if (rc) return rc;
   CUtensorMap tk, tv;
-  int rc = decode_tmap(&tk, a->k, a, a->k_ss, a->k_hs, a->k_bs);
+  rc = decode_tmap(&tk, a->k, a, a->k_ss, a->k_hs, a->k_bs);
   if (rc) return 1000 + rc;
   rc = decode_tmap(&tv, a->v, a, a->v_ss, a->v_hs, a->v_bs);
   if (rc) return 2000 + rc;
-  at[0].val.clusterDim.x = splits;
-  cfg.gridDim = dim3(splits, a->Hk, a->B);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.splits, a->Hk * groups_of(a), a->B);
+  cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes(DH);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = plan.splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
   cfg.numAttrs = 2;
-  return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, *a);
+  return (int)cudaLaunchKernelEx(&cfg, cross_decode_kernel<DH, F16, NB>, tk, tv, *a);
 }
 
-template <int DH, bool F16>
-int decode_rows(const DecodeArgs* a, cudaStream_t stream) {
-  if (a->H / a->Hk * a->Sq <= 8) return launch_decode<DH, F16, 1>(a, stream);
-  return launch_decode<DH, F16, 2>(a, stream);
-}
+// Calls f<DH, F16, NB>(a, ...) for the call's head dim, type and rows.
+#define DFL_DECODE(f, ...)                                                                              \
+  (a->dh == 64 ? (a->f16 ? (rows_of(a) <= 8 ? f<64, true, 1>(a, __VA_ARGS__) : f<64, true, 2>(a, __VA_ARGS__))       \
+                         : (rows_of(a) <= 8 ? f<64, false, 1>(a, __VA_ARGS__) : f<64, false, 2>(a, __VA_ARGS__)))    \
+               : (a->f16 ? (rows_of(a) <= 8 ? f<128, true, 1>(a, __VA_ARGS__) : f<128, true, 2>(a, __VA_ARGS__))     \
+                         : (rows_of(a) <= 8 ? f<128, false, 1>(a, __VA_ARGS__) : f<128, false, 2>(a, __VA_ARGS__))))
 
 }  // namespace
 
+extern "C" int dfl_cross_decode_takes(const DecodeArgs* a) {
+  if ((a->dh != 64 && a->dh != 128) || a->B <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk) return 0;
+  const long long rows = (long long)a->H / a->Hk * a->Sq;
+  if (rows > kMaxRows || a->B > 65535 || a->Hk * ((rows + 15) / 16) > 65535) return 0;
+  if (rows <= 16) return 1;
+  // More rows read the keys once per 16 of them, while the other kernel gives 128 rows of a head, or 256, to a CTA that walks
+  // all the keys: that leaves SMs idle where there are few tiles.  In ns: a key takes 12.5 there (20% more with a mask, which
+  // it lays out first) and 4300 go to the rest; here 17 or 11 by head dim (80% more with a mask, read value by value).
+  //   16 heads x 78 x 2355 x 64: 32.2 us there, 13.5 here; 12 x 17 x 4096 x 128: 55.8, 13.6; 32 x 64 x 4096 x 128: 56.6, 38.7
+  //   (additive mask 65.9, 76.0); 96 x 20 x 512 x 128: 11.0, 14.3; 128 x 17 x 2000 x 64: 29.0, 30.9
+  if (rows > 128 && a->Sk < 1024) return 0;
+  Plan plan;
+  if (DFL_DECODE(plan_decode, &plan)) return 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const long long tiles = (long long)a->B * a->H * (a->Sq > 128 ? (a->Sq + 255) / 256 : 1), sms = dfl_host::num_sms(dev);
+  const double here = plan.cost * (a->dh == 64 ? 11. : 17.) * (a->mask ? 1.8 : 1.);
+  const double there = (double)((tiles + sms - 1) / sms) * (4300. + 12.5 * a->Sk) * (a->mask ? 1.2 : 1.);
+  return here < 0.95 * there;
+}
+
 extern "C" int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream) {
   if (a->dh != 64 && a->dh != 128) return -2;
-  if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk || a->H / a->Hk * a->Sq > 16) return -3;
-  if (a->B > 65535 || a->Hk > 65535) return -8;
+  if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk) return -3;
+  if ((long long)a->H / a->Hk * a->Sq > kMaxRows || a->B > 65535 || (long long)a->Hk * groups_of(a) > 65535) return -8;
   auto al16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
   if (!al16(a->q) || !al16(a->k) || !al16(a->v) || !al16(a->o)) return -4;
   if ((a->q_ss | a->q_hs | a->q_bs | a->k_ss | a->k_hs | a->k_bs | a->v_ss | a->v_hs | a->v_bs | a->o_ss | a->o_hs |
        a->o_bs) % 8)
     return -5;
-  if (a->dh == 64) return a->f16 ? decode_rows<64, true>(a, stream) : decode_rows<64, false>(a, stream);
-  return a->f16 ? decode_rows<128, true>(a, stream) : decode_rows<128, false>(a, stream);
+  return DFL_DECODE(launch_decode, stream);
 }

@@ -349,6 +349,9 @@ typedef struct DecodeArgs {
   long long m_bs, m_hs, m_qs, m_ks;
   int* err;
 } DecodeArgs;
+// 1: this kernel is the faster one for the call (up to 16 query rows per key head, or more where the other would leave
+// SMs idle).
+int dfl_cross_decode_takes(const DecodeArgs* a);
 int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream);
 
 // Boolean mask [B, H, Q, Sk] (1 byte per element, element strides) -> bit rows [B, H, Q, words], words =

@@ -208,6 +208,16 @@ def test_few_queries(native, B, H, Hk, Sq, Sk, D, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", [None, "lens", "keys", "bool", "bias"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", [  # a few groups of 16 rows, the last one short; heads that end inside a group
+    (1, 16, 16, 78, 2355, 64), (2, 8, 2, 23, 1500, 128), (1, 3, 1, 17, 3001, 128), (1, 2, 1, 150, 2000, 128), (4, 3, 3, 33, 1030, 64),
+])
+def test_few_tiles(native, B, H, Hk, Sq, Sk, D, kind, dtype):
+    test_few_queries(native, B, H, Hk, Sq, Sk, D, kind, dtype)
+
+
+@pytest.mark.gpu
 def test_few_queries_rise(native):
     """Scores that rise along the keys (the running maximum moves at almost every block), and rows that differ."""
     B, H, Hk, Sq, Sk, D = 1, 8, 2, 4, 3000, 128
