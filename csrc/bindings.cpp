@@ -264,6 +264,7 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
   // that leave SMs idle split, one 128 x 256 f32 tile per CTA tile and at most 96 of them)
   l.split_ws_floats = (M + 127) / 128 * ((N + 255) / 256) <= 96 ? 96ll * 128 * 256 : 0;
   l.split_sem_count = l.split_ws_floats ? 256 : 0;
+  a.cta_mode = dfl_gemm_lora_mode(&a);
   l.tile_rows = dfl_gemm_tile_rows(&a);
   const int64_t tiles = (M + l.tile_rows - 1) / l.tile_rows;
   int64_t cap = std::min<int64_t>(l.n_adapters, l.tile_rows);
@@ -282,7 +283,7 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
     l.split_sem = reinterpret_cast<int*>(base + t_bytes + list_bytes);
     l.split_ws = reinterpret_cast<float*>(base + t_bytes + list_bytes + sem_bytes);
   }
-  a.cta_mode = l.tile_rows == 256 ? 2 : 1;  // the tile shape the lists are built for
+  if (a.cta_mode == 0) a.cta_mode = l.tile_rows == 256 ? 2 : 1;  // the tile shape the lists are built for
   DFL_CHECK_RC(dfl_gemm_lora(&a, cur_stream()), "gemm_lora");
   return res;
 }

@@ -480,6 +480,15 @@ extern "C" int dfl_gemm_tile_rows(const GemmArgs* a) {
   return use_pair(&a, 1, split_ws_of(a, dev).floats > 0, dfl_host::num_sms(dev), &wide) ? 2 * BM : BM;
 }
 
+// cta_mode of an adapter projection: 128 x 128 tiles where one round of them covers it (300 / 600 / 1000 x 2048 x 2048 without
+// adapters 22.0 / 22.6 / 23.1 us in pairs, 14.7 / 16.2 / 16.2 so; 300 x 1536 x 6144 38.6, 27.4; two rounds, 1333 x 2048 x 2048:
+// 19.4, 25.6), else as the model decides.
+extern "C" int dfl_gemm_lora_mode(const GemmArgs* a) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return (long long)((a->M + BM - 1) / BM) * ((a->N + 127) / 128) <= dfl_host::num_sms(dev) ? 3 : 0;
+}
+
 // CTAs of the launch `a` would get.
 extern "C" int dfl_gemm_ctas(const GemmArgs* a) {
   int dev = 0;

@@ -77,6 +77,7 @@ typedef struct LoraArgs {
   int* split_sem; int split_sem_count;
 } LoraArgs;
 int dfl_gemm_tile_rows(const GemmArgs* a);
+int dfl_gemm_lora_mode(const GemmArgs* a);
 int dfl_gemm_ctas(const GemmArgs* a);
 int dfl_lora_rows(int M);  // 1: so few rows that only t is used, as f32 [M, rank]
 int dfl_gemm_lora(const GemmArgs* a, cudaStream_t stream);  // a->lora set
