@@ -4,7 +4,7 @@ Contract (difflet/ops/attention.py:4-128, difflet/backends/cuda/ops_impl/attenti
 
 * ``q, k, v``: ``[B, H, S, D]`` or ``[B*H, S, D]``; the result has ``q``'s shape.
 * ``scale=None`` means 1.0 (not ``1/sqrt(D)``).
-* ``attention_mask``: bool (True = attend) or additive; ``bound_min`` / ``bound_max``
+* ``attention_mask``: bool (True = attend) or additive (integers too); ``bound_min`` / ``bound_max``
   (both or neither, exclusive with a mask) select the keys ``[bound_min, bound_max)``.
 * ``tp_q`` / ``tp_k`` / ``tp_out`` are layout hints of other hardware: accepted, ignored.
 
@@ -129,11 +129,11 @@ _MASK_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _mask_on(mask, q):
-    """A mask on q's device whose type the kernel reads (integers: non-zero = attend, as a boolean)."""
-    if mask is None:
-        return None
+    """A mask on q's device whose type the kernel reads; what is not boolean is added to the scores, integers too."""
+    if mask is None or mask.dtype == torch.bool:
+        return mask if mask is None else mask.to(q.device)
     if not mask.is_floating_point():
-        mask = mask.bool()
+        mask = mask.float()
     elif mask.dtype not in _MASK_DTYPES and q.is_cuda:  # finite values stay finite (the type's lowest masks softly)
         low = torch.finfo(torch.float32)
         mask = torch.where(mask.isfinite(), mask.clamp(low.min, low.max), mask).float()
@@ -145,7 +145,7 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     """Attention of ``q [B, H, Sq, D]`` to encoder states ``k, v [B, Hk, Sk, D]`` of another length.
 
     ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``).  ``attention_mask``: bool (True =
-    attend) or additive, broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
+    attend) or additive (integers too), broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
     ``attention``.  A query that no key is left for gives 0.  ``out`` (like q) and ``lse`` (f32 ``[B, H, Sq]``, natural
     log) are filled when given.  CUDA: bf16 and fp16 with head dim 64 or 128; anything else, and what asks for

@@ -1,0 +1,75 @@
+"""What ``ops.attention`` and ``ops.cross_attention`` accept: one meaning of a call on every device, type and path.
+
+Kernel results are compared with the 64-bit formula and the tolerances of ``test_cross_attention``."""
+
+import math
+
+import pytest
+import torch
+
+from difflet_b200 import ops
+from test_cross_attention import _check, _inputs, _ref
+
+BOTH = (ops.attention, ops.cross_attention)
+
+
+# ----------------------------------------------------------------------------- integer masks are added to the scores
+def _int_mask(B, Sq, Sk, dtype, device):
+    g = torch.Generator().manual_seed(4)
+    low = -100 if dtype == torch.int8 else -10000
+    return torch.where(torch.rand(B, 1, Sq, Sk, generator=g) < 0.6, 0, low).to(device, dtype)
+
+
+@pytest.mark.parametrize("fn", BOTH)
+@pytest.mark.parametrize("dtype", [torch.int8, torch.int32, torch.int64])
+def test_integer_masks_are_additive(fn, dtype):
+    q, k, v = _inputs(2, 4, 4, 6, 9, 16, torch.float32, "cpu")
+    m = _int_mask(2, 6, 9, dtype, "cpu")
+    want = fn(q, k, v, scale=0.25, attention_mask=m.float())
+    assert torch.allclose(fn(q, k, v, scale=0.25, attention_mask=m), want, atol=1e-6)
+    assert torch.allclose(want.double(), _ref(q, k, v, 0.25, m.float())[0], atol=1e-5)
+    got = fn(q.clone().requires_grad_(), k, v, scale=0.25, attention_mask=m)
+    assert torch.allclose(got.detach(), want, atol=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", BOTH)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Sq,D", [(3, 64), (150, 64), (150, 128)])
+def test_integer_masks_are_additive_on_cuda(native, fn, dtype, Sq, D):
+    q, k, v = _inputs(2, 4, 4, Sq, 70, D, dtype, "cuda")
+    m = _int_mask(2, Sq, 70, torch.int32, "cuda")
+    o = fn(q, k, v, scale=0.1, attention_mask=m)
+    if dtype != torch.float32:  # the kernels; -10000 masks whatever the scores are
+        _check(o, _ref(q, k, v, 0.1, m.float()), dtype, D, 70, v.abs().max().item())
+    keep = fn(q, k, v, scale=0.1, attention_mask=m == 0)
+    grad = fn(q.clone().requires_grad_(), k, v, scale=0.1, attention_mask=m).detach()
+    for other in (keep, grad):  # the library's own roundings: a few of the largest value
+        assert (o.double() - other.double()).abs().max() <= 4 * torch.finfo(dtype).eps * v.abs().max()
+
+
+@pytest.mark.gpu
+def test_masks_and_lengths_of_other_types(native):
+    """Lengths of any integer type and device, f64 masks at their lowest value, a mask of no dimension, many batch rows, and
+    the result in place of the queries."""
+    B, H, Sq, Sk, D = 2, 2, 40, 50, 64
+    q, k, v = _inputs(B, H, H, Sq, Sk, D, torch.bfloat16, "cuda")
+    all_keys = ops.cross_attention(q, k, v, scale=0.1)
+    for lens in (torch.tensor([1 << 40, 50]), torch.tensor([50, 99], dtype=torch.int16)):
+        assert torch.equal(ops.cross_attention(q, k, v, scale=0.1, kv_lens=lens), all_keys)
+    assert bool((ops.cross_attention(q, k, v, scale=0.1, kv_lens=torch.tensor([-3, 0])) == 0).all())
+    m = torch.rand(B, 1, Sq, Sk, device="cuda") < 0.5
+    want = ops.cross_attention(q, k, v, scale=0.1, attention_mask=m)
+    low = torch.zeros(m.shape, device="cuda", dtype=torch.float64).masked_fill(~m, torch.finfo(torch.float64).min)
+    low[:, :, 3] = torch.finfo(torch.float64).min  # a row at the lowest value everywhere: the mean of the values
+    o = ops.cross_attention(q, k, v, scale=0.1, attention_mask=low)
+    mean = v.double().mean(2)
+    assert bool(((o[:, :, 3].double() - mean).abs() <= 2.0 ** -7 * (mean.abs() + v.double().abs().mean(2))).all())
+    keep = torch.arange(Sq, device="cuda") != 3
+    assert torch.allclose(o[:, :, keep].float(), want[:, :, keep].float(), atol=2.0 ** -6)
+    assert torch.equal(ops.cross_attention(q, k, v, scale=0.1, attention_mask=torch.tensor(True, device="cuda")), all_keys)
+    big = _inputs(70000, 1, 1, 1, 3, 64, torch.bfloat16, "cuda")  # more batch rows than a grid axis holds
+    _check(ops.cross_attention(*big, scale=0.1), _ref(*big, 0.1), q.dtype, 64, 3, big[2].abs().max().item())
+    same = q.contiguous()
+    got = ops.cross_attention(same, k, v, scale=0.1, out=same)
+    assert got is same and torch.equal(got, all_keys)
