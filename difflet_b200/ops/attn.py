@@ -8,7 +8,8 @@ Contract (difflet/ops/attention.py:4-128, difflet/backends/cuda/ops_impl/attenti
   (both or neither, exclusive with a mask) select the keys ``[bound_min, bound_max)``.
 * ``tp_q`` / ``tp_k`` / ``tp_out`` are layout hints of other hardware: accepted, ignored.
 
-Dispatch: CUDA tensors with head dim 128, bf16, no mask, non-causal and bounds that are
+Dispatch (the kernels record no backward pass: inputs that ask for gradients take the library
+path on CUDA): CUDA tensors with head dim 128, bf16, no mask, non-causal and bounds that are
 per batch row (shape ``[B]`` or ``[B, 1, ...]``, the padded-text key windows every
 model here uses) run the tcgen05 kernel of ``csrc/attention.cu``.  Masks (boolean or
 additive), per-query windows, head dim 64 and fp16 run the tcgen05 kernel of
@@ -70,7 +71,7 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
         raise ValueError("attention_mask and bounds are mutually exclusive")
     lo, hi = _per_batch(bound_min, B), _per_batch(bound_max, B)
     simple = attention_mask is None and not causal and (bound_min is None or (lo is not None and hi is not None))
-    kernel = q.is_cuda and simple and q.shape[-1] == 128 and q.dtype == torch.bfloat16
+    kernel = q.is_cuda and simple and q.shape[-1] == 128 and q.dtype == torch.bfloat16 and not F.wants_grad(q, k, v)
     if kernel or (simple and not q.is_cuda):
         if lo is not None:
             lo = lo.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()

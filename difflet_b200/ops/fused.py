@@ -612,7 +612,7 @@ def cross_kernel_ok(q, k, v, mask=None) -> bool:
 
 def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     """softmax(scale * q k^T) v over [B, H, S, dh]; key window [kv_lo[b], kv_hi[b])."""
-    if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128:
+    if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128 and not wants_grad(q, k, v):
         return native().attention(q, k, v, float(scale), out, lse, kv_lo, kv_hi, kv_split=kv_split_mode())
     if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and cross_kernel_ok(q, k, v):
         return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse)

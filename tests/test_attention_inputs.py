@@ -73,3 +73,41 @@ def test_masks_and_lengths_of_other_types(native):
     same = q.contiguous()
     got = ops.cross_attention(same, k, v, scale=0.1, out=same)
     assert got is same and torch.equal(got, all_keys)
+
+
+# ----------------------------------------------------------------------------- gradients
+@pytest.mark.parametrize("fn", BOTH)
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_inputs_that_ask_for_gradients_stay_off_the_kernels(fn, which):
+    """Shapes and dispatch alone (tensors without data): no kernel is called, and the result has a history."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        qkv = [torch.empty(2, 2, 20, 128, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+        qkv[which].requires_grad_()
+        o = fn(*qkv, scale=0.1)
+        assert o.shape == qkv[0].shape and o.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", BOTH)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", [None, "bounds", "mask"])
+def test_gradients(native, fn, D, kind):
+    q, k, v = (t.detach().requires_grad_() for t in _inputs(2, 2, 2, 20, 33, D, torch.bfloat16, "cuda"))
+    keep = torch.ones(2, 1, 20, 33, device="cuda", dtype=torch.bool)
+    kw = {}
+    if kind == "bounds":
+        hi = torch.tensor([33, 12], device="cuda").view(2, 1, 1, 1)
+        kw = dict(bound_min=torch.zeros_like(hi), bound_max=hi)
+        keep = keep & (torch.arange(33, device="cuda") < hi)
+    elif kind == "mask":
+        keep = (torch.rand(2, 1, 20, 33, device="cuda") < 0.7) | (torch.arange(33, device="cuda") == 0)
+        kw = dict(attention_mask=keep)
+    w = torch.randn(2, 2, 20, D, device="cuda")
+    ref = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    z = (ref[0] @ ref[1].transpose(2, 3) * 0.1).masked_fill(~keep, -math.inf)
+    want = torch.autograd.grad(((z.softmax(-1) @ ref[2]) * w.double()).sum(), ref)
+    got = torch.autograd.grad((fn(q, k, v, scale=0.1, **kw) * w).sum(), (q, k, v))
+    for a, b in zip(got, want):  # the library's bf16 products: a few roundings (2^-8) of the largest value
+        assert (a.double() - b).abs().max() <= 2.0 ** -5 * b.abs().max()
