@@ -26,7 +26,9 @@ class LoraBank:
     [N, r_i]; ``scale``: one factor per adapter (numbers or a tensor; default 1).  Ranks up to 128 (shorter ones
     are padded with zeros to the longest, in steps of 16), at most 1024 adapters.
 
-    The weights must be finite (checked here; also after later changes in place).  Kept in A's type on A's device; tensors that already have the padded layout are used as they are."""
+    The weights must be finite (checked here; also after later changes in place).  Kept in A's type on A's device; tensors
+    that already have the padded layout are used as they are.  No gradient is recorded: tensors that ask for one are refused
+    outside ``torch.no_grad()``."""
 
     MAX_ADAPTERS, MAX_RANK = 1024, 128
 
@@ -43,6 +45,7 @@ class LoraBank:
                 raise ValueError(f"adapter {i}: rank {x.shape[0]} is not in 1..{self.MAX_RANK}")
             if x.dtype != a[0].dtype or y.dtype != a[0].dtype or x.device != a[0].device or y.device != a[0].device:
                 raise ValueError(f"adapter {i} differs from the first one in type or device")
+        F._no_grad("LoraBank", *a, *b, scale if torch.is_tensor(scale) else None)
         if not a[0].is_floating_point():
             raise ValueError(f"adapters are floating-point tensors, got {a[0].dtype}")
         self.n, self.in_features, self.out_features = n, K, N
@@ -94,7 +97,7 @@ def linear_lora(x, w, b=None, *, bank: LoraBank, ids, rows_per_batch: int = 0, a
     number outside the bank, which also sets the device error word) means none.  ``gate`` f32 [B, N] with
     ``gate_rows_per_batch`` rows each (0: ``rows_per_batch``, else all).  The rank-r
     intermediate is rounded to x's type once; everything is accumulated in f32 and rounded at the end."""
-    F._no_grad("linear_lora", x, b, gate, resid)
+    F._no_grad("linear_lora", x, b, gate, resid, None if isinstance(w, F.MXWeight) else w)
     if act not in (None, "none", "gelu", "gelu_tanh", "silu"):
         raise ValueError(f"act {act!r}: linear_lora has none, gelu and silu")
     if gate is not None and act not in (None, "none"):
