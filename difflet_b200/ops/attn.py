@@ -71,13 +71,15 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
         raise ValueError("attention_mask and bounds are mutually exclusive")
     lo, hi = _per_batch(bound_min, B), _per_batch(bound_max, B)
     simple = attention_mask is None and not causal and (bound_min is None or (lo is not None and hi is not None))
-    kernel = q.is_cuda and simple and q.shape[-1] == 128 and q.dtype == torch.bfloat16 and not F.wants_grad(q, k, v)
+    kernel = (q.is_cuda and simple and q.shape[-1] == v.shape[-1] == 128 and q.dtype == torch.bfloat16
+              and not F.wants_grad(q, k, v))
     if kernel or (simple and not q.is_cuda):
         if lo is not None:
             lo = lo.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
             hi = hi.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
         out = F.attention(q4, k4, v4, scale, lse=lse, kv_lo=lo, kv_hi=hi)
-    elif F.cross_kernel_ok(q, k, v, attention_mask) and not causal and k4.dtype == v4.dtype == q4.dtype and k4.shape[1] == q4.shape[1]:
+    elif (F.cross_kernel_ok(q, k, v, attention_mask) and not causal and k4.dtype == v4.dtype == q4.dtype
+          and k4.shape == v4.shape and k4.shape[1] == q4.shape[1]):
         mask = attention_mask if simple or bound_min is None else _bounds_to_mask(k4, bound_min, bound_max, None)
         if lo is not None and simple:
             lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
@@ -143,15 +145,15 @@ def _mask_on(mask, q):
 
 def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, lse=None, out=None, bound_min=None,
                     bound_max=None, **kwargs):
-    """Attention of ``q [B, H, Sq, D]`` to encoder states ``k, v [B, Hk, Sk, D]`` of another length.
+    """Attention of ``q [B, H, Sq, D]`` to encoder states ``k [B, Hk, Sk, D]``, ``v [B, Hk, Sk, Dv]`` of another length.
 
     ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``).  ``attention_mask``: bool (True =
     attend) or additive (integers too), broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
-    ``attention``.  A query that no key is left for gives 0.  ``out`` (like q) and ``lse`` (f32 ``[B, H, Sq]``, natural
-    log) are filled when given.  CUDA: bf16 and fp16 with head dim 64 or 128; anything else, and what asks for
-    gradients, runs as ``attention``."""
-    kernel = F.cross_kernel_ok(q, k, v, attention_mask)
+    ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (f32 ``[B, H, Sq]``,
+    natural log) are filled when given.  CUDA: bf16 and fp16 with D = Dv = 64 or 128; anything else, and what asks
+    for gradients, runs as ``attention``."""
+    kernel = k.shape[-1] == v.shape[-1] and F.cross_kernel_ok(q, k, v, attention_mask)
     if (kernel and q.dim() == 4 and bound_min is None and bound_max is None
             and (attention_mask is None or attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)):
         # the binding checks shapes, types and devices (ValueError)
@@ -165,15 +167,16 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         o = cross_attention(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), scale=scale, attention_mask=attention_mask,
                             lse=lse, bound_min=bound_min, bound_max=bound_max)
         return o.squeeze(0)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"q [B, H, Sq, D], k / v [B, Hk, Sk, D]; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3]:
+        raise ValueError(f"q [B, H, Sq, D], k [B, Hk, Sk, D], v [B, Hk, Sk, Dv]; got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
     B, H, Sq, D = q.shape
     if k.shape[0] != B or k.shape[3] != D or k.shape[1] < 1 or H % k.shape[1]:
         raise ValueError(f"k / v {tuple(k.shape)} do not match q {tuple(q.shape)} (H must be a multiple of Hk)")
     if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
         raise ValueError("q, k and v must share type and device")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
-        raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not match q {tuple(q.shape)} {q.dtype}")
+    if out is not None and (out.shape != (B, H, Sq, v.shape[3]) or out.dtype != q.dtype or out.device != q.device):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not {(B, H, Sq, v.shape[3])} {q.dtype}")
     if lse is not None and (lse.numel() != B * H * Sq or not lse.is_contiguous()):
         raise ValueError(f"lse must be contiguous [{B}, {H}, {Sq}]")
     lo = hi = None

@@ -111,3 +111,43 @@ def test_gradients(native, fn, D, kind):
     got = torch.autograd.grad((fn(q, k, v, scale=0.1, **kw) * w).sum(), (q, k, v))
     for a, b in zip(got, want):  # the library's bf16 products: a few roundings (2^-8) of the largest value
         assert (a.double() - b).abs().max() <= 2.0 ** -5 * b.abs().max()
+
+
+# ----------------------------------------------------------------------------- shapes
+def _wide(B, H, Hk, Sq, Sk, D, Dv, dtype, device):
+    q, k, _ = _inputs(B, H, Hk, Sq, Sk, D, dtype, device)
+    return q, k, _inputs(B, H, Hk, Sq, Sk, Dv, dtype, device, 1)[2]
+
+
+@pytest.mark.parametrize("Hk", [4, 2])
+def test_values_of_another_width(Hk):
+    q, k, v = _wide(2, 4, Hk, 6, 9, 16, 24, torch.float32, "cpu")
+    lens = torch.tensor([9, 3])
+    m = torch.rand(2, 1, 6, 9) < 0.6
+    for kw, ref in (({}, {}), (dict(attention_mask=m), dict(mask=m)), (dict(kv_lens=lens), dict(lens=lens))):
+        want = _ref(q, k, v, 0.25, **ref)[0]
+        o, out = ops.cross_attention(q, k, v, scale=0.25, **kw), torch.empty(2, 4, 6, 24)
+        assert o.shape == (2, 4, 6, 24) and torch.allclose(o.double(), want, atol=1e-5)
+        assert torch.equal(ops.cross_attention(q, k, v, scale=0.25, out=out, **kw), o) and torch.equal(out, o)
+    with pytest.raises(ValueError):
+        ops.cross_attention(q, k, v, out=torch.empty_like(q))
+    if Hk == 4:
+        assert torch.allclose(ops.attention(q, k, v, scale=0.25, attention_mask=m).double(), _ref(q, k, v, 0.25, m)[0], atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,Dv", [(64, 32), (64, 128), (128, 64), (48, 64)])
+def test_values_of_another_width_on_cuda(native, D, Dv, dtype):
+    q, k, v = _wide(2, 4, 4, 30, 41, D, Dv, dtype, "cuda")
+    m = torch.rand(2, 1, 30, 41, device="cuda") < 0.6
+    lens = torch.tensor([41, 7], device="cuda")
+    for fn in BOTH:
+        for kw in ({}, dict(mask=m)):
+            o = fn(q, k, v, scale=0.1, attention_mask=kw.get("mask"))
+            want, _, size, _ = _ref(q, k, v, 0.1, **kw)
+            assert o.shape == want.shape  # the library's form: P and the result in the type
+            assert bool(((o.double() - want).abs() <= 2 * torch.finfo(dtype).eps * (size + want.abs()) + 1e-6).all())
+    o = ops.cross_attention(q, k, v, scale=0.1, kv_lens=lens, out=torch.empty(2, 4, 30, Dv, device="cuda", dtype=dtype))
+    want, _, size, _ = _ref(q, k, v, 0.1, lens=lens)
+    assert bool(((o.double() - want).abs() <= 2 * torch.finfo(dtype).eps * (size + want.abs()) + 1e-6).all())
