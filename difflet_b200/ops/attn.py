@@ -79,7 +79,7 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
             hi = hi.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
         out = F.attention(q4, k4, v4, scale, lse=lse, kv_lo=lo, kv_hi=hi)
     elif (F.cross_kernel_ok(q, k, v, attention_mask) and not causal and k4.dtype == v4.dtype == q4.dtype
-          and k4.shape == v4.shape and k4.shape[1] == q4.shape[1]):
+          and k4.shape == v4.shape and k4.shape[:2] == q4.shape[:2]):
         mask = attention_mask if simple or bound_min is None else _bounds_to_mask(k4, bound_min, bound_max, None)
         if lo is not None and simple:
             lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
@@ -147,14 +147,16 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
                     bound_max=None, **kwargs):
     """Attention of ``q [B, H, Sq, D]`` to encoder states ``k [B, Hk, Sk, D]``, ``v [B, Hk, Sk, Dv]`` of another length.
 
-    ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``).  ``attention_mask``: bool (True =
+    ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``); where the heads are equal, or one, so may be the batch
+    rows: one of q, or of k and v, then serves all of the other side.  ``attention_mask``: bool (True =
     attend) or additive (integers too), broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
     ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (f32 ``[B, H, Sq]``,
     natural log) are filled when given.  CUDA: bf16 and fp16 with D = Dv = 64 or 128; anything else, and what asks
     for gradients, runs as ``attention``."""
     kernel = k.shape[-1] == v.shape[-1] and F.cross_kernel_ok(q, k, v, attention_mask)
-    if (kernel and q.dim() == 4 and bound_min is None and bound_max is None
+    if (kernel and q.dim() == k.dim() == 4 and k.shape[0] == q.shape[0] and k.shape[1] <= q.shape[1]
+            and bound_min is None and bound_max is None
             and (attention_mask is None or attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)):
         # the binding checks shapes, types and devices (ValueError)
         return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
@@ -171,8 +173,13 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         raise ValueError(f"q [B, H, Sq, D], k [B, Hk, Sk, D], v [B, Hk, Sk, Dv]; got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
     B, H, Sq, D = q.shape
-    if k.shape[0] != B or k.shape[3] != D or k.shape[1] < 1 or H % k.shape[1]:
+    Bk, Hk = k.shape[:2]
+    if (k.shape[3] != D or Hk < 1 or (H != 1 and H % Hk)
+            or (Bk != B and (1 not in (B, Bk) or (H != 1 and Hk not in (1, H))))):
         raise ValueError(f"k / v {tuple(k.shape)} do not match q {tuple(q.shape)} (H must be a multiple of Hk)")
+    if Bk != B or Hk > H:  # one batch row (one query head) for all
+        B, H = Bk if B == 1 else B, max(H, Hk)
+        q, k, v = q.expand(B, H, Sq, D), *(t.expand(B, *t.shape[1:]) for t in (k, v))
     if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
         raise ValueError("q, k and v must share type and device")
     if out is not None and (out.shape != (B, H, Sq, v.shape[3]) or out.dtype != q.dtype or out.device != q.device):

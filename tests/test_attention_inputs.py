@@ -151,3 +151,43 @@ def test_values_of_another_width_on_cuda(native, D, Dv, dtype):
     o = ops.cross_attention(q, k, v, scale=0.1, kv_lens=lens, out=torch.empty(2, 4, 30, Dv, device="cuda", dtype=dtype))
     want, _, size, _ = _ref(q, k, v, 0.1, lens=lens)
     assert bool(((o.double() - want).abs() <= 2 * torch.finfo(dtype).eps * (size + want.abs()) + 1e-6).all())
+
+
+SHARED = [((1, 4), (3, 4)), ((3, 4), (1, 4)), ((3, 4), (1, 1)), ((3, 1), (3, 4)), ((1, 1), (3, 4))]
+
+
+def _shared(q_rows, k_rows, device, dtype, D=16, Sq=6, Sk=9):
+    """q, k, v of one batch row or head for all of the other side, and q, k, v written out."""
+    q, k, v = _inputs(3, 4, 4, Sq, Sk, D, dtype, device)
+    q, k, v = (t[:r[0], :r[1]] for t, r in zip((q, k, v), (q_rows, k_rows, k_rows)))
+    return (q, k, v), [t.expand(3, 4, *t.shape[2:]) for t in (q, k, v)]
+
+
+@pytest.mark.parametrize("rows", SHARED)
+def test_one_batch_row_or_head_for_all(rows):
+    (q, k, v), (fq, fk, fv) = _shared(*rows, "cpu", torch.float32)
+    m = torch.rand(3, 1, 6, 9) < 0.6
+    lens = torch.tensor([9, 3, 0])
+    for kw, ref in (({}, {}), (dict(attention_mask=m), dict(mask=m)), (dict(kv_lens=lens), dict(lens=lens))):
+        o = ops.cross_attention(q, k, v, scale=0.25, **kw)
+        assert o.shape == (3, 4, 6, 16) and torch.allclose(o.double(), _ref(fq, fk, fv, 0.25, **ref)[0], atol=1e-5)
+    for bad in (((q[:, :, :, :8], k, v)), ((fq[:2], fk, fv)), ((fq, fk[:, :3], fv[:, :3])), ((fq, fk[:1, :2], fv[:1, :2]))):
+        with pytest.raises(ValueError):
+            ops.cross_attention(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", SHARED)
+def test_one_batch_row_or_head_for_all_on_cuda(native, rows, D):
+    (q, k, v), (fq, fk, fv) = _shared(*rows, "cuda", torch.bfloat16, D, 40, 70)
+    m = torch.rand(3, 1, 40, 70, device="cuda") < 0.6
+    vmax = v.abs().max().item()
+    for kw, ref in (({}, {}), (dict(attention_mask=m), dict(mask=m)), (dict(kv_lens=torch.tensor([70, 9, 0], device="cuda")),) * 2):
+        lse = torch.empty(3, 4, 40, device="cuda")
+        o = ops.cross_attention(q, k, v, scale=0.1, lse=lse, **kw)
+        _check(o, _ref(fq, fk, fv, 0.1, ref.get("mask"), ref.get("kv_lens")), q.dtype, D, 70, vmax, lse)
+    if rows in (((3, 4), (1, 4)), ((1, 4), (3, 4))):  # as ``attention`` takes them
+        o = ops.attention(q, k, v, scale=0.1, attention_mask=m)
+        want, _, size, _ = _ref(fq, fk, fv, 0.1, m)
+        assert bool(((o.double() - want).abs() <= 2 * torch.finfo(q.dtype).eps * (size + want.abs()) + 1e-6).all())
