@@ -149,7 +149,8 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
 
     ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``); where the heads are equal, or one, so may be the batch
     rows: one of q, or of k and v, then serves all of the other side.  ``attention_mask``: bool (True =
-    attend) or additive (integers too), broadcastable to ``[B, H, Sq, Sk]``.  ``kv_lens`` (integers ``[B]``): the valid keys of
+    attend) or additive (integers too), broadcastable to ``[B, H, Sq, Sk]``; moved to q's device as in ``attention``
+    (refused there with shared key heads on CUDA).  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
     ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (f32 ``[B, H, Sq]``,
     natural log) are filled when given.  CUDA: bf16 and fp16 with D = Dv = 64 or 128; anything else, and what asks
@@ -157,7 +158,8 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     kernel = k.shape[-1] == v.shape[-1] and F.cross_kernel_ok(q, k, v, attention_mask)
     if (kernel and q.dim() == k.dim() == 4 and k.shape[0] == q.shape[0] and k.shape[1] <= q.shape[1]
             and bound_min is None and bound_max is None
-            and (attention_mask is None or attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)):
+            and (attention_mask is None or ((attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)
+                                            and (attention_mask.device == q.device or k.shape[1] != q.shape[1])))):
         # the binding checks shapes, types and devices (ValueError)
         return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
                                  out=out, lse=lse)

@@ -191,3 +191,12 @@ def test_one_batch_row_or_head_for_all_on_cuda(native, rows, D):
         o = ops.attention(q, k, v, scale=0.1, attention_mask=m)
         want, _, size, _ = _ref(fq, fk, fv, 0.1, m)
         assert bool(((o.double() - want).abs() <= 2 * torch.finfo(q.dtype).eps * (size + want.abs()) + 1e-6).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", BOTH)
+def test_masks_of_the_host(native, fn):
+    q, k, v = _inputs(2, 4, 4, 40, 70, 64, torch.bfloat16, "cuda")
+    g = torch.Generator().manual_seed(0)
+    for m in (torch.rand(2, 1, 40, 70, generator=g) < 0.6, torch.randn(70, generator=g), torch.randn(40, 70, generator=g).bfloat16()):
+        assert torch.equal(fn(q, k, v, scale=0.1, attention_mask=m), fn(q, k, v, scale=0.1, attention_mask=m.cuda()))
