@@ -320,7 +320,7 @@ def add_rms_norm(x, resid=None, weight=None, *, eps=1e-6, scale=None, shift=None
     if weight is not None:
         y = y * weight.to(ct)
     if M and (scale is not None or shift is not None):
-        b = row_map.long() if row_map is not None else torch.arange(M) // (rows_per_batch or M)
+        b = row_map.long() if row_map is not None else torch.arange(M, device=x.device) // (rows_per_batch or M)
         if scale is not None:
             y = y * (1 + scale.to(ct)[b])
         if shift is not None:
@@ -659,8 +659,8 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
         return _kernels().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     Sk, rep = k.shape[2], q.shape[1] // k.shape[1]
-    idx = torch.arange(Sk)
-    keep = torch.ones(q.shape[0], Sk, dtype=torch.bool)
+    idx = torch.arange(Sk, device=q.device)
+    keep = torch.ones(q.shape[0], Sk, dtype=torch.bool, device=q.device)
     if kv_lo is not None:
         keep &= idx >= kv_lo.view(-1, 1)
     if kv_hi is not None:

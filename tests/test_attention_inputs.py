@@ -200,3 +200,15 @@ def test_masks_of_the_host(native, fn):
     g = torch.Generator().manual_seed(0)
     for m in (torch.rand(2, 1, 40, 70, generator=g) < 0.6, torch.randn(70, generator=g), torch.randn(40, 70, generator=g).bfloat16()):
         assert torch.equal(fn(q, k, v, scale=0.1, attention_mask=m), fn(q, k, v, scale=0.1, attention_mask=m.cuda()))
+
+
+# ----------------------------------------------------------------------------- tensors without data, transforms
+def test_meta_tensors():
+    q, k, v = _inputs(2, 4, 4, 6, 9, 16, torch.float32, "meta")
+    m, lens = torch.ones(2, 1, 1, 9, dtype=torch.bool, device="meta"), torch.ones(2, dtype=torch.long, device="meta")
+    for kw in ({}, dict(attention_mask=m), dict(attention_mask=m.float()), dict(kv_lens=lens)):
+        o = ops.cross_attention(q, k[:, :2], v[:, :2], **kw)
+        assert o.shape == q.shape and o.is_meta
+    x, mod = torch.empty(6, 32, device="meta"), torch.empty(2, 32, device="meta")
+    y, s = ops.add_rms_norm(x, x, scale=mod, shift=mod, rows_per_batch=3)
+    assert y.shape == s.shape == x.shape and y.is_meta
