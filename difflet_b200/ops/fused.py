@@ -30,6 +30,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
 from difflet_b200 import envs
@@ -595,19 +596,32 @@ def kv_split_mode() -> int:
 
 
 def wants_grad(*tensors) -> bool:
-    """Whether autograd would record an operation on these (None allowed)."""
+    """Whether autograd would record an operation on these, or carry their forward-mode tangents (None allowed)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
+    if fwAD._current_level >= 0:
+        return any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
     return False
+
+
+def kernel_tensors(*tensors) -> bool:
+    """Whether a kernel can be given these (None allowed): outside compilation and function transforms such as vmap, and no
+    fake tensor or other subclass."""
+    if torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None:
+        return False
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return True
 
 
 def cross_kernel_ok(q, k, v, mask=None) -> bool:
     """Whether the masked / head-dim-64 attention kernel takes these inputs (it records no backward pass: what asks
-    for gradients stays on the torch path)."""
+    for gradients stays on the torch path, and so do tracing and function transforms)."""
     return (q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in (torch.bfloat16, torch.float16)
-            and not wants_grad(q, k, v, mask))
+            and not wants_grad(q, k, v, mask) and kernel_tensors(q, k, v, mask))
 
 
 def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):

@@ -84,11 +84,11 @@ def dequantize_mx(data, scale, *, dtype: str = "float8_e4m3fn", output_dtype=tor
     if scale.dtype != torch.uint8 or scale.shape != (*data.shape[:-1], K // GROUP):
         raise ValueError(f"scale must be uint8 {(*data.shape[:-1], K // GROUP)}, got {scale.dtype} "
                          f"{tuple(scale.shape)}")
-    if (data.is_cuda and data.dtype in (torch.float8_e4m3fn, torch.float8_e5m2) and data.is_contiguous()
-            and scale.is_contiguous() and data.data_ptr() % 16 == 0
-            and output_dtype in (torch.bfloat16, torch.float16, torch.float32)):
-        from difflet_b200.ops import fused as F
+    from difflet_b200.ops import fused as F
 
+    if (data.is_cuda and data.dtype in (torch.float8_e4m3fn, torch.float8_e5m2) and data.is_contiguous()
+            and scale.is_contiguous() and output_dtype in (torch.bfloat16, torch.float16, torch.float32)
+            and F.kernel_tensors(data, scale) and data.data_ptr() % 16 == 0):
         return F._kernels().mx_dequantize(data, scale, output_dtype)
     s = torch.pow(2.0, scale.to(torch.float32) - BIAS)
     v = data.to(torch.float32).reshape(*data.shape[:-1], K // GROUP, GROUP) * s[..., None]

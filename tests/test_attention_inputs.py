@@ -212,3 +212,56 @@ def test_meta_tensors():
     x, mod = torch.empty(6, 32, device="meta"), torch.empty(2, 32, device="meta")
     y, s = ops.add_rms_norm(x, x, scale=mod, shift=mod, rows_per_batch=3)
     assert y.shape == s.shape == x.shape and y.is_meta
+
+
+def test_fake_tensors():
+    """Tracing sees the library path: no kernel is given a tensor without data."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, device="cuda", dtype=dtype)  # noqa: E731
+        for D in (64, 128):
+            q, k, v = e(2, 4, 6, D), e(2, 4, 9, D), e(2, 4, 9, D)
+            for fn in BOTH:
+                for m in (e(6, 9, dtype=torch.bool), e(2, 1, 1, 9)):
+                    o = fn(q, k, v, attention_mask=m)
+                    assert o.shape == q.shape and o.is_cuda
+            o = ops.cross_attention(q, k[:, :2], v[:, :2], kv_lens=e(2, dtype=torch.int32))
+            assert o.shape == q.shape and o.is_cuda
+        o = ops.dequantize_mx(e(4, 64, dtype=torch.float8_e4m3fn), e(4, 2, dtype=torch.uint8))
+        assert o.shape == (4, 64) and o.is_cuda
+
+
+def test_forward_mode_is_refused_where_no_tangent_is_carried():
+    import torch.autograd.forward_ad as fwAD
+
+    x = torch.randn(3, 32)
+    bank = ops.LoraBank([torch.randn(4, 32)], [torch.randn(24, 4)])
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, torch.randn(3, 32))
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.add_rms_norm(d)
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.linear_lora(d, torch.randn(24, 32), bank=bank, ids=torch.zeros(3, dtype=torch.long))
+        ops.add_rms_norm(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", BOTH)
+def test_transforms_and_tangents(native, fn):
+    import torch.autograd.forward_ad as fwAD
+
+    q, k, v = _inputs(2, 4, 4, 20, 33, 64, torch.bfloat16, "cuda")
+    m = torch.rand(20, 33, device="cuda") < 0.7
+    m[:, 0] = True
+    call = lambda q, k, v: fn(q, k, v, scale=0.1, attention_mask=m)  # noqa: E731
+    want, _, size, _ = _ref(q, k, v, 0.1, m)
+    got = torch.vmap(call)(*(torch.stack([t, t]) for t in (q, k, v)))
+    assert bool(((got[1].double() - want).abs() <= 2 * torch.finfo(q.dtype).eps * (size + want.abs())).all())
+    t = torch.randn_like(q)
+    f64 = lambda q: ((q @ k.double().transpose(2, 3) * 0.1).masked_fill(~m, -math.inf)).softmax(-1) @ v.double()  # noqa: E731
+    _, ref = torch.func.jvp(f64, (q.double(),), (t.double(),))
+    with torch.nn.attention.sdpa_kernel(torch.nn.attention.SDPBackend.MATH), fwAD.dual_level():
+        tangent = fwAD.unpack_dual(call(fwAD.make_dual(q, t), k, v)).tangent
+    assert tangent is not None  # bf16 throughout: a few roundings (2^-8) of the largest value
+    assert (tangent.double() - ref).abs().max() <= 2.0 ** -5 * ref.abs().max()
