@@ -143,6 +143,11 @@ def _mask_on(mask, q):
     return mask.to(q.device)
 
 
+def _is_key_mask(mask) -> bool:
+    """Whether a mask broadcastable to [B, H, Sq, Sk] is the same for every head and query."""
+    return all(n == 1 for n in mask.shape[-3:-1])
+
+
 def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, lse=None, out=None, bound_min=None,
                     bound_max=None, **kwargs):
     """Attention of ``q [B, H, Sq, D]`` to encoder states ``k [B, Hk, Sk, D]``, ``v [B, Hk, Sk, Dv]`` of another length.
@@ -212,19 +217,42 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         want = (B, H, Sq, k.shape[2])
         if mask.dim() > 4 or any(m not in (1, w) for m, w in zip(mask.shape[::-1], want[::-1])):
             raise ValueError(f"attention_mask {tuple(mask.shape)} does not broadcast to {want}")
+        mask = mask.reshape((1,) * (4 - mask.dim()) + mask.shape)
     scale = 1.0 if scale is None else float(scale)
     if not q.is_cuda or kernel:
         return F.cross_attention(q, k, v, scale, mask=mask, kv_lo=lo, kv_hi=hi, out=out, lse=lse)
-    if hi is not None:  # off the kernel: the window as a mask
+    # off the kernel: the window and a key mask as one mask; what lies at their excluded keys may be anything, and 0 * NaN
+    # would reach the sums
+    keys = None
+    if hi is not None:
         idx = torch.arange(k.shape[2], device=q.device)
-        win = (idx < hi[:, None]) if lo is None else (idx < hi[:, None]) & (idx >= lo[:, None])
-        win = win[:, None, None]
-        if mask is None or mask.dtype == torch.bool:
-            mask = win if mask is None else mask & win
-        else:
-            mask = mask.masked_fill(~win, float("-inf"))
+        keys = ((idx < hi[:, None]) if lo is None else (idx < hi[:, None]) & (idx >= lo[:, None]))[:, None, None]
+    if mask is not None and mask.dtype == torch.bool:
+        if _is_key_mask(mask):
+            keys, mask = mask if keys is None else keys & mask, None
+        elif keys is not None:
+            mask = mask & keys
+    elif mask is not None and keys is not None:
+        mask = mask.masked_fill(~keys, float("-inf"))
+    if keys is not None:
+        keys = keys.expand(*keys.shape[:-1], k.shape[2])
+        k, v = (t.masked_fill(~keys.transpose(2, 3), 0.0) for t in (k, v))
+        mask = keys if mask is None else mask
     rep = H // k.shape[1]
-    o = attention(q, k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1), scale=scale, attention_mask=mask, lse=lse)
+    k, v = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+    if mask is None:
+        o = attention(q, k, v, scale=scale, lse=lse)
+        return o if out is None else out.copy_(o)
+    # a row without a key attends to all of them and is cleared afterwards (softmax of nothing has no value and no gradient)
+    if mask.dtype == torch.bool:
+        empty = ~mask.any(-1, keepdim=True)
+        mask = mask | empty
+    else:
+        empty = (mask == float("-inf")).all(-1, keepdim=True)
+        mask = mask.masked_fill(empty, 0.0)
+    o = attention(q, k, v, scale=scale, attention_mask=mask, lse=lse).masked_fill(empty, 0.0)
+    if lse is not None:
+        lse.masked_fill_(empty.expand(B, H, Sq, 1).reshape(lse.shape), float("-inf"))
     return o if out is None else out.copy_(o)
 
 

@@ -681,16 +681,16 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
         keep &= idx < kv_hi.view(-1, 1)
     if mask is not None and mask.dtype == torch.bool and mask.dim() == 4 and mask.shape[1] == mask.shape[2] == 1:
         keep, mask = keep & mask[:, 0, 0], None
-    vz = v.to(ct).masked_fill(~keep[:, None, :, None], 0.0)
-    s = torch.einsum("bhqd,bhkd->bhqk", q.to(ct), k.to(ct).repeat_interleave(rep, 1)) * scale
+    kz, vz = (t.to(ct).masked_fill(~keep[:, None, :, None], 0.0).repeat_interleave(rep, 1) for t in (k, v))
+    s = torch.einsum("bhqd,bhkd->bhqk", q.to(ct), kz) * scale
     if mask is not None:
         s = s.masked_fill(~mask, float("-inf")) if mask.dtype == torch.bool else s + mask.to(ct)
     s = s.masked_fill(~keep[:, None, None], float("-inf"))
-    m = torch.logsumexp(s, -1) if Sk else s.new_full(s.shape[:-1], float("-inf"))
-    p = torch.where(torch.isinf(m)[..., None] & (m < 0)[..., None], torch.zeros_like(s), torch.softmax(s, -1))
-    o = torch.einsum("bhqk,bhkd->bhqd", p, vz.repeat_interleave(rep, 1)).to(q.dtype)
     if lse is not None:
-        lse.copy_(m.to(lse.dtype).reshape(lse.shape))
+        lse.copy_((torch.logsumexp(s, -1) if Sk else s.new_full(s.shape[:-1], float("-inf"))).to(lse.dtype).reshape(lse.shape))
+    empty = (s == float("-inf")).all(-1, keepdim=True)  # (softmax of nothing has no value and no gradient)
+    p = torch.softmax(s.masked_fill(empty, 0.0), -1).masked_fill(empty, 0.0)
+    o = torch.einsum("bhqk,bhkd->bhqd", p, vz).to(q.dtype)
     return o if out is None else out.copy_(o)
 
 

@@ -265,3 +265,62 @@ def test_transforms_and_tangents(native, fn):
         tangent = fwAD.unpack_dual(call(fwAD.make_dual(q, t), k, v)).tangent
     assert tangent is not None  # bf16 throughout: a few roundings (2^-8) of the largest value
     assert (tangent.double() - ref).abs().max() <= 2.0 ** -5 * ref.abs().max()
+
+
+# ----------------------------------------------------------------------------- excluded keys and empty rows off the kernels
+def _excluded(kind, dtype, device, Sk=33):
+    """Arguments that exclude keys, and which keys every batch row keeps."""
+    n = torch.tensor([Sk, 12, 0], device=device)
+    keep = torch.arange(Sk, device=device) < n[:, None]
+    if kind == "lens":
+        return dict(kv_lens=n), keep, torch.ones(1, 1, 20, Sk, dtype=torch.bool, device=device)
+    if kind == "keys":
+        keep = keep & (torch.arange(Sk, device=device) % 3 != 1)
+        return dict(attention_mask=keep[:, None, None]), keep, torch.ones(1, 1, 20, Sk, dtype=torch.bool, device=device)
+    own = torch.rand(1, 1, 20, Sk, generator=torch.Generator().manual_seed(0)).to(device) < 0.5
+    own[:, :, 3] = False
+    m = own if kind == "lens+bool" else torch.where(own, 0.0, -math.inf).to(dtype)
+    return dict(kv_lens=n, attention_mask=m), keep, own
+
+
+def _excluded_keys(kind, D, dtype, device, tol):
+    q, k, v = _inputs(3, 4, 2, 20, 33, D, dtype, device)
+    kw, keep, own = _excluded(kind, dtype, device)
+    gone = ~keep[:, None, :, None]
+    k, v = k.masked_fill(gone, math.nan).requires_grad_(), v.masked_fill(gone, math.inf).requires_grad_()
+    q = q.detach().requires_grad_()
+    lse = torch.empty(3, 4, 20, device=device)
+    o = ops.cross_attention(q, k, v, scale=0.1, lse=lse, **kw)
+    full = own & keep[:, None, None]
+    some = full.any(-1, keepdim=True)
+    ref = [t.detach().double().masked_fill(g, 0.0).requires_grad_() for t, g in ((q, torch.zeros_like(q).bool()), (k, gone), (v, gone))]
+    z = (ref[0] @ ref[1].repeat_interleave(2, 1).transpose(2, 3) * 0.1).masked_fill(~full & some, -math.inf)
+    want = z.softmax(-1) @ ref[2].repeat_interleave(2, 1) * some
+    assert (o.double() - want).abs().max() <= tol * want.abs().max()
+    lse_ref = torch.logsumexp(z, -1).masked_fill(~some[..., 0], -math.inf)
+    assert torch.allclose(lse.double(), lse_ref, atol=10 * tol)
+    w = torch.randn(want.shape, generator=torch.Generator().manual_seed(1), dtype=torch.float64).to(device)
+    got = torch.autograd.grad((ops.cross_attention(q, k, v, scale=0.1, **kw).double() * w).sum(), (q, k, v))
+    for a, b in zip(got, torch.autograd.grad((want * w).sum(), ref)):
+        assert (a.double() - b).abs().max() <= tol * b.abs().max()
+    out = torch.empty_like(o)
+    with torch.no_grad():
+        assert ops.cross_attention(q, k, v, scale=0.1, out=out, **kw) is out
+    assert (out.double() - want).abs().max() <= tol * want.abs().max() and bool((out[2] == 0).all())
+
+
+KINDS = ["lens", "keys", "lens+bool", "lens+bias"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_excluded_keys_and_empty_rows(kind):
+    _excluded_keys(kind, 16, torch.float32, "cpu", 2.0 ** -18)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype,tol", [(64, torch.float32, 2.0 ** -16), (40, torch.float32, 2.0 ** -16), (64, torch.bfloat16, 2.0 ** -5),
+                                         (128, torch.bfloat16, 2.0 ** -5)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_excluded_keys_and_empty_rows_off_the_kernels(native, kind, D, dtype, tol):
+    """f32, other head dims and gradients take the library path on CUDA, with the same rules."""
+    _excluded_keys(kind, D, dtype, "cuda", tol)
