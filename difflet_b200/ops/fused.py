@@ -621,14 +621,14 @@ def cross_kernel_ok(q, k, v, mask=None) -> bool:
     """Whether the masked / head-dim-64 attention kernel takes these inputs (it records no backward pass: what asks
     for gradients stays on the torch path, and so do tracing and function transforms)."""
     return (q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in (torch.bfloat16, torch.float16)
-            and not wants_grad(q, k, v, mask) and kernel_tensors(q, k, v, mask))
+            and envs.DIFFLET_KERNEL_ATTN != "sdpa" and not wants_grad(q, k, v, mask) and kernel_tensors(q, k, v, mask))
 
 
 def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     """softmax(scale * q k^T) v over [B, H, S, dh]; key window [kv_lo[b], kv_hi[b])."""
     if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128 and not wants_grad(q, k, v):
         return native().attention(q, k, v, float(scale), out, lse, kv_lo, kv_hi, kv_split=kv_split_mode())
-    if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and cross_kernel_ok(q, k, v):
+    if cross_kernel_ok(q, k, v):
         return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     if q.is_cuda and lse is None and kv_lo is None:

@@ -324,3 +324,27 @@ def test_excluded_keys_and_empty_rows(kind):
 def test_excluded_keys_and_empty_rows_off_the_kernels(native, kind, D, dtype, tol):
     """f32, other head dims and gradients take the library path on CUDA, with the same rules."""
     _excluded_keys(kind, D, dtype, "cuda", tol)
+
+
+# ----------------------------------------------------------------------------- the library baseline
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_library_baseline(native, monkeypatch, D):
+    """DIFFLET_KERNEL_ATTN=sdpa: no attention entry launches a kernel of this framework, and the results agree."""
+    from difflet_b200.ops import fused as F
+
+    q, k, v = _inputs(2, 4, 2, 40, 70, D, torch.bfloat16, "cuda")
+    fk, fv = (t.repeat_interleave(2, 1) for t in (k, v))
+    m = torch.rand(2, 1, 40, 70, device="cuda") < 0.6
+    lens = torch.tensor([70, 0], device="cuda")
+    calls = [lambda: ops.cross_attention(q, k, v, scale=0.1), lambda: ops.cross_attention(q, k, v, scale=0.1, attention_mask=m),
+             lambda: ops.cross_attention(q, k, v, scale=0.1, kv_lens=lens, attention_mask=m), lambda: ops.attention(q, fk, fv, scale=0.1),
+             lambda: ops.attention(q, fk, fv, scale=0.1, attention_mask=m), lambda: F.attention(q, fk, fv, 0.1),
+             lambda: ops.cross_attention(q[:, :, :2], k, v, scale=0.1, kv_lens=lens)]
+    kernels = [f() for f in calls]
+    monkeypatch.setenv("DIFFLET_KERNEL_ATTN", "sdpa")
+    n = F.LAUNCHES[0]
+    library = [f() for f in calls]
+    assert F.LAUNCHES[0] == n
+    for a, b in zip(kernels, library):  # both round P and the result
+        assert (a.double() - b.double()).abs().max() <= 2.0 ** -6 * v.abs().max()
