@@ -552,11 +552,12 @@ at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarTy
 
 // ---------------------------------------------------------------- cross attention
 // q [B, H, Sq, dh], k / v [B, Hk, Sk, dh]; mask: bool (true = attend) or additive, broadcastable to
-// [B, H, Sq, Sk]; kv_lo / kv_hi int32 [B].
+// [B, H, Sq, Sk]; kv_lo / kv_hi int32 [B]; p2: P in two terms.
 at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
                            const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& kv_lo,
                            const c10::optional<at::Tensor>& kv_hi, const c10::optional<at::Tensor>& out,
-                           const c10::optional<at::Tensor>& lse) {
+                           const c10::optional<at::Tensor>& lse, bool p2) {
+  TORCH_CHECK_VALUE(!p2 || !given(mask), "precise_p comes without a mask");
   TORCH_CHECK_VALUE(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q/k/v must be CUDA tensors [B, H, S, D]");
   TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
                     "cross attention runs in bfloat16 or float16, got ", q.scalar_type());
@@ -599,6 +600,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   a.v_bs = stride(v_, 0), a.v_hs = stride(v_, 1), a.v_ss = stride(v_, 2);
   a.o_bs = stride(o_, 0), a.o_hs = stride(o_, 1), a.o_ss = stride(o_, 2);
   a.f16 = q.scalar_type() == at::kHalf;
+  a.p2 = p2;
   a.scale = (float)scale;
   if (const at::Tensor* t = given(lse)) {
     TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->is_contiguous() && t->device() == q.device() &&
@@ -651,7 +653,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     d.m_bs = ms[0], d.m_hs = ms[1], d.m_qs = ms[2], d.m_ks = ms[3];
   }
   d.err = err_ptr();
-  if (dfl_cross_decode_takes(&d)) {  // too few rows to fill the other kernel's tiles: the keys are split instead
+  if (!p2 && dfl_cross_decode_takes(&d)) {  // too few rows to fill the other kernel's tiles: the keys are split instead
     DFL_CHECK_RC(dfl_cross_decode(&d, cur_stream()), "cross_attention (few queries)");
     if (!direct) o.copy_(o_);
     return o;
@@ -1320,7 +1322,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("rows_per_batch"), py::arg("row_map"), py::arg("eps"), py::arg("quant"), py::arg("blocked"),
         py::arg("out"), py::arg("s_out"));
   m.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"),
-        py::arg("mask"), py::arg("kv_lo"), py::arg("kv_hi"), py::arg("out"), py::arg("lse"));
+        py::arg("mask"), py::arg("kv_lo"), py::arg("kv_hi"), py::arg("out"), py::arg("lse"), py::arg("p2"));
   m.def("mx_dequantize", &mx_dequantize, py::arg("q"), py::arg("scales"), py::arg("dtype"));
   m.def("qkv_scatter", &qkv_scatter);
   m.def("qkv_plan", &qkv_plan);

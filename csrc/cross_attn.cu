@@ -135,5 +135,6 @@ extern "C" int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream) {
     return -5;
   if (!(a->scale > 0.f)) return -6;
   if (a->bits && ((a->bits_bs | a->bits_hs | a->bits_qs) % 4 || a->bias_tiles)) return -7;
+  if (a->p2 && (a->bits || a->bias_tiles)) return -8;
   return a->f16 ? dfl_cross_attention_f16(a, stream) : cross_entry<false>(a, stream);
 }

@@ -5,7 +5,8 @@
 //
 // A row whose mask leaves no key is 0 (log-sum-exp -inf).  One pass over the keys with a running maximum
 // and sum; statistics and accumulators are f32, P is rounded to the inputs' type for the P V
-// product (the sum uses the unrounded values).
+// product (the sum uses the unrounded values); callers that had f32 throughout before (LSE or a key window at
+// head dim 64) take the variant that splits P into two such values.
 //
 // Persistent, one CTA per SM; a work item is a block of QT * 128 queries of one head:
 //   TMA warp     Q tiles of the next item as soon as the last Q K^T of this one has read them;
@@ -214,7 +215,8 @@ DFL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
   return d;
 }
 
-template <int DH, bool F16, int QT, int MASK>
+// P2: P goes to the product as the sum of two values of the inputs' type (2^-16 of p in bf16 where one value keeps 2^-8).
+template <int DH, bool F16, int QT, int MASK, bool P2>
 __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     cross_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
@@ -340,6 +342,13 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
             const int kk = hf * (kBN / 32) + kq;
             umma_f16_ts(o_t, tmem + 128u * g + kk * 8, kHiV | (va + (uint32_t)((kk * 2048) >> 4)), idesc_pv,
                         (!first || kk > 0) ? 1u : 0u);
+          }
+          if constexpr (P2) {  // the second terms lie behind the first, in the other half of S
+#pragma unroll
+            for (int kq = 0; kq < kBN / 32; ++kq) {
+              const int kk = hf * (kBN / 32) + kq;
+              umma_f16_ts(o_t, tmem + 128u * g + 64u + kk * 8, kHiV | (va + (uint32_t)((kk * 2048) >> 4)), idesc_pv, 1u);
+            }
           }
         }
         if (last) umma_commit(&o_full[g]);
@@ -534,7 +543,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         const uint64_t sc2 = f2_pack(sc, sc), nm2 = f2_pack(-m_use, -m_use);
 #pragma unroll
         for (int qtr = 0; qtr < 4; ++qtr) {
-          uint32_t pk[16];
+          uint32_t pk[16], p2[P2 ? 16 : 1];
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const uint64_t zz = f2_pack(z[qtr * 32 + 2 * c], z[qtr * 32 + 2 * c + 1]);
@@ -547,8 +556,13 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
             const float e0 = exp2_sfu(x0), e1 = exp2_sfu(x1);
             rs[c & 1] = f2_add(rs[c & 1], f2_pack(e0, e1));
             pk[c] = pack2<F16>(e0, e1);
+            if constexpr (P2) {
+              const float2 first = unpack2<F16>(pk[c]);
+              p2[c] = pack2<F16>(e0 - first.x, e1 - first.y);
+            }
           }
           tmem_st_32x32b_x16(s_t + qtr * 16, pk);
+          if constexpr (P2) tmem_st_32x32b_x16(s_t + 64 + qtr * 16, p2);
           if (qtr & 1) {
             tmem_wait_st();
             tc_fence_before();
@@ -630,10 +644,10 @@ inline int cross_tmap(CUtensorMap* map, const void* base, int D, long long S, in
                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-template <int DH, bool F16, int QT, int MASK>
+template <int DH, bool F16, int QT, int MASK, bool P2>
 int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev) {
   using C = CrossCfg<DH, QT>;
-  auto kern = cross_attn_kernel<DH, F16, QT, MASK>;
+  auto kern = cross_attn_kernel<DH, F16, QT, MASK, P2>;
   static bool attr[16] = {false};
   if (!attr[dev & 15]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal);
@@ -662,11 +676,11 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
 }
 
 // Two ping-pong Q tiles per CTA unless one holds every query, or twice the items still fit the SMs.
-template <int DH, bool F16, int MASK>
+template <int DH, bool F16, int MASK, bool P2 = false>
 int launch_cross_qt(const CrossArgs* a, const CrossParams& p, cudaStream_t stream, int dev) {
   const long long items2 = (long long)((a->Sq + 2 * kBM - 1) / (2 * kBM)) * a->H * a->B;
-  if (a->Sq <= kBM || items2 * 2 <= dfl_host::num_sms(dev)) return launch_cross<DH, F16, 1, MASK>(a, p, stream, dev);
-  return launch_cross<DH, F16, 2, MASK>(a, p, stream, dev);
+  if (a->Sq <= kBM || items2 * 2 <= dfl_host::num_sms(dev)) return launch_cross<DH, F16, 1, MASK, P2>(a, p, stream, dev);
+  return launch_cross<DH, F16, 2, MASK, P2>(a, p, stream, dev);
 }
 
 template <int DH, bool F16>
@@ -675,6 +689,7 @@ int launch_cross_mask(const CrossArgs* a, const CrossParams& p, cudaStream_t str
     return a->bias_f32 ? launch_cross_qt<DH, F16, kBias32>(a, p, stream, dev)
                        : launch_cross_qt<DH, F16, kBias16>(a, p, stream, dev);
   if (a->bits) return launch_cross_qt<DH, F16, kBits>(a, p, stream, dev);
+  if (a->p2) return launch_cross_qt<DH, F16, kWindow, true>(a, p, stream, dev);
   return launch_cross_qt<DH, F16, kWindow>(a, p, stream, dev);
 }
 

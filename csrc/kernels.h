@@ -320,6 +320,7 @@ typedef struct CrossArgs {
   const void* bias_tiles;
   long long bias_bs, bias_hs, bias_qs, bias_ts;
   int bias_rows, bias_f32;
+  int p2;                              // P as the sum of two values of the inputs' type (no bits, no bias)
   int* err;
 } CrossArgs;
 int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream);

@@ -79,13 +79,14 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
             hi = hi.to(q.device, torch.int32 if q.is_cuda else torch.int64).contiguous()
         out = F.attention(q4, k4, v4, scale, lse=lse, kv_lo=lo, kv_hi=hi)
     elif (F.cross_kernel_ok(q, k, v, attention_mask) and not causal and k4.dtype == v4.dtype == q4.dtype
-          and k4.shape == v4.shape and k4.shape[:2] == q4.shape[:2]):
+          and k4.shape == v4.shape and k4.shape[:2] == q4.shape[:2] and (lse is None or simple)):
         mask = attention_mask if simple or bound_min is None else _bounds_to_mask(k4, bound_min, bound_max, None)
         if lo is not None and simple:
             lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
         else:
             lo = hi = None
-        out = F.cross_attention(q4, k4, v4, scale, mask=_mask_on(mask, q), kv_lo=lo, kv_hi=hi, lse=lse)
+        out = F.cross_attention(q4, k4, v4, scale, mask=_mask_on(mask, q), kv_lo=lo, kv_hi=hi, lse=lse,
+                                precise_p=lse is not None)  # (partials that are merged by their LSE: f32 up to the result)
     else:
         mask = _bounds_to_mask(k4, bound_min, bound_max, attention_mask)
         if lse is not None or not q.is_cuda:  # math path (oracle, or LSE requested off the kernel)

@@ -628,8 +628,9 @@ def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     """softmax(scale * q k^T) v over [B, H, S, dh]; key window [kv_lo[b], kv_hi[b])."""
     if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128 and not wants_grad(q, k, v):
         return native().attention(q, k, v, float(scale), out, lse, kv_lo, kv_hi, kv_split=kv_split_mode())
-    if cross_kernel_ok(q, k, v):
-        return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse)
+    if cross_kernel_ok(q, k, v):  # (a window or LSE: these have always been f32 up to the result)
+        return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse,
+                               precise_p=lse is not None or kv_lo is not None or kv_hi is not None)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     if q.is_cuda and lse is None and kv_lo is None:
         o = F.scaled_dot_product_attention(q, k, v, scale=float(scale))
@@ -658,7 +659,7 @@ def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     return o
 
 
-def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=None, lse=None):
+def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=None, lse=None, precise_p=False):
     """softmax(scale q k^T [+ mask]) v with keys of another length than the queries.
 
     q [B, H, Sq, D]; k, v [B, Hk, Sk, D] with H a multiple of Hk (query head h reads key head
@@ -666,11 +667,12 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
     the type's lowest value masks), broadcastable to [B, H, Sq, Sk]; beside it the key window
     [kv_lo[b], kv_hi[b]) (int32 [B]).  A row without a key is 0 with LSE -inf.  What k and v hold at keys
     that the window or a key mask (bool, the same for every head and query) excludes is not used.
-    CUDA: bf16 / fp16 with D 64 or 128 run the tcgen05 kernel."""
+    CUDA: bf16 / fp16 with D 64 or 128 run the tcgen05 kernel, where P is rounded to the type for its product with v, or
+    with ``precise_p`` (no mask) goes as the sum of two values of the type."""
     if q.is_cuda:
         if scale <= 0:  # the kernel scales inside the exponent, where the maximum must commute with it
             q, scale = (-q, -scale) if scale < 0 else (torch.zeros_like(q), 1.0)
-        return _kernels().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse)
+        return _kernels().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse, precise_p)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     Sk, rep = k.shape[2], q.shape[1] // k.shape[1]
     idx = torch.arange(Sk, device=q.device)

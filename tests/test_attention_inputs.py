@@ -348,3 +348,65 @@ def test_library_baseline(native, monkeypatch, D):
     assert F.LAUNCHES[0] == n
     for a, b in zip(kernels, library):  # both round P and the result
         assert (a.double() - b.double()).abs().max() <= 2.0 ** -6 * v.abs().max()
+
+
+# ----------------------------------------------------------------------------- LSE and windows: f32 up to the result
+def _check_precise(o, ref, dtype, D, Sk, vmax, lse=None):
+    """As ``_check``, with P in two terms of the type: off by u^2 (u: half a step), in fp16 by 2^-25 absolutely."""
+    want, lse_ref, size, bound = ref
+    u = torch.finfo(dtype).eps / 2
+    d = 2.0 ** -24 * (D + 4) * bound + 2.0 ** -20
+    tol = (u * u + 2 * d) * size + u * want.abs() + 1e-30
+    if dtype == torch.float16:
+        tol = tol + Sk * 2.0 ** -25 * vmax + 2.0 ** -25
+    err = (o.double() - want).abs()
+    assert bool((err <= tol).all()), f"worst {(err / tol).nan_to_num(1e9).max().item():.3g} of the tolerance"
+    if lse is not None:
+        fine = torch.isfinite(lse_ref)
+        assert torch.equal(fine, torch.isfinite(lse.double()))
+        assert bool(((lse.double() - lse_ref).abs()[fine] <= d + 2.0 ** -20 * (1 + lse_ref.abs()[fine])).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Sq,Sk,D", [(1, 1, 1, 1, 64), (2, 3, 5, 77, 64), (2, 4, 129, 128, 64), (2, 2, 501, 1024, 64), (3, 24, 1100, 130, 64),
+                                         (2, 40, 300, 2000, 64), (1, 1, 3, 200, 128), (2, 3, 257, 129, 128), (3, 20, 600, 300, 128)])
+def test_lse_and_windows_keep_f32(native, B, H, Sq, Sk, D, dtype):
+    """Head dim 64 (and fp16) with LSE or a key window was f32 up to the result: P may not be rounded to the type once."""
+    from difflet_b200.ops import fused as F
+    from difflet_b200.ops.attn import attention_with_lse
+
+    q, k, v = _inputs(B, H, H, Sq, Sk, D, dtype, "cuda", Sq + Sk)
+    vmax = v.abs().max().item()
+    lse = torch.empty(B, H, Sq, device="cuda")
+    ref = _ref(q, k, v, D ** -0.5)
+    if D == 64:
+        _check_precise(F.attention(q, k, v, D ** -0.5, lse=lse), ref, dtype, D, Sk, vmax, lse)
+        hi = torch.tensor([(Sk, 2 * Sk // 3, 0)[b] for b in range(B)], device="cuda", dtype=torch.int32)
+        lo = (hi // 5).int()
+        keep = (torch.arange(Sk, device="cuda") >= lo[:, None]) & (torch.arange(Sk, device="cuda") < hi[:, None])
+        win = _ref(q, k, v, D ** -0.5, keep[:, None, None])
+        clean = F.attention(q, k, v, D ** -0.5, kv_lo=lo, kv_hi=hi)
+        _check_precise(clean, win, dtype, D, Sk, vmax)
+        gone = ~keep[:, None, :, None]
+        dirty = F.attention(q, k.masked_fill(gone, math.nan), v.masked_fill(gone, math.inf), D ** -0.5, kv_lo=lo, kv_hi=hi)
+        assert torch.equal(dirty, clean)
+    if D == 64 or dtype == torch.float16:
+        o, lse = attention_with_lse(q, k, v, scale=D ** -0.5)
+        _check_precise(o, ref, dtype, D, Sk, vmax, lse)
+    m = torch.rand(B, 1, Sq, Sk, device="cuda") < 0.7
+    lse = torch.empty(B, H, Sq, device="cuda")
+    o = ops.attention(q, k, v, scale=D ** -0.5, attention_mask=m, lse=lse)
+    _check_precise(o, _ref(q, k, v, D ** -0.5, m), dtype, D, Sk, vmax, lse)
+    from difflet_b200 import _native
+
+    _native.check_device_errors()
+
+
+@pytest.mark.gpu
+def test_precise_p_comes_without_a_mask(native):
+    from difflet_b200.ops import fused as F
+
+    q, k, v = _inputs(1, 2, 2, 3, 5, 64, torch.bfloat16, "cuda")
+    with pytest.raises(ValueError):
+        F.cross_attention(q, k, v, 1.0, mask=torch.ones(3, 5, device="cuda", dtype=torch.bool), precise_p=True)
