@@ -158,8 +158,8 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     attend) or additive (integers too), broadcastable to ``[B, H, Sq, Sk]``; moved to q's device as in ``attention``
     (refused there with shared key heads on CUDA).  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
-    ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (f32 ``[B, H, Sq]``,
-    natural log) are filled when given.  CUDA: bf16 and fp16 with D = Dv = 64 or 128; anything else, and what asks
+    ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (``[B, H, Sq]``,
+    natural log) are filled when given (an LSE that is not contiguous f32 on q's device by a copy).  CUDA: bf16 and fp16 with D = Dv = 64 or 128; anything else, and what asks
     for gradients, runs as ``attention``."""
     kernel = k.shape[-1] == v.shape[-1] and F.cross_kernel_ok(q, k, v, attention_mask)
     if (kernel and q.dim() == k.dim() == 4 and k.shape[0] == q.shape[0] and k.shape[1] <= q.shape[1]
@@ -192,8 +192,8 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         raise ValueError("q, k and v must share type and device")
     if out is not None and (out.shape != (B, H, Sq, v.shape[3]) or out.dtype != q.dtype or out.device != q.device):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not {(B, H, Sq, v.shape[3])} {q.dtype}")
-    if lse is not None and (lse.numel() != B * H * Sq or not lse.is_contiguous()):
-        raise ValueError(f"lse must be contiguous [{B}, {H}, {Sq}]")
+    if lse is not None and lse.numel() != B * H * Sq:
+        raise ValueError(f"lse must hold [{B}, {H}, {Sq}]")
     lo = hi = None
     if kv_lens is not None:
         if bound_min is not None or bound_max is not None:

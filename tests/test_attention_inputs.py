@@ -410,3 +410,41 @@ def test_precise_p_comes_without_a_mask(native):
     q, k, v = _inputs(1, 2, 2, 3, 5, 64, torch.bfloat16, "cuda")
     with pytest.raises(ValueError):
         F.cross_attention(q, k, v, 1.0, mask=torch.ones(3, 5, device="cuda", dtype=torch.bool), precise_p=True)
+
+
+# ----------------------------------------------------------------------------- LSE of any type and layout
+def _lse_kinds(B, H, Sq, device):
+    return [torch.empty(B, H, Sq, dtype=torch.float64, device=device), torch.empty(B, Sq, H, device=device).transpose(1, 2),
+            torch.empty(B * H, Sq, dtype=torch.bfloat16, device=device), torch.empty(B, H, Sq, 2, device=device)[..., 1]]
+
+
+def _any_lse(D, dtype, device):
+    from difflet_b200.ops import fused as F
+
+    B, H, Sq, Sk = 2, 4, 30, 41
+    q, k, v = _inputs(B, H, H, Sq, Sk, D, dtype, device)
+    m = torch.rand(B, 1, Sq, Sk, generator=torch.Generator().manual_seed(0)).to(device) < 0.7
+    lens = torch.tensor([41, 7], device=device)
+    calls = [lambda t: ops.cross_attention(q, k, v, scale=0.1, lse=t), lambda t: ops.cross_attention(q, k, v, scale=0.1, attention_mask=m, lse=t),
+             lambda t: ops.cross_attention(q, k, v, scale=0.1, kv_lens=lens, lse=t), lambda t: ops.attention(q, k, v, scale=0.1, lse=t),
+             lambda t: ops.attention(q, k, v, scale=0.1, attention_mask=m, lse=t), lambda t: F.attention(q, k, v, 0.1, lse=t)]
+    for i, call in enumerate(calls if (D, dtype) != (128, torch.bfloat16) else calls[:3]):
+        want = torch.empty(B, H, Sq, device=device)
+        o = call(want)
+        for t in _lse_kinds(B, H, Sq, device):
+            if i in (3, 5) and t.dim() != 3:  # (plain attention takes the full shape)
+                continue
+            assert torch.equal(call(t), o) and torch.equal(t.reshape(B, H, Sq), want.to(t.dtype))
+    for bad in (torch.empty(B, H, Sq + 1, device=device), torch.empty(B, H, 2, dtype=torch.float64, device=device)):
+        with pytest.raises(ValueError):
+            calls[0](bad)
+
+
+def test_any_lse():
+    _any_lse(16, torch.float32, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16), (64, torch.float32)])
+def test_any_lse_on_cuda(native, D, dtype):
+    _any_lse(D, dtype, "cuda")
