@@ -219,7 +219,7 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
   }
   if (M == 0) return res;
   c10::optional<at::Tensor> out = res.dim() == 2 ? res : res.view({M, N}), resid;
-  TORCH_CHECK_VALUE(out->stride(1) == 1 && out->stride(0) % (out_f32 ? 4 : 8) == 0 &&
+  TORCH_CHECK_VALUE(out->stride(1) == 1 && (M == 1 || out->stride(0) % (out_f32 ? 4 : 8) == 0) &&
                         reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, "out needs 16-byte aligned rows");
   if (const at::Tensor* t = given(bias))
     TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 && t->dim() == 1 && t->numel() == N && t->is_contiguous() &&
@@ -245,6 +245,7 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
   a.lda = A.stride(0);
   a.ldb = B.stride(0);
   a.K = (int)K;
+  if (M == 1) a.lda = K, a.ldd = N, a.ldr = N;  // one row has no stride to speak of
   LoraArgs l{};
   a.lora = &l;
   l.a = A_l.data_ptr();

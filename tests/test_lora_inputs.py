@@ -32,3 +32,23 @@ def test_gradients_are_refused():
 @pytest.mark.gpu
 def test_gradients_are_refused_on_cuda(native):
     _gradients_are_refused("cuda", BF)
+
+
+@pytest.mark.gpu
+def test_one_row_of_any_pitch(native):
+    """A single row cut from a tensor whose rows are no whole 16-byte pieces apart: a row has no stride to speak of."""
+    K, N = 512, 256
+    x, w, b, A, B, scale = _make(4, N, K, [16, 8], "cuda")
+    bank, ids = ops.LoraBank(A, B, scale), torch.tensor([1], device="cuda")
+    y, err = _ref(x[:1], w, b, A, B, scale, ids, 2.0 ** -8)
+    for pad in (3, 4, 8):
+        wide = torch.zeros(4, K + pad, device="cuda", dtype=BF)
+        wide[:, :K] = x
+        got = ops.linear_lora(wide[:1, :K], w, b, bank=bank, ids=ids)
+        _compare(got, y, err, None, 2.0 ** -8)
+        out, resid = torch.zeros(4, N + pad, device="cuda", dtype=BF), torch.ones(4, N + pad, device="cuda", dtype=BF)
+        gate = torch.ones(1, N + pad, device="cuda")[:, :N]
+        assert torch.equal(ops.linear_lora(wide[:1, :K], w, b, bank=bank, ids=ids, out=out[:1, :N]), got)
+        assert torch.equal(out[:1, :N], got) and bool((out[1:] == 0).all() and (out[:, N:] == 0).all())
+        gated = ops.linear_lora(wide[:1, :K], w, b, bank=bank, ids=ids, gate=gate, resid=resid[:1, :N])
+        assert torch.equal(gated, ops.linear_lora(x[:1], w, b, bank=bank, ids=ids, gate=gate, resid=torch.ones(1, N, device="cuda", dtype=BF)))
