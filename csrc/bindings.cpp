@@ -457,20 +457,21 @@ std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at
     TORCH_CHECK_VALUE(v.stride(1) == 1 || D == 1, name, " needs a unit inner stride");
     return v;
   };
+  auto pitch = [&](const at::Tensor& t) { return (long long)(M == 1 ? D : t.stride(0)); };  // one row has no stride to speak of
   a.x = x2.data_ptr();
-  a.ldx = x2.stride(0);
+  a.ldx = pitch(x2);
   at::Tensor s, s2, r2;
   if (const at::Tensor* r = given(resid)) {
     like_x(*r, "resid");
     r2 = r->dim() == 2 ? *r : r->reshape({-1, D});
     TORCH_CHECK_VALUE(r2.stride(1) == 1 || D == 1, "resid needs a unit inner stride");
     a.resid = r2.data_ptr();
-    a.ldr = r2.stride(0);
+    a.ldr = pitch(r2);
     if (given(s_out)) like_x(*s_out, "resid_out");
     s = given(s_out) ? *s_out : new_like(x, x.sizes(), x.scalar_type());
     s2 = rows(s, "resid_out");
     a.s_out = s2.data_ptr();
-    a.lds = s2.stride(0);
+    a.lds = pitch(s2);
   } else {
     TORCH_CHECK_VALUE(!given(s_out), "resid_out needs resid");
   }
@@ -499,7 +500,7 @@ std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at
     TORCH_CHECK_VALUE(a.n_mod == 0 || a.n_mod == t->size(0), "scale and shift differ in their batch rows");
     a.n_mod = (int)t->size(0);
     p = t->data_ptr<float>();
-    bs = t->stride(0);
+    bs = a.n_mod == 1 ? 0 : t->stride(0);
   };
   mod(scale, "scale", a.scale, a.scale_bs);
   mod(shift, "shift", a.shift, a.shift_bs);
@@ -531,7 +532,7 @@ std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at
     y = given(out) ? *out : new_like(x, x.sizes(), x.scalar_type());
     y2 = rows(y, "out");
     a.y = y2.data_ptr();
-    a.ldy = y2.stride(0);
+    a.ldy = pitch(y2);
   }
   const int rc = dfl_add_rms_norm(&a, cur_stream());
   TORCH_CHECK_VALUE(rc != -3, "the MX output needs 16-byte aligned rows of x, resid, weight, scale and shift");
