@@ -19,9 +19,9 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "common.cuh"
+#include "found_once.h"
 #include "kernels.h"
 
 namespace {
@@ -382,8 +382,6 @@ int decode_tmap(CUtensorMap* map, const void* base, const DecodeArgs* a, long lo
 // Clusters of 1, 2, 4, 8 or 16 CTAs that are resident together (0: this size cannot be launched), found once per device.
 struct Resident {
   int clusters[5] = {0, 0, 0, 0, 0};
-  cudaError_t err = cudaSuccess;
-  std::once_flag once;
 };
 
 int rows_of(const DecodeArgs* a) { return a->H / a->Hk * a->Sq; }
@@ -398,11 +396,11 @@ struct Plan {
 
 template <int DH, bool F16, int NB>
 int plan_decode(const DecodeArgs* a, Plan* plan) {
-  static Resident resident[16];
+  static dfl_host::FoundOnce<Resident> resident[16];
   int dev = 0;
   cudaGetDevice(&dev);
-  Resident& res = resident[dev & 15];
-  std::call_once(res.once, [&] {
+  Resident res;
+  const int rc = resident[dev & 15].get(&res, [&](Resident* r) {
     auto kern = cross_decode_kernel<DH, F16, NB>;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
@@ -417,11 +415,11 @@ int plan_decode(const DecodeArgs* a, Plan* plan) {
     for (int i = 0; i < 5 && e == cudaSuccess; ++i) {
       at[0].val.clusterDim.x = 1 << i;
       cfg.gridDim = dim3((unsigned)(1 << i), 1024, 1);
-      e = cudaOccupancyMaxActiveClusters(&res.clusters[i], kern, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&r->clusters[i], kern, &cfg);
     }
-    res.err = e;
+    return (int)e;
   });
-  if (res.err != cudaSuccess) return (int)res.err;
+  if (rc) return rc;
   // CTAs per key head: each wave of clusters costs its keys per CTA and a launch, ramp and join worth about 300 keys of
   // 128 values; no CTA gets less than a turn of its warps.  64 heads of 4096 keys take 4 (1, 2, 4, 8, 16: 52, 30, 24, 28,
   // 42 us), 72 of 512 take 2 (9.0, 6.8, 9.6, 12.8, 25 us), 48 of 4096 x 64 take 8 (45, 25, 16, 12, 22 us), 480 of 1024

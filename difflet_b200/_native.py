@@ -45,7 +45,7 @@ CUDA_SOURCES = [
     "vae_gn.cu",
 ]
 CPP_SOURCES = ["bindings.cpp"]
-HEADERS = ["common.cuh", "kernels.h", "probe_noalloc.h", "gemm_epilogue.cuh", "cross_attn.cuh"]
+HEADERS = ["common.cuh", "kernels.h", "probe_noalloc.h", "gemm_epilogue.cuh", "cross_attn.cuh", "found_once.h"]
 
 NVCC_FLAGS = [
     "-gencode",
