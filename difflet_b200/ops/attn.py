@@ -58,6 +58,12 @@ def _per_batch(bound, B):
     return b
 
 
+def _edge(t, n, device):
+    """A window edge as int32 for keys [0, n): what lies past either end is that end, fractions count as in ``key < edge``."""
+    t = t.ceil() if t.is_floating_point() else t.long()
+    return t.clamp(0, n).to(device, torch.int32).contiguous()
+
+
 def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_min=None, bound_max=None,
               tp_q=False, tp_k=False, tp_out=False, lse=None, **kwargs):
     del tp_q, tp_k, tp_out, kwargs
@@ -82,7 +88,7 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
           and k4.shape == v4.shape and k4.shape[:2] == q4.shape[:2] and (lse is None or simple)):
         mask = attention_mask if simple or bound_min is None else _bounds_to_mask(k4, bound_min, bound_max, None)
         if lo is not None and simple:
-            lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
+            lo, hi = (_edge(t, k4.shape[2], q.device) for t in (lo, hi))
         else:
             lo = hi = None
         out = F.cross_attention(q4, k4, v4, scale, mask=_mask_on(mask, q), kv_lo=lo, kv_hi=hi, lse=lse,
@@ -198,10 +204,9 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     if kv_lens is not None:
         if bound_min is not None or bound_max is not None:
             raise ValueError("kv_lens and bounds are mutually exclusive")
-        if kv_lens.shape != (B,) or kv_lens.is_floating_point():
+        if kv_lens.shape != (B,) or kv_lens.is_floating_point() or kv_lens.dtype == torch.bool:
             raise ValueError(f"kv_lens must be integers [{B}]")
-        hi = kv_lens if kv_lens.dtype == torch.int32 and kv_lens.device == q.device else kv_lens.to(q.device, torch.int32)
-        hi = hi.contiguous()
+        hi = _edge(kv_lens, k.shape[2], q.device)
     elif bound_min is not None or bound_max is not None:
         if bound_min is None or bound_max is None:
             raise ValueError("bound_min and bound_max must both be provided")
@@ -211,7 +216,7 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         if lo is None or hi is None:
             attention_mask, lo, hi = _bounds_to_mask(k, bound_min, bound_max, None), None, None
         else:
-            lo, hi = (t.to(q.device, torch.int32).contiguous() for t in (lo, hi))
+            lo, hi = (_edge(t, k.shape[2], q.device) for t in (lo, hi))
     mask = attention_mask
     if mask is not None:
         mask = _mask_on(mask, q)

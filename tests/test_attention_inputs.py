@@ -448,3 +448,34 @@ def test_any_lse():
 @pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16), (64, torch.float32)])
 def test_any_lse_on_cuda(native, D, dtype):
     _any_lse(D, dtype, "cuda")
+
+
+# ----------------------------------------------------------------------------- lengths and bounds past the ends
+def _past_the_ends(D, dtype, device):
+    q, k, v = _inputs(2, 4, 4, 6, 9, D, dtype, device)
+    big = torch.iinfo(torch.int64).max
+    same = lambda a, b: torch.equal(a, b)  # noqa: E731
+    every = ops.cross_attention(q, k, v, scale=0.25, kv_lens=torch.tensor([9, 9], device=device))
+    for lens in (torch.tensor([1 << 40, big]), torch.tensor([(1 << 32) + 3, 1 << 31]), torch.tensor([9, 127], dtype=torch.int8)):
+        assert same(ops.cross_attention(q, k, v, scale=0.25, kv_lens=lens.to(device)), every)
+    assert bool((ops.cross_attention(q, k, v, scale=0.25, kv_lens=torch.tensor([-big, -(1 << 32) + 5], device=device)) == 0).all())
+    edge = lambda *n: torch.tensor(n, device=device).view(2, 1, 1, 1)  # noqa: E731
+    want = ops.cross_attention(q, k, v, scale=0.25, bound_min=edge(2, 0), bound_max=edge(9, 9))
+    for lo, hi in ((edge(2, -big), edge(big, 1 << 32)), (edge(1.5, -0.5), edge(8.5, 1e30))):
+        assert same(ops.cross_attention(q, k, v, scale=0.25, bound_min=lo, bound_max=hi), want)
+        if q.is_cuda:
+            m = (torch.arange(9, device=device) >= edge(2, 0)) & (torch.arange(9, device=device) < 9)
+            o = ops.attention(q, k, v, scale=0.25, bound_min=lo, bound_max=hi)
+            assert (o.double() - _ref(q, k, v, 0.25, m)[0]).abs().max() <= 2 * torch.finfo(dtype).eps * v.abs().max()
+    with pytest.raises(ValueError):
+        ops.cross_attention(q, k, v, kv_lens=torch.tensor([True, False], device=device))
+
+
+def test_lengths_and_bounds_past_the_ends():
+    _past_the_ends(16, torch.float32, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16), (40, torch.bfloat16), (64, torch.float32)])
+def test_lengths_and_bounds_past_the_ends_on_cuda(native, D, dtype):
+    _past_the_ends(D, dtype, "cuda")
