@@ -322,6 +322,8 @@ def add_rms_norm(x, resid=None, weight=None, *, eps=1e-6, scale=None, shift=None
         y = y * weight.to(ct)
     if M and (scale is not None or shift is not None):
         b = row_map.long() if row_map is not None else torch.arange(M, device=x.device) // (rows_per_batch or M)
+        if row_map is not None and not x.is_meta and bool(((b < 0) | (b >= (shift if scale is None else scale).shape[0])).any()):
+            raise IndexError("row_map names a row that scale / shift do not hold")
         if scale is not None:
             y = y * (1 + scale.to(ct)[b])
         if shift is not None:

@@ -34,3 +34,13 @@ def test_one_row_of_any_pitch(native, pad, dtype):
     assert torch.equal(y, want) and torch.equal(s, s_want) and y is y_out and s is s_out
     for t, was in zip(big, rest):
         assert torch.equal(t[1:], was[1:]) and torch.equal(t[:, D:], was[:, D:])
+
+
+def test_a_row_map_entry_that_does_not_exist():
+    """An error (on CUDA in the device error word); -1 is not the last row."""
+    x, mod = torch.randn(3, 8), torch.randn(2, 8)
+    for kw in (dict(scale=mod), dict(shift=mod), dict(scale=mod, shift=mod)):
+        ops.add_rms_norm(x, row_map=torch.tensor([0, 1, 1], dtype=torch.int32), **kw)
+        for bad in (-1, 2):
+            with pytest.raises(IndexError):
+                ops.add_rms_norm(x, row_map=torch.tensor([0, bad, 1], dtype=torch.int32), **kw)
