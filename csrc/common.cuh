@@ -128,6 +128,12 @@ DFL_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int kid, int
   }
 }
 
+// The same by a whole warp, with one outcome for its lanes: a lane that gave up alone would be missing from the warp's next
+// collective operation, which would then never end.
+DFL_DEVICE bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int kid, int detail, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, kid, detail, abort_flag));
+}
+
 // ---------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor) -- plain loads only.  No cross-CTA broadcast form
 // exists in this code base: a tile that several CTAs need is fetched by each.

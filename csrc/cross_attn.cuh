@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
           const uint4 b = cross_bits(p, it, 0, k0);
           w[0] = b.x, w[1] = b.y, w[2] = b.z, w[3] = b.w;
         }
-        if (!mbar_wait(&kv_full[L % R], (L / R) & 1, err, kKidCross, 140, abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&kv_full[L % R], (L / R) & 1, err, kKidCross, 140, abort_flag)) { ok = false; break; }
         uint8_t* tile = smem + C::kKV + (L % R) * C::kTile;
 #pragma unroll
         for (int c = 0; c < 4 && dirty; ++c) {  // key row 32 c + lane: 128 bytes in every chunk (the swizzle stays inside)
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
 #pragma unroll
           for (int v = 0; v < 16; ++v) bv[v] = __ldcg(bp + v * p.bias_rows);
         }
-        if (!mbar_wait(&s_full[g], s & 1, err, kKidCross, 120 + g, abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&s_full[g], s & 1, err, kKidCross, 120 + g, abort_flag)) { ok = false; break; }
         tc_fence_after();
         float z[128];
         if constexpr (is_bias(MASK)) {
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
 #pragma unroll 1
           for (int c = 0; c < DH / 8; ++c) reinterpret_cast<uint4*>(op)[c] = make_uint4(0u, 0u, 0u, 0u);
       } else {
-        if (!mbar_wait(&o_full[g], used & 1, err, kKidCross, 122 + g, abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&o_full[g], used & 1, err, kKidCross, 122 + g, abort_flag)) { ok = false; break; }
         ++used;
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum stays NaN)

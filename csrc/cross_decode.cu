@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
     for (int blk = split; blk < nb; blk += splits, ++i) {
       if (i % kGroups != warp / 2) continue;
       const int slot = i % kStages, row0 = 16 * (warp % 2), k0 = lo + blk * kStageKeys + row0, left = hi - k0;
-      if (!mbar_wait(&full[slot], (i / kStages) & 1, a.err, kKidCross, 160 + slot, abort_flag)) break;
+      if (!mbar_wait_warp(&full[slot], (i / kStages) & 1, a.err, kKidCross, 160 + slot, abort_flag)) break;
       if (left > 0) {
         // 128-byte rows in the copies' swizzle: 16-byte piece p of row r lies at p ^ (r % 8)
         uint8_t* st = smem + slot * 2 * kTile + row0 * 128;
