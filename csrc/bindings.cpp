@@ -9,6 +9,8 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 #include <limits>
 #include <string>
 #include <vector>
@@ -553,6 +555,17 @@ at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarTy
 }
 
 // ---------------------------------------------------------------- cross attention
+// Tensors that a kernel can be given in place of a differentiable torch operation: none asks for gradients or carries a
+// forward-mode tangent, and none is a wrapper (function transforms such as vmap, fake tensors).
+bool kernel_tensors(std::initializer_list<const at::Tensor*> tensors) {
+  constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
+  const bool grad = at::GradMode::is_enabled();
+  for (const at::Tensor* t : tensors)
+    if (t && ((grad && t->requires_grad()) || t->key_set().has_any(wrappers) || t->_fw_grad(0).defined())) return false;
+  return true;
+}
+
 // q [B, H, Sq, dh], k / v [B, Hk, Sk, dh]; mask: bool (true = attend) or additive, broadcastable to
 // [B, H, Sq, Sk]; kv_lo / kv_hi int32 [B]; p2: P in two terms.
 at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
@@ -560,6 +573,10 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
                            const c10::optional<at::Tensor>& kv_hi, const c10::optional<at::Tensor>& out,
                            const c10::optional<at::Tensor>& lse, bool p2) {
   TORCH_CHECK_VALUE(!p2 || !given(mask), "precise_p comes without a mask");
+  TORCH_CHECK_VALUE(kernel_tensors({&q, &k, &v, given(mask), given(kv_lo), given(kv_hi)}),
+                    "the kernel records no gradients and takes no wrapped tensors");
+  const char* choice = std::getenv("DIFFLET_KERNEL_ATTN");  // (read per call, as the other attention entries do)
+  TORCH_CHECK_VALUE(!choice || std::strcmp(choice, "sdpa"), "DIFFLET_KERNEL_ATTN=sdpa asks for the library baseline");
   TORCH_CHECK_VALUE(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q/k/v must be CUDA tensors [B, H, S, D]");
   TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
                     "cross attention runs in bfloat16 or float16, got ", q.scalar_type());

@@ -165,16 +165,14 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     (refused there with shared key heads on CUDA).  ``kv_lens`` (integers ``[B]``): the valid keys of
     each batch row; what k and v hold behind them is not used.  ``bound_min`` / ``bound_max`` as in
     ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (``[B, H, Sq]``,
-    natural log) are filled when given (an LSE that is not contiguous f32 on q's device by a copy).  CUDA: bf16 and fp16 with D = Dv = 64 or 128; anything else, and what asks
-    for gradients, runs as ``attention``."""
-    kernel = k.shape[-1] == v.shape[-1] and F.cross_kernel_ok(q, k, v, attention_mask)
-    if (kernel and q.dim() == k.dim() == 4 and k.shape[0] == q.shape[0] and k.shape[1] <= q.shape[1]
-            and bound_min is None and bound_max is None
-            and (attention_mask is None or ((attention_mask.dtype == torch.bool or attention_mask.dtype in _MASK_DTYPES)
-                                            and (attention_mask.device == q.device or k.shape[1] != q.shape[1])))):
-        # the binding checks shapes, types and devices (ValueError)
-        return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
-                                 out=out, lse=lse)
+    natural log) are filled when given (an LSE that is not contiguous f32 on q's device by a copy).  CUDA: bf16 and fp16
+    with D = Dv = 64 or 128; anything else, and what asks for gradients, runs as ``attention``."""
+    if q.is_cuda and type(q) is torch.Tensor and bound_min is None and bound_max is None and not torch.compiler.is_compiling():
+        try:  # the binding checks everything; what it refuses is looked at again below
+            return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
+                                     out=out, lse=lse)
+        except ValueError:
+            pass
     for key in ("tp_q", "tp_k", "tp_out", "causal"):
         kwargs.pop(key, None)
     if q.dim() == 3:
@@ -218,7 +216,10 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
         else:
             lo, hi = (_edge(t, k.shape[2], q.device) for t in (lo, hi))
     mask = attention_mask
+    kernel = k.shape == v.shape and F.cross_kernel_ok(q, k, v, mask)
     if mask is not None:
+        if kernel and mask.device != q.device and k.shape[1] != q.shape[1]:
+            raise ValueError("the mask must be on q's device where heads share keys")
         mask = _mask_on(mask, q)
         want = (B, H, Sq, k.shape[2])
         if mask.dim() > 4 or any(m not in (1, w) for m, w in zip(mask.shape[::-1], want[::-1])):

@@ -674,14 +674,16 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
     if q.is_cuda:
         if scale <= 0:  # the kernel scales inside the exponent, where the maximum must commute with it
             q, scale = (-q, -scale) if scale < 0 else (torch.zeros_like(q), 1.0)
+        own = lse
         if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device):
             if lse.numel() != q.shape[:-1].numel():
                 raise ValueError(f"lse {tuple(lse.shape)} does not hold {tuple(q.shape[:-1])}")
             own = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32)
-            o = _kernels().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, own, precise_p)
+        o = (_nat or _lib()).cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, own, precise_p)
+        LAUNCHES[0] += 1  # (a refused call is no launch)
+        if own is not lse:
             lse.copy_(own.reshape(lse.shape))
-            return o
-        return _kernels().cross_attention(q, k, v, scale, mask, kv_lo, kv_hi, out, lse, precise_p)
+        return o
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     Sk, rep = k.shape[2], q.shape[1] // k.shape[1]
     idx = torch.arange(Sk, device=q.device)

@@ -479,3 +479,20 @@ def test_lengths_and_bounds_past_the_ends():
 @pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16), (40, torch.bfloat16), (64, torch.float32)])
 def test_lengths_and_bounds_past_the_ends_on_cuda(native, D, dtype):
     _past_the_ends(D, dtype, "cuda")
+
+
+@pytest.mark.gpu
+def test_the_binding_refuses_what_it_would_not_differentiate(native, monkeypatch):
+    from difflet_b200.ops import fused as F
+
+    q, k, v = _inputs(1, 2, 2, 3, 5, 64, torch.bfloat16, "cuda")
+    n = F.LAUNCHES[0]
+    with pytest.raises(ValueError):
+        F.cross_attention(q.clone().requires_grad_(), k, v, 1.0)
+    monkeypatch.setenv("DIFFLET_KERNEL_ATTN", "sdpa")
+    with pytest.raises(ValueError):
+        F.cross_attention(q, k, v, 1.0)
+    assert F.LAUNCHES[0] == n  # (a refused call is no launch)
+    monkeypatch.delenv("DIFFLET_KERNEL_ATTN")
+    F.cross_attention(q, k, v, 1.0)
+    assert F.LAUNCHES[0] == n + 1
