@@ -189,8 +189,9 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
                     "adapters must be contiguous [n, r, K] and [n, N, r]");
   TORCH_CHECK_VALUE(A_l.size(2) == K, "x ", x.sizes(), " does not end in the bank's ", A_l.size(2), " inputs");
   TORCH_CHECK_VALUE(B.size(1) == K && B_l.size(1) == N, "weight ", B.sizes(), " is not [", B_l.size(1), ", ", K, "]");
-  TORCH_CHECK_VALUE(B.stride(1) == 1 && B.stride(0) % 8 == 0 && K % 8 == 0 && N % (out_f32 ? 4 : 8) == 0,
-                    "linear_lora needs rows of whole 16-byte pieces: K ", K, ", N ", N);
+  TORCH_CHECK_VALUE(B.stride(1) == 1 && B.stride(0) % 8 == 0 && K > 0 && K % 8 == 0 && N % (out_f32 ? 4 : 8) == 0 &&
+                        reinterpret_cast<uintptr_t>(B.data_ptr()) % 16 == 0,
+                    "linear_lora needs 16-byte aligned rows of whole 16-byte pieces in the weight: K ", K, ", N ", N);
   TORCH_CHECK_VALUE(scale.is_contiguous() && scale.scalar_type() == at::kFloat && scale.numel() == A_l.size(0),
                     "adapter scale must be float32 [n]");
   const c10::cuda::CUDAGuard guard(x.device());
@@ -220,7 +221,7 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
     res = new_like(x, shape, ydt);
   }
   if (M == 0) return res;
-  c10::optional<at::Tensor> out = res.dim() == 2 ? res : res.view({M, N}), resid;
+  c10::optional<at::Tensor> out = res.dim() == 2 ? res : res.view({M, N}), resid, own_gate = gate;
   TORCH_CHECK_VALUE(out->stride(1) == 1 && (M == 1 || out->stride(0) % (out_f32 ? 4 : 8) == 0) &&
                         reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, "out needs 16-byte aligned rows");
   if (const at::Tensor* t = given(bias))
@@ -235,19 +236,27 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
                       "resid must be bfloat16 ", at::IntArrayRef(shape));
     resid = t->dim() == 2 ? *t : t->reshape({M, N});
     const int64_t rpb = rows_per_batch > 0 ? rows_per_batch : M;
-    TORCH_CHECK_VALUE(gate->scalar_type() == at::kFloat && gate->dim() == 2 && gate->stride(1) == 1 && gate->size(1) >= N &&
+    TORCH_CHECK_VALUE(gate->scalar_type() == at::kFloat && gate->dim() == 2 && gate->size(1) >= N &&
                           gate->device() == x.device() && gate->size(0) * rpb >= M,
                       "gate must be float32 [B, ", N, "] with a row for every ", rpb, " rows");
+    // the epilogue reads 16 bytes at a time: other rows are laid out first, as x is
+    auto pieces = [](const at::Tensor& u, int64_t n) {
+      return u.stride(1) == 1 && (u.size(0) == 1 || u.stride(0) % n == 0) && reinterpret_cast<uintptr_t>(u.data_ptr()) % 16 == 0;
+    };
+    if (!pieces(*resid, 8)) resid = resid->clone(at::MemoryFormat::Contiguous);
+    if (!pieces(*gate, 4)) own_gate = gate->narrow(1, 0, N).clone(at::MemoryFormat::Contiguous);
   }
   GemmArgs a{};
-  gemm_epilogue_args(a, A, M, N, bias, out, epi, act_lo, act_hi, gate, rows_per_batch, resid, 1.0,
-                                    out_f32, {}, 0, 0, 0, c10::nullopt, "");
+  gemm_epilogue_args(a, A, M, N, bias, out, epi, act_lo, act_hi, own_gate, rows_per_batch, resid, 1.0,
+                     out_f32, {}, 0, 0, 0, c10::nullopt, "");
   a.A = A.data_ptr();
   a.B = B.data_ptr();
   a.lda = A.stride(0);
   a.ldb = B.stride(0);
   a.K = (int)K;
-  if (M == 1) a.lda = K, a.ldd = N, a.ldr = N;  // one row has no stride to speak of
+  // one row has no stride to speak of
+  if (M == 1) a.lda = K, a.ldd = N, a.ldr = N;
+  if (given(own_gate) && own_gate->size(0) == 1) a.gate_bstride = 0;
   LoraArgs l{};
   a.lora = &l;
   l.a = A_l.data_ptr();

@@ -52,3 +52,28 @@ def test_one_row_of_any_pitch(native):
         assert torch.equal(out[:1, :N], got) and bool((out[1:] == 0).all() and (out[:, N:] == 0).all())
         gated = ops.linear_lora(wide[:1, :K], w, b, bank=bank, ids=ids, gate=gate, resid=resid[:1, :N])
         assert torch.equal(gated, ops.linear_lora(x[:1], w, b, bank=bank, ids=ids, gate=gate, resid=torch.ones(1, N, device="cuda", dtype=BF)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 40, 300])
+def test_gate_and_residual_of_any_alignment(native, M):
+    """Rows that 16-byte accesses do not reach are laid out first, whatever kernel the number of rows selects."""
+    K, N = 128, 264
+    x, w, b, A, B, scale = _make(M, N, K, [16, 8], "cuda")
+    bank = ops.LoraBank(A, B, scale)
+    ids = torch.tensor([1, 0], device="cuda")
+    rpb = -(-M // 2)
+    gate, resid = torch.randn(2, N, device="cuda"), torch.randn(M, N, device="cuda", dtype=BF)
+    kw = dict(bank=bank, ids=ids, rows_per_batch=rpb)
+    want = ops.linear_lora(x, w, b, gate=gate, resid=resid, **kw)
+    for off, pad in ((1, 2), (0, 3), (4, 5)):
+        g, r = torch.zeros(2, N + pad + off, device="cuda"), torch.zeros(M, N + pad + off, device="cuda", dtype=BF)
+        g[:, off:off + N], r[:, off:off + N] = gate, resid
+        assert torch.equal(ops.linear_lora(x, w, b, gate=g[:, off:off + N], resid=r[:, off:off + N], **kw), want)
+    columns = resid.t().contiguous().t()  # a residual of another order, and a gate shared by all rows
+    assert torch.equal(ops.linear_lora(x, w, b, gate=gate.t().contiguous().t(), resid=columns, **kw), want)
+    one = torch.zeros(3, N + 1, device="cuda")[:1, :N]
+    got = ops.linear_lora(x, w, b, gate=one, resid=resid, gate_rows_per_batch=M, **kw)
+    assert torch.equal(got, resid)
+    with pytest.raises(ValueError):
+        ops.linear_lora(x, torch.zeros(N * K + 1, device="cuda", dtype=BF)[1:].view(N, K), b, **kw)
