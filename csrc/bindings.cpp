@@ -222,8 +222,8 @@ at::Tensor gemm_lora(const at::Tensor& x, const at::Tensor& B, const c10::option
   }
   if (M == 0) return res;
   c10::optional<at::Tensor> out = res.dim() == 2 ? res : res.view({M, N}), resid, own_gate = gate;
-  TORCH_CHECK_VALUE(out->stride(1) == 1 && (M == 1 || out->stride(0) % (out_f32 ? 4 : 8) == 0) &&
-                        reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, "out needs 16-byte aligned rows");
+  TORCH_CHECK_VALUE(out->stride(1) == 1 && (M == 1 || (out->stride(0) % (out_f32 ? 4 : 8) == 0 && out->stride(0) >= N)) &&
+                        reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, "out needs 16-byte aligned rows of its own");
   if (const at::Tensor* t = given(bias))
     TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 && t->dim() == 1 && t->numel() == N && t->is_contiguous() &&
                           t->device() == x.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
@@ -466,6 +466,7 @@ std::vector<at::Tensor> add_rms_norm(const at::Tensor& x, const c10::optional<at
   auto rows = [&](const at::Tensor& t, const char* name) {
     const at::Tensor v = t.dim() == 2 ? t : t.view({M, D});
     TORCH_CHECK_VALUE(v.stride(1) == 1 || D == 1, name, " needs a unit inner stride");
+    TORCH_CHECK_VALUE(M <= 1 || v.stride(0) >= D, "the rows of ", name, " overlap");
     return v;
   };
   auto pitch = [&](const at::Tensor& t) { return (long long)(M == 1 ? D : t.stride(0)); };  // one row has no stride to speak of

@@ -77,3 +77,13 @@ def test_gate_and_residual_of_any_alignment(native, M):
     assert torch.equal(got, resid)
     with pytest.raises(ValueError):
         ops.linear_lora(x, torch.zeros(N * K + 1, device="cuda", dtype=BF)[1:].view(N, K), b, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 300])
+def test_results_whose_rows_overlap_are_refused(native, M):
+    x, w, b, A, B, scale = _make(M, 64, 128, [16], "cuda")
+    bank, ids = ops.LoraBank(A, B, scale), torch.zeros(M, device="cuda", dtype=torch.int32)
+    for bad in (torch.empty(1, 64, device="cuda", dtype=BF).expand(M, 64), torch.empty(M * 64, device="cuda", dtype=BF).as_strided((M, 64), (32, 1))):
+        with pytest.raises(ValueError):
+            ops.linear_lora(x, w, b, bank=bank, ids=ids, out=bad)

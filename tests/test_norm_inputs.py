@@ -44,3 +44,17 @@ def test_a_row_map_entry_that_does_not_exist():
         for bad in (-1, 2):
             with pytest.raises(IndexError):
                 ops.add_rms_norm(x, row_map=torch.tensor([0, bad, 1], dtype=torch.int32), **kw)
+
+
+@pytest.mark.gpu
+def test_results_whose_rows_overlap_are_refused(native):
+    """One row of memory for all rows (expand), or rows that run into one another."""
+    x = torch.randn(5, 64, device="cuda")
+    one, close = torch.empty(1, 64, device="cuda").expand(5, 64), torch.empty(400, device="cuda").as_strided((5, 64), (32, 1))
+    for bad in (one, close):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.add_rms_norm(x, out=bad)
+        with pytest.raises(ValueError, match="overlap"):
+            ops.add_rms_norm(x, x, resid_out=bad)
+    y, s = ops.add_rms_norm(one, one)  # (inputs may)
+    assert torch.equal(s, one + one)
