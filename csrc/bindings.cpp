@@ -613,13 +613,14 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) == 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0));
     return ok;
   };
-  const at::Tensor q_ = fits(q) ? q : q.contiguous();
+  // (a copy, where `contiguous` would hand back a tensor that is contiguous from an odd start)
+  auto laid_out = [&](const at::Tensor& t) { return fits(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
+  const at::Tensor q_ = laid_out(q);
   // a head axis that is one head repeated (expand) needs no copy: every query head reads key head 0
   const bool one = a.Hk > 1 && k.stride(1) == 0 && v.stride(1) == 0;
   at::Tensor k_ = one ? k.narrow(1, 0, 1) : k, v_ = one ? v.narrow(1, 0, 1) : v;
   if (one) a.Hk = 1;
-  if (!fits(k_)) k_ = k_.contiguous();
-  if (!fits(v_)) v_ = v_.contiguous();
+  k_ = laid_out(k_), v_ = laid_out(v_);
   auto stride = [](const at::Tensor& t, int d) { return (long long)(t.size(d) == 1 ? t.size(3) : t.stride(d)); };
   const bool direct = fits(o);
   at::Tensor o_ = direct ? o : new_like(o, o.sizes(), o.scalar_type());

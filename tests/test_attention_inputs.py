@@ -496,3 +496,24 @@ def test_the_binding_refuses_what_it_would_not_differentiate(native, monkeypatch
     monkeypatch.delenv("DIFFLET_KERNEL_ATTN")
     F.cross_attention(q, k, v, 1.0)
     assert F.LAUNCHES[0] == n + 1
+
+
+# ----------------------------------------------------------------------------- layouts
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 200])
+@pytest.mark.parametrize("off", [1, 3, 4])
+def test_contiguous_from_an_odd_start(native, Sq, off):
+    """Contiguous q, k, v and out that start where no copy engine can address them."""
+    q, k, v = (t.contiguous() for t in _inputs(2, 4, 2, Sq, 300, 64, torch.bfloat16, "cuda"))
+    want = ops.cross_attention(q, k, v, scale=0.1)
+
+    def moved(t):
+        u = torch.empty(t.numel() + off, device="cuda", dtype=t.dtype)[off:].view(t.shape)
+        return u.copy_(t)
+
+    for args in ((moved(q), k, v), (q, moved(k), v), (q, k, moved(v)), (moved(q), moved(k), moved(v))):
+        assert torch.equal(ops.cross_attention(*args, scale=0.1), want)
+    out = moved(torch.zeros_like(q))
+    assert ops.cross_attention(q, k, v, scale=0.1, out=out) is out and torch.equal(out, want)
+    one = torch.empty(3, 64 + off, device="cuda", dtype=q.dtype)[:1, :64].view(1, 1, 1, 64).copy_(q[:1, :1, :1])
+    assert torch.equal(ops.cross_attention(one, k[:1, :1], v[:1, :1], scale=0.1), ops.cross_attention(q[:1, :1, :1], k[:1, :1], v[:1, :1], scale=0.1))
