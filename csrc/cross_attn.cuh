@@ -78,7 +78,7 @@ struct CrossCfg {
   static constexpr int kProducerWarp = 4 * QT, kMmaWarp = 4 * QT + 1, kCleanWarp = 4 * QT + 2;
   static constexpr int kTile = 128 * DH * 2;
   static constexpr int kChunks = DH / 64;
-  static constexpr int kRing = DH == 64 ? 8 : (QT == 2 ? 4 : 5);  // (three slots: 360 -> 388 us at 512 keys)
+  static constexpr int kRing = DH == 64 ? 8 : 4;  // (QT = 2, three slots: 360 -> 388 us at 512 keys)
   static constexpr int kQ = 0, kKV = QT * kTile;
   static constexpr int kOut = kKV + kRing * kTile;  // 4 KB per softmax warp: 32 rows x 64 columns on their way out
   static constexpr int kBar = kOut + 4 * QT * 4096;
@@ -88,6 +88,7 @@ struct CrossCfg {
   static constexpr uint32_t kTmemCols = QT == 2 ? 512 : 256;
   static constexpr uint32_t kOCol = 128 * QT;  // S_g at 128 g, O_g at kOCol + DH g
   static_assert(kTotal <= 232448, "shared memory budget");
+  static_assert(kRing % 2 == 0, "a slot holds K or V for good: the cleaning warp then waits for every phase of a V slot");
   static_assert(kOCol + DH * QT <= kTmemCols, "tensor memory");
 };
 

@@ -517,3 +517,31 @@ def test_contiguous_from_an_odd_start(native, Sq, off):
     assert ops.cross_attention(q, k, v, scale=0.1, out=out) is out and torch.equal(out, want)
     one = torch.empty(3, 64 + off, device="cuda", dtype=q.dtype)[:1, :64].view(1, 1, 1, 64).copy_(q[:1, :1, :1])
     assert torch.equal(ops.cross_attention(one, k[:1, :1], v[:1, :1], scale=0.1), ops.cross_attention(q[:1, :1, :1], k[:1, :1], v[:1, :1], scale=0.1))
+
+
+# ----------------------------------------------------------------------------- lengths beside masks
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["bool", "bias", "bias32", "key bias", "keys"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", [(4, 32, 4, 94, 1429, 128), (3, 12, 3, 473, 1402, 128), (2, 48, 6, 123, 1231, 128), (3, 12, 12, 700, 900, 128),
+                                            (4, 32, 8, 104, 906, 64), (2, 6, 2, 5, 3000, 128)])
+def test_lengths_beside_masks(native, B, H, Hk, Sq, Sk, D, kind, dtype):
+    """Both exclude keys; many key tiles for one query tile a CTA, whose copies land in any order."""
+    q, k, v = _inputs(B, H, Hk, Sq, Sk, D, dtype, "cuda")
+    lens = torch.tensor([Sk, Sk // 2, 1, 0][:B], device="cuda")
+    if kind == "key bias":
+        m = torch.randn(1, Sk, generator=torch.Generator().manual_seed(0)).to("cuda", dtype)
+    else:
+        from test_cross_attention import _mask
+
+        m = _mask(kind, B, H, Sq, Sk, "cuda", dtype)
+    gone = (torch.arange(Sk, device="cuda") >= lens[:, None])[:, None, :, None]
+    k, v = k.masked_fill(gone, math.nan), v.masked_fill(gone, math.inf)
+    lse = torch.empty(B, H, Sq, device="cuda")
+    o = ops.cross_attention(q, k, v, scale=D ** -0.5, attention_mask=m, kv_lens=lens, lse=lse)
+    _check(o, _ref(q, k, v, D ** -0.5, m, lens), dtype, D, Sk, v[v.isfinite()].abs().max().item(), lse)
+    for _ in range(20):
+        assert torch.equal(ops.cross_attention(q, k, v, scale=D ** -0.5, attention_mask=m, kv_lens=lens), o)
+    from difflet_b200 import _native
+
+    _native.check_device_errors()
