@@ -14,7 +14,7 @@ per batch row (shape ``[B]`` or ``[B, 1, ...]``, the padded-text key windows eve
 model here uses) run the tcgen05 kernel of ``csrc/attention.cu``.  Masks (boolean or
 additive), per-query windows, head dim 64 and fp16 run the tcgen05 kernel of
 ``csrc/cross_attn.cuh``, which ``cross_attention`` always takes.  Anything else on CUDA
-(causal, other head dims, fp32) is the library path:
+(causal, other head dims, values of another width, fp32, tracing and function transforms) is the library path:
 ``torch.nn.functional.scaled_dot_product_attention``.  CPU tensors run the fp32 / fp64
 oracle of ``ops.fused``.
 
@@ -167,7 +167,8 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     ``attention``.  A query that no key is left for gives 0.  ``out`` (``[B, H, Sq, Dv]``) and ``lse`` (``[B, H, Sq]``,
     natural log) are filled when given (an LSE that is not contiguous f32 on q's device by a copy).  CUDA: bf16 and fp16
     with D = Dv = 64 or 128; anything else, and what asks for gradients, runs as ``attention``."""
-    if q.is_cuda and type(q) is torch.Tensor and bound_min is None and bound_max is None and not torch.compiler.is_compiling():
+    if (q.is_cuda and type(q) is torch.Tensor and q.dtype in F.CROSS_DTYPES and q.shape[-1] in (64, 128)
+            and bound_min is None and bound_max is None and not torch.compiler.is_compiling()):
         try:  # the binding checks everything; what it refuses is looked at again below
             return F.cross_attention(q, k, v, 1.0 if scale is None else float(scale), mask=attention_mask, kv_hi=kv_lens,
                                      out=out, lse=lse)

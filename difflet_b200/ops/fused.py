@@ -619,11 +619,14 @@ def kernel_tensors(*tensors) -> bool:
     return True
 
 
+CROSS_DTYPES = (torch.bfloat16, torch.float16)
+
+
 def cross_kernel_ok(q, k, v, mask=None) -> bool:
     """Whether the masked / head-dim-64 attention kernel takes these inputs (it records no backward pass: what asks
     for gradients stays on the torch path, and so do tracing and function transforms)."""
-    return (q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in (torch.bfloat16, torch.float16)
-            and envs.DIFFLET_KERNEL_ATTN != "sdpa" and not wants_grad(q, k, v, mask) and kernel_tensors(q, k, v, mask))
+    return (q.is_cuda and q.shape[-1] in (64, 128) and q.dtype in CROSS_DTYPES and kernel_tensors(q, k, v, mask)
+            and not wants_grad(q, k, v, mask) and envs.DIFFLET_KERNEL_ATTN != "sdpa")
 
 
 def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):

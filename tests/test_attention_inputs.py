@@ -545,3 +545,16 @@ def test_lengths_beside_masks(native, B, H, Hk, Sq, Sk, D, kind, dtype):
     from difflet_b200 import _native
 
     _native.check_device_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_compiled_calls_trace_the_library_path(native, D):
+    """A whole-graph trace (no code generation) meets no opaque native call."""
+    q, k, v = _inputs(2, 4, 4, 20, 33, D, torch.bfloat16, "cuda")
+    m = torch.rand(20, 33, device="cuda") < 0.7
+    m[:, 0] = True
+    for fn in BOTH:
+        call = torch.compile(lambda q, k, v: fn(q, k, v, scale=0.1, attention_mask=m), backend="eager", fullgraph=True)  # noqa: B023
+        want, _, size, _ = _ref(q, k, v, 0.1, m)
+        assert bool(((call(q, k, v).double() - want).abs() <= 2 * torch.finfo(q.dtype).eps * (size + want.abs())).all())
