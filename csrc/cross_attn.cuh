@@ -24,7 +24,8 @@
 // finished, and P_g(first tile of an item) is signalled only after its warpgroup has read O_g of the
 // item before, so neither P nor O needs a barrier of its own.
 //
-// 40 heads x 32760 queries x 512 keys x 128: 349 us (984 TFLOP/s; the products alone take 205 at the library's rate, the
+// 40 heads x 32760 queries x 512 keys x 128: 342 - 349 us in a loop over one state's tensors (1005 - 984 TFLOP/s), 413 (831) with
+// three states' in turn (the products alone take 205 at the library's rate, the
 // exponentials 180 at the SFU's).  What is left is the round trip of a Q tile (scores, exponentials, P, next
 // scores: 3650 cycles for 2 x 1024 of products), which two tiles do not fill, and the turn of the items.  Measured
 // and slower or equal: part of the exponentials on the FMA pipe (387 us), an MMA warp per Q tile (402), three K / V slots
