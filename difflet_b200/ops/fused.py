@@ -633,9 +633,12 @@ def attention(q, k, v, scale, *, out=None, lse=None, kv_lo=None, kv_hi=None):
     """softmax(scale * q k^T) v over [B, H, S, dh]; key window [kv_lo[b], kv_hi[b])."""
     if q.is_cuda and envs.DIFFLET_KERNEL_ATTN != "sdpa" and q.shape[-1] == 128 and not wants_grad(q, k, v):
         return native().attention(q, k, v, float(scale), out, lse, kv_lo, kv_hi, kv_split=kv_split_mode())
-    if cross_kernel_ok(q, k, v):  # (a window or LSE: these have always been f32 up to the result)
-        return cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out, lse=lse,
-                               precise_p=lse is not None or kv_lo is not None or kv_hi is not None)
+    if cross_kernel_ok(q, k, v) and k.shape == v.shape and k.shape[0] == q.shape[0] and k.dtype == v.dtype == q.dtype:
+        # (a window or LSE: these have always been f32 up to the result)
+        own = out is None or (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device)
+        o = cross_attention(q, k, v, float(scale), kv_lo=kv_lo, kv_hi=kv_hi, out=out if own else None, lse=lse,
+                            precise_p=lse is not None or kv_lo is not None or kv_hi is not None)
+        return o if own else out.copy_(o)
     ct = torch.float64 if q.dtype == torch.float64 else torch.float32
     if q.is_cuda and lse is None and kv_lo is None:
         o = F.scaled_dot_product_attention(q, k, v, scale=float(scale))

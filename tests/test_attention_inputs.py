@@ -558,3 +558,24 @@ def test_compiled_calls_trace_the_library_path(native, D):
         call = torch.compile(lambda q, k, v: fn(q, k, v, scale=0.1, attention_mask=m), backend="eager", fullgraph=True)  # noqa: B023
         want, _, size, _ = _ref(q, k, v, 0.1, m)
         assert bool(((call(q, k, v).double() - want).abs() <= 2 * torch.finfo(q.dtype).eps * (size + want.abs())).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_fused_attention_keeps_what_it_took(native, dtype):
+    """``ops.fused.attention`` at head dim 64: values of another width, one batch row of keys, a result of another type."""
+    from difflet_b200.ops import fused as F
+
+    q, k, v = _inputs(3, 4, 4, 30, 41, 64, dtype, "cuda")
+    wide = _inputs(3, 4, 4, 30, 41, 32, dtype, "cuda", 1)[2]
+    hi = torch.tensor([41, 7, 30], device="cuda", dtype=torch.int32)
+    lo = torch.zeros_like(hi)
+    eps = torch.finfo(dtype).eps
+    for args, full in (((q, k, wide), (q, k, wide)), ((q, k[:1], v[:1]), (q, k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)))):
+        for kw, ref in (({}, {}), (dict(kv_lo=lo, kv_hi=hi), dict(lens=hi))):
+            o = F.attention(*args, 0.1, **kw)
+            want, _, size, _ = _ref(*full, 0.1, **ref)
+            assert bool(((o.double() - want).abs() <= 2 * eps * (size + want.abs()) + 1e-6).all())
+    want = F.attention(q, k, v, 0.1)
+    out = torch.empty(3, 4, 30, 64, device="cuda")
+    assert F.attention(q, k, v, 0.1, out=out) is out and torch.equal(out, want.float())
