@@ -124,6 +124,12 @@ def linear_lora(x, w, b=None, *, bank: LoraBank, ids, rows_per_batch: int = 0, a
     if ids.shape[0] != want:
         raise ValueError(f"{want} ids expected for {M} rows" + (f" of {rows_per_batch} a batch" if rows_per_batch > 0 else "")
                          + f", got {ids.shape[0]}")
+    if b is not None and tuple(b.shape) != (N,):
+        raise ValueError(f"bias must be [{N}], got {tuple(b.shape)}")
+    if gate is not None and (gate.dim() != 2 or gate.shape[1] < N or gate.shape[0] * (rpb if rpb > 0 else M) < M):
+        raise ValueError(f"gate must be [B, {N}] with a row for every {rpb if rpb > 0 else M} rows, got {tuple(gate.shape)}")
+    if resid is not None and tuple(resid.shape) != (*x.shape[:-1], N):
+        raise ValueError(f"resid must be {(*x.shape[:-1], N)}, got {tuple(resid.shape)}")
     if isinstance(w, F.MXWeight):
         if w.compute == "mx":
             raise NotImplementedError("linear_lora beside a block-scaled weight: use MXWeight(compute='dequant')")

@@ -87,3 +87,28 @@ def test_results_whose_rows_overlap_are_refused(native, M):
     for bad in (torch.empty(1, 64, device="cuda", dtype=BF).expand(M, 64), torch.empty(M * 64, device="cuda", dtype=BF).as_strided((M, 64), (32, 1))):
         with pytest.raises(ValueError):
             ops.linear_lora(x, w, b, bank=bank, ids=ids, out=bad)
+
+
+def _shape_refusals(device, dtype):
+    """A bias, gate or residual that would only broadcast is refused on every device."""
+    x, w, b, A, B, scale = _make(6, 24, 32, [4, 4], device, dtype)
+    bank, ids = ops.LoraBank(A, B, scale), torch.zeros(6, dtype=torch.long, device=device)
+    gate, resid = torch.ones(6, 24, device=device), torch.ones(6, 24, device=device, dtype=dtype)
+    kw = dict(bank=bank, ids=ids)
+    for bad in (dict(gate=gate[:1], resid=resid, gate_rows_per_batch=1), dict(gate=gate[:, :16], resid=resid), dict(gate=gate[0], resid=resid),
+                dict(gate=gate[:1], resid=resid[:1]), dict(gate=gate[:1], resid=resid[:, :1]), dict(gate=gate[:2], resid=resid, gate_rows_per_batch=2)):
+        with pytest.raises(ValueError):
+            ops.linear_lora(x, w, b, **kw, **bad)
+    for bad in (b[:1], b[None]):
+        with pytest.raises(ValueError):
+            ops.linear_lora(x, w, bad, **kw)
+    ops.linear_lora(x, w, b, gate=gate[:1], resid=resid, **kw)
+
+
+def test_shapes_that_only_broadcast_are_refused():
+    _shape_refusals("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_shapes_that_only_broadcast_are_refused_on_cuda(native):
+    _shape_refusals("cuda", BF)
