@@ -60,8 +60,11 @@ def _per_batch(bound, B):
 
 def _edge(t, n, device):
     """A window edge as int32 for keys [0, n): what lies past either end is that end, fractions count as in ``key < edge``."""
-    t = t.ceil() if t.is_floating_point() else t.long()
-    return t.clamp(0, n).to(device, torch.int32).contiguous()
+    if t.is_floating_point():
+        t = t.ceil().clamp(0, n)
+    elif t.dtype == torch.int64:  # (the kernels clamp what fits 32 bits)
+        t = t.clamp(0, n)
+    return t.to(device, torch.int32).contiguous()
 
 
 def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_min=None, bound_max=None,
@@ -94,6 +97,8 @@ def attention(q, k, v, *, scale=None, causal=False, attention_mask=None, bound_m
         out = F.cross_attention(q4, k4, v4, scale, mask=_mask_on(mask, q), kv_lo=lo, kv_hi=hi, lse=lse,
                                 precise_p=lse is not None)  # (partials that are merged by their LSE: f32 up to the result)
     else:
+        if simple and lo is not None:  # (one edge per batch row, whatever shape it came in)
+            bound_min, bound_max = (t.view(B, 1, 1, 1) for t in (lo, hi))
         mask = _bounds_to_mask(k4, bound_min, bound_max, attention_mask)
         if lse is not None or not q.is_cuda:  # math path (oracle, or LSE requested off the kernel)
             out = _oracle_masked(q4, k4, v4, scale, causal, mask, lse)

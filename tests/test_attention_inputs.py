@@ -579,3 +579,25 @@ def test_fused_attention_keeps_what_it_took(native, dtype):
     want = F.attention(q, k, v, 0.1)
     out = torch.empty(3, 4, 30, 64, device="cuda")
     assert F.attention(q, k, v, 0.1, out=out) is out and torch.equal(out, want.float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", BOTH)
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.bfloat16), (40, torch.float32)])
+def test_bounds_of_one_edge_per_batch_row_off_the_kernels(native, fn, D, dtype):
+    """[B], [B, 1] and scalar bounds mean the same with and without gradients, at head dims with and without a kernel."""
+    q, k, v = _inputs(3, 2, 2, 20, 33, D, dtype, "cuda")
+    lo, hi = torch.tensor([0, 3, 5], device="cuda"), torch.tensor([33, 12, 5 + 28], device="cuda")
+    keep = (torch.arange(33, device="cuda") >= lo[:, None]) & (torch.arange(33, device="cuda") < hi[:, None])
+    want, _, size, _ = _ref(q, k, v, 0.1, keep[:, None, None])
+    tol = 2 * torch.finfo(dtype).eps * (size + want.abs()) + 2.0 ** -20
+    for shape in ((3,), (3, 1), (3, 1, 1, 1)):
+        kw = dict(bound_min=lo.view(shape), bound_max=hi.view(shape))
+        for grad in (False, True):
+            o = fn(q.detach().clone().requires_grad_(grad), k, v, scale=0.1, **kw)
+            assert o.requires_grad == grad and bool(((o.double() - want).abs() <= tol).all())
+    one = dict(bound_min=torch.tensor(2, device="cuda"), bound_max=torch.tensor(30, device="cuda"))
+    want, _, size, _ = _ref(q, k, v, 0.1, ((torch.arange(33, device="cuda") >= 2) & (torch.arange(33, device="cuda") < 30))[None, None, None])
+    for grad in (False, True):
+        o = fn(q.detach().clone().requires_grad_(grad), k, v, scale=0.1, **one)
+        assert bool(((o.double() - want).abs() <= 2 * torch.finfo(dtype).eps * (size + want.abs()) + 2.0 ** -20).all())
