@@ -3,70 +3,9 @@
 // The kernels live in torch-free .cu translation units behind the C interface
 // in kernels.h; this file only validates tensors, picks strides and streams,
 // and forwards.  Every entry point raises on a non-zero launcher status.
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
-
-#include <algorithm>
-#include <cstdlib>
-#include <cstring>
-#include <limits>
-#include <string>
-#include <vector>
-
-#include "kernels.h"
+#include "bindings.h"
 
 namespace {
-
-#define DFL_CHECK_RC(rc, what) TORCH_CHECK((rc) == 0, what, " launch failed with status ", (rc))
-
-void check_bf16_cuda(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16");
-}
-
-void check_rowmajor(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.dim() == 2, name, " must be 2-D");
-  TORCH_CHECK(t.stride(1) == 1, name, " must have a unit inner stride");
-}
-
-// Per-device 4-int error word (see common.cuh).
-at::Tensor& error_buffer(int device) {
-  static at::Tensor bufs[16];
-  TORCH_CHECK(device >= 0 && device < 16, "device index out of range");
-  if (!bufs[device].defined()) {
-    bufs[device] = at::zeros({4}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
-  }
-  return bufs[device];
-}
-
-int* err_ptr() {
-  int dev = c10::cuda::current_device();
-  return error_buffer(dev).data_ptr<int>();
-}
-
-cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
-
-const void* opt_ptr(const c10::optional<at::Tensor>& t) {
-  return (t.has_value() && t->defined()) ? t->data_ptr() : nullptr;
-}
-
-// at::empty on t's device without the dispatcher (a microsecond of a small call).
-at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype) {
-  return at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt);
-}
-
-int dtype_code(const at::Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return kDtypeF32;
-    case at::kBFloat16: return kDtypeBf16;
-    case at::kHalf: return kDtypeF16;
-    default: TORCH_CHECK_VALUE(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
-  }
-}
-
-const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 
 // ---------------------------------------------------------------------------
 // Output + epilogue fields shared by the bf16 and MXFP8 GEMMs.  With out_peer
@@ -562,18 +501,6 @@ at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarTy
   DFL_CHECK_RC(dfl_mx_dequantize(q.data_ptr(), sf.data_ptr(), out.data_ptr(), q.numel(), dtype_code(out, "output"),
                                  q.scalar_type() == at::kFloat8_e5m2, cur_stream()), "mx_dequantize");
   return out;
-}
-
-// ---------------------------------------------------------------- cross attention
-// Tensors that a kernel can be given in place of a differentiable torch operation: none asks for gradients or carries a
-// forward-mode tangent, and none is a wrapper (function transforms such as vmap, fake tensors).
-bool kernel_tensors(std::initializer_list<const at::Tensor*> tensors) {
-  constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
-                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
-  const bool grad = at::GradMode::is_enabled();
-  for (const at::Tensor* t : tensors)
-    if (t && ((grad && t->requires_grad()) || t->key_set().has_any(wrappers) || t->_fw_grad(0).defined())) return false;
-  return true;
 }
 
 // q [B, H, Sq, dh], k / v [B, Hk, Sk, dh]; mask: bool (true = attend) or additive, broadcastable to
@@ -1309,6 +1236,8 @@ at::Tensor rel_l1(const at::Tensor& a, const at::Tensor& b) {
 
 }  // namespace
 
+void bind_layer(py::module_& m);  // bindings_layer.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "difflet_b200 native sm_100a kernels";
   m.def("gemm_set_pair_auto", [](bool on) { dfl_gemm_set_pair_auto(on ? 1 : 0); });
@@ -1403,4 +1332,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("m2") = py::none(), py::arg("m_out") = py::none(), py::arg("coeffs"), py::arg("store_last"),
         py::arg("swap_ab") = false);
   m.def("rel_l1", &rel_l1);
+  bind_layer(m);
 }

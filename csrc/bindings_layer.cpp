@@ -1,0 +1,112 @@
+// torch bindings of the layer operators: gated projection, embedding lookup, windowed attention.
+#include "bindings.h"
+
+namespace {
+
+// Rows that the copy engine can address: unit inner stride, 16-byte aligned rows; anything else is laid out anew.
+at::Tensor rows16(const at::Tensor& t) {
+  const bool fits = t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) > 0)) &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+long long row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? (t.size(1) + 7) / 8 * 8 : t.stride(0); }
+
+bool is16(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+
+// ---------------------------------------------------------------- gated projection
+// x [..., K], wg / wu [F, K] of one 16-bit type -> {h [..., F]} or, to keep the projections for the gradients, {h, g, u}
+// (g, u [M, F] with padded rows).
+std::vector<at::Tensor> gated_linear(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act, bool keep) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && wg.dim() == 2 && wu.dim() == 2, "x [..., K] and weights [F, K] must be CUDA tensors");
+  TORCH_CHECK_VALUE(is16(x), "gated_linear runs in bfloat16 or float16 on CUDA, got ", x.scalar_type());
+  for (const at::Tensor* t : {&wg, &wu})
+    TORCH_CHECK_VALUE(t->device() == x.device() && t->scalar_type() == x.scalar_type(), "x and the weights must share type and device");
+  const int64_t K = x.size(-1), F = wg.size(0);
+  TORCH_CHECK_VALUE(wg.size(1) == K && wu.sizes() == wg.sizes(), "weights ", wg.sizes(), " and ", wu.sizes(), " must both be [F, ", K, "]");
+  TORCH_CHECK_VALUE(K > 0 && K % 8 == 0 && K < (1 << 30) && F < (1 << 30), "K must be a multiple of 8, got ", K);
+  TORCH_CHECK_VALUE(act >= kGluSilu && act <= kGluGeluErf, "unknown activation");
+  const c10::cuda::CUDAGuard guard(x.device());
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = F;
+  at::Tensor h = new_like(x, shape, x.scalar_type());
+  const int64_t M = x.numel() / K, Fp = (F + 7) / 8 * 8;
+  TORCH_CHECK_VALUE(M < (1ll << 30), "too many rows");
+  std::vector<at::Tensor> out{h};
+  GluArgs a{};
+  if (keep)
+    for (int i = 0; i < 2; ++i) out.push_back(new_like(x, {M, Fp}, x.scalar_type()).narrow(1, 0, F));
+  if (M == 0 || F == 0) return out;
+  const at::Tensor x2 = rows16(x.reshape({M, K})), g2 = rows16(wg), u2 = rows16(wu);
+  a.x = x2.data_ptr(), a.ldx = row_stride(x2);
+  a.wg = g2.data_ptr(), a.ldwg = row_stride(g2);
+  a.wu = u2.data_ptr(), a.ldwu = row_stride(u2);
+  a.h = h.data_ptr(), a.ldh = F;
+  if (keep) a.g = out[1].data_ptr(), a.u = out[2].data_ptr(), a.lds = Fp;
+  a.M = (int)M, a.K = (int)K, a.F = (int)F, a.act = (int)act;
+  a.f16 = x.scalar_type() == at::kHalf;
+  a.err = err_ptr();
+  DFL_CHECK_RC(dfl_glu(&a, cur_stream()), "gated_linear");
+  return out;
+}
+
+// Gradients of gated_linear: {dx, dwg, dwu} (undefined where not needed) from dh and what the forward kept.
+std::vector<at::Tensor> gated_linear_grad(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                                          const at::Tensor& g, const at::Tensor& u, int64_t act, bool need_dx, bool need_dwg,
+                                          bool need_dwu) {
+  const int64_t K = x.size(-1), F = wg.size(0), M = x.numel() / std::max<int64_t>(K, 1);
+  TORCH_CHECK_VALUE(dh.is_cuda() && dh.device() == x.device() && dh.scalar_type() == x.scalar_type() && dh.numel() == M * F,
+                    "the gradient ", dh.sizes(), " ", dh.scalar_type(), " does not match the output");
+  TORCH_CHECK_VALUE(g.dim() == 2 && g.size(0) == M && g.size(1) == F && g.sizes() == u.sizes() && g.strides() == u.strides() &&
+                        g.scalar_type() == x.scalar_type() && g.stride(1) == 1 && g.stride(0) % 8 == 0,
+                    "g and u are what the forward kept");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor dx, dwg, dwu;
+  if (need_dx) dx = new_like(x, x.sizes(), x.scalar_type());
+  if (need_dwg) dwg = new_like(wg, wg.sizes(), x.scalar_type());
+  if (need_dwu) dwu = new_like(wu, wu.sizes(), x.scalar_type());
+  if (M == 0 || F == 0) {
+    for (at::Tensor* t : {&dx, &dwg, &dwu})
+      if (t->defined()) t->zero_();
+    return {dx, dwg, dwu};
+  }
+  at::Tensor d2 = dh.reshape({M, F});
+  if (F > 1 && (d2.stride(1) != 1 || (M > 1 && d2.stride(0) < F))) d2 = d2.contiguous();
+  const int64_t Fp = (F + 7) / 8 * 8;
+  const at::Tensor dgu = new_like(x, {2, M, Fp}, x.scalar_type());
+  GluGradArgs e{};
+  e.dh = d2.data_ptr(), e.lddh = M > 1 ? d2.stride(0) : F;
+  e.g = g.data_ptr(), e.u = u.data_ptr(), e.lds = Fp;
+  TORCH_CHECK_VALUE(M <= 1 || g.stride(0) == Fp, "g and u are what the forward kept");
+  e.dg = dgu.data_ptr(), e.du = dgu[1].data_ptr();
+  e.M = M, e.F = (int)F, e.act = (int)act, e.f16 = x.scalar_type() == at::kHalf;
+  DFL_CHECK_RC(dfl_glu_grad(&e, cur_stream()), "gated_linear (gradient of the product)");
+  const at::Tensor x2 = rows16(x.reshape({M, K})), g2 = rows16(wg), u2 = rows16(wu);
+  GluGemmArgs a{};
+  a.dg = e.dg, a.du = e.du, a.lds = Fp;
+  a.x = x2.data_ptr(), a.ldx = row_stride(x2);
+  a.wg = g2.data_ptr(), a.ldwg = row_stride(g2);
+  a.wu = u2.data_ptr(), a.ldwu = row_stride(u2);
+  a.M = (int)M, a.K = (int)K, a.F = (int)F, a.f16 = e.f16;
+  a.err = err_ptr();
+  at::Tensor ws;
+  if (need_dx) {
+    a.dx = dx.data_ptr();
+    a.ws_floats = dfl_glu_dx_ws(a.M, a.K, a.F);
+    if (a.ws_floats) ws = new_like(x, {a.ws_floats}, at::kFloat), a.ws = ws.data_ptr<float>();
+    DFL_CHECK_RC(dfl_glu_dx(&a, cur_stream()), "gated_linear (gradient of x)");
+  }
+  if (need_dwg || need_dwu) {
+    a.dwg = need_dwg ? dwg.data_ptr() : nullptr;
+    a.dwu = need_dwu ? dwu.data_ptr() : nullptr;
+    DFL_CHECK_RC(dfl_glu_dw(&a, cur_stream()), "gated_linear (gradients of the weights)");
+  }
+  return {dx, dwg, dwu};
+}
+
+}  // namespace
+
+void bind_layer(py::module_& m) {
+  m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("act"), py::arg("keep"));
+  m.def("gated_linear_grad", &gated_linear_grad, py::arg("dh"), py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("g"), py::arg("u"),
+        py::arg("act"), py::arg("need_dx"), py::arg("need_dwg"), py::arg("need_dwu"));
+}

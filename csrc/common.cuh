@@ -38,6 +38,8 @@ enum KernelId : int {
   kKidConv = 6,
   kKidCross = 7,
   kKidLora = 8,
+  kKidGlu = 9,
+  kKidEmbed = 10,
 };
 
 DFL_DEVICE void record_error(int* err, int code, int kid, int d0, int d1) {

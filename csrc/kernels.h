@@ -490,6 +490,41 @@ int dfl_rel_l1_blocks(long long n, int num_sms);
 int dfl_rel_l1(const void* a, const void* b, long long n, float* scratch, int blocks, float* out,
                cudaStream_t stream);
 
+// ------------------------------------------------------------------ gated projection
+enum { kGluSilu = 0, kGluGelu = 1, kGluGeluErf = 2 };  // activations (kGluGelu: tanh form)
+// h = act(x Wg^T) * (x Wu^T); with g / u the two projections are kept beside it (for the gradients).  16-bit types
+// (f16: fp16, else bf16); row strides in elements, 16-byte aligned rows of x, wg, wu, g and u, any rows of h.
+typedef struct GluArgs {
+  const void* x; const void* wg; const void* wu;  // [M, K], [F, K], [F, K]
+  long long ldx, ldwg, ldwu;
+  void* h; long long ldh;                         // [M, F]
+  void* g; void* u; long long lds;                // [M, F] or NULL
+  int M, K, F, act, f16;
+  int* err;
+} GluArgs;
+int dfl_glu(const GluArgs* a, cudaStream_t stream);
+// dg = dh * u * act'(g), du = dh * act(g): [M, F]; rows of g, u, dg and du 16-byte aligned, of dh any.
+typedef struct GluGradArgs {
+  const void* dh; long long lddh;
+  const void* g; const void* u; void* dg; void* du; long long lds;
+  long long M;
+  int F, act, f16;
+} GluGradArgs;
+int dfl_glu_grad(const GluGradArgs* a, cudaStream_t stream);
+// dx = dg Wg + du Wu  [M, K];  dWg = dg^T x, dWu = du^T x  [F, K] (each may be NULL).  Rows 16-byte aligned.
+typedef struct GluGemmArgs {
+  const void* dg; const void* du; long long lds;
+  const void* x; const void* wg; const void* wu;
+  long long ldx, ldwg, ldwu;
+  void* dx; void* dwg; void* dwu;                 // contiguous
+  float* ws; long long ws_floats;                 // partial sums of dx (dfl_glu_dx_ws) or NULL
+  int M, K, F, f16;
+  int* err;
+} GluGemmArgs;
+int dfl_glu_dx(const GluGemmArgs* a, cudaStream_t stream);
+int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream);
+long long dfl_glu_dx_ws(int M, int K, int F);     // floats
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,7 @@ CUDA_SOURCES = [
     "gemm.cu",
     "gemm2.cu",
     "lora.cu",
+    "glu.cu",
     "norm.cu",
     "add_norm.cu",
     "attention.cu",
@@ -44,8 +45,9 @@ CUDA_SOURCES = [
     "vae.cu",
     "vae_gn.cu",
 ]
-CPP_SOURCES = ["bindings.cpp"]
-HEADERS = ["common.cuh", "kernels.h", "probe_noalloc.h", "gemm_epilogue.cuh", "cross_attn.cuh", "found_once.h"]
+CPP_SOURCES = ["bindings.cpp", "bindings_layer.cpp"]
+HEADERS = ["common.cuh", "kernels.h", "probe_noalloc.h", "gemm_epilogue.cuh", "cross_attn.cuh", "found_once.h", "pair.cuh",
+           "bindings.h"]
 
 NVCC_FLAGS = [
     "-gencode",

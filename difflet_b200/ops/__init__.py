@@ -11,6 +11,7 @@ _EXPORTS = {
     "ParallelEmbedding": "linear",
     "LoraBank": "lora",
     "linear_lora": "lora",
+    "gated_linear": "gated",
     "LayerNorm": "norm",
     "RMSNorm": "norm",
     "CustomRMSNorm": "norm",

@@ -16,6 +16,7 @@ Ops:
   linear_qkv    linear whose q/k/v column blocks go through qkv_scatter inside the
                 GEMM epilogue (no round trip of the qkv rows through HBM)
   linear_lora   linear with low-rank adapters of many requests accumulated beside the weight
+  gated_linear  act(x Wg^T) * (x Wu^T) as one kernel, with its gradients
   linear_group  two linear / linear_qkv calls with one epilogue kind as one launch
   row_sumsq     per-row sums of squares of q / k column blocks (TP across-heads RMS)
   attention     softmax(scale q k^T) v with key window and LSE
@@ -253,6 +254,29 @@ def linear_lora(x, w, b, bank, ids, rows_per_id=0, *, act=None, act_lo=0, act_hi
         y = resid.to(ct) + gate[:, :N].to(ct).repeat_interleave(gate_rows_per_batch or M, 0)[:M] * y
     y = y.to(torch.float32 if out_f32 else x.dtype)
     return y if out is None else out.copy_(y)
+
+
+# activation of gated_linear -> code of the native kernels
+GATED_ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 1, "gelu_erf": 2}
+
+
+def gated_linear(x, w_gate, w_up, act="silu"):
+    """``act(x w_gate^T) * (x w_up^T)`` in torch operations (f32 up to the result, f64 for f64): the oracle."""
+    ct = torch.float64 if x.dtype == torch.float64 else torch.float32
+    g, u = x.to(ct) @ w_gate.to(ct).t(), x.to(ct) @ w_up.to(ct).t()
+    a = F.silu(g) if act == "silu" else F.gelu(g, approximate="none" if act == "gelu_erf" else "tanh")
+    return (a * u).to(x.dtype)
+
+
+def gated_linear_native(x, w_gate, w_up, act, keep: bool):
+    """The kernel: (h,) or, with ``keep``, (h, g, u)."""
+    return _kernels().gated_linear(x, w_gate, w_up, GATED_ACTS[act], keep)
+
+
+def gated_linear_grad_native(dh, x, w_gate, w_up, g, u, act, need):
+    """(dx, dw_gate, dw_up), None where ``need`` is false."""
+    LAUNCHES[0] += int(need[0]) + int(need[1] or need[2])
+    return _kernels().gated_linear_grad(dh, x, w_gate, w_up, g, u, GATED_ACTS[act], *need)
 
 
 def _no_grad(name: str, *tensors) -> None:
@@ -603,9 +627,12 @@ def wants_grad(*tensors) -> bool:
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    if fwAD._current_level >= 0:
-        return any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
-    return False
+    return has_tangent(*tensors)
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of these carries a forward-mode tangent (None allowed)."""
+    return fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def kernel_tensors(*tensors) -> bool:

@@ -1,0 +1,55 @@
+"""The gated projection of a feed-forward block, and its gradients.
+
+``gated_linear`` evaluates ``act(x W_gate^T) * (x W_up^T)`` (the first half of the SwiGLU / gated-GELU blocks of the
+prompt encoders) as one kernel: both products, the activation and the multiplication (``csrc/glu.cu``).  The down projection
+is an ordinary ``linear``.  The weights stay as checkpoints hold them, two [F, K] tensors or the halves of one.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from difflet_b200.ops import fused as F
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, act):
+        h, g, u = F.gated_linear_native(x, w_gate, w_up, act, True)
+        ctx.act = act
+        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        need = [bool(n) for n in ctx.needs_input_grad[:3]]
+        return (*F.gated_linear_grad_native(dh, *ctx.saved_tensors, ctx.act, need), None)
+
+
+def gated_linear(x, w_gate, w_up, *, act="silu"):
+    """``act(x w_gate^T) * (x w_up^T)``: x [..., K]; w_gate, w_up [F, K] -> [..., F].
+
+    ``act``: "silu", "gelu" / "gelu_tanh" (tanh form) or "gelu_erf".  Products are accumulated and the activation is
+    evaluated in f32; the result is rounded to x's type once.  Differentiable in all three (once): the two projections are
+    kept in x's type for it.  CUDA: bf16 and fp16 with K a multiple of 8; other types and sizes, tracing,
+    function transforms and forward-mode tangents run as torch operations."""
+    if act not in F.GATED_ACTS:
+        raise ValueError(f"act {act!r}: one of {sorted(F.GATED_ACTS)}")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:
+        raise ValueError(f"x [..., K] and two weights [F, K] expected, got {tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}")
+    for name, t in (("w_gate", w_gate), ("w_up", w_up)):
+        if t.dtype != x.dtype or t.device != x.device:
+            raise ValueError(f"{name} {t.dtype} on {t.device} does not match x {x.dtype} on {x.device}")
+    if not x.is_floating_point():
+        raise ValueError(f"gated_linear needs floating-point tensors, got {x.dtype}")
+    if (x.is_cuda and x.dtype in F.CROSS_DTYPES and x.shape[-1] > 0 and x.shape[-1] % 8 == 0 and F.kernel_tensors(x, w_gate, w_up)
+            and not F.has_tangent(x, w_gate, w_up)):
+        if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+            return _GatedLinear.apply(x, w_gate, w_up, act)
+        return F.gated_linear_native(x, w_gate, w_up, act, False)[0]
+    return F.gated_linear(x, w_gate, w_up, act)
+
+
+__all__ = ["gated_linear"]
