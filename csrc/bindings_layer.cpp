@@ -103,10 +103,69 @@ std::vector<at::Tensor> gated_linear_grad(const at::Tensor& dh, const at::Tensor
   return {dx, dwg, dwu};
 }
 
+// ---------------------------------------------------------------- embedding lookup
+at::Tensor integer_ids(const at::Tensor& ids) {  // contiguous int32 or int64
+  const bool as_is = ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong;
+  return (as_is ? ids : ids.to(at::kLong)).contiguous();
+}
+
+// scale * w[ids]: ids of any shape, w [V, D] -> [..., D].
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale) {
+  TORCH_CHECK_VALUE(w.is_cuda() && w.dim() == 2 && ids.device() == w.device(), "ids and weight [V, D] must be on one CUDA device");
+  TORCH_CHECK_VALUE(at::isIntegralType(ids.scalar_type(), false), "ids must be integers, got ", ids.scalar_type());
+  EmbedArgs a{};
+  a.dtype = dtype_code(w, "weight");
+  a.V = w.size(0);
+  TORCH_CHECK_VALUE(w.size(1) < (1 << 30), "the rows are too long");
+  a.D = (int)w.size(1);
+  const c10::cuda::CUDAGuard guard(w.device());
+  std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+  shape.push_back(a.D);
+  at::Tensor y = new_like(w, shape, w.scalar_type());
+  if (y.numel() == 0) return y;
+  const at::Tensor i = integer_ids(ids), t = w.stride(1) == 1 || a.D == 1 ? w : w.contiguous();
+  a.ids = i.data_ptr(), a.id_bytes = (int)i.element_size();
+  a.w = t.data_ptr(), a.ldw = t.stride(0);
+  a.y = y.data_ptr();
+  a.n = i.numel();
+  a.scale = (float)scale;
+  a.err = err_ptr();
+  DFL_CHECK_RC(dfl_embed(&a, cur_stream()), "embedding");
+  return y;
+}
+
+// Gradient of the above: dy [..., D] for ids -> [V, D]; pad: the row that gets none (-1: every row gets its own).
+at::Tensor embedding_grad(const at::Tensor& dy, const at::Tensor& ids, int64_t V, double scale, int64_t pad) {
+  TORCH_CHECK_VALUE(dy.is_cuda() && dy.dim() >= 1 && ids.device() == dy.device() && at::isIntegralType(ids.scalar_type(), false),
+                    "dy [..., D] and integer ids must be on one CUDA device");
+  EmbedGradArgs a{};
+  a.dtype = dtype_code(dy, "dy");
+  a.n = ids.numel(), a.V = V;
+  TORCH_CHECK_VALUE(dy.size(-1) < (1 << 30) && a.n < (1ll << 30) && V < (1ll << 30), "too many ids or rows");
+  a.D = (int)dy.size(-1);
+  TORCH_CHECK_VALUE(dy.numel() == a.n * a.D, "dy ", dy.sizes(), " does not match ", a.n, " ids");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  at::Tensor dw = new_like(dy, {V, a.D}, dy.scalar_type());
+  if (dw.numel() == 0) return dw;
+  if (a.n == 0) return dw.zero_();
+  const at::Tensor i = integer_ids(ids), d = dy.contiguous();
+  a.ids = i.data_ptr(), a.id_bytes = (int)i.element_size();
+  a.dy = d.data_ptr(), a.dw = dw.data_ptr();
+  a.scale = (float)scale;
+  a.pad = pad;
+  a.ws_bytes = dfl_embed_grad_ws(a.n, a.V, a.D);
+  const at::Tensor ws = new_like(dy, {a.ws_bytes}, at::kByte);
+  a.ws = ws.data_ptr();
+  DFL_CHECK_RC(dfl_embed_grad(&a, cur_stream()), "embedding (gradient)");
+  return dw;
+}
+
 }  // namespace
 
 void bind_layer(py::module_& m) {
   m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("act"), py::arg("keep"));
   m.def("gated_linear_grad", &gated_linear_grad, py::arg("dh"), py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("g"), py::arg("u"),
         py::arg("act"), py::arg("need_dx"), py::arg("need_dwg"), py::arg("need_dwu"));
+  m.def("embedding", &embedding, py::arg("ids"), py::arg("w"), py::arg("scale"));
+  m.def("embedding_grad", &embedding_grad, py::arg("dy"), py::arg("ids"), py::arg("V"), py::arg("scale"), py::arg("pad"));
 }

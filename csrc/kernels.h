@@ -525,6 +525,31 @@ int dfl_glu_dx(const GluGemmArgs* a, cudaStream_t stream);
 int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream);
 long long dfl_glu_dx_ws(int M, int K, int F);     // floats
 
+// ------------------------------------------------------------------ embedding lookup
+// y[i] = scale * w[ids[i]]; ids of 4 or 8 bytes; an id outside [0, V) gives 0 and sets the error word.
+typedef struct EmbedArgs {
+  const void* ids; int id_bytes;
+  const void* w; long long ldw;      // [V, D], rows ldw elements apart
+  void* y;                           // [n, D] contiguous
+  long long n, V;
+  int D, dtype;
+  float scale;
+  int* err;
+} EmbedArgs;
+int dfl_embed(const EmbedArgs* a, cudaStream_t stream);
+// dw[v] = scale * sum of dy[i] over the i with ids[i] = v, in ascending order; 0 for v = pad (-1: none).
+typedef struct EmbedGradArgs {
+  const void* ids; int id_bytes;
+  const void* dy;                    // [n, D] contiguous
+  void* dw;                          // [V, D] contiguous
+  long long n, V, pad;
+  int D, dtype;
+  float scale;
+  void* ws; long long ws_bytes;      // dfl_embed_grad_ws, 16-byte aligned
+} EmbedGradArgs;
+long long dfl_embed_grad_ws(long long n, long long V, int D);
+int dfl_embed_grad(const EmbedGradArgs* a, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

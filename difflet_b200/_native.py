@@ -30,6 +30,7 @@ CUDA_SOURCES = [
     "gemm2.cu",
     "lora.cu",
     "glu.cu",
+    "embed.cu",
     "norm.cu",
     "add_norm.cu",
     "attention.cu",

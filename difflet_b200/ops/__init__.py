@@ -23,6 +23,7 @@ _EXPORTS = {
     "joint_ring_attention": "attn",
     "ulysses_attention": "attn",
     "joint_ulysses_attention": "attn",
+    "embedding": "embeddings",
     "apply_rotary_emb": "embeddings",
     "apply_rotary_emb_fp32": "embeddings",
     "apply_rotary_emb_slices": "embeddings",

@@ -1,4 +1,8 @@
-"""Rotary embeddings of the public op surface (difflet/ops/embeddings.py; laws of
+"""Embedding lookup and rotary embeddings.
+
+``embedding``: rows of a table, scaled, with a gradient for the table (``csrc/embed.cu``).
+
+Rotary embeddings of the public op surface (difflet/ops/embeddings.py; laws of
 difflet/backends/_torch_megatron/embeddings.py:13-37).  Tables are full head-dim
 ``cos`` / ``sin`` with each frequency repeated for its (even, odd) pair.  The built-in
 models rotate q/k inside the fused norm + RoPE + scatter kernel instead."""
@@ -6,6 +10,52 @@ models rotate q/k inside the fused norm + RoPE + scatter kernel instead."""
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as TF
+from torch.autograd.function import once_differentiable
+
+from difflet_b200.ops import fused as F
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, pad):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.pad = weight.shape[0], scale, pad
+        return F.embedding(ids, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return None, F.embedding_grad(dy, *ctx.saved_tensors, ctx.rows, ctx.scale, ctx.pad), None, None
+
+
+def embedding(ids, weight, *, scale=1.0, padding_idx=None):
+    """``scale * weight[ids]``: ids of any shape and integer type, weight [V, D] -> [..., D].
+
+    The product is formed in f32 and rounded once.  Differentiable in ``weight`` (once): the gradient is a dense [V, D] of its
+    type, every row summed in f32 in the order of the ids; the row ``padding_idx`` (negative: from the end) gets none.
+    CUDA: bf16, fp16 and fp32; an id outside the table gives a row of zeros and no gradient, and sets the device error word
+    (``_native.check_device_errors`` raises it); on the CPU it raises IndexError.  Other types, tracing, function transforms and
+    forward-mode tangents run as torch operations."""
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError(f"weight must be floating-point [V, D], got {tuple(weight.shape)} {weight.dtype}")
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+        raise ValueError(f"ids must be integers, got {ids.dtype}")
+    if ids.device != weight.device:
+        raise ValueError(f"ids on {ids.device}, weight on {weight.device}")
+    V, scale = weight.shape[0], float(scale)
+    pad = -1
+    if padding_idx is not None:
+        pad = int(padding_idx) + (V if padding_idx < 0 else 0)
+        if not 0 <= pad < V:
+            raise ValueError(f"padding_idx {padding_idx} is not a row of {V}")
+    if weight.is_cuda and weight.dtype in F.EMBED_DTYPES and F.kernel_tensors(ids, weight) and not F.has_tangent(weight):
+        if torch.is_grad_enabled() and weight.requires_grad:
+            return _Embedding.apply(ids, weight, scale, pad)
+        return F.embedding(ids, weight, scale)
+    ct = torch.float64 if weight.dtype == torch.float64 else torch.float32
+    rows = TF.embedding(ids.long(), weight, padding_idx=None if pad < 0 else pad)
+    return (rows.to(ct) * scale).to(weight.dtype)
 
 
 def apply_rotary_emb(hidden_states, freqs_cos, freqs_sin):
@@ -33,4 +83,4 @@ def apply_rotary_emb_slices(hidden_states, freqs_cos, freqs_sin):
     return apply_rotary_emb(hidden_states, freqs_cos, freqs_sin)
 
 
-__all__ = ["apply_rotary_emb", "apply_rotary_emb_fp32", "apply_rotary_emb_slices"]
+__all__ = ["embedding", "apply_rotary_emb", "apply_rotary_emb_fp32", "apply_rotary_emb_slices"]

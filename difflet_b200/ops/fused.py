@@ -21,6 +21,7 @@ Ops:
   row_sumsq     per-row sums of squares of q / k column blocks (TP across-heads RMS)
   attention     softmax(scale q k^T) v with key window and LSE
   cross_attention attention with masks, shared key heads, head dim 64 / 128, bf16 / fp16
+  embedding     scaled rows of a table, with its gradient by grouped ids
   gemv          modulation linears (M <= 8), f32 in/out, optional SiLU
   euler_step    x += dt * (u + s (c - u)) on f32 latents (+ bf16 mirror)
   timestep_embed sinusoidal features
@@ -738,6 +739,30 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
     p = torch.softmax(s.masked_fill(empty, 0.0), -1).masked_fill(empty, 0.0)
     o = torch.einsum("bhqk,bhkd->bhqd", p, vz).to(q.dtype)
     return o if out is None else out.copy_(o)
+
+
+# --------------------------------------------------------------------------- embedding lookup
+EMBED_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def embedding(ids, w, scale=1.0):
+    """``scale * w[ids]`` without a gradient: the kernel on CUDA, torch operations elsewhere."""
+    if w.is_cuda:
+        return _kernels().embedding(ids, w, float(scale))
+    ct = torch.float64 if w.dtype == torch.float64 else torch.float32
+    return (w[ids.long()].to(ct) * scale).to(w.dtype)
+
+
+def embedding_grad(dy, ids, V, scale=1.0, pad=-1):
+    """[V, D]: row v is ``scale`` times the sum of dy over the ids that are v (0 for v = pad)."""
+    if dy.is_cuda:
+        LAUNCHES[0] += 1  # (two kernels)
+        return _kernels().embedding_grad(dy, ids, int(V), float(scale), int(pad))
+    ct = torch.float64 if dy.dtype == torch.float64 else torch.float32
+    i, d = ids.reshape(-1).long(), dy.reshape(-1, dy.shape[-1]).to(ct)
+    keep = (i != pad) & (i >= 0) & (i < V)
+    dw = torch.zeros(V, d.shape[1], dtype=ct, device=dy.device).index_add_(0, i[keep], d[keep])
+    return (dw * scale).to(dy.dtype)
 
 
 # --------------------------------------------------------------------------- convolution
