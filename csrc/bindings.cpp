@@ -504,13 +504,15 @@ at::Tensor mx_dequantize(const at::Tensor& q, const at::Tensor& sf, at::ScalarTy
 }
 
 // q [B, H, Sq, dh], k / v [B, Hk, Sk, dh]; mask: bool (true = attend) or additive, broadcastable to
-// [B, H, Sq, Sk]; kv_lo / kv_hi int32 [B]; p2: P in two terms.
-at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
+// [B, H, Sq, Sk]; kv_lo / kv_hi int32 [B]; p2: P in two terms; slide > 0: a causal window that slides with the queries, beside the
+// first `sinks` keys, from position start[b] on.
+at::Tensor cross_attention_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
                            const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& kv_lo,
                            const c10::optional<at::Tensor>& kv_hi, const c10::optional<at::Tensor>& out,
-                           const c10::optional<at::Tensor>& lse, bool p2) {
+                           const c10::optional<at::Tensor>& lse, bool p2, int64_t slide, int64_t sinks,
+                           const c10::optional<at::Tensor>& start) {
   TORCH_CHECK_VALUE(!p2 || !given(mask), "precise_p comes without a mask");
-  TORCH_CHECK_VALUE(kernel_tensors({&q, &k, &v, given(mask), given(kv_lo), given(kv_hi)}),
+  TORCH_CHECK_VALUE(kernel_tensors({&q, &k, &v, given(mask), given(kv_lo), given(kv_hi), given(start)}),
                     "the kernel records no gradients and takes no wrapped tensors");
   const char* choice = std::getenv("DIFFLET_KERNEL_ATTN");  // (read per call, as the other attention entries do)
   TORCH_CHECK_VALUE(!choice || std::strcmp(choice, "sdpa"), "DIFFLET_KERNEL_ATTN=sdpa asks for the library baseline");
@@ -582,6 +584,17 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   };
   a.kv_lo = edge(kv_lo, "kv_lo", edges[0]);
   a.kv_hi = edge(kv_hi, "kv_lens", edges[1]);
+  at::Tensor first;
+  if (slide > 0) {
+    a.slide = (int)std::min<int64_t>(slide, std::numeric_limits<int>::max());
+    a.sinks = (int)std::min<int64_t>(sinks, a.Sk);
+    if (const at::Tensor* t = given(start)) {
+      TORCH_CHECK_VALUE(at::isIntegralType(t->scalar_type(), false) && t->dim() == 1 && t->size(0) == a.B, "q_start must be integers [", a.B, "]");
+      first = (t->scalar_type() == at::kLong ? t->clamp(std::numeric_limits<int>::min(), std::numeric_limits<int>::max()) : *t)
+                  .to(at::TensorOptions().device(q.device()).dtype(at::kInt)).contiguous();
+      a.start = first.data_ptr<int>();
+    }
+  }
   at::Tensor m, aux;
   int mdt = 0;  // -1: boolean, else the type of an additive mask
   long long ms[4] = {0, 0, 0, 0};
@@ -609,6 +622,8 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     d.mask_dtype = mdt;
     d.m_bs = ms[0], d.m_hs = ms[1], d.m_qs = ms[2], d.m_ks = ms[3];
   }
+  d.slide = a.slide, d.sinks = a.sinks, d.start = a.start;
+  d.span = (int)std::min<int64_t>(a.Sk, a.slide ? (int64_t)a.slide + a.sinks + a.Sq - 1 : a.Sk);
   d.err = err_ptr();
   if (!p2 && dfl_cross_decode_takes(&d)) {  // too few rows to fill the other kernel's tiles: the keys are split instead
     DFL_CHECK_RC(dfl_cross_decode(&d, cur_stream()), "cross_attention (few queries)");
@@ -658,6 +673,20 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   DFL_CHECK_RC(dfl_cross_attention(&a, cur_stream()), "cross_attention");
   if (!direct) o.copy_(o_);
   return o;
+}
+
+at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
+                           const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& kv_lo,
+                           const c10::optional<at::Tensor>& kv_hi, const c10::optional<at::Tensor>& out,
+                           const c10::optional<at::Tensor>& lse, bool p2) {
+  return cross_attention_call(q, k, v, scale, mask, kv_lo, kv_hi, out, lse, p2, 0, 0, c10::nullopt);
+}
+
+at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale, int64_t window, int64_t sinks,
+                            const c10::optional<at::Tensor>& kv_lens, const c10::optional<at::Tensor>& q_start,
+                            const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& lse) {
+  TORCH_CHECK_VALUE(window >= 1 && sinks >= 0, "window must be at least 1 and sinks at least 0, got ", window, " and ", sinks);
+  return cross_attention_call(q, k, v, scale, c10::nullopt, c10::nullopt, kv_lens, out, lse, false, window, sinks, q_start);
 }
 
 // Head-scatter description shared by the standalone qkv_scatter kernel and the GEMM
@@ -1282,6 +1311,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out"), py::arg("s_out"));
   m.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"),
         py::arg("mask"), py::arg("kv_lo"), py::arg("kv_hi"), py::arg("out"), py::arg("lse"), py::arg("p2"));
+  m.def("window_attention", &window_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"),
+        py::arg("sinks"), py::arg("kv_lens") = py::none(), py::arg("q_start") = py::none(), py::arg("out") = py::none(),
+        py::arg("lse") = py::none());
   m.def("mx_dequantize", &mx_dequantize, py::arg("q"), py::arg("scales"), py::arg("dtype"));
   m.def("qkv_scatter", &qkv_scatter);
   m.def("qkv_plan", &qkv_plan);

@@ -136,5 +136,6 @@ extern "C" int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream) {
   if (!(a->scale > 0.f)) return -6;
   if (a->bits && ((a->bits_bs | a->bits_hs | a->bits_qs) % 4 || a->bias_tiles)) return -7;
   if (a->p2 && (a->bits || a->bias_tiles)) return -8;
+  if (a->slide && (a->slide < 0 || a->sinks < 0 || a->bits || a->bias_tiles || a->p2 || a->kv_lo)) return -9;
   return a->f16 ? dfl_cross_attention_f16(a, stream) : cross_entry<false>(a, stream);
 }

@@ -34,7 +34,8 @@
 // the turn of an item (366).
 //
 // Masks: a key window [lo, hi) per batch row (tiles outside it are skipped), bits (kBits: packed
-// by cross_mask_bits, per query or shared by all queries) or an additive bias (kBias16 / kBias32).
+// by cross_mask_bits, per query or shared by all queries), an additive bias (kBias16 / kBias32), or a causal window that
+// slides with the queries beside the first keys (kSlide: only the tiles that some query of the block sees are read).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -51,8 +52,8 @@ constexpr int kBN = 128;      // keys per tile
 constexpr int kChunk = 16384;  // 128 rows x 64 values: one swizzle chunk
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-enum { kWindow = 0, kBits = 1, kBias16 = 2, kBias32 = 3 };  // kBias16: of the inputs' type, kBias32: f32
-constexpr bool is_bias(int mask) { return mask >= kBias16; }
+enum { kWindow = 0, kBits = 1, kBias16 = 2, kBias32 = 3, kSlide = 4 };  // kBias16: of the inputs' type, kBias32: f32
+constexpr bool is_bias(int mask) { return mask == kBias16 || mask == kBias32; }
 
 struct CrossParams {
   void* o;
@@ -71,6 +72,10 @@ struct CrossParams {
   const uint4* bias;
   long long bias_bs, bias_hs, bias_qs, bias_ts;  // batch, head, 32-query block, key tile
   int bias_rows;                                 // queries per block: 32, or 1 (one row for all)
+  // kSlide: query i of batch row b stands at p = start[b] + i (start NULL: keys - Sq) and sees the keys up to p that are
+  // among the last `slide` or the first `sinks`
+  const int* start;
+  int slide, sinks;
 };
 
 template <int DH, int QT>
@@ -170,6 +175,7 @@ struct CrossItems {
     window(p);
   }
   DFL_DEVICE bool more(const CrossParams& p) const { return b < p.B; }
+  DFL_DEVICE int tile(int j) const { return t0 + j; }
   DFL_DEVICE void next(const CrossParams& p) {
     const int was = b;
     qb += dq, h += dh, b += db;
@@ -188,6 +194,55 @@ struct CrossItems {
   }
 };
 
+// The same where a window slides with the queries: the tiles of the first keys, then those of the window.
+template <int QT>
+struct SlideItems {
+  int q0, h, b, n;
+  int lo, hi, sinks; // keys that a query of this block may see: [0, sinks) and [lo, hi)
+  long long p0;      // position of the block's first query (a start may be any 32-bit value)
+  int qb, dq, dh, db, len, start, n_sink, t_win;
+  DFL_DEVICE explicit SlideItems(const CrossParams& p) {
+    const int i = blockIdx.x, g = gridDim.x;
+    qb = i % p.n_qb, h = (i / p.n_qb) % p.H, b = i / p.n_qb / p.H;
+    dq = g % p.n_qb, dh = (g / p.n_qb) % p.H, db = g / p.n_qb / p.H;
+    row(p);
+  }
+  DFL_DEVICE bool more(const CrossParams& p) const { return b < p.B; }
+  DFL_DEVICE void next(const CrossParams& p) {
+    const int was = b;
+    qb += dq, h += dh, b += db;
+    if (qb >= p.n_qb) qb -= p.n_qb, ++h;
+    if (h >= p.H) h -= p.H, ++b;
+    if (b != was) row(p);
+    else block(p);
+  }
+  DFL_DEVICE void row(const CrossParams& p) {
+    if (b >= p.B) return;
+    len = p.kv_hi ? min(p.Sk, max(0, __ldcg(p.kv_hi + b))) : p.Sk;
+    start = p.start ? __ldcg(p.start + b) : len - p.Sq;
+    block(p);
+  }
+  DFL_DEVICE void block(const CrossParams& p) {
+    q0 = qb * (QT * kBM);
+    p0 = (long long)start + q0;
+    hi = (int)max(0ll, min((long long)len, (long long)start + min(q0 + QT * kBM, p.Sq)));
+    lo = (int)min((long long)p.Sk, max(0ll, p0 - p.slide + 1));
+    sinks = min(p.sinks, hi);
+    n_sink = (sinks + kBN - 1) / kBN;
+    t_win = max(n_sink, lo / kBN);
+    n = n_sink + (hi > lo ? max(0, (hi + kBN - 1) / kBN - t_win) : 0);
+  }
+  DFL_DEVICE int tile(int j) const { return j < n_sink ? j : t_win + j - n_sink; }
+};
+template <int MASK, int QT>
+struct ItemsOf {
+  using T = CrossItems<QT>;
+};
+template <int QT>
+struct ItemsOf<kSlide, QT> {
+  using T = SlideItems<QT>;
+};
+
 // The words of key tile k0 for one row of a bit mask (whole 128-key groups are stored).
 template <class Item>
 DFL_DEVICE uint4 cross_bits(const CrossParams& p, const Item& it, int q, int k0) {
@@ -197,7 +252,8 @@ DFL_DEVICE uint4 cross_bits(const CrossParams& p, const Item& it, int q, int k0)
 // Whether tile k0 holds V rows of keys that no query of this batch row may see.
 template <int MASK, class Item>
 DFL_DEVICE bool cross_dirty(const CrossParams& p, const Item& it, int k0) {
-  if (it.lo > k0 || it.hi < min(k0 + kBN, p.Sk)) return true;
+  if constexpr (MASK == kSlide) return it.hi < k0 + kBN || (it.lo > k0 && it.sinks < k0 + kBN);
+  else if (it.lo > k0 || it.hi < min(k0 + kBN, p.Sk)) return true;
   if (MASK == kBits && p.key_bits) {
     const uint4 w = cross_bits(p, it, 0, k0);
     return (w.x & w.y & w.z & w.w) != 0xffffffffu;
@@ -224,6 +280,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
                       const CrossParams p, int* err) {
   using C = CrossCfg<DH, QT>;
+  using Items = typename ItemsOf<MASK, QT>::T;
   constexpr int R = C::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -240,7 +297,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const bool cleaning = p.kv_lo || p.kv_hi || (MASK == kBits && p.key_bits);  // masked keys may hold anything
+  const bool cleaning = MASK == kSlide || p.kv_lo || p.kv_hi || (MASK == kBits && p.key_bits);  // masked keys may hold anything
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kNumBars; ++i) {
@@ -276,7 +333,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       for (int i = 0; i < R; ++i) issued[i] = false, issued_par[i] = 0;
       bool ok = true;
       int L = 0, used = 0;  // used: items with key tiles so far
-      for (CrossItems<QT> it(p); it.more(p) && ok; it.next(p)) {
+      for (Items it(p); it.more(p) && ok; it.next(p)) {
         if (it.n == 0) continue;
         const int hk = it.h / p.rep;
         for (int j = 0; j < it.n && ok; ++j) {
@@ -287,7 +344,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
             uint8_t* dst = smem + C::kKV + slot * C::kTile;
             mbar_arrive_expect_tx(&kv_full[slot], C::kTile);
             for (int c = 0; c < C::kChunks; ++c)
-              tma_load_4d(dst + c * kChunk, which == 0 ? &tk : &tv, &kv_full[slot], c * 64, (it.t0 + j) * kBN, hk, it.b);
+              tma_load_4d(dst + c * kChunk, which == 0 ? &tk : &tv, &kv_full[slot], c * 64, it.tile(j) * kBN, hk, it.b);
             issued[slot] = true;
             issued_par[slot] = par;
             if (j == 0 && which == 0) {  // the item's first keys are on their way: now its queries
@@ -368,7 +425,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         clean_par ^= 1u << slot;
         return mbar_wait(&v_clean[slot], par, err, kKidCross, 116, abort_flag);
       };
-      for (CrossItems<QT> it(p); it.more(p) && ok; it.next(p)) {
+      for (Items it(p); it.more(p) && ok; it.next(p)) {
         if (it.n == 0) continue;
         for (int j = 0; j < it.n && ok; ++j, ++s) {
           if (!wait_load(2 * s, 113)) { ok = false; break; }
@@ -403,9 +460,9 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     int s = 0;
     // every V tile passes here in order (its phase of v_clean[slot] completes once), so neither this
     // warp nor the MMA warp can be a phase of a slot ahead of the other
-    for (CrossItems<QT> it(p); cleaning && it.more(p) && ok; it.next(p)) {
+    for (Items it(p); cleaning && it.more(p) && ok; it.next(p)) {
       for (int j = 0; j < it.n && ok; ++j, ++s) {
-        const int k0 = (it.t0 + j) * kBN, L = 2 * s + 1;
+        const int k0 = it.tile(j) * kBN, L = 2 * s + 1;
         const bool dirty = cross_dirty<MASK>(p, it, k0);
         uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
         if (MASK == kBits && p.key_bits && dirty) {
@@ -417,7 +474,9 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4 && dirty; ++c) {  // key row 32 c + lane: 128 bytes in every chunk (the swizzle stays inside)
           const int r = 32 * c + lane, key = k0 + r;
-          if (key < it.lo || key >= it.hi || !((w[c] >> lane) & 1u)) {
+          bool drop = key < it.lo || key >= it.hi || !((w[c] >> lane) & 1u);
+          if constexpr (MASK == kSlide) drop = key >= it.hi || (key < it.lo && key >= it.sinks);
+          if (drop) {
 #pragma unroll
             for (int ch = 0; ch < C::kChunks; ++ch)
 #pragma unroll
@@ -444,12 +503,12 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     const float grow = is_bias(MASK) ? 8.f * kLn2 : 8.f;
     bool ok = true;
     int s = 0, used = 0;
-    for (CrossItems<QT> it(p); it.more(p) && ok; it.next(p)) {
+    for (Items it(p); it.more(p) && ok; it.next(p)) {
       const int qrow = it.q0 + g * kBM + row;
       const bool live = qrow < p.Sq;
       float m = -INFINITY, l = 0.f;  // running maximum (log2 units; bias: natural units) and sum
       for (int j = 0; j < it.n; ++j, ++s) {
-        const int k0 = (it.t0 + j) * kBN;
+        const int k0 = it.tile(j) * kBN;
         uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);
         if (MASK == kBits && live) keep = cross_bits(p, it, qrow, k0);
         // bias: 64 registers of it are on their way while the scores are awaited (16 bit: the whole
@@ -458,7 +517,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         const uint4* bp = nullptr;
         if constexpr (is_bias(MASK)) {
           const int qc = min(qrow, p.Sq - 1);  // (rows behind the last query read a valid one)
-          bp = p.bias + it.b * p.bias_bs + it.h * p.bias_hs + (qc / 32) * p.bias_qs + (it.t0 + j) * p.bias_ts +
+          bp = p.bias + it.b * p.bias_bs + it.h * p.bias_hs + (qc / 32) * p.bias_qs + it.tile(j) * p.bias_ts +
                (p.bias_rows > 1 ? qc % 32 : 0);
 #pragma unroll
           for (int v = 0; v < 16; ++v) bv[v] = __ldcg(bp + v * p.bias_rows);
@@ -508,7 +567,17 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
               if (!((w[c / 32] >> (c % 32)) & 1u)) z[c] = -INFINITY;
           }
         }
-        if (k0 < it.lo || k0 + kBN > it.hi) {
+        if constexpr (MASK == kSlide) {
+          // this row's keys, from k0 on: up to its own position, the last `slide` or the first `sinks` of them
+          const long long p_row = it.p0 + g * kBM + row;
+          const int up = (int)max(0ll, min(p_row + 1, (long long)it.hi)) - k0, sk = it.sinks - k0;
+          const int from = (int)max(0ll, min(p_row - p.slide + 1, (long long)p.Sk)) - k0;
+          if (up < kBN || (from > 0 && sk < kBN)) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (c >= up || (c < from && c >= sk)) z[c] = -INFINITY;
+          }
+        } else if (k0 < it.lo || k0 + kBN > it.hi) {
 #pragma unroll
           for (int c = 0; c < 128; ++c)
             if (k0 + c < it.lo || k0 + c >= it.hi) z[c] = -INFINITY;
@@ -691,6 +760,7 @@ int launch_cross_mask(const CrossArgs* a, const CrossParams& p, cudaStream_t str
     return a->bias_f32 ? launch_cross_qt<DH, F16, kBias32>(a, p, stream, dev)
                        : launch_cross_qt<DH, F16, kBias16>(a, p, stream, dev);
   if (a->bits) return launch_cross_qt<DH, F16, kBits>(a, p, stream, dev);
+  if (a->slide) return launch_cross_qt<DH, F16, kSlide>(a, p, stream, dev);
   if (a->p2) return launch_cross_qt<DH, F16, kWindow, true>(a, p, stream, dev);
   return launch_cross_qt<DH, F16, kWindow>(a, p, stream, dev);
 }
@@ -711,6 +781,8 @@ int cross_entry(const CrossArgs* a, cudaStream_t stream) {
   p.bias = reinterpret_cast<const uint4*>(a->bias_tiles);
   p.bias_bs = a->bias_bs, p.bias_hs = a->bias_hs, p.bias_qs = a->bias_qs, p.bias_ts = a->bias_ts;
   p.bias_rows = a->bias_rows;
+  p.start = a->start;
+  p.slide = a->slide, p.sinks = a->sinks;
   int dev = 0;
   cudaGetDevice(&dev);
   return a->dh == 64 ? launch_cross_mask<64, F16>(a, p, stream, dev) : launch_cross_mask<128, F16>(a, p, stream, dev);

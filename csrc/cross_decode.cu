@@ -70,6 +70,27 @@ DFL_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Keys of a batch row that its queries may see: [0, sinks) and [lo, hi); start: position of the first query.
+struct Keys {
+  int lo, hi, sinks, start;
+};
+template <bool SLIDE>
+DFL_DEVICE Keys keys_of(const DecodeArgs& a, int b) {
+  Keys k{};
+  k.hi = a.kv_hi ? min(a.Sk, a.kv_hi[b]) : a.Sk;
+  if constexpr (SLIDE) {
+    k.hi = max(0, k.hi);
+    k.start = a.start ? a.start[b] : k.hi - a.Sq;
+    const long long start = k.start;  // (any 32-bit value)
+    k.hi = (int)max(0ll, min((long long)k.hi, start + a.Sq));
+    k.lo = (int)min((long long)a.Sk, max(0ll, start - a.slide + 1));
+    k.sinks = min(min(a.sinks, k.hi), k.lo);
+  } else {
+    k.lo = a.kv_lo ? max(0, a.kv_lo[b]) : 0;
+  }
+  return k;
+}
+
 // Score of (row, key) after the mask: -inf when excluded.
 DFL_DEVICE float masked_score(const DecodeArgs& a, float s, int b, int h, int q, int k) {
   const float z = s * a.scale;
@@ -169,7 +190,7 @@ DFL_DEVICE void ldmatrix_x4_trans(uint32_t (&r)[4], const uint8_t* p) {
                : "memory");
 }
 // NB: blocks of eight query rows.  The last warp fills the ring.
-template <int DH, bool F16, int NB>
+template <int DH, bool F16, int NB, bool SLIDE>
 __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
     cross_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const DecodeArgs a) {
   constexpr int KC = DH / 32, DT = DH / 16;
@@ -196,15 +217,19 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
     fence_proxy_async_shared();
   }
   griddep_wait();  // (launched while the kernel before it ends)
-  const int lo = a.kv_lo ? max(0, a.kv_lo[b]) : 0, hi = a.kv_hi ? min(a.Sk, a.kv_hi[b]) : a.Sk;
-  const int nb = hi > lo ? (hi - lo + kStageKeys - 1) / kStageKeys : 0;
+  const Keys keys = keys_of<SLIDE>(a, b);
+  const int lo = keys.lo, hi = keys.hi;
+  // stages: of the first keys, then of [lo, hi)
+  const int ns = SLIDE ? (keys.sinks + kStageKeys - 1) / kStageKeys : 0;
+  const int nb = ns + (hi > lo ? (hi - lo + kStageKeys - 1) / kStageKeys : 0);
+  auto stage_key = [&](int blk) { return SLIDE && blk < ns ? blk * kStageKeys : lo + (blk - ns) * kStageKeys; };
   __syncthreads();
 
   if (warp == kWarps) {
     if (lane == 0) {
       int i = 0;
       for (int blk = split; blk < nb; blk += splits, ++i) {
-        const int slot = i % kStages, k0 = lo + blk * kStageKeys;
+        const int slot = i % kStages, k0 = stage_key(blk);
         if (!mbar_wait(&empty[slot], ((i / kStages) & 1) ^ 1u, a.err, kKidCross, 150 + slot, abort_flag)) break;
         uint8_t* st = smem + slot * 2 * kTile;
         mbar_arrive_expect_tx(&full[slot], 2 * kTile);
@@ -246,7 +271,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
     int i = 0;
     for (int blk = split; blk < nb; blk += splits, ++i) {
       if (i % kGroups != warp / 2) continue;
-      const int slot = i % kStages, row0 = 16 * (warp % 2), k0 = lo + blk * kStageKeys + row0, left = hi - k0;
+      const int slot = i % kStages, row0 = 16 * (warp % 2), k0 = stage_key(blk) + row0;
+      const int left = (SLIDE && blk < ns ? keys.sinks : hi) - k0;
       if (!mbar_wait_warp(&full[slot], (i / kStages) & 1, a.err, kKidCross, 160 + slot, abort_flag)) break;
       if (left > 0) {
         // 128-byte rows in the copies' swizzle: 16-byte piece p of row r lies at p ^ (r % 8)
@@ -267,7 +293,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
           for (int e = 0; e < 2 * NB; ++e) s[n][e] += s2[n][e];
         }
         // s[n][2 h + e]: row quad + 8 h, key 8 n + 2 t + e
-        const bool plain = a.mask == nullptr && left >= kKeys;  // (rows past R are not stored, whatever they hold)
+        // (rows past R are not stored, whatever they hold; a single query sees every key that is read)
+        const bool plain = (SLIDE ? a.Sq == 1 : a.mask == nullptr) && left >= kKeys;
         float f[NB];
         bool moved = false;
 #pragma unroll
@@ -280,7 +307,10 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2)
               const int key = 8 * n + 2 * t + e;
               float& z = s[n][2 * h + e];
               if (plain) z *= a.scale;
-              else z = quad + 8 * h < R && key < left ? masked_score(a, z, b, hrow[h], qrow[h], k0 + key) : -INFINITY;
+              else if constexpr (SLIDE) {
+                const long long at = (long long)keys.start + qrow[h];
+                z = key < left && k0 + key <= at && (k0 + key > at - a.slide || k0 + key < a.sinks) ? z * a.scale : -INFINITY;
+              } else z = quad + 8 * h < R && key < left ? masked_score(a, z, b, hrow[h], qrow[h], k0 + key) : -INFINITY;
               mx = fmaxf(mx, z);
             }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -394,14 +424,14 @@ struct Plan {
   long long cost;
 };
 
-template <int DH, bool F16, int NB>
+template <int DH, bool F16, int NB, bool SLIDE>
 int plan_decode(const DecodeArgs* a, Plan* plan) {
   static dfl_host::FoundOnce<Resident> resident[16];
   int dev = 0;
   cudaGetDevice(&dev);
   Resident res;
   const int rc = resident[dev & 15].get(&res, [&](Resident* r) {
-    auto kern = cross_decode_kernel<DH, F16, NB>;
+    auto kern = cross_decode_kernel<DH, F16, NB, SLIDE>;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(32 * (kWarps + 1), 1, 1);
     cfg.dynamicSmemBytes = smem_bytes(DH);
@@ -427,7 +457,7 @@ int plan_decode(const DecodeArgs* a, Plan* plan) {
   const long long heads = (long long)a->B * a->Hk * groups_of(a);
   plan->cost = -1;
   for (int i = 0; i < 5; ++i) {
-    const long long fit = res.clusters[i], keys = (a->Sk + (1 << i) - 1) >> i;
+    const long long fit = res.clusters[i], keys = ((long long)a->span + (1 << i) - 1) >> i;
     if (fit <= 0 || (i > 0 && keys < kGroups * kStageKeys)) continue;
     const long long cost = (heads + fit - 1) / fit * (keys + 300 * 128 / DH);
     if (plan->cost < 0 || cost < plan->cost) plan->cost = cost, plan->splits = 1 << i;
@@ -435,10 +465,10 @@ int plan_decode(const DecodeArgs* a, Plan* plan) {
   return 0;
 }
 
-template <int DH, bool F16, int NB>
+template <int DH, bool F16, int NB, bool SLIDE>
 int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
   Plan plan;
-  int rc = plan_decode<DH, F16, NB>(a, &plan);
+  int rc = plan_decode<DH, F16, NB, SLIDE>(a, &plan);
   if (rc) return rc;
   CUtensorMap tk, tv;
   rc = decode_tmap(&tk, a->k, a, a->k_ss, a->k_hs, a->k_bs);
@@ -458,15 +488,16 @@ int launch_decode(const DecodeArgs* a, cudaStream_t stream) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return (int)cudaLaunchKernelEx(&cfg, cross_decode_kernel<DH, F16, NB>, tk, tv, *a);
+  return (int)cudaLaunchKernelEx(&cfg, cross_decode_kernel<DH, F16, NB, SLIDE>, tk, tv, *a);
 }
 
-// Calls f<DH, F16, NB>(a, ...) for the call's head dim, type and rows.
-#define DFL_DECODE(f, ...)                                                                              \
-  (a->dh == 64 ? (a->f16 ? (rows_of(a) <= 8 ? f<64, true, 1>(a, __VA_ARGS__) : f<64, true, 2>(a, __VA_ARGS__))       \
-                         : (rows_of(a) <= 8 ? f<64, false, 1>(a, __VA_ARGS__) : f<64, false, 2>(a, __VA_ARGS__)))    \
-               : (a->f16 ? (rows_of(a) <= 8 ? f<128, true, 1>(a, __VA_ARGS__) : f<128, true, 2>(a, __VA_ARGS__))     \
-                         : (rows_of(a) <= 8 ? f<128, false, 1>(a, __VA_ARGS__) : f<128, false, 2>(a, __VA_ARGS__))))
+// Calls f<DH, F16, NB, SLIDE>(a, ...) for the call's head dim, type, rows and mask.
+#define DFL_DECODE_ROWS(f, dh, f16, ...)                                                                             \
+  (a->slide ? (rows_of(a) <= 8 ? f<dh, f16, 1, true>(a, __VA_ARGS__) : f<dh, f16, 2, true>(a, __VA_ARGS__))          \
+            : (rows_of(a) <= 8 ? f<dh, f16, 1, false>(a, __VA_ARGS__) : f<dh, f16, 2, false>(a, __VA_ARGS__)))
+#define DFL_DECODE(f, ...)                                                                                           \
+  (a->dh == 64 ? (a->f16 ? DFL_DECODE_ROWS(f, 64, true, __VA_ARGS__) : DFL_DECODE_ROWS(f, 64, false, __VA_ARGS__))   \
+               : (a->f16 ? DFL_DECODE_ROWS(f, 128, true, __VA_ARGS__) : DFL_DECODE_ROWS(f, 128, false, __VA_ARGS__)))
 
 }  // namespace
 
@@ -480,20 +511,21 @@ extern "C" int dfl_cross_decode_takes(const DecodeArgs* a) {
   // it lays out first) and 4300 go to the rest; here 17 or 11 by head dim (80% more with a mask, read value by value).
   //   16 heads x 78 x 2355 x 64: 32.2 us there, 13.5 here; 12 x 17 x 4096 x 128: 55.8, 13.6; 32 x 64 x 4096 x 128: 56.6, 38.7
   //   (additive mask 65.9, 76.0); 96 x 20 x 512 x 128: 11.0, 14.3; 128 x 17 x 2000 x 64: 29.0, 30.9
-  if (rows > 128 && a->Sk < 1024) return 0;
+  if (rows > 128 && a->span < 1024) return 0;
   Plan plan;
   if (DFL_DECODE(plan_decode, &plan)) return 0;
   int dev = 0;
   cudaGetDevice(&dev);
   const long long tiles = (long long)a->B * a->H * (a->Sq > 128 ? (a->Sq + 255) / 256 : 1), sms = dfl_host::num_sms(dev);
   const double here = plan.cost * (a->dh == 64 ? 11. : 17.) * (a->mask ? 1.8 : 1.);
-  const double there = (double)((tiles + sms - 1) / sms) * (4300. + 12.5 * a->Sk) * (a->mask ? 1.2 : 1.);
+  const double there = (double)((tiles + sms - 1) / sms) * (4300. + 12.5 * a->span) * (a->mask ? 1.2 : 1.);
   return here < 0.95 * there;
 }
 
 extern "C" int dfl_cross_decode(const DecodeArgs* a, cudaStream_t stream) {
   if (a->dh != 64 && a->dh != 128) return -2;
-  if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk) return -3;
+  if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk || a->span <= 0) return -3;
+  if (a->slide && (a->slide < 0 || a->sinks < 0 || a->mask || a->kv_lo)) return -9;
   if ((long long)a->H / a->Hk * a->Sq > kMaxRows || a->B > 65535 || (long long)a->Hk * groups_of(a) > 65535) return -8;
   auto al16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
   if (!al16(a->q) || !al16(a->k) || !al16(a->v) || !al16(a->o)) return -4;

@@ -321,6 +321,10 @@ typedef struct CrossArgs {
   long long bias_bs, bias_hs, bias_qs, bias_ts;
   int bias_rows, bias_f32;
   int p2;                              // P as the sum of two values of the inputs' type (no bits, no bias)
+  // slide > 0: query i of batch row b stands at p = start[b] + i (NULL: the row's keys - Sq) and sees key j <= p where
+  // j > p - slide or j < sinks (kv_hi: the row's keys; no other mask)
+  int slide, sinks;
+  const int* start;
   int* err;
 } CrossArgs;
 int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream);
@@ -349,6 +353,9 @@ typedef struct DecodeArgs {
   const void* mask;                    // NULL, bool bytes (mask_dtype -1) or an additive mask
   int mask_dtype;
   long long m_bs, m_hs, m_qs, m_ks;
+  int slide, sinks;                    // as in CrossArgs
+  const int* start;
+  int span;                            // keys of a row that are read at most (Sk where nothing slides)
   int* err;
 } DecodeArgs;
 // 1: this kernel is the faster one for the call (up to 16 query rows per key head, or more where the other would leave

@@ -19,6 +19,7 @@ _EXPORTS = {
     "add_rms_norm": "norm",
     "attention": "attn",
     "cross_attention": "attn",
+    "window_attention": "attn",
     "ring_attention": "attn",
     "joint_ring_attention": "attn",
     "ulysses_attention": "attn",

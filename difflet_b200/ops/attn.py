@@ -269,6 +269,64 @@ def cross_attention(q, k, v, *, scale=None, attention_mask=None, kv_lens=None, l
     return o if out is None else out.copy_(o)
 
 
+def _positions(q, k, kv_lens, q_start):
+    """Valid keys and the first query's position of each batch row, int64 [B]."""
+    B, Sk = q.shape[0], k.shape[2]
+    lens = torch.full((B,), Sk, device=q.device) if kv_lens is None else kv_lens.to(q.device, torch.int64).clamp(0, Sk)
+    return lens, lens - q.shape[2] if q_start is None else q_start.to(q.device, torch.int64)
+
+
+def window_attention(q, k, v, *, window, sinks=0, scale=None, kv_lens=None, q_start=None, lse=None, out=None):
+    """Causal attention to the last ``window`` keys and to the first ``sinks`` ones, which stay visible.
+
+    q [B, H, Sq, D]; k, v [B, Hk, Sk, D] (the cache), ``Hk`` divides ``H`` (query head h reads key head ``h // (H // Hk)``); any
+    strides.  Query i of batch row b stands at position ``p = q_start[b] + i`` and sees the keys ``j <= p`` with ``j > p - window``
+    or ``j < sinks``, among the row's ``kv_lens[b]`` valid ones (integers ``[B]``; None: all).  ``q_start`` (an integer or integers
+    ``[B]``; None: ``kv_lens - Sq``, the queries are the newest keys' own): 0 for prompts that are padded behind their ends.  A
+    window of ``Sk`` or more is plain causal attention.  ``scale=None`` means 1.0 as in ``attention``.
+
+    A query without a visible key gives 0 (LSE -inf).  What k and v hold at keys that no query of the call sees is not used; a
+    value that only some queries see must be finite (it meets the others with weight 0).  ``out`` (``[B, H, Sq, D]``) and ``lse``
+    (``[B, H, Sq]``, natural log) are filled when given.  CUDA: bf16 and fp16 with D 64 or 128, whose P is rounded to
+    the type for its product with v; only the tiles that some query sees are read, and few queries share the keys among many
+    CTAs.  Anything else, and what asks for gradients, runs as ``cross_attention`` under the same mask."""
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q [B, H, Sq, D], k and v [B, Hk, Sk, D]; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, H, Sq, _ = q.shape
+    if k.shape[1] < 1 or H % k.shape[1]:
+        raise ValueError(f"the query heads ({H}) must be a multiple of the key heads ({k.shape[1]})")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must share type and device")
+    if q_start is not None and not torch.is_tensor(q_start):
+        q_start = torch.full((B,), int(q_start), device=q.device)
+    for name, t in (("kv_lens", kv_lens), ("q_start", q_start)):
+        if t is not None and (t.shape != (B,) or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool):
+            raise ValueError(f"{name} must be integers [{B}]")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not match q {tuple(q.shape)} {q.dtype}")
+    if lse is not None and lse.numel() != B * H * Sq:
+        raise ValueError(f"lse must hold [{B}, {H}, {Sq}]")
+    scale = 1.0 if scale is None else float(scale)
+    if F.cross_kernel_ok(q, k, v) and F.kernel_tensors(kv_lens, q_start):
+        own = lse
+        if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device):
+            own = torch.empty(B, H, Sq, device=q.device, dtype=torch.float32)
+        o = F.window_attention(q, k, v, scale, window, sinks, kv_lens=kv_lens, q_start=q_start, out=out, lse=own)
+        if own is not lse:
+            lse.copy_(own.reshape(lse.shape))
+        return o
+    lens, first = _positions(q, k, kv_lens, q_start)
+    j = torch.arange(k.shape[2], device=q.device)
+    p = (first[:, None] + torch.arange(Sq, device=q.device))[:, :, None]
+    seen = (j <= p) & ((j > p - window) | (j < sinks)) & (j < lens[:, None, None])
+    keys = seen.any(1)[:, None, :, None]  # (what no query sees may be anything, and 0 * NaN would reach the sums)
+    k, v = (t.masked_fill(~keys, 0.0) for t in (k, v))
+    return cross_attention(q, k, v, scale=scale, attention_mask=seen[:, None], lse=lse, out=out)
+
+
 def attention_with_lse(q, k, v, *, scale, bound_min=None, bound_max=None):
     """(out, lse) of one key block: lse fp32 [B, H, Sq] (natural log)."""
     lse = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float64 if q.dtype == torch.float64
@@ -425,5 +483,5 @@ def joint_ulysses_attention(q_img, q_txt, image_k, image_v, text_k, text_v, *, s
     return img_out, torch.cat(parts, 1)
 
 
-__all__ = ["attention", "cross_attention", "ring_attention", "joint_ring_attention", "ulysses_attention",
+__all__ = ["attention", "cross_attention", "window_attention", "ring_attention", "joint_ring_attention", "ulysses_attention",
            "joint_ulysses_attention", "attention_with_lse", "merge_partials"]

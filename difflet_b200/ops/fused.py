@@ -20,6 +20,7 @@ Ops:
   linear_group  two linear / linear_qkv calls with one epilogue kind as one launch
   row_sumsq     per-row sums of squares of q / k column blocks (TP across-heads RMS)
   attention     softmax(scale q k^T) v with key window and LSE
+  window_attention causal attention to the last and the first keys (head dim 64 / 128, bf16 / fp16)
   cross_attention attention with masks, shared key heads, head dim 64 / 128, bf16 / fp16
   embedding     scaled rows of a table, with its gradient by grouped ids
   gemv          modulation linears (M <= 8), f32 in/out, optional SiLU
@@ -739,6 +740,15 @@ def cross_attention(q, k, v, scale, *, mask=None, kv_lo=None, kv_hi=None, out=No
     p = torch.softmax(s.masked_fill(empty, 0.0), -1).masked_fill(empty, 0.0)
     o = torch.einsum("bhqk,bhkd->bhqd", p, vz).to(q.dtype)
     return o if out is None else out.copy_(o)
+
+
+def window_attention(q, k, v, scale, window, sinks, *, kv_lens=None, q_start=None, out=None, lse=None):
+    """The kernel of ``ops.window_attention`` (CUDA tensors that ``cross_kernel_ok`` takes; an LSE is contiguous f32)."""
+    if scale <= 0:  # as in cross_attention
+        q, scale = (-q, -scale) if scale < 0 else (torch.zeros_like(q), 1.0)
+    o = (_nat or _lib()).window_attention(q, k, v, scale, window, sinks, kv_lens, q_start, out, lse)
+    LAUNCHES[0] += 1  # (a refused call is no launch)
+    return o
 
 
 # --------------------------------------------------------------------------- embedding lookup
