@@ -63,14 +63,20 @@ inline int dtype_code(const at::Tensor& t, const char* name) {
 
 inline const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 
-// ---------------------------------------------------------------- cross attention
+// No wrapper among these (function transforms such as vmap, fake tensors) and no forward-mode tangent.
+inline bool plain_tensors(std::initializer_list<const at::Tensor*> tensors) {
+  constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
+  for (const at::Tensor* t : tensors)
+    if (t && (t->key_set().has_any(wrappers) || t->_fw_grad(0).defined())) return false;
+  return true;
+}
+
 // Tensors that a kernel can be given in place of a differentiable torch operation: none asks for gradients or carries a
 // forward-mode tangent, and none is a wrapper (function transforms such as vmap, fake tensors).
 inline bool kernel_tensors(std::initializer_list<const at::Tensor*> tensors) {
-  constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
-                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
-  const bool grad = at::GradMode::is_enabled();
-  for (const at::Tensor* t : tensors)
-    if (t && ((grad && t->requires_grad()) || t->key_set().has_any(wrappers) || t->_fw_grad(0).defined())) return false;
-  return true;
+  if (at::GradMode::is_enabled())
+    for (const at::Tensor* t : tensors)
+      if (t && t->requires_grad()) return false;
+  return plain_tensors(tensors);
 }

@@ -1,7 +1,35 @@
 // torch bindings of the layer operators: gated projection, embedding lookup, windowed attention.
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "bindings.h"
 
 namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients computed by kernels, for a backward pass that may itself be recorded: they carry an error for whoever
+// differentiates them.
+template <class Compute>
+variable_list once_differentiable(const char* name, Compute compute) {
+  const bool recorded = at::GradMode::is_enabled();
+  variable_list grads;
+  {
+    const at::NoGradGuard off;
+    grads = compute();
+  }
+  if (!recorded) return grads;
+  variable_list given;
+  for (const at::Tensor& t : grads)
+    if (t.defined()) given.push_back(t.detach().set_requires_grad(true));
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " can be differentiated once only", (int64_t)given.size());
+  const variable_list held = (*error)(std::move(given));
+  size_t i = 0;
+  for (at::Tensor& t : grads)
+    if (t.defined()) t = held[i++];
+  return grads;
+}
 
 // Rows that the copy engine can address: unit inner stride, 16-byte aligned rows; anything else is laid out anew.
 at::Tensor rows16(const at::Tensor& t) {
@@ -16,7 +44,7 @@ bool is16(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.sc
 // ---------------------------------------------------------------- gated projection
 // x [..., K], wg / wu [F, K] of one 16-bit type -> {h [..., F]} or, to keep the projections for the gradients, {h, g, u}
 // (g, u [M, F] with padded rows).
-std::vector<at::Tensor> gated_linear(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act, bool keep) {
+std::vector<at::Tensor> gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act, bool keep) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && wg.dim() == 2 && wu.dim() == 2, "x [..., K] and weights [F, K] must be CUDA tensors");
   TORCH_CHECK_VALUE(is16(x), "gated_linear runs in bfloat16 or float16 on CUDA, got ", x.scalar_type());
   for (const at::Tensor* t : {&wg, &wu})
@@ -45,12 +73,15 @@ std::vector<at::Tensor> gated_linear(const at::Tensor& x, const at::Tensor& wg, 
   a.M = (int)M, a.K = (int)K, a.F = (int)F, a.act = (int)act;
   a.f16 = x.scalar_type() == at::kHalf;
   a.err = err_ptr();
+  at::Tensor ws;
+  a.ws_floats = dfl_glu_ws(0, a.M, a.K, a.F);
+  if (a.ws_floats) ws = new_like(x, {a.ws_floats}, at::kFloat), a.ws = ws.data_ptr<float>();
   DFL_CHECK_RC(dfl_glu(&a, cur_stream()), "gated_linear");
   return out;
 }
 
 // Gradients of gated_linear: {dx, dwg, dwu} (undefined where not needed) from dh and what the forward kept.
-std::vector<at::Tensor> gated_linear_grad(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+std::vector<at::Tensor> gated_backward(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                                           const at::Tensor& g, const at::Tensor& u, int64_t act, bool need_dx, bool need_dwg,
                                           bool need_dwu) {
   const int64_t K = x.size(-1), F = wg.size(0), M = x.numel() / std::max<int64_t>(K, 1);
@@ -88,11 +119,12 @@ std::vector<at::Tensor> gated_linear_grad(const at::Tensor& dh, const at::Tensor
   a.wu = u2.data_ptr(), a.ldwu = row_stride(u2);
   a.M = (int)M, a.K = (int)K, a.F = (int)F, a.f16 = e.f16;
   a.err = err_ptr();
-  at::Tensor ws;
+  at::Tensor ws;  // (one for both products, which run one after the other)
+  const int dw = need_dwg && need_dwu ? 2 : 3;
+  a.ws_floats = std::max(need_dx ? dfl_glu_ws(1, a.M, a.K, a.F) : 0, need_dwg || need_dwu ? dfl_glu_ws(dw, a.M, a.K, a.F) : 0);
+  if (a.ws_floats) ws = new_like(x, {a.ws_floats}, at::kFloat), a.ws = ws.data_ptr<float>();
   if (need_dx) {
     a.dx = dx.data_ptr();
-    a.ws_floats = dfl_glu_dx_ws(a.M, a.K, a.F);
-    if (a.ws_floats) ws = new_like(x, {a.ws_floats}, at::kFloat), a.ws = ws.data_ptr<float>();
     DFL_CHECK_RC(dfl_glu_dx(&a, cur_stream()), "gated_linear (gradient of x)");
   }
   if (need_dwg || need_dwu) {
@@ -103,6 +135,30 @@ std::vector<at::Tensor> gated_linear_grad(const at::Tensor& dh, const at::Tensor
   return {dx, dwg, dwu};
 }
 
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act) {
+    std::vector<at::Tensor> hgu = gated_forward(x, wg, wu, act, true);
+    ctx->save_for_backward({x, wg, wu, hgu[1], hgu[2]});
+    ctx->saved_data["act"] = act;
+    return hgu[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dh) {
+    return once_differentiable("gated_linear", [&]() -> variable_list {
+      const variable_list s = ctx->get_saved_variables();
+      std::vector<at::Tensor> d = gated_backward(dh[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["act"].toInt(),
+                                                 ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+      return {d[0], d[1], d[2], at::Tensor()};
+    });
+  }
+};
+
+at::Tensor gated_linear(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act) {
+  TORCH_CHECK_VALUE(plain_tensors({&x, &wg, &wu}), "the kernel takes no wrapped tensors and no tangents");
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad()))
+    return GatedLinear::apply(x, wg, wu, act);
+  return gated_forward(x, wg, wu, act, false)[0];
+}
+
 // ---------------------------------------------------------------- embedding lookup
 at::Tensor integer_ids(const at::Tensor& ids) {  // contiguous int32 or int64
   const bool as_is = ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong;
@@ -110,7 +166,7 @@ at::Tensor integer_ids(const at::Tensor& ids) {  // contiguous int32 or int64
 }
 
 // scale * w[ids]: ids of any shape, w [V, D] -> [..., D].
-at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale) {
+at::Tensor embedding_forward(const at::Tensor& ids, const at::Tensor& w, double scale) {
   TORCH_CHECK_VALUE(w.is_cuda() && w.dim() == 2 && ids.device() == w.device(), "ids and weight [V, D] must be on one CUDA device");
   TORCH_CHECK_VALUE(at::isIntegralType(ids.scalar_type(), false), "ids must be integers, got ", ids.scalar_type());
   EmbedArgs a{};
@@ -160,12 +216,38 @@ at::Tensor embedding_grad(const at::Tensor& dy, const at::Tensor& ids, int64_t V
   return dw;
 }
 
+struct Embedding : torch::autograd::Function<Embedding> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& w, double scale, int64_t pad) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["pad"] = pad;
+    return embedding_forward(ids, w, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    return once_differentiable("embedding", [&]() -> variable_list {
+      return {at::Tensor(), embedding_grad(dy[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
+                                           ctx->saved_data["scale"].toDouble(), ctx->saved_data["pad"].toInt()), at::Tensor(), at::Tensor()};
+    });
+  }
+};
+
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale, const c10::optional<int64_t>& padding_idx) {
+  TORCH_CHECK_VALUE(plain_tensors({&ids, &w}), "the kernel takes no wrapped tensors and no tangents");
+  TORCH_CHECK_VALUE(w.dim() == 2, "weight must be [V, D], got ", w.sizes());
+  int64_t pad = -1;
+  if (padding_idx.has_value()) {
+    pad = *padding_idx + (*padding_idx < 0 ? w.size(0) : 0);
+    TORCH_CHECK_VALUE(pad >= 0 && pad < w.size(0), "padding_idx ", *padding_idx, " is not a row of ", w.size(0));
+  }
+  if (at::GradMode::is_enabled() && w.requires_grad()) return Embedding::apply(ids, w, scale, pad);
+  return embedding_forward(ids, w, scale);
+}
+
 }  // namespace
 
 void bind_layer(py::module_& m) {
-  m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("act"), py::arg("keep"));
-  m.def("gated_linear_grad", &gated_linear_grad, py::arg("dh"), py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("g"), py::arg("u"),
-        py::arg("act"), py::arg("need_dx"), py::arg("need_dwg"), py::arg("need_dwu"));
-  m.def("embedding", &embedding, py::arg("ids"), py::arg("w"), py::arg("scale"));
+  m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("wg"), py::arg("wu"), py::arg("act"));
+  m.def("embedding", &embedding, py::arg("ids"), py::arg("w"), py::arg("scale"), py::arg("padding_idx") = py::none());
   m.def("embedding_grad", &embedding_grad, py::arg("dy"), py::arg("ids"), py::arg("V"), py::arg("scale"), py::arg("pad"));
 }

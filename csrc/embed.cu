@@ -3,14 +3,14 @@
 // Lookup: bound by its bytes; a thread moves 16-byte pieces (single values where a row is no multiple of them).  The product
 // is formed in f32 and rounded once.
 //
-// Gradient: dW[v] = scale * sum of dy[i] over the tokens i with id v.  Every row of dW is written once, by the warp that sums it,
-// zeros among them; f32 sums in ascending order of i, so the result does not depend on the order of atomics.
+// Gradient: dW[v] = scale * sum of dy[i] over the tokens i with id v: f32 sums in ascending order of i, so the result does not
+// depend on the order of atomics, rounded once.  Bound by writing dW, nearly all of it zeros.
 //   embed_sort_kernel  one cluster groups the tokens by id: count (a warp adds equal ids at once), give every id that occurs a
 //                      range of the list, place.  Where the range lies and in which order tokens arrive there is left to chance;
-//                      ids with more than 32 tokens are put in ascending order here, the rest by the warp that sums them.
-//                      Their tokens are cut into items of 64.
-//   embed_sum_kernel   warps take (item, 32 pieces of a row), then rows.  An item's sums are kept in f32 and the
-//                      last warp of a row's piece adds them in order.
+//                      ids with more than 32 tokens are put in ascending order here, the rest by the warps that sum them.
+//                      Meanwhile the other clusters fill dW with zeros.
+//   embed_sum_kernel   a warp takes 128 pieces of an item (an id's tokens, at most 64 of them).  The sums of an id's items are
+//                      kept in f32 and added in order by the last warp of the piece.
 // A sort by value is not needed for that, and a scan over the vocabulary neither.
 #include <algorithm>
 
@@ -27,9 +27,12 @@ constexpr int kCluster = 8, kSortThreads = 1024, kFew = 32, kItem = 64, kByWarp 
 constexpr int kWindow = 1 << 18;  // tokens whose order a CTA finds by one bitmap in shared memory (32 KB)
 
 struct Item {
-  int row, begin, len, part;  // part: of the partial sums, -1 where the item is the whole row
-  int first, items, ticket, pad;  // of the row: first part, items, index of its counters
+  int row, begin, len, part;  // begin: in the list; part: of the partial sums, -1: none
+  int first, items, ticket, order;  // of the row: first part, items, index of its counters
 };
+
+// An item's tokens: in any order, in ascending order, or the only one of its row, which `begin` is itself.
+enum { kAnyOrder = 0, kInOrder = 1, kOnly = 2 };
 
 struct EmbedWs {
   int* count;   // [V]
@@ -38,14 +41,14 @@ struct EmbedWs {
   int* list;    // [n]
   int* tmp;     // [n]
   int* many;    // [n / 32]: rows with more than kFew tokens
-  Item* items;  // [n / 32]
+  Item* items;  // [n + n / 32]
   int* ticket;  // [n / 32][pieces]
   int* head;    // list length, rows in `many`, items, parts, tickets
   float* part;  // [n / 32][D]
 };
 
 __host__ __device__ inline long long up16(long long b) { return (b + 15) / 16 * 16; }
-// (an item of at most 64 tokens belongs to a row of more than 32: there are at most n / 32 of them)
+// (ids with more than 32 tokens have at most n / 32 items)
 inline long long embed_layout(long long n, long long V, int D, char* base, EmbedWs* w) {
   long long at = 0;
   const long long m = n / kFew + 1, chunks = (D + 31) / 32;
@@ -61,7 +64,7 @@ inline long long embed_layout(long long n, long long V, int D, char* base, Embed
   r.list = reinterpret_cast<int*>(take(4 * n));
   r.tmp = reinterpret_cast<int*>(take(4 * n));
   r.many = reinterpret_cast<int*>(take(4 * m));
-  r.items = reinterpret_cast<Item*>(take((long long)sizeof(Item) * m));
+  r.items = reinterpret_cast<Item*>(take((long long)sizeof(Item) * (n + m)));
   r.ticket = reinterpret_cast<int*>(take(4 * m * chunks));
   r.head = reinterpret_cast<int*>(take(64));
   r.part = reinterpret_cast<float*>(take(4 * m * D));
@@ -85,17 +88,17 @@ struct Value<kDtypeF32> {
 };
 template <>
 struct Value<kDtypeBf16> {
-  using T = __nv_bfloat16;
+  using T = uint16_t;
   static constexpr int kWide = 8;
-  static DFL_DEVICE float get(T v) { return __bfloat162float(v); }
-  static DFL_DEVICE T put(float v) { return __float2bfloat16_rn(v); }
+  static DFL_DEVICE float get(T v) { return __uint_as_float((uint32_t)v << 16); }
+  static DFL_DEVICE T put(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 };
 template <>
 struct Value<kDtypeF16> {
-  using T = __half;
+  using T = uint16_t;
   static constexpr int kWide = 8;
-  static DFL_DEVICE float get(T v) { return __half2float(v); }
-  static DFL_DEVICE T put(float v) { return __float2half_rn(v); }
+  static DFL_DEVICE float get(T v) { return __half2float(__ushort_as_half(v)); }
+  static DFL_DEVICE T put(float v) { return __half_as_ushort(__float2half_rn(v)); }
 };
 
 template <class T, int VEC>
@@ -113,15 +116,20 @@ __global__ void __launch_bounds__(256) embed_kernel(EmbedArgs a, int lanes) {
     const long long id = id_at(a.ids, a.id_bytes, i);
     const bool in = id >= 0 && id < a.V;
     if (!in && lane == 0) record_error(a.err, kErrBounds, kKidEmbed, 1, (int)i);
-    const P* src = reinterpret_cast<const P*>(reinterpret_cast<const typename V::T*>(a.w) + (in ? id * a.ldw : 0));
-    P* dst = reinterpret_cast<P*>(reinterpret_cast<typename V::T*>(a.y) + i * a.D);
-#pragma unroll 4
-    for (int c = lane; c < pieces; c += lanes) {
-      P x;
-      if (in) x = src[c];
+    const P* __restrict__ src = reinterpret_cast<const P*>(reinterpret_cast<const typename V::T*>(a.w) + (in ? id * a.ldw : 0));
+    P* __restrict__ dst = reinterpret_cast<P*>(reinterpret_cast<typename V::T*>(a.y) + i * a.D);
+    for (int c0 = lane; c0 < pieces; c0 += 4 * lanes) {
+      P x[4];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x.v[e] = in ? V::put(a.scale * V::get(x.v[e])) : V::put(0.f);
-      dst[c] = x;
+      for (int u = 0; u < 4; ++u)
+        if (in && c0 + u * lanes < pieces) x[u] = src[c0 + u * lanes];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (c0 + u * lanes >= pieces) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[u].v[e] = in ? V::put(a.scale * V::get(x[u].v[e])) : V::put(0.f);
+        dst[c0 + u * lanes] = x[u];
+      }
     }
   }
 }
@@ -144,6 +152,14 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   __shared__ int sums[kSortThreads / 32];
   griddep_wait();
   constexpr int kAll = kCluster * kSortThreads;
+  if (blockIdx.x >= kCluster) {  // zeros
+    const long long bytes = a.V * a.D * (a.dtype == kDtypeF32 ? 4 : 2), whole = bytes / 16, step = (long long)(gridDim.x - kCluster) * kSortThreads;
+    const long long at = (long long)(blockIdx.x - kCluster) * kSortThreads + threadIdx.x;
+    uint4* d = reinterpret_cast<uint4*>(a.dw);
+    for (long long i = at; i < whole; i += step) d[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (at < bytes - whole * 16) reinterpret_cast<uint8_t*>(a.dw)[whole * 16 + at] = 0;
+    return;
+  }
   const int me = blockIdx.x * kSortThreads + threadIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   auto sync = [] {
     __threadfence();
@@ -177,16 +193,17 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
     const int at = warp_add(w.head, c);
     if (first) w.start[id] = at;
     const bool large = c > kFew;
+    const int items = (c + kItem - 1) / kItem, it = warp_add(w.head + 2, items);
+    int part = 0, ticket = 0;
     if (__any_sync(0xffffffffu, large)) {
-      const int items = large ? (c + kItem - 1) / kItem : 0;
-      const int slot = warp_add(w.head + 1, large), it = warp_add(w.head + 2, items), part = warp_add(w.head + 3, items > 1 ? items : 0);
-      const int ticket = warp_add(w.head + 4, items > 1);
-      if (large) {
-        w.many[slot] = id;
-        for (int k = 0; k < items; ++k)
-          w.items[it + k] = Item{id, at + k * kItem, min(kItem, c - k * kItem), items > 1 ? part + k : -1, part, items, ticket, 0};
-      }
+      const int slot = warp_add(w.head + 1, large);
+      part = warp_add(w.head + 3, items > 1 ? items : 0);
+      ticket = warp_add(w.head + 4, items > 1);
+      if (large) w.many[slot] = id;
     }
+    for (int k = 0; k < items; ++k)
+      w.items[it + k] = Item{id, c == 1 ? (int)i : at + k * kItem, min(kItem, c - k * kItem), items > 1 ? part + k : -1, part, items, ticket,
+                           c == 1 ? kOnly : large ? kInOrder : kAnyOrder};
   }
   sync();
   for (long long i = me; i < a.n; i += kAll) {
@@ -201,14 +218,25 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   for (int j = me / 32; j < rows; j += kAll / 32) {
     const int id = __ldcg(w.many + j), c = __ldcg(w.count + id), at = __ldcg(w.start + id);
     if (c > kByWarp) continue;
-    for (int k = lane; k < c; k += 32) {
-      const int mine = __ldcg(w.list + at + k);
-      int place = 0;
-      for (int o = 0; o < c; ++o) place += __ldcg(w.list + at + o) < mine;
-      w.tmp[at + place] = mine;
+    int mine[kByWarp / 32], place[kByWarp / 32];
+#pragma unroll
+    for (int e = 0; e < kByWarp / 32; ++e) {
+      mine[e] = e * 32 + lane < c ? __ldcg(w.list + at + e * 32 + lane) : 0x7fffffff;
+      place[e] = 0;
+    }
+#pragma unroll
+    for (int o = 0; o < kByWarp / 32; ++o) {
+      if (o * 32 >= c) break;
+      for (int s = 0; s < 32; ++s) {  // (what lies behind the last token is above all)
+        const int x = __shfl_sync(0xffffffffu, mine[o], s);
+#pragma unroll
+        for (int e = 0; e < kByWarp / 32; ++e) place[e] += x < mine[e];
+      }
     }
     __syncwarp();
-    for (int k = lane; k < c; k += 32) w.list[at + k] = w.tmp[at + k];
+#pragma unroll
+    for (int e = 0; e < kByWarp / 32; ++e)
+      if (e * 32 + lane < c) w.list[at + place[e]] = mine[e];
   }
   for (int j = blockIdx.x; j < rows; j += kCluster) {
     const int id = __ldcg(w.many + j), c = __ldcg(w.count + id), at = __ldcg(w.start + id);
@@ -251,90 +279,102 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   }
 }
 
+// A warp takes 32 U pieces of an item: lane l the pieces l, l + 32, ...; the next item is on its way meanwhile.
+// 16384 tokens of 8000 ids x 3584, bf16: see embed_train in the table; U = 4 with two tokens in flight 104 us, U = 1 with eight
+// (and the item read when its turn comes) 61.
+constexpr int kU = 2, kTokens = 4;
+
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256) embed_sum_kernel(EmbedGradArgs a, EmbedWs w) {
   using V = Value<DT>;
   using P = Piece<typename V::T, VEC>;
   griddep_wait();
-  const int lane = threadIdx.x % 32, pieces = a.D / VEC, chunks = (pieces + 31) / 32;
+  const int lane = threadIdx.x % 32, pieces = a.D / VEC, chunks = (pieces + 32 * kU - 1) / (32 * kU);
   const long long warps = (long long)gridDim.x * 8, me = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const typename V::T* dy = reinterpret_cast<const typename V::T*>(a.dy);
+  const typename V::T* __restrict__ dy = reinterpret_cast<const typename V::T*>(a.dy);
   typename V::T* dw = reinterpret_cast<typename V::T*>(a.dw);
-  auto add = [&](float (&s)[VEC], const P& x) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s[e] += V::get(x.v[e]);
-  };
-  auto piece_of = [&](int token, int c) { return reinterpret_cast<const P*>(dy + (long long)token * a.D) + c; };
-  auto put = [&](long long row, int c, const float (&s)[VEC]) {
-    P x;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) x.v[e] = V::put(a.scale * s[e]);
-    reinterpret_cast<P*>(dw + row * a.D)[c] = x;
-  };
 
   const long long items = (long long)__ldcg(w.head + 2) * chunks;
-  for (long long t = me; t < items; t += warps) {
-    const Item it = w.items[t / chunks];
-    const int chunk = (int)(t % chunks), c = chunk * 32 + lane;
-    float s[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-    const int t0 = lane < it.len ? __ldcg(w.list + it.begin + lane) : 0, t1 = lane + 32 < it.len ? __ldcg(w.list + it.begin + 32 + lane) : 0;
-#pragma unroll 8
-    for (int k = 0; k < it.len; ++k) {
-      const int token = __shfl_sync(0xffffffffu, k < 32 ? t0 : t1, k % 32);
-      if (c < pieces) add(s, *piece_of(token, c));
-    }
-    if (it.part < 0) {
-      if (c < pieces) put(it.row, c, s);
-      continue;
-    }
-    if (c < pieces)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) __stcg(w.part + (long long)it.part * a.D + c * VEC + e, s[e]);
-    __threadfence();
-    __syncwarp();
-    int last = 0;
-    if (lane == 0) last = atomicAdd(w.ticket + (long long)it.ticket * chunks + chunk, 1) == it.items - 1;
-    if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-    __threadfence();
-    if (c >= pieces) continue;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < it.items; ++k)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s[e] += __ldcg(w.part + (long long)(it.first + k) * a.D + c * VEC + e);
-    put(it.row, c, s);
+  Item it{};
+  int t0 = 0, t1 = 0;
+  auto tokens = [&] {  // the item's tokens, one or two to a lane
+    t0 = it.order == kOnly ? it.begin : lane < it.len ? __ldcg(w.list + it.begin + lane) : 0x7fffffff;
+    t1 = lane + 32 < it.len ? __ldcg(w.list + it.begin + 32 + lane) : 0;
+  };
+  if (me < items) {
+    it = w.items[me / chunks];
+    tokens();
   }
-
-  for (long long v = me; v < a.V; v += warps) {
-    const int n = __ldcg(w.count + v);
-    if (n > kFew) continue;  // (an item's)
-    int token = 0;
-    if (n > 0) {  // this row's tokens in ascending order, one to a lane
-      const int at = __ldcg(w.start + v);
-      const int mine = lane < n ? __ldcg(w.list + at + lane) : 0x7fffffff;
-      int place = 0;
-      for (int k = 0; k < n; ++k) place += __shfl_sync(0xffffffffu, mine, k) < mine;
-      for (int k = 0; k < n; ++k) {
-        const int at_k = __shfl_sync(0xffffffffu, place, k), t = __shfl_sync(0xffffffffu, mine, k);
-        if (at_k == lane) token = t;
-      }
-    }
-#pragma unroll 2
-    for (int c0 = 0; c0 < pieces; c0 += 32) {
-      const int c = c0 + lane;
-      float s[VEC];
+  for (long long t = me; t < items; t += warps) {
+    const Item nx = w.items[min(t + warps, items - 1) / chunks];
+    const int chunk = (int)(t % chunks), c0 = chunk * 32 * kU + lane;
+    float s[kU][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const int t = __shfl_sync(0xffffffffu, token, k);
-        if (c < pieces) add(s, *piece_of(t, c));
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[u][e] = 0.f;
+    if (it.order == kAnyOrder) {  // one token to a lane, in ascending order
+      int place = 0;
+      for (int k = 0; k < it.len; ++k) place += __shfl_sync(0xffffffffu, t0, k) < t0;
+      const int mine = t0;
+      for (int k = 0; k < it.len; ++k) {
+        const int to = __shfl_sync(0xffffffffu, place, k), x = __shfl_sync(0xffffffffu, mine, k);
+        if (to == lane) t0 = x;
       }
-      if (c < pieces) put(v, c, s);
     }
+    for (int k = 0; k < it.len; k += kTokens) {
+      P x[kTokens][kU];
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) {
+        if (k + j >= it.len) break;
+        const P* src = reinterpret_cast<const P*>(dy + (long long)__shfl_sync(0xffffffffu, k < 32 ? t0 : t1, (k + j) % 32) * a.D);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) x[j][u] = src[min(c0 + 32 * u, pieces - 1)];  // (lanes past the row's end read it, and store nothing)
+      }
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) {
+        if (k + j >= it.len) break;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) s[u][e] += V::get(x[j][u].v[e]);
+      }
+    }
+    bool whole = true;
+    if (it.part >= 0) {
+      float* part = w.part + (long long)it.part * a.D;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (c0 + 32 * u < pieces)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) __stcg(part + (c0 + 32 * u) * VEC + e, s[u][e]);
+      __threadfence();
+      __syncwarp();
+      int last = 0;
+      if (lane == 0) last = atomicAdd(w.ticket + (long long)it.ticket * chunks + chunk, 1) == it.items - 1;
+      whole = __shfl_sync(0xffffffffu, last, 0);
+      if (whole) __threadfence();
+#pragma unroll
+      for (int u = 0; u < kU && whole; ++u) {
+        const float* from = w.part + (long long)it.first * a.D + min(c0 + 32 * u, pieces - 1) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[u][e] = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < it.items; ++k)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) s[u][e] += __ldcg(from + (long long)k * a.D + e);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (!whole || c0 + 32 * u >= pieces) break;
+      P x;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x.v[e] = V::put(a.scale * s[u][e]);
+      reinterpret_cast<P*>(dw + it.row * (long long)a.D)[c0 + 32 * u] = x;
+    }
+    it = nx;
+    tokens();
   }
 }
 
@@ -345,8 +385,8 @@ int launch_embed(const EmbedArgs* a, cudaStream_t stream) {
   constexpr int W = Value<DT>::kWide;
   const bool wide = a->D % W == 0 && a->ldw % W == 0 && al16(a->w) && al16(a->y);
   const int pieces = wide ? a->D / W : a->D;
-  int lanes = 32;
-  while (lanes < 256 && lanes < pieces) lanes *= 2;
+  int lanes = 8;
+  while (lanes < 256 && 4 * lanes < pieces) lanes *= 2;  // (a thread has four pieces in flight)
   const long long rows = 256 / lanes, blocks = (a->n + rows - 1) / rows;
   const unsigned grid = (unsigned)std::min<long long>(blocks, 1 << 20);
   return (int)(wide ? dfl_host::launch_early(embed_kernel<DT, W>, grid, 256, 0, stream, *a, lanes)
@@ -357,7 +397,7 @@ template <int DT>
 int launch_sum(const EmbedGradArgs* a, const EmbedWs& w, cudaStream_t stream) {
   constexpr int W = Value<DT>::kWide;
   const bool wide = a->D % W == 0 && al16(a->dy) && al16(a->dw);
-  const long long work = a->V + a->n / kFew * ((a->D / (wide ? W : 1) + 31) / 32);
+  const long long work = (a->n + a->n / kFew) * ((a->D / (wide ? W : 1) + 32 * kU - 1) / (32 * kU));  // (at most)
   const unsigned grid = (unsigned)std::min<long long>((work + 7) / 8, 148 * 8);
   return (int)(wide ? dfl_host::launch_early(embed_sum_kernel<DT, W>, grid, 256, 0, stream, *a, w)
                     : dfl_host::launch_early(embed_sum_kernel<DT, 1>, grid, 256, 0, stream, *a, w));
@@ -379,10 +419,13 @@ extern "C" long long dfl_embed_grad_ws(long long n, long long V, int D) { return
 
 extern "C" int dfl_embed_grad(const EmbedGradArgs* a, cudaStream_t stream) {
   if (a->n <= 0 || a->D <= 0 || a->V <= 0 || a->n >= (1ll << 30) || a->V >= (1ll << 30) || (a->id_bytes != 4 && a->id_bytes != 8)) return -2;
-  if (!al16(a->ws)) return -3;
+  if (!al16(a->ws) || !al16(a->dw)) return -3;
   EmbedWs w;
   if (embed_layout(a->n, a->V, a->D, reinterpret_cast<char*>(a->ws), &w) > a->ws_bytes) return -4;
-  const cudaError_t e = dfl_host::launch_early(embed_sort_kernel, kCluster, kSortThreads, 0, stream, *a, w);
+  // (14 clusters for the zeros; fewer where dW is small)
+  const long long fill = (a->V * a->D * (a->dtype == kDtypeF32 ? 4 : 2) + 16 * kCluster * kSortThreads - 1) / (16 * kCluster * kSortThreads);
+  const unsigned clusters = 1 + (unsigned)std::min<long long>(fill, 14);
+  const cudaError_t e = dfl_host::launch_early(embed_sort_kernel, clusters * kCluster, kSortThreads, 0, stream, *a, w);
   if (e != cudaSuccess) return (int)e;
   switch (a->dtype) {
     case kDtypeF32: return launch_sum<kDtypeF32>(a, w, stream);

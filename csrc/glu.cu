@@ -13,8 +13,10 @@
 //   dx       the K loop runs over dg Wg, then du Wu, in one accumulator; the weights are read as they lie ([F, K]: the
 //            second operand with its columns contiguous)
 //   dW       both operands lie with their columns contiguous ([M, F] and [M, K]); nothing is transposed in memory
-// Tiles of 256 x 256 by CTA pairs, or 128 x 128 by single CTAs where those fill the SMs better (glu_plan).
+// Tiles of 256 x 256 by CTA pairs, of 128 x 256 or of 128 x 128 by single CTAs; what is left after whole rounds of tiles may be
+// split along the sum, the parts added by a kernel behind (glu_plan).
 #include <algorithm>
+#include <cstdlib>
 #include <cstring>
 
 #include <cuda_fp16.h>
@@ -28,12 +30,19 @@ using namespace dfl;
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
 
-constexpr int BM = 128, BK = 64, STAGES = 6, kThreads = 192;
-constexpr int kOpBytes = 128 * BK * 2;  // each CTA loads 128 rows (or columns) of both operands per stage
-constexpr int kStageBytes = 2 * kOpBytes;
-constexpr int kBarOff = STAGES * kStageBytes;
-constexpr int kSmem = kBarOff + (2 * STAGES + 4) * 8 + 16 + 1024;
-static_assert(kSmem <= 232448, "shared memory budget");
+constexpr int BM = 128, BK = 64, kThreads = 192;
+// CG: CTAs per tile (2: a pair).  A tile is 128 CG rows and BN accumulator columns; each CTA loads 128 rows of the first operand
+// and BN / CG rows (or columns) of the second per stage.
+template <int CG, int BN>
+struct Cfg {
+  static constexpr int kA = BM * BK * 2, kCols = BN / CG, kB = kCols * BK * 2, kStage = kA + kB;
+  static constexpr int kStages = kStage > 32768 ? 4 : 6;
+  static constexpr int kBarOff = kStages * kStage;
+  static constexpr int kRowsOff = (kBarOff + (2 * kStages + 4) * 8 + 16 + 15) / 16 * 16;  // 32 x 33 16-bit values per epilogue warp
+  static constexpr int kSmem = kRowsOff + 4 * 32 * 33 * 2 + 1024;
+  static_assert(kSmem <= 232448, "shared memory budget");
+};
+constexpr int kChunk = 64 * BK * 2;  // 64 columns of an operand whose columns are contiguous
 constexpr int kGroupM = 16;  // tile raster: 16 M blocks per group, for L2 reuse
 
 struct GluParams {
@@ -42,9 +51,11 @@ struct GluParams {
   void* g;           // forward: the kept projections
   void* u;
   long long ldd, lds;
-  float* ws;         // dx: partial sums [splits][M][N]
   int M, N, K;       // of one problem: rows and columns of the output, length of the sums (of each segment)
-  int num_m, num_n, tiles, splits;
+  int num_m, num_n, tiles;  // tiles of one problem
+  // Items: `whole` tiles, then the rest of them in `splits` parts each, whose sums go to ws [tile of the rest][part][row][column].
+  int whole, splits, items;
+  float* ws;
   int act;
 };
 
@@ -103,37 +114,51 @@ template <int MODE>
 DFL_DEVICE int k_blocks(const GluParams& p) { return (p.K + BK - 1) / BK * (MODE == kDx ? 2 : 1); }
 
 struct Tile {
-  int which, mb, nb, split, kb0, kb1;
+  int which, mb, nb, kb0, kb1;
+  int part;  // of the rest's sums, -1: the whole sum
 };
 template <int MODE>
 DFL_DEVICE Tile tile_of(const GluParams& p, int t) {
   Tile r;
-  r.split = t % p.splits;
-  t /= p.splits;
+  const int n = k_blocks<MODE>(p);
+  r.part = -1, r.kb0 = 0, r.kb1 = n;
+  if (t >= p.whole && p.splits > 1) {
+    r.part = t - p.whole;
+    const int s = r.part % p.splits, per = (n + p.splits - 1) / p.splits;
+    t = p.whole + r.part / p.splits;
+    r.kb0 = min(n, s * per), r.kb1 = min(n, r.kb0 + per);
+  }
   r.which = t / p.tiles;
   t -= r.which * p.tiles;
   const int group = t / (kGroupM * p.num_n), first = group * kGroupM, gm = min(kGroupM, p.num_m - first);
   t -= group * kGroupM * p.num_n;
   r.mb = first + t % gm, r.nb = t / gm;
-  const int n = k_blocks<MODE>(p), per = (n + p.splits - 1) / p.splits;
-  r.kb0 = min(n, r.split * per), r.kb1 = min(n, r.kb0 + per);
   return r;
 }
 
-// 32 columns of a row: whole 16-byte pieces where the row allows it.
+// 32 columns of the rows of a warp (lane: row): whole 16-byte pieces where every row allows it, else through shared memory, so that
+// the lanes write along a row (a row each would cost a line per lane and value).
 template <bool F16>
-DFL_DEVICE void store_cols(void* base, long long at, const float (&v)[32], int cols, bool wide) {
+DFL_DEVICE void store_cols(void* base, long long row0, int rows, long long ld, int col, const float (&v)[32], int cols, bool wide,
+                           uint16_t (*stage)[33]) {
+  const int lane = threadIdx.x % 32;
+  uint32_t w[16];
+#pragma unroll
+  for (int q = 0; q < 16; ++q) w[q] = pack2<F16>(v[2 * q], v[2 * q + 1]);
   if (wide && cols >= 32) {
-    uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + at);
+    uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + (row0 + lane) * ld + col);
+    if (lane < rows)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      d[q] = make_uint4(pack2<F16>(v[8 * q], v[8 * q + 1]), pack2<F16>(v[8 * q + 2], v[8 * q + 3]),
-                        pack2<F16>(v[8 * q + 4], v[8 * q + 5]), pack2<F16>(v[8 * q + 6], v[8 * q + 7]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < cols) store1<F16>(base, at + j, v[j]);
+      for (int q = 0; q < 4; ++q) d[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    return;
   }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 16; ++q) stage[lane][2 * q] = (uint16_t)w[q], stage[lane][2 * q + 1] = (uint16_t)(w[q] >> 16);
+  __syncwarp();
+  uint16_t* d = reinterpret_cast<uint16_t*>(base) + row0 * ld + col + lane;
+  if (lane < cols)
+    for (int r = 0; r < rows; ++r) d[r * ld] = stage[r][lane];
 }
 
 template <int CG>
@@ -142,14 +167,14 @@ DFL_DEVICE void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, i
   else tma_load_2d(dst, map, bar, c0, c1);
 }
 
-// CG: CTAs per tile (2: a pair).  A tile is 128 CG rows and 128 CG accumulator columns.
-template <int MODE, int CG, bool F16>
+template <int MODE, int CG, int BN, bool F16>
 __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant__ GluParams p, int* err) {
-  constexpr int BN = 128 * CG;
+  using C = Cfg<CG, BN>;
+  constexpr int STAGES = C::kStages;
   constexpr uint32_t kTmemCols = 2 * BN;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kBarOff);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -159,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
-  const int items = p.tiles * (MODE == kDw ? (p.d[1] ? 2 : 1) : 1) * p.splits;
+  const int items = p.items;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -206,10 +231,10 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
             ok = false;
             break;
           }
-          uint8_t* sa = smem + stage * kStageBytes;
-          uint8_t* sb = sa + kOpBytes;
+          uint8_t* sa = smem + stage * C::kStage;
+          uint8_t* sb = sa + C::kA;
           uint64_t* bar = &full_bar[stage];
-          if (rank == 0) mbar_arrive_expect_tx(bar, CG * kStageBytes);
+          if (rank == 0) mbar_arrive_expect_tx(bar, CG * C::kStage);
           const int m0 = it.mb * BM * CG + (int)rank * BM;
           if constexpr (MODE == kForward) {
             load_tile<CG>(sa, &p.a[0], bar, kb * BK, m0);
@@ -218,20 +243,20 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
               load_tile<CG>(sb, &p.b[rank], bar, kb * BK, n0);
             } else {
               load_tile<CG>(sb, &p.b[0], bar, kb * BK, n0);
-              load_tile<CG>(sb + kOpBytes / 2, &p.b[1], bar, kb * BK, n0);
+              load_tile<CG>(sb + C::kB / 2, &p.b[1], bar, kb * BK, n0);
             }
           } else if constexpr (MODE == kDx) {
             const int half = (p.K + BK - 1) / BK, seg = kb >= half, k0 = (kb - seg * half) * BK;
-            const int n0 = it.nb * BN + (int)rank * 128;
             load_tile<CG>(sa, &p.a[seg], bar, k0, m0);
-            load_tile<CG>(sb, &p.b[seg], bar, n0, k0);
-            load_tile<CG>(sb + kOpBytes / 2, &p.b[seg], bar, n0 + 64, k0);
+#pragma unroll
+            for (int c = 0; c < C::kCols / 64; ++c)
+              load_tile<CG>(sb + c * kChunk, &p.b[seg], bar, it.nb * BN + (int)rank * C::kCols + 64 * c, k0);
           } else {
-            const int n0 = it.nb * BN + (int)rank * 128;
             load_tile<CG>(sa, &p.a[it.which], bar, m0, kb * BK);
-            load_tile<CG>(sa + kOpBytes / 2, &p.a[it.which], bar, m0 + 64, kb * BK);
-            load_tile<CG>(sb, &p.b[0], bar, n0, kb * BK);
-            load_tile<CG>(sb + kOpBytes / 2, &p.b[0], bar, n0 + 64, kb * BK);
+            load_tile<CG>(sa + kChunk, &p.a[it.which], bar, m0 + 64, kb * BK);
+#pragma unroll
+            for (int c = 0; c < C::kCols / 64; ++c)
+              load_tile<CG>(sb + c * kChunk, &p.b[0], bar, it.nb * BN + (int)rank * C::kCols + 64 * c, kb * BK);
           }
           issued |= 1 << stage;
           issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
@@ -251,9 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
       constexpr uint32_t kF16Bits = F16 ? (1u << 7) | (1u << 10) : 0u;  // clears the two bf16 format bits
       constexpr uint32_t idesc = make_idesc_bf16_f32(BM * CG, BN, a_mn, b_mn) & ~kF16Bits;
       // K-major: rows of 64 K values, 16 of them 32 bytes apart.  MN-major: chunks of 64 columns, 64 rows of K each;
-      // 16 rows are 2048 bytes, the next chunk is kOpBytes / 2 away.
+      // 16 rows are 2048 bytes.
       auto desc = [](uint32_t addr, int k, bool mn) {
-        return mn ? make_sdesc_sw128(addr + k * 2048, kOpBytes / 2, 1024) : make_sdesc_sw128(addr + k * 32, 16, 1024);
+        return mn ? make_sdesc_sw128(addr + k * 2048, kChunk, 1024) : make_sdesc_sw128(addr + k * 32, 16, 1024);
       };
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -269,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(smem + stage * kStageBytes), b_addr = a_addr + kOpBytes;
+          const uint32_t a_addr = smem_u32(smem + stage * C::kStage), b_addr = a_addr + C::kA;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
             const uint32_t more = (kb > it.kb0 || k > 0) ? 1u : 0u;
@@ -292,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     }
   } else {
     const int sub = warp & 3;  // the tensor-memory lane quarter that this warp may read
+    uint16_t(*stage_rows)[33] = reinterpret_cast<uint16_t(*)[33]>(smem + C::kRowsOff) + 32 * sub;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = first; t < items; t += step) {
@@ -305,7 +331,19 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
         if (CG == 1 || rank == 0) mbar_arrive(&tempty_bar[acc]);
         else mbar_arrive_cta0(&tempty_bar[acc]);
       };
-      if constexpr (MODE == kForward) {
+      const int row0 = row - lane, rows = min(32, p.M - row0);  // the warp's
+      if (it.part >= 0) {  // sums of a part: the whole tile, whatever lies outside
+        float* part = p.ws + (long long)it.part * (BM * CG * BN) + ((int)rank * BM + sub * 32 + lane) * BN;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tbase + c, r);
+          tmem_wait_ld();
+          if (c + 32 == BN) release();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) reinterpret_cast<uint4*>(part + c)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+        }
+      } else if constexpr (MODE == kForward) {
         const bool wide = p.ldd % 8 == 0 && (reinterpret_cast<uintptr_t>(p.d[0]) & 15) == 0;
 #pragma unroll 1
         for (int c = 0; c < BN / 2; c += 32) {
@@ -315,13 +353,13 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
           tmem_wait_ld();
           if (c + 32 == BN / 2) release();
           const int col = it.nb * (BN / 2) + c, cols = p.N - col;
-          if (row >= p.M || cols <= 0) continue;
+          if (rows <= 0 || cols <= 0) continue;
           float g[32], u[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) g[j] = __uint_as_float(gr[j]), u[j] = __uint_as_float(ur[j]);
           if (p.g) {
-            store_cols<F16>(p.g, row * p.lds + col, g, cols, true);
-            store_cols<F16>(p.u, row * p.lds + col, u, cols, true);
+            store_cols<F16>(p.g, row0, rows, p.lds, col, g, cols, true, stage_rows);
+            store_cols<F16>(p.u, row0, rows, p.lds, col, u, cols, true, stage_rows);
           }
           if (p.act == kGluSilu) {
 #pragma unroll
@@ -333,10 +371,9 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 32; ++j) u[j] *= act_of<kGluGeluErf>(g[j]);
           }
-          store_cols<F16>(p.d[0], row * p.ldd + col, u, cols, wide);
+          store_cols<F16>(p.d[0], row0, rows, p.ldd, col, u, cols, wide, stage_rows);
         }
       } else {
-        const bool none = it.kb0 >= it.kb1;  // (a sum over nothing)
 #pragma unroll 1
         for (int c = 0; c < BN; c += 32) {
           uint32_t r[32];
@@ -344,18 +381,11 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
           tmem_wait_ld();
           if (c + 32 == BN) release();
           const int col = it.nb * BN + c, cols = p.N - col;
-          if (row >= p.M || cols <= 0) continue;
+          if (rows <= 0 || cols <= 0) continue;
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : __uint_as_float(r[j]);
-          if (MODE == kDx && p.splits > 1) {  // N is a multiple of 8
-            float4* d = reinterpret_cast<float4*>(p.ws + ((long long)it.split * p.M + row) * p.N + col);
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (4 * q < cols) d[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-          } else {
-            store_cols<F16>(p.d[it.which], row * p.ldd + col, v, cols, true);
-          }
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          store_cols<F16>(p.d[it.which], row0, rows, p.ldd, col, v, cols, true, stage_rows);
         }
       }
       acc ^= 1;
@@ -375,17 +405,132 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
   }
 }
 
-// dx from its partial sums, added in order.
+// ---------------------------------------------------------------------------
+// Few rows: bound by reading both weights once (4 F K bytes).  A CTA of 8 warps owns 16 output columns; its warps take 128-wide
+// pieces of K in turn and multiply on the warp-level m16n8k16 instruction, the weights' rows as the 16-row operand
+// straight from global memory (both operands in the same permuted K order, so that a lane loads 16 contiguous bytes).  The
+// warps' sums are added in their order.
+// ---------------------------------------------------------------------------
+constexpr int kRowsMax = 32;
+
 template <bool F16>
-__global__ void __launch_bounds__(256) glu_join_kernel(const float* ws, void* dx, long long n, int splits) {
+DFL_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+DFL_DEVICE uint4 ld_once(const uint16_t* p) {  // read once: no L1 allocation
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+  return r;
+}
+
+// NB: groups of 8 rows.
+template <int NB, bool F16>
+__global__ void __launch_bounds__(256, NB == 4 ? 1 : 2) glu_rows_kernel(GluArgs a) {
+  constexpr int U = NB == 4 ? 2 : 4;  // pieces of 32 K values in flight
+  __shared__ float red[8][2][16][8 * NB + 1];
   griddep_wait();
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
-    float4 s = __ldcg(reinterpret_cast<const float4*>(ws + i));
-    for (int k = 1; k < splits; ++k) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(ws + k * n + i));
-      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = lane / 4, t = lane % 4;
+  const int n0 = blockIdx.x * 16, r0 = min(n0 + quad, a.F - 1), r1 = min(n0 + quad + 8, a.F - 1);
+  const uint16_t* w[4] = {reinterpret_cast<const uint16_t*>(a.wg) + r0 * a.ldwg, reinterpret_cast<const uint16_t*>(a.wg) + r1 * a.ldwg,
+                          reinterpret_cast<const uint16_t*>(a.wu) + r0 * a.ldwu, reinterpret_cast<const uint16_t*>(a.wu) + r1 * a.ldwu};
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x);
+  float c[2][NB][4];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int g = 0; g < NB; ++g) c[s][g][0] = c[s][g][1] = c[s][g][2] = c[s][g][3] = 0.f;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  for (int k0 = warp * 32 * U; k0 < a.K; k0 += 8 * 32 * U) {
+    uint4 v[U][4], b[U][NB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + 32 * u + 8 * t;  // K is a multiple of 8: a lane's piece is inside or outside
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u][i] = k < a.K ? ld_once(w[i] + k) : zero;
     }
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(dx) + i) = make_uint2(pack2<F16>(s.x, s.y), pack2<F16>(s.z, s.w));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + 32 * u + 8 * t;
+#pragma unroll
+      for (int g = 0; g < NB; ++g)
+        b[u][g] = k < a.K && 8 * g + quad < a.M ? __ldcg(reinterpret_cast<const uint4*>(x + (8 * g + quad) * a.ldx + k)) : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int g = 0; g < NB; ++g)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          mma16816<F16>(c[s][g], v[u][2 * s].x, v[u][2 * s + 1].x, v[u][2 * s].y, v[u][2 * s + 1].y, b[u][g].x, b[u][g].y);
+          mma16816<F16>(c[s][g], v[u][2 * s].z, v[u][2 * s + 1].z, v[u][2 * s].w, v[u][2 * s + 1].w, b[u][g].z, b[u][g].w);
+        }
+  }
+  // c[s][g][2 i + e]: column quad + 8 i of the gate (s = 0) or the other projection, row 8 g + 2 t + e
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int g = 0; g < NB; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[warp][s][quad + 8 * (i / 2)][8 * g + 2 * t + i % 2] = c[s][g][i];
+  __syncthreads();
+  const int n = threadIdx.x % 16, col = n0 + n;
+  if (col >= a.F) return;
+  for (int m = threadIdx.x / 16; m < a.M; m += 16) {
+    float g = 0.f, u = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g += red[k][0][n][m], u += red[k][1][n][m];
+    if (a.g) store1<F16>(a.g, m * a.lds + col, g), store1<F16>(a.u, m * a.lds + col, u);
+    const float v = a.act == kGluSilu ? act_of<kGluSilu>(g) : a.act == kGluGelu ? act_of<kGluGelu>(g) : act_of<kGluGeluErf>(g);
+    store1<F16>(a.h, m * a.ldh + col, v * u);
+  }
+}
+
+template <bool F16>
+int launch_rows(const GluArgs* a, cudaStream_t stream) {
+  const auto kern = a->M <= 8 ? glu_rows_kernel<1, F16> : a->M <= 16 ? glu_rows_kernel<2, F16> : glu_rows_kernel<4, F16>;
+  return (int)dfl_host::launch_early(kern, (unsigned)((a->F + 15) / 16), 256, 0, stream, *a);
+}
+
+// The rest's tiles from their parts, added in order: a thread takes 4 columns of a row.
+template <int MODE, bool F16>
+__global__ void __launch_bounds__(256) glu_join_kernel(const __grid_constant__ GluParams p, int rows, int BN, int rest) {
+  griddep_wait();
+  const int cols = MODE == kForward ? BN / 2 : BN, quads = cols / 4;
+  const long long n = (long long)rest * rows * quads, tile = (long long)rows * BN;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int q = (int)(i % quads) * 4, r = (int)(i / quads % rows), t = (int)(i / quads / rows);
+    const Tile it = tile_of<MODE>(p, p.whole + t * p.splits);
+    const int row = it.mb * rows + r, col = it.nb * cols + q;
+    if (row >= p.M || col >= p.N) continue;
+    const float* from = p.ws + (long long)t * p.splits * tile + (long long)r * BN + q;
+    float v[2][4] = {};
+    for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+      for (int h = 0; h < (MODE == kForward ? 2 : 1); ++h) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(from + s * tile + h * cols));
+        v[h][0] += x.x, v[h][1] += x.y, v[h][2] += x.z, v[h][3] += x.w;
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (col + e >= p.N) break;
+      if constexpr (MODE == kForward) {
+        const float g = v[0][e], u = v[1][e];
+        if (p.g) store1<F16>(p.g, row * p.lds + col + e, g), store1<F16>(p.u, row * p.lds + col + e, u);
+        const float a = p.act == kGluSilu ? act_of<kGluSilu>(g) : p.act == kGluGelu ? act_of<kGluGelu>(g) : act_of<kGluGeluErf>(g);
+        store1<F16>(p.d[0], row * p.ldd + col + e, a * u);
+      } else {
+        store1<F16>(p.d[it.which], row * p.ldd + col + e, v[0][e]);
+      }
+    }
   }
 }
 
@@ -432,28 +577,69 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// CTAs per tile: pairs take 256 x 256 in the time (per K block) that a single CTA needs for about 1.6 tiles of 128 x 128;
-// whichever needs fewer rounds' time.
-int glu_ctas(long long rows, long long cols, int problems, int sms) {
-  auto tiles = [&](int n) { return ((rows + n - 1) / n) * ((cols + n - 1) / n) * problems; };
-  const long long pairs = (tiles(256) + sms / 2 - 1) / (sms / 2), singles = (tiles(128) + sms - 1) / sms;
-  return pairs * 16 <= singles * 10 ? 2 : 1;
+// How a product is laid out.  Per K block an SM needs (cycles): a pair's 256 x 256 tile 560 (its products: 524), a 128 x 256 tile
+// 750 and a 128 x 128 tile 512 (both bound by the copies: 48 and 32 KB).  What is left after whole rounds is split along the
+// sum where that is shorter: every part of a tile costs its sums' way through L2, the join a launch.
+struct Plan {
+  int cg, bn, whole, splits;
+};
+template <int MODE>
+Plan glu_plan(long long rows, long long cols, int problems, int blocks, int sms) {
+  static const int force = getenv("GLU_FORCE") ? atoi(getenv("GLU_FORCE")) : 0;
+  static const int nosplit = getenv("GLU_NOSPLIT") ? 1 : 0;
+  struct Shape {
+    int cg, bn;
+    double block;
+  };
+  constexpr Shape shapes[3] = {{2, 256, 560.}, {1, 256, 750.}, {1, 128, 512.}};
+  Plan best{};
+  double least = 0.;
+  int idx = 0;
+  for (const Shape& s : shapes) {
+    if (++idx != force && force) continue;
+    const int width = MODE == kForward ? s.bn / 2 : s.bn;
+    const long long tiles = (rows + 128 * s.cg - 1) / (128 * s.cg) * ((cols + width - 1) / width) * problems, slots = sms / s.cg;
+    const long long rounds = tiles / slots, rest = tiles % slots;
+    const auto take = [&](long long whole, int splits, double cost) {
+      if (best.cg == 0 || cost < least) best = Plan{s.cg, s.bn, (int)whole, splits}, least = cost;
+    };
+    take(tiles, 1, (double)(rounds + (rest > 0)) * blocks * s.block);
+    if (rest == 0 || nosplit) continue;
+    for (int n = 2; n <= slots / rest && blocks / n >= 4 && n <= 32; ++n)
+      if ((n - 1) * ((blocks + n - 1) / n) < blocks)  // (every part holds something)
+      take(rounds * slots, n, (rounds * blocks + (blocks + n - 1) / n) * s.block + 6000. + rest * n * 128. * s.cg * s.bn * 8 / 2600.);
+  }
+  return best;
 }
 
-template <int MODE, int CG, bool F16>
-int launch_glu(const GluParams& p, int problems, int sms, int dev, int* err, cudaStream_t stream) {
-  auto kern = glu_kernel<MODE, CG, F16>;
+template <int MODE>
+int setup(GluParams& p, const Plan& plan, int problems) {
+  const long long width = MODE == kForward ? plan.bn / 2 : plan.bn, m = ((long long)p.M + 128 * plan.cg - 1) / (128 * plan.cg),
+                  n = (p.N + width - 1) / width;
+  if (m * n * problems > (1 << 28)) return -9;
+  p.num_m = (int)m, p.num_n = (int)n, p.tiles = (int)(m * n);
+  p.whole = plan.whole, p.splits = plan.splits;
+  p.items = p.whole + (p.tiles * problems - p.whole) * p.splits;
+  return 0;
+}
+long long ws_floats(const Plan& plan, long long items) {
+  return plan.splits > 1 ? (items - plan.whole) * 128ll * plan.cg * plan.bn : 0;
+}
+
+template <int MODE, int CG, int BN, bool F16>
+int launch_glu(const GluParams& p, int sms, int dev, int* err, cudaStream_t stream) {
+  auto kern = glu_kernel<MODE, CG, BN, F16>;
+  constexpr int smem = Cfg<CG, BN>::kSmem;
   static bool attr[16] = {false};
   if (!attr[dev & 15]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     attr[dev & 15] = true;
   }
-  const long long items = (long long)p.tiles * problems * p.splits, slots = sms / CG;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CG * std::min(items, slots)), 1, 1);
+  cfg.gridDim = dim3((unsigned)(CG * std::min(p.items, sms / CG)), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -463,47 +649,67 @@ int launch_glu(const GluParams& p, int problems, int sms, int dev, int* err, cud
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = CG == 2 ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, kern, p, err);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, err);
+  if (e != cudaSuccess || p.splits == 1) return (int)e;
+  const int rest = (p.items - p.whole) / p.splits;
+  const long long threads = (long long)rest * BM * CG * (MODE == kForward ? BN / 8 : BN / 4);
+  return (int)dfl_host::launch_early(glu_join_kernel<MODE, F16>, (unsigned)std::min<long long>((threads + 255) / 256, 148 * 8), 256, 0, stream, p,
+                                     BM * CG, BN, rest);
 }
 
 template <int MODE>
-int launch_mode(const GluParams& p, int cg, int f16, int problems, int sms, int dev, int* err, cudaStream_t stream) {
-  if (cg == 2)
-    return f16 ? launch_glu<MODE, 2, true>(p, problems, sms, dev, err, stream)
-               : launch_glu<MODE, 2, false>(p, problems, sms, dev, err, stream);
-  return f16 ? launch_glu<MODE, 1, true>(p, problems, sms, dev, err, stream)
-             : launch_glu<MODE, 1, false>(p, problems, sms, dev, err, stream);
+int launch_mode(const GluParams& p, const Plan& plan, int f16, int sms, int dev, int* err, cudaStream_t stream) {
+  if (p.splits > 1 && !p.ws) return -10;
+  if (plan.cg == 2) return f16 ? launch_glu<MODE, 2, 256, true>(p, sms, dev, err, stream) : launch_glu<MODE, 2, 256, false>(p, sms, dev, err, stream);
+  if (plan.bn == 256) return f16 ? launch_glu<MODE, 1, 256, true>(p, sms, dev, err, stream) : launch_glu<MODE, 1, 256, false>(p, sms, dev, err, stream);
+  return f16 ? launch_glu<MODE, 1, 128, true>(p, sms, dev, err, stream) : launch_glu<MODE, 1, 128, false>(p, sms, dev, err, stream);
 }
 
-int tiles_of(GluParams& p, int cg, int cols) {
-  const long long m = ((long long)p.M + 128 * cg - 1) / (128 * cg), n = ((long long)p.N + cols - 1) / cols;
-  if (m * n > (1 << 28)) return -9;
-  p.num_m = (int)m, p.num_n = (int)n, p.tiles = (int)(m * n);
-  return 0;
-}
+int blocks_of(int K) { return (K + BK - 1) / BK; }
+Plan plan_forward(int M, int K, int F, int sms) { return glu_plan<kForward>(M, F, 1, blocks_of(K), sms); }
+Plan plan_dx(int M, int K, int F, int sms) { return glu_plan<kDx>(M, K, 1, 2 * blocks_of(F), sms); }
+Plan plan_dw(int M, int K, int F, int problems, int sms) { return glu_plan<kDw>(F, K, problems, blocks_of(M), sms); }
 
 }  // namespace
+
+// Floats that a call's parts take; what: 0 forward, 1 dx, 2 dW of both weights, 3 of one.
+extern "C" long long dfl_glu_ws(int what, int M, int K, int F) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = dfl_host::num_sms(dev);
+  if (what == 0 && M <= kRowsMax) return 0;
+  const Plan plan = what == 0 ? plan_forward(M, K, F, sms) : what == 1 ? plan_dx(M, K, F, sms) : plan_dw(M, K, F, what == 2 ? 2 : 1, sms);
+  GluParams p{};
+  p.M = what >= 2 ? F : M, p.N = what == 0 ? F : K;
+  const int rc = what == 0 ? setup<kForward>(p, plan, 1) : what == 1 ? setup<kDx>(p, plan, 1) : setup<kDw>(p, plan, what == 2 ? 2 : 1);
+  return rc ? 0 : ws_floats(plan, p.items);
+}
 
 extern "C" int dfl_glu(const GluArgs* a, cudaStream_t stream) {
   if (a->M <= 0 || a->F <= 0 || a->K <= 0 || a->K % 8 || a->act < 0 || a->act > kGluGeluErf) return -2;
   if (!al16(a->x) || !al16(a->wg) || !al16(a->wu) || (a->ldx | a->ldwg | a->ldwu) % 8) return -3;
   if (a->g && (!a->u || !al16(a->g) || !al16(a->u) || a->lds % 8 || a->lds < a->F)) return -4;
+  if (a->M <= kRowsMax) return a->f16 ? launch_rows<true>(a, stream) : launch_rows<false>(a, stream);
   int dev = 0;
   cudaGetDevice(&dev);
-  const int sms = dfl_host::num_sms(dev), cg = glu_ctas(a->M, 2ll * a->F, 1, sms);
+  const int sms = dfl_host::num_sms(dev);
+  const Plan plan = plan_forward(a->M, a->K, a->F, sms);
   GluParams p;
   std::memset(&p, 0, sizeof(p));
   int rc = dfl_host::make_tmap_2d_bf16(&p.a[0], a->x, a->K, a->M, a->ldx, BK, BM, true);
   if (rc) return 1000 + rc;
-  rc = dfl_host::make_tmap_2d_bf16(&p.b[0], a->wg, a->K, a->F, a->ldwg, BK, 64 * cg, true);
+  rc = dfl_host::make_tmap_2d_bf16(&p.b[0], a->wg, a->K, a->F, a->ldwg, BK, plan.bn / 2, true);
   if (rc) return 2000 + rc;
-  rc = dfl_host::make_tmap_2d_bf16(&p.b[1], a->wu, a->K, a->F, a->ldwu, BK, 64 * cg, true);
+  rc = dfl_host::make_tmap_2d_bf16(&p.b[1], a->wu, a->K, a->F, a->ldwu, BK, plan.bn / 2, true);
   if (rc) return 3000 + rc;
   p.d[0] = a->h, p.ldd = a->ldh;
   p.g = a->g, p.u = a->u, p.lds = a->lds;
-  p.M = a->M, p.N = a->F, p.K = a->K, p.splits = 1, p.act = a->act;
-  rc = tiles_of(p, cg, 64 * cg);
-  return rc ? rc : launch_mode<kForward>(p, cg, a->f16, 1, sms, dev, a->err, stream);
+  p.M = a->M, p.N = a->F, p.K = a->K, p.act = a->act;
+  rc = setup<kForward>(p, plan, 1);
+  if (rc) return rc;
+  if (ws_floats(plan, p.items) > a->ws_floats || !al16(a->ws)) return -10;
+  p.ws = a->ws;
+  return launch_mode<kForward>(p, plan, a->f16, sms, dev, a->err, stream);
 }
 
 extern "C" int dfl_glu_grad(const GluGradArgs* a, cudaStream_t stream) {
@@ -524,15 +730,14 @@ static int check_gemm(const GluGemmArgs* a) {
   return 0;
 }
 
-extern "C" long long dfl_glu_dx_ws(int M, int K, int F) { return 0; }
-
 extern "C" int dfl_glu_dx(const GluGemmArgs* a, cudaStream_t stream) {
   int rc = check_gemm(a);
   if (rc) return rc;
   if (!al16(a->wg) || !al16(a->wu) || !al16(a->dx) || (a->ldwg | a->ldwu) % 8) return -3;
   int dev = 0;
   cudaGetDevice(&dev);
-  const int sms = dfl_host::num_sms(dev), cg = glu_ctas(a->M, a->K, 1, sms);
+  const int sms = dfl_host::num_sms(dev);
+  const Plan plan = plan_dx(a->M, a->K, a->F, sms);
   GluParams p;
   std::memset(&p, 0, sizeof(p));
   for (int i = 0; i < 2; ++i) {
@@ -542,9 +747,12 @@ extern "C" int dfl_glu_dx(const GluGemmArgs* a, cudaStream_t stream) {
     if (rc) return 2000 + rc;
   }
   p.d[0] = a->dx, p.ldd = a->K;
-  p.M = a->M, p.N = a->K, p.K = a->F, p.splits = 1;
-  rc = tiles_of(p, cg, 128 * cg);
-  return rc ? rc : launch_mode<kDx>(p, cg, a->f16, 1, sms, dev, a->err, stream);
+  p.M = a->M, p.N = a->K, p.K = a->F;
+  rc = setup<kDx>(p, plan, 1);
+  if (rc) return rc;
+  if (ws_floats(plan, p.items) > a->ws_floats || !al16(a->ws)) return -10;
+  p.ws = a->ws;
+  return launch_mode<kDx>(p, plan, a->f16, sms, dev, a->err, stream);
 }
 
 extern "C" int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream) {
@@ -553,7 +761,8 @@ extern "C" int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream) {
   if (!al16(a->x) || a->ldx % 8 || !al16(a->dwg) || !al16(a->dwu) || (!a->dwg && !a->dwu)) return -3;
   int dev = 0;
   cudaGetDevice(&dev);
-  const int problems = a->dwg && a->dwu ? 2 : 1, sms = dfl_host::num_sms(dev), cg = glu_ctas(a->F, a->K, problems, sms);
+  const int problems = a->dwg && a->dwu ? 2 : 1, sms = dfl_host::num_sms(dev);
+  const Plan plan = plan_dw(a->M, a->K, a->F, problems, sms);
   GluParams p;
   std::memset(&p, 0, sizeof(p));
   int n = 0;
@@ -567,7 +776,10 @@ extern "C" int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream) {
   rc = dfl_host::make_tmap_2d_bf16(&p.b[0], a->x, a->K, a->M, a->ldx, 64, BK, true);
   if (rc) return 2000 + rc;
   p.ldd = a->K;
-  p.M = a->F, p.N = a->K, p.K = a->M, p.splits = 1;
-  rc = tiles_of(p, cg, 128 * cg);
-  return rc ? rc : launch_mode<kDw>(p, cg, a->f16, problems, sms, dev, a->err, stream);
+  p.M = a->F, p.N = a->K, p.K = a->M;
+  rc = setup<kDw>(p, plan, problems);
+  if (rc) return rc;
+  if (ws_floats(plan, p.items) > a->ws_floats || !al16(a->ws)) return -10;
+  p.ws = a->ws;
+  return launch_mode<kDw>(p, plan, a->f16, sms, dev, a->err, stream);
 }

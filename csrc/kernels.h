@@ -507,6 +507,7 @@ typedef struct GluArgs {
   void* h; long long ldh;                         // [M, F]
   void* g; void* u; long long lds;                // [M, F] or NULL
   int M, K, F, act, f16;
+  float* ws; long long ws_floats;                 // dfl_glu_ws(0, ...) or NULL
   int* err;
 } GluArgs;
 int dfl_glu(const GluArgs* a, cudaStream_t stream);
@@ -524,13 +525,14 @@ typedef struct GluGemmArgs {
   const void* x; const void* wg; const void* wu;
   long long ldx, ldwg, ldwu;
   void* dx; void* dwg; void* dwu;                 // contiguous
-  float* ws; long long ws_floats;                 // partial sums of dx (dfl_glu_dx_ws) or NULL
+  float* ws; long long ws_floats;                 // dfl_glu_ws or NULL
   int M, K, F, f16;
   int* err;
 } GluGemmArgs;
 int dfl_glu_dx(const GluGemmArgs* a, cudaStream_t stream);
 int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream);
-long long dfl_glu_dx_ws(int M, int K, int F);     // floats
+// Floats of a call's partial sums: forward (what = 0), dx (1), dW of both weights (2) or of one (3).
+long long dfl_glu_ws(int what, int M, int K, int F);
 
 // ------------------------------------------------------------------ embedding lookup
 // y[i] = scale * w[ids[i]]; ids of 4 or 8 bytes; an id outside [0, V) gives 0 and sets the error word.

@@ -27,6 +27,8 @@ instead.  Semantics: difflet/backends/neuron/ops_impl/attention.py:435-713.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 import torch.nn.functional as TF
 
@@ -290,7 +292,14 @@ def window_attention(q, k, v, *, window, sinks=0, scale=None, kv_lens=None, q_st
     (``[B, H, Sq]``, natural log) are filled when given.  CUDA: bf16 and fp16 with D 64 or 128, whose P is rounded to
     the type for its product with v; only the tiles that some query sees are read, and few queries share the keys among many
     CTAs.  Anything else, and what asks for gradients, runs as ``cross_attention`` under the same mask."""
-    window, sinks = int(window), int(sinks)
+    if (q.is_cuda and type(q) is torch.Tensor and q.dtype in F.CROSS_DTYPES and (q_start is None or type(q_start) is torch.Tensor)
+            and not torch.compiler.is_compiling()):
+        try:  # the binding checks everything; what it refuses is looked at again below
+            return F.window_attention(q, k, v, 1.0 if scale is None else float(scale), window, sinks, kv_lens=kv_lens,
+                                      q_start=q_start, out=out, lse=lse)
+        except (ValueError, TypeError):
+            pass
+    window, sinks = (min(operator.index(n), 2 ** 62) for n in (window, sinks))
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:

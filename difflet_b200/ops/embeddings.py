@@ -10,23 +10,11 @@ models rotate q/k inside the fused norm + RoPE + scatter kernel instead."""
 from __future__ import annotations
 
 import torch
-import torch.nn.functional as TF
-from torch.autograd.function import once_differentiable
 
 from difflet_b200.ops import fused as F
 
 
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, pad):
-        ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.pad = weight.shape[0], scale, pad
-        return F.embedding(ids, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        return None, F.embedding_grad(dy, *ctx.saved_tensors, ctx.rows, ctx.scale, ctx.pad), None, None
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def embedding(ids, weight, *, scale=1.0, padding_idx=None):
@@ -37,25 +25,25 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
     CUDA: bf16, fp16 and fp32; an id outside the table gives a row of zeros and no gradient, and sets the device error word
     (``_native.check_device_errors`` raises it); on the CPU it raises IndexError.  Other types, tracing, function transforms and
     forward-mode tangents run as torch operations."""
+    if weight.is_cuda and type(weight) in _PLAIN and not torch.compiler.is_compiling():
+        try:  # the binding checks everything; what it refuses is looked at again below
+            y = (F._nat or F._lib()).embedding(ids, weight, scale, padding_idx)
+            F.LAUNCHES[0] += 1
+            return y
+        except ValueError:
+            pass
     if weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError(f"weight must be floating-point [V, D], got {tuple(weight.shape)} {weight.dtype}")
     if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
         raise ValueError(f"ids must be integers, got {ids.dtype}")
     if ids.device != weight.device:
         raise ValueError(f"ids on {ids.device}, weight on {weight.device}")
-    V, scale = weight.shape[0], float(scale)
-    pad = -1
+    V, pad = weight.shape[0], None
     if padding_idx is not None:
         pad = int(padding_idx) + (V if padding_idx < 0 else 0)
         if not 0 <= pad < V:
             raise ValueError(f"padding_idx {padding_idx} is not a row of {V}")
-    if weight.is_cuda and weight.dtype in F.EMBED_DTYPES and F.kernel_tensors(ids, weight) and not F.has_tangent(weight):
-        if torch.is_grad_enabled() and weight.requires_grad:
-            return _Embedding.apply(ids, weight, scale, pad)
-        return F.embedding(ids, weight, scale)
-    ct = torch.float64 if weight.dtype == torch.float64 else torch.float32
-    rows = TF.embedding(ids.long(), weight, padding_idx=None if pad < 0 else pad)
-    return (rows.to(ct) * scale).to(weight.dtype)
+    return F.embedding(ids, weight, float(scale), pad)
 
 
 def apply_rotary_emb(hidden_states, freqs_cos, freqs_sin):

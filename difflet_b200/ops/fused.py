@@ -270,17 +270,6 @@ def gated_linear(x, w_gate, w_up, act="silu"):
     return (a * u).to(x.dtype)
 
 
-def gated_linear_native(x, w_gate, w_up, act, keep: bool):
-    """The kernel: (h,) or, with ``keep``, (h, g, u)."""
-    return _kernels().gated_linear(x, w_gate, w_up, GATED_ACTS[act], keep)
-
-
-def gated_linear_grad_native(dh, x, w_gate, w_up, g, u, act, need):
-    """(dx, dw_gate, dw_up), None where ``need`` is false."""
-    LAUNCHES[0] += int(need[0]) + int(need[1] or need[2])
-    return _kernels().gated_linear_grad(dh, x, w_gate, w_up, g, u, GATED_ACTS[act], *need)
-
-
 def _no_grad(name: str, *tensors) -> None:
     """The kernels record no backward pass: refuse inputs whose gradient would be lost silently."""
     if wants_grad(*tensors):
@@ -752,15 +741,10 @@ def window_attention(q, k, v, scale, window, sinks, *, kv_lens=None, q_start=Non
 
 
 # --------------------------------------------------------------------------- embedding lookup
-EMBED_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
-
-
-def embedding(ids, w, scale=1.0):
-    """``scale * w[ids]`` without a gradient: the kernel on CUDA, torch operations elsewhere."""
-    if w.is_cuda:
-        return _kernels().embedding(ids, w, float(scale))
+def embedding(ids, w, scale=1.0, pad=None):
+    """``scale * w[ids]`` in torch operations (f32 up to the result, f64 for f64): the oracle."""
     ct = torch.float64 if w.dtype == torch.float64 else torch.float32
-    return (w[ids.long()].to(ct) * scale).to(w.dtype)
+    return (F.embedding(ids.long(), w, padding_idx=pad).to(ct) * scale).to(w.dtype)
 
 
 def embedding_grad(dy, ids, V, scale=1.0, pad=-1):

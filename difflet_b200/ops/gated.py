@@ -8,24 +8,11 @@ is an ordinary ``linear``.  The weights stay as checkpoints hold them, two [F, K
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from difflet_b200.ops import fused as F
 
 
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, act):
-        h, g, u = F.gated_linear_native(x, w_gate, w_up, act, True)
-        ctx.act = act
-        ctx.save_for_backward(x, w_gate, w_up, g, u)
-        return h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh):
-        need = [bool(n) for n in ctx.needs_input_grad[:3]]
-        return (*F.gated_linear_grad_native(dh, *ctx.saved_tensors, ctx.act, need), None)
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def gated_linear(x, w_gate, w_up, *, act="silu"):
@@ -35,6 +22,13 @@ def gated_linear(x, w_gate, w_up, *, act="silu"):
     evaluated in f32; the result is rounded to x's type once.  Differentiable in all three (once): the two projections are
     kept in x's type for it.  CUDA: bf16 and fp16 with K a multiple of 8; other types and sizes, tracing,
     function transforms and forward-mode tangents run as torch operations."""
+    if x.is_cuda and act in F.GATED_ACTS and type(x) in _PLAIN and not torch.compiler.is_compiling():
+        try:  # the binding checks everything; what it refuses is looked at again below
+            h = (F._nat or F._lib()).gated_linear(x, w_gate, w_up, F.GATED_ACTS[act])
+            F.LAUNCHES[0] += 1
+            return h
+        except ValueError:
+            pass
     if act not in F.GATED_ACTS:
         raise ValueError(f"act {act!r}: one of {sorted(F.GATED_ACTS)}")
     if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:
@@ -44,11 +38,6 @@ def gated_linear(x, w_gate, w_up, *, act="silu"):
             raise ValueError(f"{name} {t.dtype} on {t.device} does not match x {x.dtype} on {x.device}")
     if not x.is_floating_point():
         raise ValueError(f"gated_linear needs floating-point tensors, got {x.dtype}")
-    if (x.is_cuda and x.dtype in F.CROSS_DTYPES and x.shape[-1] > 0 and x.shape[-1] % 8 == 0 and F.kernel_tensors(x, w_gate, w_up)
-            and not F.has_tangent(x, w_gate, w_up)):
-        if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
-            return _GatedLinear.apply(x, w_gate, w_up, act)
-        return F.gated_linear_native(x, w_gate, w_up, act, False)[0]
     return F.gated_linear(x, w_gate, w_up, act)
 
 
