@@ -669,6 +669,13 @@ at::Tensor cross_attention_call(const at::Tensor& q, const at::Tensor& k, const 
     a.bias_hs = t.H > 1 ? nq * nt * a.bias_ts : 0;
     a.bias_bs = t.B > 1 ? t.H * nq * nt * a.bias_ts : 0;
   }
+  if (a.slide) {
+    dfl_cross_slide_plan(&a);
+    if (a.splits > 1) {
+      aux = new_like(q, {(int64_t)a.splits * a.B * a.H * a.Sq * (a.dh + 1)}, at::kFloat);
+      a.parts = aux.data_ptr<float>();
+    }
+  }
   a.err = err_ptr();
   DFL_CHECK_RC(dfl_cross_attention(&a, cur_stream()), "cross_attention");
   if (!direct) o.copy_(o_);

@@ -42,9 +42,12 @@ long long row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? (t.size(1) +
 bool is16(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
 
 // ---------------------------------------------------------------- gated projection
-// x [..., K], wg / wu [F, K] of one 16-bit type -> {h [..., F]} or, to keep the projections for the gradients, {h, g, u}
-// (g, u [M, F] with padded rows).
-std::vector<at::Tensor> gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act, bool keep) {
+// x as rows [M, K] that the copy engine can address.
+at::Tensor rows_of(const at::Tensor& x, int64_t M, int64_t K) { return rows16(x.dim() == 2 ? x : x.reshape({M, K})); }
+
+// x [..., K], wg / wu [F, K] of one 16-bit type -> h [..., F]; kept: where the projections are wanted for the gradients,
+// [2, M, F] with padded rows.
+at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act, at::Tensor* kept) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && wg.dim() == 2 && wu.dim() == 2, "x [..., K] and weights [F, K] must be CUDA tensors");
   TORCH_CHECK_VALUE(is16(x), "gated_linear runs in bfloat16 or float16 on CUDA, got ", x.scalar_type());
   for (const at::Tensor* t : {&wg, &wu})
@@ -59,17 +62,15 @@ std::vector<at::Tensor> gated_forward(const at::Tensor& x, const at::Tensor& wg,
   at::Tensor h = new_like(x, shape, x.scalar_type());
   const int64_t M = x.numel() / K, Fp = (F + 7) / 8 * 8;
   TORCH_CHECK_VALUE(M < (1ll << 30), "too many rows");
-  std::vector<at::Tensor> out{h};
   GluArgs a{};
-  if (keep)
-    for (int i = 0; i < 2; ++i) out.push_back(new_like(x, {M, Fp}, x.scalar_type()).narrow(1, 0, F));
-  if (M == 0 || F == 0) return out;
-  const at::Tensor x2 = rows16(x.reshape({M, K})), g2 = rows16(wg), u2 = rows16(wu);
+  if (kept) *kept = new_like(x, {2, M, Fp}, x.scalar_type());
+  if (M == 0 || F == 0) return h;
+  const at::Tensor x2 = rows_of(x, M, K), g2 = rows16(wg), u2 = rows16(wu);
   a.x = x2.data_ptr(), a.ldx = row_stride(x2);
   a.wg = g2.data_ptr(), a.ldwg = row_stride(g2);
   a.wu = u2.data_ptr(), a.ldwu = row_stride(u2);
   a.h = h.data_ptr(), a.ldh = F;
-  if (keep) a.g = out[1].data_ptr(), a.u = out[2].data_ptr(), a.lds = Fp;
+  if (kept) a.g = kept->data_ptr(), a.u = reinterpret_cast<uint16_t*>(a.g) + M * Fp, a.lds = Fp;
   a.M = (int)M, a.K = (int)K, a.F = (int)F, a.act = (int)act;
   a.f16 = x.scalar_type() == at::kHalf;
   a.err = err_ptr();
@@ -77,19 +78,15 @@ std::vector<at::Tensor> gated_forward(const at::Tensor& x, const at::Tensor& wg,
   a.ws_floats = dfl_glu_ws(0, a.M, a.K, a.F);
   if (a.ws_floats) ws = new_like(x, {a.ws_floats}, at::kFloat), a.ws = ws.data_ptr<float>();
   DFL_CHECK_RC(dfl_glu(&a, cur_stream()), "gated_linear");
-  return out;
+  return h;
 }
 
 // Gradients of gated_linear: {dx, dwg, dwu} (undefined where not needed) from dh and what the forward kept.
-std::vector<at::Tensor> gated_backward(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
-                                          const at::Tensor& g, const at::Tensor& u, int64_t act, bool need_dx, bool need_dwg,
-                                          bool need_dwu) {
-  const int64_t K = x.size(-1), F = wg.size(0), M = x.numel() / std::max<int64_t>(K, 1);
-  TORCH_CHECK_VALUE(dh.is_cuda() && dh.device() == x.device() && dh.scalar_type() == x.scalar_type() && dh.numel() == M * F,
-                    "the gradient ", dh.sizes(), " ", dh.scalar_type(), " does not match the output");
-  TORCH_CHECK_VALUE(g.dim() == 2 && g.size(0) == M && g.size(1) == F && g.sizes() == u.sizes() && g.strides() == u.strides() &&
-                        g.scalar_type() == x.scalar_type() && g.stride(1) == 1 && g.stride(0) % 8 == 0,
-                    "g and u are what the forward kept");
+variable_list gated_backward(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& kept,
+                             int64_t act, bool need_dx, bool need_dwg, bool need_dwu) {
+  const int64_t K = x.size(-1), F = wg.size(0), M = x.numel() / K, Fp = (F + 7) / 8 * 8;
+  TORCH_CHECK(dh.device() == x.device() && dh.scalar_type() == x.scalar_type() && dh.numel() == M * F, "the gradient ", dh.sizes(), " ",
+              dh.scalar_type(), " does not match the output");
   const c10::cuda::CUDAGuard guard(x.device());
   at::Tensor dx, dwg, dwu;
   if (need_dx) dx = new_like(x, x.sizes(), x.scalar_type());
@@ -100,18 +97,16 @@ std::vector<at::Tensor> gated_backward(const at::Tensor& dh, const at::Tensor& x
       if (t->defined()) t->zero_();
     return {dx, dwg, dwu};
   }
-  at::Tensor d2 = dh.reshape({M, F});
+  at::Tensor d2 = dh.dim() == 2 ? dh : dh.reshape({M, F});
   if (F > 1 && (d2.stride(1) != 1 || (M > 1 && d2.stride(0) < F))) d2 = d2.contiguous();
-  const int64_t Fp = (F + 7) / 8 * 8;
   const at::Tensor dgu = new_like(x, {2, M, Fp}, x.scalar_type());
   GluGradArgs e{};
   e.dh = d2.data_ptr(), e.lddh = M > 1 ? d2.stride(0) : F;
-  e.g = g.data_ptr(), e.u = u.data_ptr(), e.lds = Fp;
-  TORCH_CHECK_VALUE(M <= 1 || g.stride(0) == Fp, "g and u are what the forward kept");
-  e.dg = dgu.data_ptr(), e.du = dgu[1].data_ptr();
+  e.g = kept.data_ptr(), e.u = reinterpret_cast<const uint16_t*>(e.g) + M * Fp, e.lds = Fp;
+  e.dg = dgu.data_ptr(), e.du = reinterpret_cast<uint16_t*>(e.dg) + M * Fp;
   e.M = M, e.F = (int)F, e.act = (int)act, e.f16 = x.scalar_type() == at::kHalf;
   DFL_CHECK_RC(dfl_glu_grad(&e, cur_stream()), "gated_linear (gradient of the product)");
-  const at::Tensor x2 = rows16(x.reshape({M, K})), g2 = rows16(wg), u2 = rows16(wu);
+  const at::Tensor x2 = rows_of(x, M, K), g2 = rows16(wg), u2 = rows16(wu);
   GluGemmArgs a{};
   a.dg = e.dg, a.du = e.du, a.lds = Fp;
   a.x = x2.data_ptr(), a.ldx = row_stride(x2);
@@ -137,17 +132,19 @@ std::vector<at::Tensor> gated_backward(const at::Tensor& dh, const at::Tensor& x
 
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act) {
-    std::vector<at::Tensor> hgu = gated_forward(x, wg, wu, act, true);
-    ctx->save_for_backward({x, wg, wu, hgu[1], hgu[2]});
+    at::Tensor kept;
+    const at::Tensor h = gated_forward(x, wg, wu, act, &kept);
+    ctx->save_for_backward({x, wg, wu, kept});
     ctx->saved_data["act"] = act;
-    return hgu[0];
+    return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dh) {
     return once_differentiable("gated_linear", [&]() -> variable_list {
       const variable_list s = ctx->get_saved_variables();
-      std::vector<at::Tensor> d = gated_backward(dh[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["act"].toInt(),
-                                                 ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
-      return {d[0], d[1], d[2], at::Tensor()};
+      variable_list d = gated_backward(dh[0], s[0], s[1], s[2], s[3], ctx->saved_data["act"].toInt(), ctx->needs_input_grad(0),
+                                       ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+      d.emplace_back();
+      return d;
     });
   }
 };
@@ -156,7 +153,7 @@ at::Tensor gated_linear(const at::Tensor& x, const at::Tensor& wg, const at::Ten
   TORCH_CHECK_VALUE(plain_tensors({&x, &wg, &wu}), "the kernel takes no wrapped tensors and no tangents");
   if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad()))
     return GatedLinear::apply(x, wg, wu, act);
-  return gated_forward(x, wg, wu, act, false)[0];
+  return gated_forward(x, wg, wu, act, nullptr);
 }
 
 // ---------------------------------------------------------------- embedding lookup

@@ -1,4 +1,6 @@
 // Cross attention: bf16 variants, argument checks and the bit packing of boolean masks.
+#include <algorithm>
+
 #include "cross_attn.cuh"
 
 extern "C" int dfl_cross_attention_f16(const CrossArgs* a, cudaStream_t stream);
@@ -124,6 +126,28 @@ extern "C" int dfl_cross_mask_bits(const MaskBitsArgs* a, cudaStream_t stream) {
   return (int)dfl_host::launch_early(cross_mask_bits_kernel, (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, stream, *a);
 }
 
+// How a sliding window is laid out (q_tiles, splits): rounds of items, each of which costs its key tiles (a tile pair about 4300 cycles
+// at head dim 128 and 3000 at 64, a lone tile 3600 and 2600) and about 4000 for its turn; parts cost their rows' way through L2
+// and a launch.  The blocks are taken as equally long, as they are but for the first window.
+extern "C" void dfl_cross_slide_plan(CrossArgs* a) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const long long sms = dfl_host::num_sms(dev), rows = (long long)a->B * a->H * a->Sq;
+  double least = -1.;
+  for (int qt = 1; qt <= 2; ++qt) {
+    if (qt == 2 && a->Sq <= kBM) break;
+    const long long items = ((long long)a->Sq + qt * kBM - 1) / (qt * kBM) * a->H * a->B;
+    const long long span = std::min<long long>(a->Sk, (long long)a->slide + std::min(a->Sq, qt * kBM));
+    const long long tiles = std::max<long long>(1, (span + kBN - 1) / kBN + (a->Sk > span ? (a->sinks + kBN - 1) / kBN : 0));
+    const double step = qt == 2 ? (a->dh == 64 ? 3000. : 4300.) : (a->dh == 64 ? 2600. : 3600.);
+    for (int s = 1; s <= 16 && s <= tiles; ++s) {
+      const double rounds = s == 1 && items > sms ? (double)items / sms : (double)((items * s + sms - 1) / sms);
+      const double cost = rounds * ((tiles + s - 1) / s * step + 4000.) + (s > 1 ? 6000. + (double)s * rows * a->dh * 8 / 2600. : 0.);
+      if (least < 0. || cost < least) least = cost, a->q_tiles = qt, a->splits = s;
+    }
+  }
+}
+
 extern "C" int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream) {
   if (a->dh != 64 && a->dh != 128) return -2;
   if (a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->H % a->Hk) return -3;
@@ -137,5 +161,6 @@ extern "C" int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream) {
   if (a->bits && ((a->bits_bs | a->bits_hs | a->bits_qs) % 4 || a->bias_tiles)) return -7;
   if (a->p2 && (a->bits || a->bias_tiles)) return -8;
   if (a->slide && (a->slide < 0 || a->sinks < 0 || a->bits || a->bias_tiles || a->p2 || a->kv_lo)) return -9;
+  if (a->slide && (a->splits < 1 || (a->splits > 1 && !a->parts) || !al16(a->parts) || (a->q_tiles != 1 && a->q_tiles != 2))) return -10;
   return a->f16 ? dfl_cross_attention_f16(a, stream) : cross_entry<false>(a, stream);
 }

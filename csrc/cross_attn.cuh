@@ -76,6 +76,10 @@ struct CrossParams {
   // among the last `slide` or the first `sinks`
   const int* start;
   int slide, sinks;
+  // The key tiles of a block in `splits` parts, joined by cross_join_kernel: f32 rows and log-sum-exps (log2 units), [part][B, H, Sq]
+  int splits;
+  float* part_o;
+  float* part_l;
 };
 
 template <int DH, int QT>
@@ -194,30 +198,34 @@ struct CrossItems {
   }
 };
 
-// The same where a window slides with the queries: the tiles of the first keys, then those of the window.
+// The same where a window slides with the queries: the tiles of the first keys, then those of the window, or a part of them.
+// Heads first, the last queries before the first ones: blocks with many keys lead, those with few fill the last round
+// (12 heads x 32760 queries, window 9360: see the table).
 template <int QT>
 struct SlideItems {
   int q0, h, b, n;
   int lo, hi, sinks; // keys that a query of this block may see: [0, sinks) and [lo, hi)
   long long p0;      // position of the block's first query (a start may be any 32-bit value)
-  int qb, dq, dh, db, len, start, n_sink, t_win;
+  int sp, qb, ds, dh, db, dq, len, start, n_sink, t_win, j0;
   DFL_DEVICE explicit SlideItems(const CrossParams& p) {
-    const int i = blockIdx.x, g = gridDim.x;
-    qb = i % p.n_qb, h = (i / p.n_qb) % p.H, b = i / p.n_qb / p.H;
-    dq = g % p.n_qb, dh = (g / p.n_qb) % p.H, db = g / p.n_qb / p.H;
+    const int i = blockIdx.x / p.splits, g = gridDim.x / p.splits;
+    sp = blockIdx.x % p.splits, ds = gridDim.x % p.splits;
+    h = i % p.H, b = i / p.H % p.B, qb = p.n_qb - 1 - i / p.H / p.B;
+    dh = g % p.H, db = g / p.H % p.B, dq = g / p.H / p.B;
     row(p);
   }
-  DFL_DEVICE bool more(const CrossParams& p) const { return b < p.B; }
+  DFL_DEVICE bool more(const CrossParams& p) const { return qb >= 0; }
   DFL_DEVICE void next(const CrossParams& p) {
     const int was = b;
-    qb += dq, h += dh, b += db;
-    if (qb >= p.n_qb) qb -= p.n_qb, ++h;
+    sp += ds, h += dh, b += db, qb -= dq;
+    if (sp >= p.splits) sp -= p.splits, ++h;
     if (h >= p.H) h -= p.H, ++b;
+    if (b >= p.B) b -= p.B, --qb;
     if (b != was) row(p);
     else block(p);
   }
   DFL_DEVICE void row(const CrossParams& p) {
-    if (b >= p.B) return;
+    if (qb < 0) return;
     len = p.kv_hi ? min(p.Sk, max(0, __ldcg(p.kv_hi + b))) : p.Sk;
     start = p.start ? __ldcg(p.start + b) : len - p.Sq;
     block(p);
@@ -231,8 +239,14 @@ struct SlideItems {
     n_sink = (sinks + kBN - 1) / kBN;
     t_win = max(n_sink, lo / kBN);
     n = n_sink + (hi > lo ? max(0, (hi + kBN - 1) / kBN - t_win) : 0);
+    j0 = 0;
+    if (p.splits > 1) {
+      const int per = (n + p.splits - 1) / p.splits;
+      j0 = min(n, sp * per);
+      n = min(per, n - j0);
+    }
   }
-  DFL_DEVICE int tile(int j) const { return j < n_sink ? j : t_win + j - n_sink; }
+  DFL_DEVICE int tile(int j) const { return j0 + j < n_sink ? j0 + j : t_win + j0 + j - n_sink; }
 };
 template <int MASK, int QT>
 struct ItemsOf {
@@ -646,6 +660,32 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         l += (a0 + a1) + (b0 + b1);
       }
       if (!ok) break;
+      if constexpr (MASK == kSlide) {
+        if (p.splits > 1) {  // a part: the row as it is weighted by its own maximum and sum
+          const long long r = (((long long)it.sp * p.B + it.b) * p.H + it.h) * p.Sq + qrow;
+          if (it.n > 0) {
+            if (!mbar_wait_warp(&o_full[g], used & 1, err, kKidCross, 122 + g, abort_flag)) { ok = false; break; }
+            ++used;
+            tc_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+            for (int c = 0; c < DH; c += 32) {
+              uint32_t o_raw[32];
+              tmem_ld_32x32b_x32(o_t + c, o_raw);
+              tmem_wait_ld();
+              if (!live) continue;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                reinterpret_cast<float4*>(p.part_o + r * DH + c)[e] =
+                    make_float4(__uint_as_float(o_raw[4 * e]) * inv, __uint_as_float(o_raw[4 * e + 1]) * inv,
+                                __uint_as_float(o_raw[4 * e + 2]) * inv, __uint_as_float(o_raw[4 * e + 3]) * inv);
+            }
+            tc_fence_before();  // O_g has been read before this thread's next P_g signal
+          }
+          if (live) p.part_l[r] = l == 0.f ? -INFINITY : m + log2f(l);
+          continue;
+        }
+      }
       // this item's rows
       uint16_t* op = reinterpret_cast<uint16_t*>(p.o) + it.b * p.o_bs + it.h * p.o_hs + (long long)qrow * p.o_ss;
       if (it.n == 0) {
@@ -702,6 +742,35 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
   if (warp == C::kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
 }
 
+// A block's rows from its parts, added in order; a thread takes 4 values of a row.
+template <int DH, bool F16>
+__global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p) {
+  griddep_wait();
+  const long long rows = (long long)p.B * p.H * p.Sq;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * (DH / 4); i += (long long)gridDim.x * 256) {
+    const long long r = i / (DH / 4);
+    const int d = (int)(i % (DH / 4)) * 4;
+    float top = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, __ldcg(p.part_l + s * rows + r));
+    const float use = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+      const float l = __ldcg(p.part_l + s * rows + r);
+      if (l == -INFINITY) continue;  // (nothing was stored for it)
+      const float f = exp2_sfu(l - use);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * rows + r) * DH + d));
+      o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+      sum += f;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const long long q = r % p.Sq, h = r / p.Sq % p.H, b = r / p.Sq / p.H;
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + b * p.o_bs + h * p.o_hs + q * p.o_ss + d) =
+        make_uint2(pack2<F16>(o.x * inv, o.y * inv), pack2<F16>(o.z * inv, o.w * inv));
+    if (p.lse && d == 0) p.lse[r] = sum == 0.f ? -INFINITY : (use + log2f(sum)) * kLn2;
+  }
+}
+
 inline int cross_tmap(CUtensorMap* map, const void* base, int D, long long S, int H, int B, long long ss, long long hs,
                       long long bs, bool f16, bool out = false) {
   dfl_host::EncodeTiledFn fn = dfl_host::get_encode_tiled();
@@ -741,14 +810,19 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
   rc = cross_tmap(&to, a->o, DH, a->Sq, a->H, a->B, a->o_ss, a->o_hs, a->o_bs, F16, true);
   if (rc) return 4000 + rc;
   p.n_qb = (a->Sq + QT * kBM - 1) / (QT * kBM);
-  const long long items = (long long)p.n_qb * a->H * a->B;
+  const long long items = (long long)p.n_qb * a->H * a->B * p.splits;
   const int sms = dfl_host::num_sms(dev);
-  return (int)dfl_host::launch_early(kern, (unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream, tq, tk, tv, to, p, a->err);
+  const cudaError_t e = dfl_host::launch_early(kern, (unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream, tq, tk, tv, to, p, a->err);
+  if (MASK != kSlide || p.splits == 1 || e != cudaSuccess) return (int)e;
+  const long long blocks = ((long long)a->B * a->H * a->Sq * (DH / 4) + 255) / 256;
+  return (int)dfl_host::launch_early(cross_join_kernel<DH, F16>, (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream, p);
 }
 
 // Two ping-pong Q tiles per CTA unless one holds every query, or twice the items still fit the SMs.
 template <int DH, bool F16, int MASK, bool P2 = false>
 int launch_cross_qt(const CrossArgs* a, const CrossParams& p, cudaStream_t stream, int dev) {
+  if constexpr (MASK == kSlide)
+    return a->q_tiles == 1 ? launch_cross<DH, F16, 1, MASK, P2>(a, p, stream, dev) : launch_cross<DH, F16, 2, MASK, P2>(a, p, stream, dev);
   const long long items2 = (long long)((a->Sq + 2 * kBM - 1) / (2 * kBM)) * a->H * a->B;
   if (a->Sq <= kBM || items2 * 2 <= dfl_host::num_sms(dev)) return launch_cross<DH, F16, 1, MASK, P2>(a, p, stream, dev);
   return launch_cross<DH, F16, 2, MASK, P2>(a, p, stream, dev);
@@ -783,6 +857,9 @@ int cross_entry(const CrossArgs* a, cudaStream_t stream) {
   p.bias_rows = a->bias_rows;
   p.start = a->start;
   p.slide = a->slide, p.sinks = a->sinks;
+  p.splits = a->slide ? a->splits : 1;
+  p.part_o = a->parts;
+  p.part_l = a->parts + (long long)p.splits * a->B * a->H * a->Sq * a->dh;
   int dev = 0;
   cudaGetDevice(&dev);
   return a->dh == 64 ? launch_cross_mask<64, F16>(a, p, stream, dev) : launch_cross_mask<128, F16>(a, p, stream, dev);

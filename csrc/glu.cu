@@ -16,7 +16,6 @@
 // Tiles of 256 x 256 by CTA pairs, of 128 x 256 or of 128 x 128 by single CTAs; what is left after whole rounds of tiles may be
 // split along the sum, the parts added by a kernel behind (glu_plan).
 #include <algorithm>
-#include <cstdlib>
 #include <cstring>
 
 #include <cuda_fp16.h>
@@ -30,7 +29,8 @@ using namespace dfl;
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
 
-constexpr int BM = 128, BK = 64, kThreads = 192;
+constexpr int BM = 128, BK = 64;
+constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;  // copies, products, then the results: two warps to a lane quarter
 // CG: CTAs per tile (2: a pair).  A tile is 128 CG rows and BN accumulator columns; each CTA loads 128 rows of the first operand
 // and BN / CG rows (or columns) of the second per stage.
 template <int CG, int BN>
@@ -39,7 +39,7 @@ struct Cfg {
   static constexpr int kStages = kStage > 32768 ? 4 : 6;
   static constexpr int kBarOff = kStages * kStage;
   static constexpr int kRowsOff = (kBarOff + (2 * kStages + 4) * 8 + 16 + 15) / 16 * 16;  // 32 x 33 16-bit values per epilogue warp
-  static constexpr int kSmem = kRowsOff + 4 * 32 * 33 * 2 + 1024;
+  static constexpr int kSmem = kRowsOff + kEpiWarps * 32 * 33 * 2 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 constexpr int kChunk = 64 * BK * 2;  // 64 columns of an operand whose columns are contiguous
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 128 * CG);  // (CTA 0's copy is the one used)
+      mbar_init(&tempty_bar[a], 32 * kEpiWarps * CG);  // (CTA 0's copy is the one used)
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -317,7 +317,8 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     }
   } else {
     const int sub = warp & 3;  // the tensor-memory lane quarter that this warp may read
-    uint16_t(*stage_rows)[33] = reinterpret_cast<uint16_t(*)[33]>(smem + C::kRowsOff) + 32 * sub;
+    const int half = (warp - 2) / 4;  // of the tile's columns
+    uint16_t(*stage_rows)[33] = reinterpret_cast<uint16_t(*)[33]>(smem + C::kRowsOff) + 32 * (warp - 2);
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = first; t < items; t += step) {
@@ -335,23 +336,23 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
       if (it.part >= 0) {  // sums of a part: the whole tile, whatever lies outside
         float* part = p.ws + (long long)it.part * (BM * CG * BN) + ((int)rank * BM + sub * 32 + lane) * BN;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
           uint32_t r[32];
           tmem_ld_32x32b_x32(tbase + c, r);
           tmem_wait_ld();
-          if (c + 32 == BN) release();
+          if (c + 32 == (half + 1) * (BN / 2)) release();
 #pragma unroll
           for (int q = 0; q < 8; ++q) reinterpret_cast<uint4*>(part + c)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
         }
       } else if constexpr (MODE == kForward) {
         const bool wide = p.ldd % 8 == 0 && (reinterpret_cast<uintptr_t>(p.d[0]) & 15) == 0;
 #pragma unroll 1
-        for (int c = 0; c < BN / 2; c += 32) {
+        for (int c = half * (BN / 4); c < (half + 1) * (BN / 4); c += 32) {
           uint32_t gr[32], ur[32];
           tmem_ld_32x32b_x32(tbase + c, gr);
           tmem_ld_32x32b_x32(tbase + BN / 2 + c, ur);
           tmem_wait_ld();
-          if (c + 32 == BN / 2) release();
+          if (c + 32 == (half + 1) * (BN / 4)) release();
           const int col = it.nb * (BN / 2) + c, cols = p.N - col;
           if (rows <= 0 || cols <= 0) continue;
           float g[32], u[32];
@@ -375,11 +376,11 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
         }
       } else {
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
           uint32_t r[32];
           tmem_ld_32x32b_x32(tbase + c, r);
           tmem_wait_ld();
-          if (c + 32 == BN) release();
+          if (c + 32 == (half + 1) * (BN / 2)) release();
           const int col = it.nb * BN + c, cols = p.N - col;
           if (rows <= 0 || cols <= 0) continue;
           float v[32];
@@ -578,15 +579,14 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // How a product is laid out.  Per K block an SM needs (cycles): a pair's 256 x 256 tile 560 (its products: 524), a 128 x 256 tile
-// 750 and a 128 x 128 tile 512 (both bound by the copies: 48 and 32 KB).  What is left after whole rounds is split along the
-// sum where that is shorter: every part of a tile costs its sums' way through L2, the join a launch.
+// 750 and a 128 x 128 tile 512 (both bound by the copies: 48 and 32 KB); a tile's results 2500, or 1250, beside the next
+// tile's products.  What is left after whole rounds is split along the sum where that is shorter: every part of a tile costs
+// its sums' way through L2, the join a launch.
 struct Plan {
   int cg, bn, whole, splits;
 };
 template <int MODE>
 Plan glu_plan(long long rows, long long cols, int problems, int blocks, int sms) {
-  static const int force = getenv("GLU_FORCE") ? atoi(getenv("GLU_FORCE")) : 0;
-  static const int nosplit = getenv("GLU_NOSPLIT") ? 1 : 0;
   struct Shape {
     int cg, bn;
     double block;
@@ -594,20 +594,19 @@ Plan glu_plan(long long rows, long long cols, int problems, int blocks, int sms)
   constexpr Shape shapes[3] = {{2, 256, 560.}, {1, 256, 750.}, {1, 128, 512.}};
   Plan best{};
   double least = 0.;
-  int idx = 0;
   for (const Shape& s : shapes) {
-    if (++idx != force && force) continue;
     const int width = MODE == kForward ? s.bn / 2 : s.bn;
     const long long tiles = (rows + 128 * s.cg - 1) / (128 * s.cg) * ((cols + width - 1) / width) * problems, slots = sms / s.cg;
     const long long rounds = tiles / slots, rest = tiles % slots;
     const auto take = [&](long long whole, int splits, double cost) {
       if (best.cg == 0 || cost < least) best = Plan{s.cg, s.bn, (int)whole, splits}, least = cost;
     };
-    take(tiles, 1, (double)(rounds + (rest > 0)) * blocks * s.block);
-    if (rest == 0 || nosplit) continue;
+    const double results = s.bn * 10., whole = std::max(blocks * s.block, results);
+    take(tiles, 1, (rounds + (rest > 0)) * whole + results);
+    if (rest == 0) continue;
     for (int n = 2; n <= slots / rest && blocks / n >= 4 && n <= 32; ++n)
       if ((n - 1) * ((blocks + n - 1) / n) < blocks)  // (every part holds something)
-      take(rounds * slots, n, (rounds * blocks + (blocks + n - 1) / n) * s.block + 6000. + rest * n * 128. * s.cg * s.bn * 8 / 2600.);
+        take(rounds * slots, n, rounds * whole + (blocks + n - 1) / n * s.block + results + 6000. + rest * n * 128. * s.cg * s.bn * 8 / 2600.);
   }
   return best;
 }

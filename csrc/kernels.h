@@ -325,8 +325,11 @@ typedef struct CrossArgs {
   // j > p - slide or j < sinks (kv_hi: the row's keys; no other mask)
   int slide, sinks;
   const int* start;
+  int q_tiles, splits;                 // by dfl_cross_slide_plan: query tiles to a CTA, parts of the keys
+  float* parts;                        // splits > 1: splits * B * H * Sq * (dh + 1) floats
   int* err;
 } CrossArgs;
+void dfl_cross_slide_plan(CrossArgs* a);
 int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream);
 
 // Additive mask [B, H, Q, Sk] (its unbroadcast extents, element strides) -> 32-query x 128-key blocks
