@@ -39,6 +39,7 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
@@ -50,6 +51,7 @@ using namespace dfl;
 constexpr int kBM = 128;      // queries per Q tile
 constexpr int kBN = 128;      // keys per tile
 constexpr int kChunk = 16384;  // 128 rows x 64 values: one swizzle chunk
+constexpr int kMaxParts = 8;   // of the keys of a block
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 enum { kWindow = 0, kBits = 1, kBias16 = 2, kBias32 = 3, kSlide = 4 };  // kBias16: of the inputs' type, kBias32: f32
@@ -661,28 +663,36 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       }
       if (!ok) break;
       if constexpr (MASK == kSlide) {
-        if (p.splits > 1) {  // a part: the row as it is weighted by its own maximum and sum
-          const long long r = (((long long)it.sp * p.B + it.b) * p.H + it.h) * p.Sq + qrow;
+        if (p.splits > 1) {  // a part: the row as it is weighted by its own maximum and sum, in f32; `to` addresses the parts
           if (it.n > 0) {
             if (!mbar_wait_warp(&o_full[g], used & 1, err, kKidCross, 122 + g, abort_flag)) { ok = false; break; }
             ++used;
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint8_t* stage = smem + C::kOut + warp * 4096;  // 32 rows x 32 values, swizzled as below
+            const int r0 = it.q0 + g * kBM + (warp & 3) * 32;
 #pragma unroll 1
             for (int c = 0; c < DH; c += 32) {
+              if (lane == 0) bulk_wait_read();
+              __syncwarp();
               uint32_t o_raw[32];
               tmem_ld_32x32b_x32(o_t + c, o_raw);
               tmem_wait_ld();
-              if (!live) continue;
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<float4*>(p.part_o + r * DH + c)[e] =
-                    make_float4(__uint_as_float(o_raw[4 * e]) * inv, __uint_as_float(o_raw[4 * e + 1]) * inv,
-                                __uint_as_float(o_raw[4 * e + 2]) * inv, __uint_as_float(o_raw[4 * e + 3]) * inv);
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) * 16)) =
+                    make_float4(__uint_as_float(o_raw[4 * i]) * inv, __uint_as_float(o_raw[4 * i + 1]) * inv,
+                                __uint_as_float(o_raw[4 * i + 2]) * inv, __uint_as_float(o_raw[4 * i + 3]) * inv);
+              fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0 && r0 < p.Sq) {
+                tma_store_4d(&to, stage, c, r0, it.h, it.sp * p.B + it.b);
+                bulk_commit();
+              }
             }
             tc_fence_before();  // O_g has been read before this thread's next P_g signal
           }
-          if (live) p.part_l[r] = l == 0.f ? -INFINITY : m + log2f(l);
+          if (live) p.part_l[(((long long)it.sp * p.B + it.b) * p.H + it.h) * p.Sq + qrow] = l == 0.f ? -INFINITY : m + log2f(l);
           continue;
         }
       }
@@ -746,40 +756,46 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
 template <int DH, bool F16>
 __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p) {
   griddep_wait();
+  constexpr int kRows = 256 / (DH / 4);
+  const int d = threadIdx.x % (DH / 4) * 4;
   const long long rows = (long long)p.B * p.H * p.Sq;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * (DH / 4); i += (long long)gridDim.x * 256) {
-    const long long r = i / (DH / 4);
-    const int d = (int)(i % (DH / 4)) * 4;
-    float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, __ldcg(p.part_l + s * rows + r));
-    const float use = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-      const float l = __ldcg(p.part_l + s * rows + r);
-      if (l == -INFINITY) continue;  // (nothing was stored for it)
-      const float f = exp2_sfu(l - use);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * rows + r) * DH + d));
-      o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
-      sum += f;
+  for (int bh = blockIdx.y; bh < p.B * p.H; bh += gridDim.y)
+    for (int q = blockIdx.x * kRows + threadIdx.x / (DH / 4); q < p.Sq; q += gridDim.x * kRows) {
+      const long long r = (long long)bh * p.Sq + q;
+      float l[kMaxParts], top = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < kMaxParts; ++s) {
+        l[s] = s < p.splits ? __ldcg(p.part_l + s * rows + r) : -INFINITY;
+        top = fmaxf(top, l[s]);
+      }
+      const float use = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kMaxParts; ++s) {
+        if (s >= p.splits || l[s] == -INFINITY) continue;  // (nothing was stored for it)
+        const float f = exp2_sfu(l[s] - use);
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * rows + r) * DH + d));
+        o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+        sum += f;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + bh / p.H * p.o_bs + bh % p.H * p.o_hs + (long long)q * p.o_ss + d) =
+          make_uint2(pack2<F16>(o.x * inv, o.y * inv), pack2<F16>(o.z * inv, o.w * inv));
+      if (p.lse && d == 0) p.lse[r] = sum == 0.f ? -INFINITY : (use + log2f(sum)) * kLn2;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const long long q = r % p.Sq, h = r / p.Sq % p.H, b = r / p.Sq / p.H;
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + b * p.o_bs + h * p.o_hs + q * p.o_ss + d) =
-        make_uint2(pack2<F16>(o.x * inv, o.y * inv), pack2<F16>(o.z * inv, o.w * inv));
-    if (p.lse && d == 0) p.lse[r] = sum == 0.f ? -INFINITY : (use + log2f(sum)) * kLn2;
-  }
 }
 
 inline int cross_tmap(CUtensorMap* map, const void* base, int D, long long S, int H, int B, long long ss, long long hs,
-                      long long bs, bool f16, bool out = false) {
+                      long long bs, bool f16, bool out = false, bool f32 = false) {
   dfl_host::EncodeTiledFn fn = dfl_host::get_encode_tiled();
   if (!fn) return 999;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)hs * 2, (cuuint64_t)bs * 2};
-  cuuint32_t box[4] = {64, out ? 32u : 128u, 1, 1};
+  const cuuint64_t e = f32 ? 4 : 2;
+  cuuint64_t strides[3] = {(cuuint64_t)ss * e, (cuuint64_t)hs * e, (cuuint64_t)bs * e};
+  cuuint32_t box[4] = {f32 ? 32u : 64u, out ? 32u : 128u, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  return (int)fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+  return (int)fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
@@ -807,15 +823,26 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
   if (rc) return 2000 + rc;
   rc = cross_tmap(&tv, a->v, DH, a->Sk, a->Hk, a->B, a->v_ss, a->v_hs, a->v_bs, F16);
   if (rc) return 3000 + rc;
-  rc = cross_tmap(&to, a->o, DH, a->Sq, a->H, a->B, a->o_ss, a->o_hs, a->o_bs, F16, true);
+  if (MASK == kSlide && p.splits > 1)
+    rc = cross_tmap(&to, p.part_o, DH, a->Sq, a->H, a->B * p.splits, DH, (long long)a->Sq * DH, (long long)a->H * a->Sq * DH, F16, true, true);
+  else
+    rc = cross_tmap(&to, a->o, DH, a->Sq, a->H, a->B, a->o_ss, a->o_hs, a->o_bs, F16, true);
   if (rc) return 4000 + rc;
   p.n_qb = (a->Sq + QT * kBM - 1) / (QT * kBM);
   const long long items = (long long)p.n_qb * a->H * a->B * p.splits;
   const int sms = dfl_host::num_sms(dev);
   const cudaError_t e = dfl_host::launch_early(kern, (unsigned)(items < sms ? items : sms), C::kThreads, C::kTotal, stream, tq, tk, tv, to, p, a->err);
   if (MASK != kSlide || p.splits == 1 || e != cudaSuccess) return (int)e;
-  const long long blocks = ((long long)a->B * a->H * a->Sq * (DH / 4) + 255) / 256;
-  return (int)dfl_host::launch_early(cross_join_kernel<DH, F16>, (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a->Sq + 1024 / DH - 1) / (1024 / DH)), (unsigned)std::min<long long>((long long)a->B * a->H, 65535), 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, cross_join_kernel<DH, F16>, p);
 }
 
 // Two ping-pong Q tiles per CTA unless one holds every query, or twice the items still fit the SMs.

@@ -86,14 +86,29 @@ DFL_DEVICE void store1(void* p, long long i, float v) {
 
 // act(x) = x s(x), and its derivative s + x s'(x).  SiLU: s = 1 / (1 + e^-x).  GELU, tanh form:
 // 0.5 (1 + tanh z) = 1 / (1 + e^-2z), z = sqrt(2 / pi) (x + 0.044715 x^3), which keeps the relative accuracy where
-// the result is small.  Exact GELU: s = erfc(-x / sqrt 2) / 2, s' = e^(-x^2 / 2) / sqrt(2 pi).
+// the result is small.  Exact GELU: s = Phi(x) = erfc(-x / sqrt 2) / 2, s' = e^(-x^2 / 2) / sqrt(2 pi); with z = |x|,
+// Phi(-z) = e^(-z^2 / 2) t p(t), t = 1 / (1 + 0.3 z), p of degree 7 fitted to least relative error over 0 <= z <= 14
+// (1.5e-7; 4e-6 at z = 13, where the rounding of z^2 counts).  erfcf took 28 us where this takes 24 (1000 x 1024 x 2816, g and u kept).
 DFL_DEVICE float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }  // (2^126 < e^-x gives 0, as it should)
 DFL_DEVICE float gelu_arg(float x) { return 1.5957691216057308f * x * (1.f + 0.044715f * x * x); }
+DFL_DEVICE float2 normal(float x) {  // (Phi(x), e^(-x^2 / 2))
+  const float z = fabsf(x), t = __fdividef(1.f, 1.f + 0.3f * z), e = __expf(-0.5f * z * z);
+  float p = 0.035675063729286194f;
+  p = fmaf(p, t, -0.15720424056053162f);
+  p = fmaf(p, t, 0.20635543763637543f);
+  p = fmaf(p, t, -0.05368535965681076f);
+  p = fmaf(p, t, 0.12856251001358032f);
+  p = fmaf(p, t, 0.09991323202848434f);
+  p = fmaf(p, t, 0.12075399607419968f);
+  p = fmaf(p, t, 0.11962929368019104f);
+  const float low = e * t * p;
+  return make_float2(x > 0.f ? 1.f - low : low, e);
+}
 template <int ACT>
 DFL_DEVICE float act_of(float x) {
   if constexpr (ACT == kGluSilu) return x * sigmoid(x);
   if constexpr (ACT == kGluGelu) return x * sigmoid(gelu_arg(x));
-  return 0.5f * x * erfcf(-0.7071067811865476f * x);
+  return x * normal(x).x;
 }
 template <int ACT>
 DFL_DEVICE float2 act_grad(float x) {  // (act, act')
@@ -105,8 +120,8 @@ DFL_DEVICE float2 act_grad(float x) {  // (act, act')
     const float s = sigmoid(gelu_arg(x));
     return make_float2(x * s, s * (1.f + x * (1.f - s) * 1.5957691216057308f * (1.f + 3.f * 0.044715f * x * x)));
   }
-  const float s = 0.5f * erfcf(-0.7071067811865476f * x);
-  return make_float2(x * s, s + x * 0.3989422804014327f * __expf(-0.5f * x * x));
+  const float2 n = normal(x);
+  return make_float2(x * n.x, n.x + x * 0.3989422804014327f * n.y);
 }
 
 // K blocks [kb0, kb1) of split item `split`; a block is (segment, offset) in the two-segment sums of dx.
