@@ -313,7 +313,8 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const bool cleaning = MASK == kSlide || p.kv_lo || p.kv_hi || (MASK == kBits && p.key_bits);  // masked keys may hold anything
+  const bool cleaning = MASK != kSlide && (p.kv_lo || p.kv_hi || (MASK == kBits && p.key_bits));  // masked keys may hold anything
+  uint64_t* v_raw = v_clean;  // kSlide: V tiles that the cleaning warp passes on (the others go straight to the products)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kNumBars; ++i) {
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     if (lane == 0) {
       // load L (K_s: 2 s, V_s: 2 s + 1 over all steps s) goes to slot L % R, use (L / R)
       bool issued[R], q_issued[2] = {false, false};
-      uint32_t issued_par[R];
+      uint32_t issued_par[R], raw = 0, raw_par = 0;  // raw: a bit per slot whose copy was counted on v_raw; raw_par: parity of its next phase
       for (int i = 0; i < R; ++i) issued[i] = false, issued_par[i] = 0;
       bool ok = true;
       int L = 0, used = 0;  // used: items with key tiles so far
@@ -358,9 +359,14 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
             const uint32_t par = (L / R) & 1;
             if (!mbar_wait(&kv_empty[slot], par ^ 1u, err, kKidCross, 100 + which, abort_flag)) { ok = false; break; }
             uint8_t* dst = smem + C::kKV + slot * C::kTile;
-            mbar_arrive_expect_tx(&kv_full[slot], C::kTile);
+            uint64_t* full = &kv_full[slot];
+            if constexpr (MASK == kSlide) {
+              raw &= ~(1u << slot);
+              if (which == 1 && cross_dirty<MASK>(p, it, it.tile(j) * kBN)) full = &v_raw[slot], raw |= 1u << slot, raw_par ^= 1u << slot;
+            }
+            mbar_arrive_expect_tx(full, C::kTile);
             for (int c = 0; c < C::kChunks; ++c)
-              tma_load_4d(dst + c * kChunk, which == 0 ? &tk : &tv, &kv_full[slot], c * 64, it.tile(j) * kBN, hk, it.b);
+              tma_load_4d(dst + c * kChunk, which == 0 ? &tk : &tv, full, c * 64, it.tile(j) * kBN, hk, it.b);
             issued[slot] = true;
             issued_par[slot] = par;
             if (j == 0 && which == 0) {  // the item's first keys are on their way: now its queries
@@ -381,7 +387,10 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         for (int g = 0; g < QT; ++g)
           if (q_issued[g]) mbar_wait(&q_full[g], 0, nullptr, 0, 0, nullptr, 200000000LL), mbar_wait(&q_full[g], 1, nullptr, 0, 0, nullptr, 200000000LL);
         for (int i = 0; i < R; ++i)
-          if (issued[i]) mbar_wait(&kv_full[i], issued_par[i], nullptr, 0, 0, nullptr, 200000000LL);
+          if (issued[i]) {
+            if ((raw >> i) & 1u) mbar_wait(&v_raw[i], ((raw_par >> i) & 1u) ^ 1u, nullptr, 0, 0, nullptr, 200000000LL);
+            else mbar_wait(&kv_full[i], issued_par[i], nullptr, 0, 0, nullptr, 200000000LL);
+          }
       }
     }
   } else if (warp == C::kMmaWarp) {
@@ -474,6 +483,40 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     bool ok = true;
     int s = 0;
+    auto clean = [&](const Items& it, int k0, uint8_t* tile, const uint32_t (&w)[4]) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {  // key row 32 c + lane: 128 bytes in every chunk (the swizzle stays inside)
+        const int r = 32 * c + lane, key = k0 + r;
+        bool drop = key < it.lo || key >= it.hi || !((w[c] >> lane) & 1u);
+        if constexpr (MASK == kSlide) drop = key >= it.hi || (key < it.lo && key >= it.sinks);
+        if (drop) {
+#pragma unroll
+          for (int ch = 0; ch < C::kChunks; ++ch)
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<uint4*>(tile + ch * kChunk + r * 128 + ((v + lane) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+    };
+    if constexpr (MASK == kSlide) {
+      // Only the tiles that hold keys which no query of the block sees pass here, a few at the window's ends: their copies are counted
+      // on v_raw[slot], this warp's arrival completes kv_full[slot] in their place, and until it has the slot is not filled again, so
+      // neither side can be a phase of it ahead.  (With every tile passing here, as below, 32760 queries took 7 % more.)
+      uint32_t par = 0;  // a bit per slot: parity of its next phase
+      for (Items it(p); it.more(p) && ok; it.next(p)) {
+        for (int j = 0; j < it.n && ok; ++j, ++s) {
+          const int k0 = it.tile(j) * kBN, slot = (2 * s + 1) % R;
+          if (!cross_dirty<MASK>(p, it, k0)) continue;
+          if (!mbar_wait_warp(&v_raw[slot], (par >> slot) & 1u, err, kKidCross, 141, abort_flag)) { ok = false; break; }
+          par ^= 1u << slot;
+          const uint32_t all[4] = {~0u, ~0u, ~0u, ~0u};
+          clean(it, k0, smem + C::kKV + slot * C::kTile, all);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[slot]);
+        }
+      }
+    }
     // every V tile passes here in order (its phase of v_clean[slot] completes once), so neither this
     // warp nor the MMA warp can be a phase of a slot ahead of the other
     for (Items it(p); cleaning && it.more(p) && ok; it.next(p)) {
@@ -487,19 +530,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         }
         if (!mbar_wait_warp(&kv_full[L % R], (L / R) & 1, err, kKidCross, 140, abort_flag)) { ok = false; break; }
         uint8_t* tile = smem + C::kKV + (L % R) * C::kTile;
-#pragma unroll
-        for (int c = 0; c < 4 && dirty; ++c) {  // key row 32 c + lane: 128 bytes in every chunk (the swizzle stays inside)
-          const int r = 32 * c + lane, key = k0 + r;
-          bool drop = key < it.lo || key >= it.hi || !((w[c] >> lane) & 1u);
-          if constexpr (MASK == kSlide) drop = key >= it.hi || (key < it.lo && key >= it.sinks);
-          if (drop) {
-#pragma unroll
-            for (int ch = 0; ch < C::kChunks; ++ch)
-#pragma unroll
-              for (int v = 0; v < 8; ++v)
-                *reinterpret_cast<uint4*>(tile + ch * kChunk + r * 128 + ((v + lane) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
+        if (dirty) clean(it, k0, tile, w);
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_clean[L % R]);
