@@ -586,6 +586,7 @@ at::Tensor cross_attention_call(const at::Tensor& q, const at::Tensor& k, const 
   a.kv_hi = edge(kv_hi, "kv_lens", edges[1]);
   at::Tensor first;
   if (slide > 0) {
+    TORCH_CHECK_VALUE(a.Sq < (1 << 29) && a.Sk < (1 << 29), "a length is too large");
     a.slide = (int)std::min<int64_t>(slide, std::numeric_limits<int>::max());
     a.sinks = (int)std::min<int64_t>(sinks, a.Sk);
     if (const at::Tensor* t = given(start)) {

@@ -161,6 +161,6 @@ extern "C" int dfl_cross_attention(const CrossArgs* a, cudaStream_t stream) {
   if (a->bits && ((a->bits_bs | a->bits_hs | a->bits_qs) % 4 || a->bias_tiles)) return -7;
   if (a->p2 && (a->bits || a->bias_tiles)) return -8;
   if (a->slide && (a->slide < 0 || a->sinks < 0 || a->bits || a->bias_tiles || a->p2 || a->kv_lo)) return -9;
-  if (a->slide && (a->splits < 1 || a->splits > kMaxParts || (a->splits > 1 && !a->parts) || !al16(a->parts) || (a->q_tiles != 1 && a->q_tiles != 2))) return -10;
+  if (a->slide && (a->splits < 1 || a->splits > kMaxParts || (a->splits > 1 && !a->parts) || !al16(a->parts) || (a->q_tiles != 1 && a->q_tiles != 2) || a->Sq >= (1 << 29) || a->Sk >= (1 << 29))) return -10;
   return a->f16 ? dfl_cross_attention_f16(a, stream) : cross_entry<false>(a, stream);
 }

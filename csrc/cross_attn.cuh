@@ -207,13 +207,17 @@ struct CrossItems {
 
 // The same where a window slides with the queries: the tiles of the first keys, then those of the window, or a part of them.
 // Heads first, the last queries before the first ones: blocks with many keys lead, those with few fill the last round
-// (12 heads x 32760 queries, window 9360: see the table).
+// (12 heads x 32760 queries, window 9360: 2145 -> 1926 us).  Measured and slower: a window's tiles from its first key on,
+// wherever that lies (24 heads x 8192, window 128: 95 -> 104 us), query tiles that pass over the tiles none of their rows sees (82 -> 87),
+// a fifth slot in place of the buffers that rows leave through (32760 queries: 1646 -> 1713).
 template <int QT>
 struct SlideItems {
   int q0, h, b, n;
-  int lo, hi, sinks; // keys that a query of this block may see: [0, sinks) and [lo, hi)
-  long long p0;      // position of the block's first query (a start may be any 32-bit value)
-  int sp, qb, ds, dh, db, dq, len, start, n_sink, t_win, j0;
+  int lo, hi, sinks;  // keys that a query of this block may see: [0, sinks) and [lo, hi)
+  // Query i sees key j where j <= i + start and j > i - back (back = slide - start; both held to +- 2^29, beyond every length: the
+  // launcher's limit, so 32 bits do)
+  int start, back;
+  int sp, qb, ds, dh, db, dq, len, n_sink, t_win, j0;
   DFL_DEVICE explicit SlideItems(const CrossParams& p) {
     const int i = blockIdx.x / p.splits, g = gridDim.x / p.splits;
     sp = blockIdx.x % p.splits, ds = gridDim.x % p.splits;
@@ -234,14 +238,15 @@ struct SlideItems {
   DFL_DEVICE void row(const CrossParams& p) {
     if (qb < 0) return;
     len = p.kv_hi ? min(p.Sk, max(0, __ldcg(p.kv_hi + b))) : p.Sk;
-    start = p.start ? __ldcg(p.start + b) : len - p.Sq;
+    const long long first = p.start ? __ldcg(p.start + b) : len - p.Sq;
+    start = (int)max(-(1ll << 29), min(1ll << 29, first));
+    back = (int)max(-(1ll << 29), min(1ll << 29, p.slide - first));
     block(p);
   }
   DFL_DEVICE void block(const CrossParams& p) {
     q0 = qb * (QT * kBM);
-    p0 = (long long)start + q0;
-    hi = (int)max(0ll, min((long long)len, (long long)start + min(q0 + QT * kBM, p.Sq)));
-    lo = (int)min((long long)p.Sk, max(0ll, p0 - p.slide + 1));
+    hi = max(0, min(len, start + min(q0 + QT * kBM, p.Sq)));
+    lo = min(p.Sk, max(0, q0 - back + 1));
     sinks = min(p.sinks, hi);
     n_sink = (sinks + kBN - 1) / kBN;
     t_win = max(n_sink, lo / kBN);
@@ -294,6 +299,19 @@ DFL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
   return d;
 }
 
+// Register split for QT = 2: 128 threads with 64 and 256 with 216, or 88 and 208 where the items' state needs more
+// (32760 queries: 1870 -> 1840 us).
+template <int MASK>
+DFL_DEVICE void fewer_registers() {
+  if constexpr (MASK == kSlide) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+}
+template <int MASK>
+DFL_DEVICE void more_registers() {
+  if constexpr (MASK == kSlide) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+}
+
 // P2: P goes to the product as the sum of two values of the inputs' type (2^-16 of p in bf16 where one value keeps 2^-8).
 template <int DH, bool F16, int QT, int MASK, bool P2>
 __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
@@ -344,10 +362,10 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
   // (launched while the kernel before it, the mask's own among them, ends: what that writes is read past L1)
   griddep_wait();
 
-  // Register split for QT = 2: 128 x 64 + 256 x 216 = 63488 <= 384 x 168 at launch (checked by the
-  // launcher); every warp of a warpgroup executes its setmaxnreg.
+  // Register split for QT = 2: 128 x 64 + 256 x 216 = 63488 (kSlide: 128 x 88 + 256 x 208 = 64512) <= 384 x 168 at launch
+  // (checked by the launcher); every warp of a warpgroup executes its setmaxnreg.
   if (warp == C::kProducerWarp) {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (QT == 2) fewer_registers<MASK>();
     if (lane == 0) {
       // load L (K_s: 2 s, V_s: 2 s + 1 over all steps s) goes to slot L % R, use (L / R)
       bool issued[R], q_issued[2] = {false, false};
@@ -399,7 +417,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       }
     }
   } else if (warp == C::kMmaWarp) {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (QT == 2) fewer_registers<MASK>();
     if (lane == 0) {
       constexpr uint32_t kF16Bits = F16 ? (1u << 7) | (1u << 10) : 0u;  // clears the two bf16 format bits
       constexpr uint32_t idesc_qk = make_idesc_bf16_f32(kBM, kBN, 0, 0) & ~kF16Bits;
@@ -485,7 +503,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       }
     }
   } else if (warp == C::kCleanWarp) {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (QT == 2) fewer_registers<MASK>();
     bool ok = true;
     int s = 0;
     auto clean = [&](const Items& it, int k0, uint8_t* tile, const uint32_t (&w)[4]) {
@@ -542,9 +560,9 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
       }
     }
   } else if (warp >= C::kProducerWarp) {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");  // the idle warp
+    if constexpr (QT == 2) fewer_registers<MASK>();  // the idle warp
   } else {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (QT == 2) more_registers<MASK>();
     const int g = warp / 4;
     const int row = (warp & 3) * 32 + lane;  // row of the Q tile == tensor-memory lane
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -621,9 +639,7 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         }
         if constexpr (MASK == kSlide) {
           // this row's keys, from k0 on: up to its own position, the last `slide` or the first `sinks` of them
-          const long long p_row = it.p0 + g * kBM + row;
-          const int up = (int)max(0ll, min(p_row + 1, (long long)it.hi)) - k0, sk = it.sinks - k0;
-          const int from = (int)max(0ll, min(p_row - p.slide + 1, (long long)p.Sk)) - k0;
+          const int up = min(qrow + it.start + 1, it.hi) - k0, from = qrow - it.back + 1 - k0, sk = it.sinks - k0;
           if (up < kBN || (from > 0 && sk < kBN)) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {  // (as bits: two instructions a score where the comparisons take five)
@@ -852,7 +868,7 @@ int launch_cross(const CrossArgs* a, CrossParams p, cudaStream_t stream, int dev
       cudaFuncAttributes fa;
       e = cudaFuncGetAttributes(&fa, kern);
       if (e != cudaSuccess) return (int)e;
-      if (fa.numRegs * C::kThreads < 128 * 64 + 256 * 216) return -11;
+      if (fa.numRegs * C::kThreads < (MASK == kSlide ? 128 * 88 + 256 * 208 : 128 * 64 + 256 * 216)) return -11;
     }
     attr[dev & 15] = true;
   }
