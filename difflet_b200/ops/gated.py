@@ -27,8 +27,10 @@ def gated_linear(x, w_gate, w_up, *, act="silu"):
             h = (F._nat or F._lib()).gated_linear(x, w_gate, w_up, F.GATED_ACTS[act])
             F.LAUNCHES[0] += 1
             return h
-        except ValueError:
+        except (ValueError, TypeError):
             pass
+    if isinstance(w_gate, F.MXWeight) or isinstance(w_up, F.MXWeight):
+        raise NotImplementedError("gated_linear with block-scaled weights: dequantize() them first")
     if act not in F.GATED_ACTS:
         raise ValueError(f"act {act!r}: one of {sorted(F.GATED_ACTS)}")
     if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:

@@ -13,7 +13,9 @@ Ops: ``attention``, ``linear`` (bias + optional GELU / SiLU on a column window),
 ``linear_gate_resid`` (``resid + gate * (x W^T + b)``), ``ln_modulate`` (LayerNorm / RMSNorm
 with affine and per-batch shift / scale), ``rms_norm``, ``quantize_mx`` (OCP-MX E4M3 +
 E8M0 per 32), ``linear_mx`` (block-scaled GEMM on quantized operands), ``gemv``,
-``add_rms_norm`` (residual addition + RMSNorm), ``cross_attention`` (masks, key counts, shared key heads).
+``add_rms_norm`` (residual addition + RMSNorm), ``cross_attention`` (masks, key counts, shared key heads),
+``window_attention`` (causal, the last and the first keys), ``gated_linear`` (act(x W_gate^T) * (x W_up^T)) and
+``embedding`` (scaled rows of a table); the last two record gradients as ``ops.gated_linear`` and ``ops.embedding`` only.
 """
 
 from __future__ import annotations
@@ -177,7 +179,47 @@ def _(q, k, v, scale, attention_mask=None, kv_lens=None):
     return torch.empty_like(q)
 
 
+@torch.library.custom_op(f"{_NS}::window_attention", mutates_args=())
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
+                     kv_lens: Optional[torch.Tensor] = None, q_start: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention to the last ``window`` and the first ``sinks`` keys of a cache."""
+    from difflet_b200.ops.attn import window_attention as _window
+
+    return _window(q, k, v, window=window, sinks=sinks, scale=scale, kv_lens=kv_lens, q_start=q_start)
+
+
+@window_attention.register_fake
+def _(q, k, v, scale, window, sinks=0, kv_lens=None, q_start=None):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op(f"{_NS}::gated_linear", mutates_args=())
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: str = "silu") -> torch.Tensor:
+    """act(x w_gate^T) * (x w_up^T)."""
+    from difflet_b200.ops.gated import gated_linear as _gated
+
+    return _gated(x, w_gate, w_up, act=act)
+
+
+@gated_linear.register_fake
+def _(x, w_gate, w_up, act="silu"):
+    return x.new_empty(x.shape[:-1] + (w_gate.shape[0],))
+
+
+@torch.library.custom_op(f"{_NS}::embedding", mutates_args=())
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[ids]."""
+    from difflet_b200.ops.embeddings import embedding as _embedding
+
+    return _embedding(ids, weight, scale=scale)
+
+
+@embedding.register_fake
+def _(ids, weight, scale=1.0):
+    return weight.new_empty(ids.shape + (weight.shape[1],))
+
+
 OPS = ("attention", "linear", "linear_gate_resid", "ln_modulate", "rms_norm", "quantize_mx", "linear_mx", "gemv",
-       "add_rms_norm", "cross_attention")
+       "add_rms_norm", "cross_attention", "window_attention", "gated_linear", "embedding")
 
 __all__ = list(OPS)
