@@ -46,7 +46,7 @@ bool is16(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.sc
 at::Tensor rows_of(const at::Tensor& x, int64_t M, int64_t K) { return rows16(x.dim() == 2 ? x : x.reshape({M, K})); }
 
 // x [..., K], wg / wu [F, K] of one 16-bit type -> h [..., F]; kept: where the projections are wanted for the gradients,
-// [2, M, F] with padded rows.
+// f32 [2, M, F] with padded rows.
 at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act, at::Tensor* kept) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && wg.dim() == 2 && wu.dim() == 2, "x [..., K] and weights [F, K] must be CUDA tensors");
   TORCH_CHECK_VALUE(is16(x), "gated_linear runs in bfloat16 or float16 on CUDA, got ", x.scalar_type());
@@ -63,14 +63,14 @@ at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Te
   const int64_t M = x.numel() / K, Fp = (F + 7) / 8 * 8;
   TORCH_CHECK_VALUE(M < (1ll << 30), "too many rows");
   GluArgs a{};
-  if (kept) *kept = new_like(x, {2, M, Fp}, x.scalar_type());
+  if (kept) *kept = new_like(x, {2, M, Fp}, at::kFloat);
   if (M == 0 || F == 0) return h;
   const at::Tensor x2 = rows_of(x, M, K), g2 = rows16(wg), u2 = rows16(wu);
   a.x = x2.data_ptr(), a.ldx = row_stride(x2);
   a.wg = g2.data_ptr(), a.ldwg = row_stride(g2);
   a.wu = u2.data_ptr(), a.ldwu = row_stride(u2);
   a.h = h.data_ptr(), a.ldh = F;
-  if (kept) a.g = kept->data_ptr(), a.u = reinterpret_cast<uint16_t*>(a.g) + M * Fp, a.lds = Fp;
+  if (kept) a.g = kept->data_ptr<float>(), a.u = a.g + M * Fp, a.lds = Fp;
   a.M = (int)M, a.K = (int)K, a.F = (int)F, a.act = (int)act;
   a.f16 = x.scalar_type() == at::kHalf;
   a.err = err_ptr();
@@ -102,7 +102,7 @@ variable_list gated_backward(const at::Tensor& dh, const at::Tensor& x, const at
   const at::Tensor dgu = new_like(x, {2, M, Fp}, x.scalar_type());
   GluGradArgs e{};
   e.dh = d2.data_ptr(), e.lddh = M > 1 ? d2.stride(0) : F;
-  e.g = kept.data_ptr(), e.u = reinterpret_cast<const uint16_t*>(e.g) + M * Fp, e.lds = Fp;
+  e.g = kept.data_ptr<float>(), e.u = e.g + M * Fp, e.lds = Fp;
   e.dg = dgu.data_ptr(), e.du = reinterpret_cast<uint16_t*>(e.dg) + M * Fp;
   e.M = M, e.F = (int)F, e.act = (int)act, e.f16 = x.scalar_type() == at::kHalf;
   DFL_CHECK_RC(dfl_glu_grad(&e, cur_stream()), "gated_linear (gradient of the product)");

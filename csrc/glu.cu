@@ -7,9 +7,9 @@
 // ring of shared-memory stages filled by tiled copies):
 //   forward  an accumulator holds the same columns of g and u side by side (Wg's and Wu's rows are the two halves of the
 //            tile's second operand; in a CTA pair each CTA loads one of them), so act(g) * u needs no exchange; x is read
-//            once for both.  With gradients to come, g and u are stored too, rounded to the type (at most 2^-8 of each
-//            value in bf16; the gradients are rounded to it anyway: the alternative, computing them again, costs another
-//            4 M F K operations).
+//            once for both.  With gradients to come, g and u are stored too, in f32: rounded to the type they made the
+//            gradients' error 1.8 times that of their own rounding, where the rounding of dg and du alone makes it 1.4 times
+//            (4 M F bytes more to write and to read: 3 % of a 4096 x 3584 x 18944 step; computing them again: 4 M F K operations).
 //   dx       the K loop runs over dg Wg, then du Wu, in one accumulator; the weights are read as they lie ([F, K]: the
 //            second operand with its columns contiguous)
 //   dW       both operands lie with their columns contiguous ([M, F] and [M, K]); nothing is transposed in memory
@@ -48,8 +48,8 @@ constexpr int kGroupM = 16;  // tile raster: 16 M blocks per group, for L2 reuse
 struct GluParams {
   CUtensorMap a[2], b[2];
   void* d[2];        // outputs (forward: h; dW: one for each problem)
-  void* g;           // forward: the kept projections
-  void* u;
+  float* g;          // forward: the kept projections
+  float* u;
   long long ldd, lds;
   int M, N, K;       // of one problem: rows and columns of the output, length of the sums (of each segment)
   int num_m, num_n, tiles;  // tiles of one problem
@@ -151,6 +151,12 @@ DFL_DEVICE Tile tile_of(const GluParams& p, int t) {
   return r;
 }
 
+// A whole 32-byte sector at once: a row a lane, stores of 16 bytes would write every sector twice.
+DFL_DEVICE void st_sector(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h)
+               : "memory");
+}
+
 // 32 columns of the rows of a warp (lane: row): whole 16-byte pieces where every row allows it, else through shared memory, so that
 // the lanes write along a row (a row each would cost a line per lane and value).
 template <bool F16>
@@ -161,10 +167,16 @@ DFL_DEVICE void store_cols(void* base, long long row0, int rows, long long ld, i
 #pragma unroll
   for (int q = 0; q < 16; ++q) w[q] = pack2<F16>(v[2 * q], v[2 * q + 1]);
   if (wide && cols >= 32) {
-    uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + (row0 + lane) * ld + col);
-    if (lane < rows)
+    uint16_t* d = reinterpret_cast<uint16_t*>(base) + (row0 + lane) * ld + col;
+    if (lane >= rows) return;
+    if (ld % 16 == 0 && (reinterpret_cast<uintptr_t>(base) & 31) == 0) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) d[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      for (int q = 0; q < 2; ++q)
+        st_sector(d + 16 * q, w[8 * q], w[8 * q + 1], w[8 * q + 2], w[8 * q + 3], w[8 * q + 4], w[8 * q + 5], w[8 * q + 6], w[8 * q + 7]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) reinterpret_cast<uint4*>(d)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    }
     return;
   }
   __syncwarp();
@@ -174,6 +186,20 @@ DFL_DEVICE void store_cols(void* base, long long row0, int rows, long long ld, i
   uint16_t* d = reinterpret_cast<uint16_t*>(base) + row0 * ld + col + lane;
   if (lane < cols)
     for (int r = 0; r < rows; ++r) d[r * ld] = stage[r][lane];
+}
+
+DFL_DEVICE void keep_cols(float* d, const float (&v)[32], int cols) {  // (rows are 32-byte aligned)
+  if (cols >= 32) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      st_sector(d + 8 * q, __float_as_uint(v[8 * q]), __float_as_uint(v[8 * q + 1]), __float_as_uint(v[8 * q + 2]),
+                __float_as_uint(v[8 * q + 3]), __float_as_uint(v[8 * q + 4]), __float_as_uint(v[8 * q + 5]),
+                __float_as_uint(v[8 * q + 6]), __float_as_uint(v[8 * q + 7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < cols) d[j] = v[j];
+  }
 }
 
 template <int CG>
@@ -357,7 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
           tmem_wait_ld();
           if (c + 32 == (half + 1) * (BN / 2)) release();
 #pragma unroll
-          for (int q = 0; q < 8; ++q) reinterpret_cast<uint4*>(part + c)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+          for (int q = 0; q < 4; ++q)
+            st_sector(part + c + 8 * q, r[8 * q], r[8 * q + 1], r[8 * q + 2], r[8 * q + 3], r[8 * q + 4], r[8 * q + 5], r[8 * q + 6], r[8 * q + 7]);
         }
       } else if constexpr (MODE == kForward) {
         const bool wide = p.ldd % 8 == 0 && (reinterpret_cast<uintptr_t>(p.d[0]) & 15) == 0;
@@ -374,8 +401,10 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
 #pragma unroll
           for (int j = 0; j < 32; ++j) g[j] = __uint_as_float(gr[j]), u[j] = __uint_as_float(ur[j]);
           if (p.g) {
-            store_cols<F16>(p.g, row0, rows, p.lds, col, g, cols, true, stage_rows);
-            store_cols<F16>(p.u, row0, rows, p.lds, col, u, cols, true, stage_rows);
+            if (lane < rows) {
+              keep_cols(p.g + row * p.lds + col, g, cols);
+              keep_cols(p.u + row * p.lds + col, u, cols);
+            }
           }
           if (p.act == kGluSilu) {
 #pragma unroll
@@ -504,7 +533,7 @@ __global__ void __launch_bounds__(256, NB == 4 ? 1 : 2) glu_rows_kernel(GluArgs 
     float g = 0.f, u = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) g += red[k][0][n][m], u += red[k][1][n][m];
-    if (a.g) store1<F16>(a.g, m * a.lds + col, g), store1<F16>(a.u, m * a.lds + col, u);
+    if (a.g) a.g[m * a.lds + col] = g, a.u[m * a.lds + col] = u;
     const float v = a.act == kGluSilu ? act_of<kGluSilu>(g) : a.act == kGluGelu ? act_of<kGluGelu>(g) : act_of<kGluGeluErf>(g);
     store1<F16>(a.h, m * a.ldh + col, v * u);
   }
@@ -540,7 +569,7 @@ __global__ void __launch_bounds__(256) glu_join_kernel(const __grid_constant__ G
       if (col + e >= p.N) break;
       if constexpr (MODE == kForward) {
         const float g = v[0][e], u = v[1][e];
-        if (p.g) store1<F16>(p.g, row * p.lds + col + e, g), store1<F16>(p.u, row * p.lds + col + e, u);
+        if (p.g) p.g[row * p.lds + col + e] = g, p.u[row * p.lds + col + e] = u;
         const float a = p.act == kGluSilu ? act_of<kGluSilu>(g) : p.act == kGluGelu ? act_of<kGluGelu>(g) : act_of<kGluGeluErf>(g);
         store1<F16>(p.d[0], row * p.ldd + col + e, a * u);
       } else {
@@ -550,7 +579,7 @@ __global__ void __launch_bounds__(256) glu_join_kernel(const __grid_constant__ G
   }
 }
 
-// dg, du: 8 columns a thread.  Bound by its bytes (10 M F).
+// dg, du: 8 columns a thread.  Bound by its bytes (14 M F): 4096 x 18944 see gated_train in the table.
 template <bool F16, int ACT>
 __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
   griddep_wait();
@@ -562,11 +591,15 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
     const int col = (int)(i - row * per_row) * 8, cols = min(8, a.F - col);
     const long long at = row * a.lds + col;
     // (the rows of g, u, dg and du are padded to whole pieces)
-    const uint4 gv = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.g) + at));
-    const uint4 uv = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.u) + at));
-    float d[8];
+    float g[8], u[8], d[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(a.g + at) + h), y = __ldcs(reinterpret_cast<const float4*>(a.u + at) + h);
+      g[4 * h] = x.x, g[4 * h + 1] = x.y, g[4 * h + 2] = x.z, g[4 * h + 3] = x.w;
+      u[4 * h] = y.x, u[4 * h + 1] = y.y, u[4 * h + 2] = y.z, u[4 * h + 3] = y.w;
+    }
     if (wide && cols == 8) {
-      const uint4 dv = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.dh) + row * a.lddh + col));
+      const uint4 dv = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.dh) + row * a.lddh + col));
       const uint32_t w[4] = {dv.x, dv.y, dv.z, dv.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -577,13 +610,11 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = e < cols ? load1<F16>(a.dh, row * a.lddh + col + e) : 0.f;
     }
-    const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
     uint32_t og[4], ou[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 g = unpack2<F16>(gw[e]), u = unpack2<F16>(uw[e]);
-      const float2 x = act_grad<ACT>(g.x), y = act_grad<ACT>(g.y);
-      og[e] = pack2<F16>(d[2 * e] * u.x * x.y, d[2 * e + 1] * u.y * y.y);
+      const float2 x = act_grad<ACT>(g[2 * e]), y = act_grad<ACT>(g[2 * e + 1]);
+      og[e] = pack2<F16>(d[2 * e] * u[2 * e] * x.y, d[2 * e + 1] * u[2 * e + 1] * y.y);
       ou[e] = pack2<F16>(d[2 * e] * x.x, d[2 * e + 1] * y.x);
     }
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.dg) + at) = make_uint4(og[0], og[1], og[2], og[3]);
@@ -702,7 +733,8 @@ extern "C" long long dfl_glu_ws(int what, int M, int K, int F) {
 extern "C" int dfl_glu(const GluArgs* a, cudaStream_t stream) {
   if (a->M <= 0 || a->F <= 0 || a->K <= 0 || a->K % 8 || a->act < 0 || a->act > kGluGeluErf) return -2;
   if (!al16(a->x) || !al16(a->wg) || !al16(a->wu) || (a->ldx | a->ldwg | a->ldwu) % 8) return -3;
-  if (a->g && (!a->u || !al16(a->g) || !al16(a->u) || a->lds % 8 || a->lds < a->F)) return -4;
+  auto al32 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 31) == 0; };
+  if (a->g && (!a->u || !al32(a->g) || !al32(a->u) || a->lds % 8 || a->lds < a->F)) return -4;
   if (a->M <= kRowsMax) return a->f16 ? launch_rows<true>(a, stream) : launch_rows<false>(a, stream);
   int dev = 0;
   cudaGetDevice(&dev);
@@ -721,7 +753,7 @@ extern "C" int dfl_glu(const GluArgs* a, cudaStream_t stream) {
   p.M = a->M, p.N = a->F, p.K = a->K, p.act = a->act;
   rc = setup<kForward>(p, plan, 1);
   if (rc) return rc;
-  if (ws_floats(plan, p.items) > a->ws_floats || !al16(a->ws)) return -10;
+  if (ws_floats(plan, p.items) > a->ws_floats || (reinterpret_cast<uintptr_t>(a->ws) & 31)) return -10;
   p.ws = a->ws;
   return launch_mode<kForward>(p, plan, a->f16, sms, dev, a->err, stream);
 }
@@ -764,7 +796,7 @@ extern "C" int dfl_glu_dx(const GluGemmArgs* a, cudaStream_t stream) {
   p.M = a->M, p.N = a->K, p.K = a->F;
   rc = setup<kDx>(p, plan, 1);
   if (rc) return rc;
-  if (ws_floats(plan, p.items) > a->ws_floats || !al16(a->ws)) return -10;
+  if (ws_floats(plan, p.items) > a->ws_floats || (reinterpret_cast<uintptr_t>(a->ws) & 31)) return -10;
   p.ws = a->ws;
   return launch_mode<kDx>(p, plan, a->f16, sms, dev, a->err, stream);
 }
@@ -793,7 +825,7 @@ extern "C" int dfl_glu_dw(const GluGemmArgs* a, cudaStream_t stream) {
   p.M = a->F, p.N = a->K, p.K = a->M;
   rc = setup<kDw>(p, plan, problems);
   if (rc) return rc;
-  if (ws_floats(plan, p.items) > a->ws_floats || !al16(a->ws)) return -10;
+  if (ws_floats(plan, p.items) > a->ws_floats || (reinterpret_cast<uintptr_t>(a->ws) & 31)) return -10;
   p.ws = a->ws;
   return launch_mode<kDw>(p, plan, a->f16, sms, dev, a->err, stream);
 }

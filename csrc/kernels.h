@@ -503,21 +503,21 @@ int dfl_rel_l1(const void* a, const void* b, long long n, float* scratch, int bl
 // ------------------------------------------------------------------ gated projection
 enum { kGluSilu = 0, kGluGelu = 1, kGluGeluErf = 2 };  // activations (kGluGelu: tanh form)
 // h = act(x Wg^T) * (x Wu^T); with g / u the two projections are kept beside it (for the gradients).  16-bit types
-// (f16: fp16, else bf16); row strides in elements, 16-byte aligned rows of x, wg, wu, g and u, any rows of h.
+// (f16: fp16, else bf16), g and u f32; row strides in elements, 16-byte aligned rows of x, wg, wu, g and u, any rows of h.
 typedef struct GluArgs {
   const void* x; const void* wg; const void* wu;  // [M, K], [F, K], [F, K]
   long long ldx, ldwg, ldwu;
   void* h; long long ldh;                         // [M, F]
-  void* g; void* u; long long lds;                // [M, F] or NULL
+  float* g; float* u; long long lds;              // [M, F] or NULL
   int M, K, F, act, f16;
   float* ws; long long ws_floats;                 // dfl_glu_ws(0, ...) or NULL
   int* err;
 } GluArgs;
 int dfl_glu(const GluArgs* a, cudaStream_t stream);
-// dg = dh * u * act'(g), du = dh * act(g): [M, F]; rows of g, u, dg and du 16-byte aligned, of dh any.
+// dg = dh * u * act'(g), du = dh * act(g): [M, F]; rows of g, u, dg and du lds elements (a multiple of 8) apart, of dh any.
 typedef struct GluGradArgs {
   const void* dh; long long lddh;
-  const void* g; const void* u; void* dg; void* du; long long lds;
+  const float* g; const float* u; void* dg; void* du; long long lds;
   long long M;
   int F, act, f16;
 } GluGradArgs;
