@@ -279,13 +279,14 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   }
 }
 
-// A warp takes 32 U pieces of an item: lane l the pieces l, l + 32, ...; the next item is on its way meanwhile.
-// 16384 tokens of 8000 ids x 3584, bf16: see embed_train in the table; U = 4 with two tokens in flight 104 us, U = 1 with eight
-// (and the item read when its turn comes) 61.
+// A warp takes 32 U pieces of an item: lane l the pieces l, l + 32, ...; the next item is on its way meanwhile.  What counts is
+// the loads in flight (most ids occur once): the whole gradient of 16384 tokens x 3584 over 152064 rows takes 240 us with three CTAs an SM,
+// U = 2 and four tokens in flight (two CTAs 247; U = 4 and two tokens 254, U = 1 and four 250, and eight 254), 32768 tokens
+// x 4096 over 32000 rows 166 (181, 172, 186, 196).
 constexpr int kU = 2, kTokens = 4;
 
 template <int DT, int VEC>
-__global__ void __launch_bounds__(256) embed_sum_kernel(EmbedGradArgs a, EmbedWs w) {
+__global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, EmbedWs w) {
   using V = Value<DT>;
   using P = Piece<typename V::T, VEC>;
   griddep_wait();

@@ -545,37 +545,37 @@ int launch_rows(const GluArgs* a, cudaStream_t stream) {
   return (int)dfl_host::launch_early(kern, (unsigned)((a->F + 15) / 16), 256, 0, stream, *a);
 }
 
-// The rest's tiles from their parts, added in order: a thread takes 4 columns of a row.
-template <int MODE, bool F16>
-__global__ void __launch_bounds__(256) glu_join_kernel(const __grid_constant__ GluParams p, int rows, int BN, int rest) {
+// The rest's tiles from their parts, added in order: a thread takes 4 columns of a row.  (A block stays within a tile.)
+template <int MODE, int ROWS, int BN, bool F16>
+__global__ void __launch_bounds__(256) glu_join_kernel(const __grid_constant__ GluParams p) {
   griddep_wait();
-  const int cols = MODE == kForward ? BN / 2 : BN, quads = cols / 4;
-  const long long n = (long long)rest * rows * quads, tile = (long long)rows * BN;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const int q = (int)(i % quads) * 4, r = (int)(i / quads % rows), t = (int)(i / quads / rows);
-    const Tile it = tile_of<MODE>(p, p.whole + t * p.splits);
-    const int row = it.mb * rows + r, col = it.nb * cols + q;
-    if (row >= p.M || col >= p.N) continue;
-    const float* from = p.ws + (long long)t * p.splits * tile + (long long)r * BN + q;
-    float v[2][4] = {};
-    for (int s = 0; s < p.splits; ++s)
+  constexpr int kCols = MODE == kForward ? BN / 2 : BN, kQuads = kCols / 4, kBlocks = ROWS * kQuads / 256;
+  constexpr int kTile = ROWS * BN;
+  const int t = blockIdx.x / kBlocks, i = blockIdx.x % kBlocks * 256 + threadIdx.x, r = i / kQuads, q = i % kQuads * 4;
+  const Tile it = tile_of<MODE>(p, p.whole + t * p.splits);
+  const int row = it.mb * ROWS + r, col = it.nb * kCols + q;
+  if (row >= p.M || col >= p.N) return;
+  const float* from = p.ws + (long long)t * p.splits * kTile + r * BN + q;
+  float v[2][4] = {};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s)
 #pragma unroll
-      for (int h = 0; h < (MODE == kForward ? 2 : 1); ++h) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(from + s * tile + h * cols));
-        v[h][0] += x.x, v[h][1] += x.y, v[h][2] += x.z, v[h][3] += x.w;
-      }
+    for (int h = 0; h < (MODE == kForward ? 2 : 1); ++h) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(from + (long long)s * kTile + h * kCols));
+      v[h][0] += x.x, v[h][1] += x.y, v[h][2] += x.z, v[h][3] += x.w;
+    }
+  if constexpr (MODE == kForward) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (col + e >= p.N) break;
-      if constexpr (MODE == kForward) {
-        const float g = v[0][e], u = v[1][e];
-        if (p.g) p.g[row * p.lds + col + e] = g, p.u[row * p.lds + col + e] = u;
-        const float a = p.act == kGluSilu ? act_of<kGluSilu>(g) : p.act == kGluGelu ? act_of<kGluGelu>(g) : act_of<kGluGeluErf>(g);
-        store1<F16>(p.d[0], row * p.ldd + col + e, a * u);
-      } else {
-        store1<F16>(p.d[it.which], row * p.ldd + col + e, v[0][e]);
-      }
+      const float g = v[0][e], u = v[1][e];
+      if (p.g) p.g[row * p.lds + col + e] = g, p.u[row * p.lds + col + e] = u;
+      const float a = p.act == kGluSilu ? act_of<kGluSilu>(g) : p.act == kGluGelu ? act_of<kGluGelu>(g) : act_of<kGluGeluErf>(g);
+      store1<F16>(p.d[0], row * p.ldd + col + e, a * u);
     }
+  } else {  // (N and the rows' pitch are multiples of 8)
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.d[it.which]) + row * p.ldd + col) =
+        make_uint2(pack2<F16>(v[0][0], v[0][1]), pack2<F16>(v[0][2], v[0][3]));
   }
 }
 
@@ -697,9 +697,8 @@ int launch_glu(const GluParams& p, int sms, int dev, int* err, cudaStream_t stre
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, err);
   if (e != cudaSuccess || p.splits == 1) return (int)e;
   const int rest = (p.items - p.whole) / p.splits;
-  const long long threads = (long long)rest * BM * CG * (MODE == kForward ? BN / 8 : BN / 4);
-  return (int)dfl_host::launch_early(glu_join_kernel<MODE, F16>, (unsigned)std::min<long long>((threads + 255) / 256, 148 * 8), 256, 0, stream, p,
-                                     BM * CG, BN, rest);
+  constexpr int rows = BM * CG, blocks = rows * (MODE == kForward ? BN / 8 : BN / 4) / 256;
+  return (int)dfl_host::launch_early(glu_join_kernel<MODE, rows, BN, F16>, (unsigned)(rest * blocks), 256, 0, stream, p);
 }
 
 template <int MODE>
