@@ -13,6 +13,7 @@
 //                      kept in f32 and added in order by the last warp of the piece.
 // A sort by value is not needed for that, and a scan over the vocabulary neither.
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -73,7 +74,8 @@ inline long long embed_layout(long long n, long long V, int D, char* base, Embed
 }
 
 DFL_DEVICE long long id_at(const void* ids, int bytes, long long i) {
-  return bytes == 8 ? __ldg(reinterpret_cast<const long long*>(ids) + i) : (long long)__ldg(reinterpret_cast<const int*>(ids) + i);
+  // (launched while the kernel before ends: what that writes is read past L1, here and below)
+  return bytes == 8 ? __ldcg(reinterpret_cast<const long long*>(ids) + i) : (long long)__ldcg(reinterpret_cast<const int*>(ids) + i);
 }
 
 // Types: a piece is VEC values.
@@ -101,36 +103,108 @@ struct Value<kDtypeF16> {
   static DFL_DEVICE T put(float v) { return __half_as_ushort(__float2half_rn(v)); }
 };
 
-template <class T, int VEC>
-struct alignas(sizeof(T) * VEC) Piece {
-  T v[VEC];
-};
-
-template <int DT, int VEC>
-__global__ void __launch_bounds__(256) embed_kernel(EmbedArgs a, int lanes) {
-  using V = Value<DT>;
-  using P = Piece<typename V::T, VEC>;
-  griddep_wait();
-  const int pieces = a.D / VEC, sub = threadIdx.x / lanes, lane = threadIdx.x % lanes, rows = 256 / lanes;
-  for (long long i = (long long)blockIdx.x * rows + sub; i < a.n; i += (long long)gridDim.x * rows) {
-    const long long id = id_at(a.ids, a.id_bytes, i);
-    const bool in = id >= 0 && id < a.V;
-    if (!in && lane == 0) record_error(a.err, kErrBounds, kKidEmbed, 1, (int)i);
-    const P* __restrict__ src = reinterpret_cast<const P*>(reinterpret_cast<const typename V::T*>(a.w) + (in ? id * a.ldw : 0));
-    P* __restrict__ dst = reinterpret_cast<P*>(reinterpret_cast<typename V::T*>(a.y) + i * a.D);
-    for (int c0 = lane; c0 < pieces; c0 += 4 * lanes) {
-      P x[4];
+// A piece: 16 bytes (WIDE) or a single value, and its values added to s.
+template <int DT, bool WIDE>
+struct Piece {
+  using T = typename Value<DT>::T;
+  static constexpr int N = WIDE ? Value<DT>::kWide : 1;
+  using R = std::conditional_t<WIDE, uint4, T>;
+  static DFL_DEVICE R load(const T* p) { return __ldcg(reinterpret_cast<const R*>(p)); }
+  static DFL_DEVICE void add(float (&s)[N], R r) {
+    if constexpr (!WIDE) {
+      s[0] += Value<DT>::get(r);
+    } else {
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (in && c0 + u * lanes < pieces) x[u] = src[c0 + u * lanes];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (c0 + u * lanes >= pieces) break;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[u].v[e] = in ? V::put(a.scale * V::get(x[u].v[e])) : V::put(0.f);
-        dst[c0 + u * lanes] = x[u];
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == kDtypeF32) {
+          s[i] += __uint_as_float(w[i]);
+        } else {
+          float2 f;
+          if constexpr (DT == kDtypeBf16) f = unpack_bf16x2(w[i]);
+          else f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          s[2 * i] += f.x, s[2 * i + 1] += f.y;
+        }
       }
     }
+  }
+  static DFL_DEVICE void store(T* p, const float (&s)[N], float scale) {
+    if constexpr (!WIDE) {
+      *p = Value<DT>::put(scale * s[0]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == kDtypeF32) {
+          w[i] = __float_as_uint(scale * s[i]);
+        } else if constexpr (DT == kDtypeBf16) {
+          w[i] = pack_bf16x2(scale * s[2 * i], scale * s[2 * i + 1]);
+        } else {
+          const __half2 h = __floats2half2_rn(scale * s[2 * i], scale * s[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+};
+
+// A piece of 16 bytes, each of its values times s.
+template <int DT>
+DFL_DEVICE uint32_t scaled_word(uint32_t w, float s) {
+  if constexpr (DT == kDtypeF32) {
+    return __float_as_uint(s * __uint_as_float(w));
+  } else if constexpr (DT == kDtypeBf16) {
+    const float2 f = unpack_bf16x2(w);
+    return pack_bf16x2(s * f.x, s * f.y);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
+    const __half2 h = __floats2half2_rn(s * f.x, s * f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// `lanes` threads to a row, four pieces of it (WIDE: of 16 bytes, else single values) in flight in each; the next row's id is on
+// its way meanwhile.
+template <int DT, bool WIDE>
+__global__ void __launch_bounds__(256, 5) embed_kernel(EmbedArgs a, int lanes) {
+  using V = Value<DT>;
+  using T = typename V::T;
+  griddep_wait();
+  const int pieces = WIDE ? a.D / V::kWide : a.D, lane = threadIdx.x % lanes, rows = 256 / lanes;
+  const long long step = (long long)gridDim.x * rows;
+  long long i = (long long)blockIdx.x * rows + threadIdx.x / lanes;
+  if (i >= a.n) return;
+  long long id = id_at(a.ids, a.id_bytes, i);
+  for (; i < a.n; i += step) {
+    const long long next = id_at(a.ids, a.id_bytes, min(i + step, a.n - 1));
+    const bool in = id >= 0 && id < a.V;
+    if (!in && lane == 0) record_error(a.err, kErrBounds, kKidEmbed, 1, (int)i);
+    const T* src = reinterpret_cast<const T*>(a.w) + (in ? id * a.ldw : 0);
+    T* dst = reinterpret_cast<T*>(a.y) + i * a.D;
+    for (int c = lane; c < pieces; c += 4 * lanes) {
+      const int n = in ? (pieces - c + lanes - 1) / lanes : 0;  // pieces of this thread from here on
+      if constexpr (WIDE) {
+        const uint4* s = reinterpret_cast<const uint4*>(src) + c;
+        uint4* d = reinterpret_cast<uint4*>(dst) + c;
+        uint4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = u < n ? __ldcg(s + u * lanes) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (c + u * lanes < pieces)
+            d[u * lanes] = make_uint4(scaled_word<DT>(x[u].x, a.scale), scaled_word<DT>(x[u].y, a.scale), scaled_word<DT>(x[u].z, a.scale),
+                                      scaled_word<DT>(x[u].w, a.scale));
+      } else {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = u < n ? V::get(__ldcg(src + c + u * lanes)) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (c + u * lanes < pieces) dst[c + u * lanes] = V::put(a.scale * x[u]);
+      }
+    }
+    id = next;
   }
 }
 
@@ -280,35 +354,42 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
 }
 
 // A warp takes 32 U pieces of an item: lane l the pieces l, l + 32, ...; the next item is on its way meanwhile.  What counts is
-// the loads in flight (most ids occur once): the whole gradient of 16384 tokens x 3584 over 152064 rows takes 240 us with three CTAs an SM,
+// the loads in flight (most ids occur once): the whole gradient of 16384 tokens x 3584 over 152064 rows took 240 us with three CTAs an SM,
 // U = 2 and four tokens in flight (two CTAs 247; U = 4 and two tokens 254, U = 1 and four 250, and eight 254), 32768 tokens
-// x 4096 over 32000 rows 166 (181, 172, 186, 196).
+// x 4096 over 32000 rows 166 (181, 172, 186, 196); the pieces as whole words 221 and 164.
 constexpr int kU = 2, kTokens = 4;
 
-template <int DT, int VEC>
+template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, EmbedWs w) {
-  using V = Value<DT>;
-  using P = Piece<typename V::T, VEC>;
+  using P = Piece<DT, WIDE>;
+  using T = typename P::T;
+  constexpr int VEC = P::N;
   griddep_wait();
   const int lane = threadIdx.x % 32, pieces = a.D / VEC, chunks = (pieces + 32 * kU - 1) / (32 * kU);
   const long long warps = (long long)gridDim.x * 8, me = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const typename V::T* __restrict__ dy = reinterpret_cast<const typename V::T*>(a.dy);
-  typename V::T* dw = reinterpret_cast<typename V::T*>(a.dw);
+  const T* dy = reinterpret_cast<const T*>(a.dy);
+  T* dw = reinterpret_cast<T*>(a.dw);
 
-  const long long items = (long long)__ldcg(w.head + 2) * chunks;
+  // (item, chunk) by item * chunks + chunk, advanced without divisions
+  const int items = __ldcg(w.head + 2), d_item = (int)(warps / chunks), d_chunk = (int)(warps % chunks);
+  long long item = me / chunks;
+  int chunk = (int)(me % chunks);
   Item it{};
   int t0 = 0, t1 = 0;
   auto tokens = [&] {  // the item's tokens, one or two to a lane
     t0 = it.order == kOnly ? it.begin : lane < it.len ? __ldcg(w.list + it.begin + lane) : 0x7fffffff;
     t1 = lane + 32 < it.len ? __ldcg(w.list + it.begin + 32 + lane) : 0;
   };
-  if (me < items) {
-    it = w.items[me / chunks];
+  if (item < items) {
+    it = w.items[item];
     tokens();
   }
-  for (long long t = me; t < items; t += warps) {
-    const Item nx = w.items[min(t + warps, items - 1) / chunks];
-    const int chunk = (int)(t % chunks), c0 = chunk * 32 * kU + lane;
+  while (item < items) {
+    int to_chunk = chunk + d_chunk;
+    item += d_item + (to_chunk >= chunks);
+    to_chunk -= to_chunk >= chunks ? chunks : 0;
+    const Item nx = w.items[min(item, items - 1ll)];
+    const int c0 = chunk * 32 * kU + lane;
     float s[kU][VEC];
 #pragma unroll
     for (int u = 0; u < kU; ++u)
@@ -324,21 +405,19 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
       }
     }
     for (int k = 0; k < it.len; k += kTokens) {
-      P x[kTokens][kU];
+      typename P::R x[kTokens][kU];
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) {
         if (k + j >= it.len) break;
-        const P* src = reinterpret_cast<const P*>(dy + (long long)__shfl_sync(0xffffffffu, k < 32 ? t0 : t1, (k + j) % 32) * a.D);
+        const T* src = dy + (long long)__shfl_sync(0xffffffffu, k < 32 ? t0 : t1, (k + j) % 32) * a.D;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) x[j][u] = src[min(c0 + 32 * u, pieces - 1)];  // (lanes past the row's end read it, and store nothing)
+        for (int u = 0; u < kU; ++u) x[j][u] = P::load(src + min(c0 + 32 * u, pieces - 1) * VEC);  // (lanes past the row's end read it, and store nothing)
       }
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) {
         if (k + j >= it.len) break;
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[u][e] += V::get(x[j][u].v[e]);
+        for (int u = 0; u < kU; ++u) P::add(s[u], x[j][u]);
       }
     }
     bool whole = true;
@@ -369,12 +448,9 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       if (!whole || c0 + 32 * u >= pieces) break;
-      P x;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x.v[e] = V::put(a.scale * s[u][e]);
-      reinterpret_cast<P*>(dw + it.row * (long long)a.D)[c0 + 32 * u] = x;
+      P::store(dw + it.row * (long long)a.D + (c0 + 32 * u) * VEC, s[u], a.scale);
     }
-    it = nx;
+    it = nx, chunk = to_chunk;
     tokens();
   }
 }
@@ -389,9 +465,9 @@ int launch_embed(const EmbedArgs* a, cudaStream_t stream) {
   int lanes = 8;
   while (lanes < 256 && 4 * lanes < pieces) lanes *= 2;  // (a thread has four pieces in flight)
   const long long rows = 256 / lanes, blocks = (a->n + rows - 1) / rows;
-  const unsigned grid = (unsigned)std::min<long long>(blocks, 1 << 20);
-  return (int)(wide ? dfl_host::launch_early(embed_kernel<DT, W>, grid, 256, 0, stream, *a, lanes)
-                    : dfl_host::launch_early(embed_kernel<DT, 1>, grid, 256, 0, stream, *a, lanes));
+  const unsigned grid = (unsigned)std::min<long long>(blocks, 148 * 5);
+  return (int)(wide ? dfl_host::launch_early(embed_kernel<DT, true>, grid, 256, 0, stream, *a, lanes)
+                    : dfl_host::launch_early(embed_kernel<DT, false>, grid, 256, 0, stream, *a, lanes));
 }
 
 template <int DT>
@@ -400,8 +476,8 @@ int launch_sum(const EmbedGradArgs* a, const EmbedWs& w, cudaStream_t stream) {
   const bool wide = a->D % W == 0 && al16(a->dy) && al16(a->dw);
   const long long work = (a->n + a->n / kFew) * ((a->D / (wide ? W : 1) + 32 * kU - 1) / (32 * kU));  // (at most)
   const unsigned grid = (unsigned)std::min<long long>((work + 7) / 8, 148 * 8);
-  return (int)(wide ? dfl_host::launch_early(embed_sum_kernel<DT, W>, grid, 256, 0, stream, *a, w)
-                    : dfl_host::launch_early(embed_sum_kernel<DT, 1>, grid, 256, 0, stream, *a, w));
+  return (int)(wide ? dfl_host::launch_early(embed_sum_kernel<DT, true>, grid, 256, 0, stream, *a, w)
+                    : dfl_host::launch_early(embed_sum_kernel<DT, false>, grid, 256, 0, stream, *a, w));
 }
 
 }  // namespace

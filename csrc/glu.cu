@@ -75,8 +75,9 @@ DFL_DEVICE float2 unpack2(uint32_t v) {
 }
 template <bool F16>
 DFL_DEVICE float load1(const void* p, long long i) {
-  if constexpr (F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-  else return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  const uint16_t v = __ldcg(reinterpret_cast<const uint16_t*>(p) + i);
+  if constexpr (F16) return __half2float(__ushort_as_half(v));
+  else return __bfloat162float(__ushort_as_bfloat16(v));
 }
 template <bool F16>
 DFL_DEVICE void store1(void* p, long long i, float v) {
@@ -471,11 +472,8 @@ DFL_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-DFL_DEVICE uint4 ld_once(const uint16_t* p) {  // read once: no L1 allocation
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
-  return r;
-}
+// (launched while the kernel before ends: what that writes is read past L1)
+DFL_DEVICE uint4 ld_once(const uint16_t* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
 
 // NB: groups of 8 rows.
 template <int NB, bool F16>
@@ -594,12 +592,12 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
     float g[8], u[8], d[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4 x = __ldcs(reinterpret_cast<const float4*>(a.g + at) + h), y = __ldcs(reinterpret_cast<const float4*>(a.u + at) + h);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(a.g + at) + h), y = __ldcg(reinterpret_cast<const float4*>(a.u + at) + h);
       g[4 * h] = x.x, g[4 * h + 1] = x.y, g[4 * h + 2] = x.z, g[4 * h + 3] = x.w;
       u[4 * h] = y.x, u[4 * h + 1] = y.y, u[4 * h + 2] = y.z, u[4 * h + 3] = y.w;
     }
     if (wide && cols == 8) {
-      const uint4 dv = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.dh) + row * a.lddh + col));
+      const uint4 dv = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.dh) + row * a.lddh + col));
       const uint32_t w[4] = {dv.x, dv.y, dv.z, dv.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
