@@ -1,6 +1,6 @@
 // Embedding lookup y[i] = scale * W[ids[i]] and its gradient (sm_100a), f32, bf16 or fp16.
 //
-// Lookup: bound by its bytes; a thread moves 16-byte pieces (single values where a row is no multiple of them).  The product
+// Lookup: bound by its bytes; a thread moves pieces of 16 bytes, or of 8, 4 or 2 where the rows' length or start asks for it.  The product
 // is formed in f32 and rounded once.
 //
 // Gradient: dW[v] = scale * sum of dy[i] over the tokens i with id v: f32 sums in ascending order of i, so the result does not
@@ -9,11 +9,10 @@
 //                      range of the list, place.  Where the range lies and in which order tokens arrive there is left to chance;
 //                      ids with more than 32 tokens are put in ascending order here, the rest by the warps that sum them.
 //                      Meanwhile the other clusters fill dW with zeros.
-//   embed_sum_kernel   a warp takes 128 pieces of an item (an id's tokens, at most 64 of them).  The sums of an id's items are
+//   embed_sum_kernel   a warp takes up to 1 KB of an item (an id's tokens, at most 64 of them).  The sums of an id's items are
 //                      kept in f32 and added in order by the last warp of the piece.
 // A sort by value is not needed for that, and a scan over the vocabulary neither.
 #include <algorithm>
-#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -78,100 +77,82 @@ DFL_DEVICE long long id_at(const void* ids, int bytes, long long i) {
   return bytes == 8 ? __ldcg(reinterpret_cast<const long long*>(ids) + i) : (long long)__ldcg(reinterpret_cast<const int*>(ids) + i);
 }
 
-// Types: a piece is VEC values.
-template <int DT>
-struct Value;
+// A piece of a row: B = 16, 8, 4 or 2 bytes, the most that every row's start and length allow.
+template <int B>
+struct Bytes;
 template <>
-struct Value<kDtypeF32> {
-  using T = float;
-  static constexpr int kWide = 4;
-  static DFL_DEVICE float get(float v) { return v; }
-  static DFL_DEVICE float put(float v) { return v; }
+struct Bytes<16> {
+  using R = uint4;
 };
 template <>
-struct Value<kDtypeBf16> {
-  using T = uint16_t;
-  static constexpr int kWide = 8;
-  static DFL_DEVICE float get(T v) { return __uint_as_float((uint32_t)v << 16); }
-  static DFL_DEVICE T put(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+struct Bytes<8> {
+  using R = uint2;
 };
 template <>
-struct Value<kDtypeF16> {
-  using T = uint16_t;
-  static constexpr int kWide = 8;
-  static DFL_DEVICE float get(T v) { return __half2float(__ushort_as_half(v)); }
-  static DFL_DEVICE T put(float v) { return __half_as_ushort(__float2half_rn(v)); }
+struct Bytes<4> {
+  using R = uint32_t;
+};
+template <>
+struct Bytes<2> {
+  using R = uint16_t;
 };
 
-// A piece: 16 bytes (WIDE) or a single value, and its values added to s.
-template <int DT, bool WIDE>
+template <int DT, int B>
 struct Piece {
-  using T = typename Value<DT>::T;
-  static constexpr int N = WIDE ? Value<DT>::kWide : 1;
-  using R = std::conditional_t<WIDE, uint4, T>;
-  static DFL_DEVICE R load(const T* p) { return __ldcg(reinterpret_cast<const R*>(p)); }
-  static DFL_DEVICE void add(float (&s)[N], R r) {
-    if constexpr (!WIDE) {
-      s[0] += Value<DT>::get(r);
+  using R = typename Bytes<B>::R;
+  static constexpr int kSize = DT == kDtypeF32 ? 4 : 2, N = B / kSize;  // values
+  static_assert(B >= kSize, "a piece holds whole values");
+  static DFL_DEVICE R load(const void* p) { return __ldcg(reinterpret_cast<const R*>(p)); }
+  static DFL_DEVICE void values(R r, float (&v)[N]) {
+    if constexpr (B == 2) {
+      v[0] = DT == kDtypeBf16 ? __uint_as_float((uint32_t)r << 16) : __half2float(__ushort_as_half(r));
     } else {
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < B / 4; ++i) {
         if constexpr (DT == kDtypeF32) {
-          s[i] += __uint_as_float(w[i]);
+          v[i] = __uint_as_float(w[i]);
         } else {
-          float2 f;
-          if constexpr (DT == kDtypeBf16) f = unpack_bf16x2(w[i]);
-          else f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          s[2 * i] += f.x, s[2 * i + 1] += f.y;
+          const float2 f = DT == kDtypeBf16 ? unpack_bf16x2(w[i]) : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x, v[2 * i + 1] = f.y;
         }
       }
     }
   }
-  static DFL_DEVICE void store(T* p, const float (&s)[N], float scale) {
-    if constexpr (!WIDE) {
-      *p = Value<DT>::put(scale * s[0]);
+  static DFL_DEVICE void store(void* p, const float (&v)[N], float scale) {  // scale * v, rounded once
+    if constexpr (B == 2) {
+      *reinterpret_cast<uint16_t*>(p) = DT == kDtypeBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(scale * v[0]))
+                                                         : __half_as_ushort(__float2half_rn(scale * v[0]));
     } else {
-      uint32_t w[4];
+      R r;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < B / 4; ++i) {
         if constexpr (DT == kDtypeF32) {
-          w[i] = __float_as_uint(scale * s[i]);
+          w[i] = __float_as_uint(scale * v[i]);
         } else if constexpr (DT == kDtypeBf16) {
-          w[i] = pack_bf16x2(scale * s[2 * i], scale * s[2 * i + 1]);
+          w[i] = pack_bf16x2(scale * v[2 * i], scale * v[2 * i + 1]);
         } else {
-          const __half2 h = __floats2half2_rn(scale * s[2 * i], scale * s[2 * i + 1]);
+          const __half2 h = __floats2half2_rn(scale * v[2 * i], scale * v[2 * i + 1]);
           w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
       }
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<R*>(p) = r;
     }
   }
 };
 
-// A piece of 16 bytes, each of its values times s.
-template <int DT>
-DFL_DEVICE uint32_t scaled_word(uint32_t w, float s) {
-  if constexpr (DT == kDtypeF32) {
-    return __float_as_uint(s * __uint_as_float(w));
-  } else if constexpr (DT == kDtypeBf16) {
-    const float2 f = unpack_bf16x2(w);
-    return pack_bf16x2(s * f.x, s * f.y);
-  } else {
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
-    const __half2 h = __floats2half2_rn(s * f.x, s * f.y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
+// Pieces that a thread has in flight: 64 bytes, or 16 loads.
+template <int B>
+constexpr int kFlight = B == 16 ? 4 : B == 8 ? 8 : 16;
 
-// `lanes` threads to a row, four pieces of it (WIDE: of 16 bytes, else single values) in flight in each; the next row's id is on
-// its way meanwhile.
-template <int DT, bool WIDE>
+// `lanes` threads to a row; the next row's id is on its way meanwhile.
+template <int DT, int B>
 __global__ void __launch_bounds__(256, 5) embed_kernel(EmbedArgs a, int lanes) {
-  using V = Value<DT>;
-  using T = typename V::T;
+  using P = Piece<DT, B>;
+  constexpr int U = kFlight<B>;
   griddep_wait();
-  const int pieces = WIDE ? a.D / V::kWide : a.D, lane = threadIdx.x % lanes, rows = 256 / lanes;
+  const int pieces = a.D / P::N, lane = threadIdx.x % lanes, rows = 256 / lanes;
   const long long step = (long long)gridDim.x * rows;
   long long i = (long long)blockIdx.x * rows + threadIdx.x / lanes;
   if (i >= a.n) return;
@@ -180,29 +161,19 @@ __global__ void __launch_bounds__(256, 5) embed_kernel(EmbedArgs a, int lanes) {
     const long long next = id_at(a.ids, a.id_bytes, min(i + step, a.n - 1));
     const bool in = id >= 0 && id < a.V;
     if (!in && lane == 0) record_error(a.err, kErrBounds, kKidEmbed, 1, (int)i);
-    const T* src = reinterpret_cast<const T*>(a.w) + (in ? id * a.ldw : 0);
-    T* dst = reinterpret_cast<T*>(a.y) + i * a.D;
-    for (int c = lane; c < pieces; c += 4 * lanes) {
-      const int n = in ? (pieces - c + lanes - 1) / lanes : 0;  // pieces of this thread from here on
-      if constexpr (WIDE) {
-        const uint4* s = reinterpret_cast<const uint4*>(src) + c;
-        uint4* d = reinterpret_cast<uint4*>(dst) + c;
-        uint4 x[4];
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.w) + (in ? id * a.ldw * P::kSize : 0);
+    uint8_t* dst = reinterpret_cast<uint8_t*>(a.y) + i * a.D * P::kSize;
+    for (int c = lane; c < pieces; c += U * lanes) {
+      typename P::R x[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = u < n ? __ldcg(s + u * lanes) : make_uint4(0u, 0u, 0u, 0u);
+      for (int u = 0; u < U; ++u) x[u] = in && c + u * lanes < pieces ? P::load(src + (long long)(c + u * lanes) * B) : typename P::R{};
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (c + u * lanes < pieces)
-            d[u * lanes] = make_uint4(scaled_word<DT>(x[u].x, a.scale), scaled_word<DT>(x[u].y, a.scale), scaled_word<DT>(x[u].z, a.scale),
-                                      scaled_word<DT>(x[u].w, a.scale));
-      } else {
-        float x[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = u < n ? V::get(__ldcg(src + c + u * lanes)) : 0.f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (c + u * lanes < pieces) dst[c + u * lanes] = V::put(a.scale * x[u]);
-      }
+      for (int u = 0; u < U; ++u)
+        if (c + u * lanes < pieces) {
+          float v[P::N];
+          P::values(x[u], v);
+          P::store(dst + (long long)(c + u * lanes) * B, v, a.scale);
+        }
     }
     id = next;
   }
@@ -353,22 +324,25 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   }
 }
 
-// A warp takes 32 U pieces of an item: lane l the pieces l, l + 32, ...; the next item is on its way meanwhile.  What counts is
+// A warp takes 32 U pieces of an item (lane l the pieces l, l + 32, ...), T tokens at a time; the next item is on its way meanwhile.  What counts is
 // the loads in flight (most ids occur once): the whole gradient of 16384 tokens x 3584 over 152064 rows took 240 us with three CTAs an SM,
 // U = 2 and four tokens in flight (two CTAs 247; U = 4 and two tokens 254, U = 1 and four 250, and eight 254), 32768 tokens
 // x 4096 over 32000 rows 166 (181, 172, 186, 196); the pieces as whole words 221 and 164.
-constexpr int kU = 2, kTokens = 4;
+template <int B>
+constexpr int kU = B == 16 ? 2 : B == 8 ? 4 : 8;
+template <int B>
+constexpr int kTokens = B >= 8 ? 4 : 2;
 
-template <int DT, bool WIDE>
+template <int DT, int B>
 __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, EmbedWs w) {
-  using P = Piece<DT, WIDE>;
-  using T = typename P::T;
-  constexpr int VEC = P::N;
+  using P = Piece<DT, B>;
+  constexpr int VEC = P::N, U = kU<B>, T = kTokens<B>;
   griddep_wait();
-  const int lane = threadIdx.x % 32, pieces = a.D / VEC, chunks = (pieces + 32 * kU - 1) / (32 * kU);
+  const int lane = threadIdx.x % 32, pieces = a.D / VEC, chunks = (pieces + 32 * U - 1) / (32 * U);
   const long long warps = (long long)gridDim.x * 8, me = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const T* dy = reinterpret_cast<const T*>(a.dy);
-  T* dw = reinterpret_cast<T*>(a.dw);
+  const uint8_t* dy = reinterpret_cast<const uint8_t*>(a.dy);
+  uint8_t* dw = reinterpret_cast<uint8_t*>(a.dw);
+  const long long row_bytes = (long long)a.D * P::kSize;
 
   // (item, chunk) by item * chunks + chunk, advanced without divisions
   const int items = __ldcg(w.head + 2), d_item = (int)(warps / chunks), d_chunk = (int)(warps % chunks);
@@ -389,10 +363,10 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
     item += d_item + (to_chunk >= chunks);
     to_chunk -= to_chunk >= chunks ? chunks : 0;
     const Item nx = w.items[min(item, items - 1ll)];
-    const int c0 = chunk * 32 * kU + lane;
-    float s[kU][VEC];
+    const int c0 = chunk * 32 * U + lane;
+    float s[U][VEC];
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s[u][e] = 0.f;
     if (it.order == kAnyOrder) {  // one token to a lane, in ascending order
@@ -404,30 +378,35 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
         if (to == lane) t0 = x;
       }
     }
-    for (int k = 0; k < it.len; k += kTokens) {
-      typename P::R x[kTokens][kU];
+    for (int k = 0; k < it.len; k += T) {
+      typename P::R x[T][U];
 #pragma unroll
-      for (int j = 0; j < kTokens; ++j) {
+      for (int j = 0; j < T; ++j) {
         if (k + j >= it.len) break;
-        const T* src = dy + (long long)__shfl_sync(0xffffffffu, k < 32 ? t0 : t1, (k + j) % 32) * a.D;
+        const uint8_t* src = dy + (long long)__shfl_sync(0xffffffffu, k < 32 ? t0 : t1, (k + j) % 32) * row_bytes;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) x[j][u] = P::load(src + min(c0 + 32 * u, pieces - 1) * VEC);  // (lanes past the row's end read it, and store nothing)
+        for (int u = 0; u < U; ++u) x[j][u] = P::load(src + (long long)min(c0 + 32 * u, pieces - 1) * B);  // (lanes past the row's end read it, and store nothing)
       }
 #pragma unroll
-      for (int j = 0; j < kTokens; ++j) {
+      for (int j = 0; j < T; ++j) {
         if (k + j >= it.len) break;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) P::add(s[u], x[j][u]);
+        for (int u = 0; u < U; ++u) {
+          float v[VEC];
+          P::values(x[j][u], v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) s[u][e] += v[e];
+        }
       }
     }
     bool whole = true;
     if (it.part >= 0) {
       float* part = w.part + (long long)it.part * a.D;
 #pragma unroll
-      for (int u = 0; u < kU; ++u)
+      for (int u = 0; u < U; ++u)
         if (c0 + 32 * u < pieces)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) __stcg(part + (c0 + 32 * u) * VEC + e, s[u][e]);
+          for (int e = 0; e < VEC; ++e) __stcg(part + (long long)(c0 + 32 * u) * VEC + e, s[u][e]);
       __threadfence();
       __syncwarp();
       int last = 0;
@@ -435,8 +414,8 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
       whole = __shfl_sync(0xffffffffu, last, 0);
       if (whole) __threadfence();
 #pragma unroll
-      for (int u = 0; u < kU && whole; ++u) {
-        const float* from = w.part + (long long)it.first * a.D + min(c0 + 32 * u, pieces - 1) * VEC;
+      for (int u = 0; u < U && whole; ++u) {
+        const float* from = w.part + (long long)it.first * a.D + (long long)min(c0 + 32 * u, pieces - 1) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s[u][e] = 0.f;
 #pragma unroll 4
@@ -446,9 +425,9 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
       }
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (!whole || c0 + 32 * u >= pieces) break;
-      P::store(dw + it.row * (long long)a.D + (c0 + 32 * u) * VEC, s[u], a.scale);
+      P::store(dw + it.row * row_bytes + (long long)(c0 + 32 * u) * B, s[u], a.scale);
     }
     it = nx, chunk = to_chunk;
     tokens();
@@ -457,57 +436,59 @@ __global__ void __launch_bounds__(256, 3) embed_sum_kernel(EmbedGradArgs a, Embe
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <int DT>
-int launch_embed(const EmbedArgs* a, cudaStream_t stream) {
-  constexpr int W = Value<DT>::kWide;
-  const bool wide = a->D % W == 0 && a->ldw % W == 0 && al16(a->w) && al16(a->y);
-  const int pieces = wide ? a->D / W : a->D;
-  int lanes = 8;
-  while (lanes < 256 && 4 * lanes < pieces) lanes *= 2;  // (a thread has four pieces in flight)
-  const long long rows = 256 / lanes, blocks = (a->n + rows - 1) / rows;
-  const unsigned grid = (unsigned)std::min<long long>(blocks, 148 * 5);
-  return (int)(wide ? dfl_host::launch_early(embed_kernel<DT, true>, grid, 256, 0, stream, *a, lanes)
-                    : dfl_host::launch_early(embed_kernel<DT, false>, grid, 256, 0, stream, *a, lanes));
+// Bytes of a piece: what divides the rows' length and pitch and both starts.
+int piece_bytes(long long row, long long pitch, const void* a, const void* b) {
+  const uintptr_t all = (uintptr_t)row | (uintptr_t)pitch | reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b);
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
-template <int DT>
-int launch_sum(const EmbedGradArgs* a, const EmbedWs& w, cudaStream_t stream) {
-  constexpr int W = Value<DT>::kWide;
-  const bool wide = a->D % W == 0 && al16(a->dy) && al16(a->dw);
-  const long long work = (a->n + a->n / kFew) * ((a->D / (wide ? W : 1) + 32 * kU - 1) / (32 * kU));  // (at most)
-  const unsigned grid = (unsigned)std::min<long long>((work + 7) / 8, 148 * 8);
-  return (int)(wide ? dfl_host::launch_early(embed_sum_kernel<DT, true>, grid, 256, 0, stream, *a, w)
-                    : dfl_host::launch_early(embed_sum_kernel<DT, false>, grid, 256, 0, stream, *a, w));
+template <int DT, int B>
+int launch_embed(const EmbedArgs* a, cudaStream_t stream) {
+  const int pieces = a->D / Piece<DT, B>::N;
+  int lanes = 8;
+  while (lanes < 256 && kFlight<B> * lanes < pieces) lanes *= 2;
+  const long long rows = 256 / lanes, blocks = (a->n + rows - 1) / rows;
+  return (int)dfl_host::launch_early(embed_kernel<DT, B>, (unsigned)std::min<long long>(blocks, 148 * 5), 256, 0, stream, *a, lanes);
 }
+
+template <int DT, int B>
+int launch_sum(const EmbedGradArgs* a, const EmbedWs& w, cudaStream_t stream) {
+  const int pieces = a->D / Piece<DT, B>::N;
+  const long long work = (a->n + a->n / kFew) * ((pieces + 32 * kU<B> - 1) / (32 * kU<B>));  // (at most)
+  return (int)dfl_host::launch_early(embed_sum_kernel<DT, B>, (unsigned)std::min<long long>((work + 7) / 8, 148 * 8), 256, 0, stream, *a, w);
+}
+
+// Calls f<type, bytes>(...).
+#define DFL_EMBED(f, dtype, bytes, ...)                                                                           \
+  ((dtype) == kDtypeF32                                                                                           \
+       ? ((bytes) == 16 ? f<kDtypeF32, 16>(__VA_ARGS__) : (bytes) == 8 ? f<kDtypeF32, 8>(__VA_ARGS__) : f<kDtypeF32, 4>(__VA_ARGS__)) \
+   : (dtype) == kDtypeBf16                                                                                        \
+       ? ((bytes) == 16 ? f<kDtypeBf16, 16>(__VA_ARGS__) : (bytes) == 8 ? f<kDtypeBf16, 8>(__VA_ARGS__)           \
+          : (bytes) == 4 ? f<kDtypeBf16, 4>(__VA_ARGS__) : f<kDtypeBf16, 2>(__VA_ARGS__))                         \
+       : ((bytes) == 16 ? f<kDtypeF16, 16>(__VA_ARGS__) : (bytes) == 8 ? f<kDtypeF16, 8>(__VA_ARGS__)             \
+          : (bytes) == 4 ? f<kDtypeF16, 4>(__VA_ARGS__) : f<kDtypeF16, 2>(__VA_ARGS__)))
 
 }  // namespace
 
 extern "C" int dfl_embed(const EmbedArgs* a, cudaStream_t stream) {
   if (a->n <= 0 || a->D <= 0 || a->V < 0 || (a->id_bytes != 4 && a->id_bytes != 8)) return -2;
-  switch (a->dtype) {
-    case kDtypeF32: return launch_embed<kDtypeF32>(a, stream);
-    case kDtypeBf16: return launch_embed<kDtypeBf16>(a, stream);
-    case kDtypeF16: return launch_embed<kDtypeF16>(a, stream);
-    default: return -1;
-  }
+  if (a->dtype != kDtypeF32 && a->dtype != kDtypeBf16 && a->dtype != kDtypeF16) return -1;
+  const int size = a->dtype == kDtypeF32 ? 4 : 2, bytes = piece_bytes((long long)a->D * size, a->ldw * size, a->w, a->y);
+  return DFL_EMBED(launch_embed, a->dtype, bytes, a, stream);
 }
 
 extern "C" long long dfl_embed_grad_ws(long long n, long long V, int D) { return embed_layout(n, V, D, nullptr, nullptr); }
 
 extern "C" int dfl_embed_grad(const EmbedGradArgs* a, cudaStream_t stream) {
   if (a->n <= 0 || a->D <= 0 || a->V <= 0 || a->n >= (1ll << 30) || a->V >= (1ll << 30) || (a->id_bytes != 4 && a->id_bytes != 8)) return -2;
+  if (a->dtype != kDtypeF32 && a->dtype != kDtypeBf16 && a->dtype != kDtypeF16) return -1;
   if (!al16(a->ws) || !al16(a->dw)) return -3;
   EmbedWs w;
   if (embed_layout(a->n, a->V, a->D, reinterpret_cast<char*>(a->ws), &w) > a->ws_bytes) return -4;
+  const int size = a->dtype == kDtypeF32 ? 4 : 2, bytes = piece_bytes((long long)a->D * size, 0, a->dy, a->dw);
   // (14 clusters for the zeros; fewer where dW is small)
-  const long long fill = (a->V * a->D * (a->dtype == kDtypeF32 ? 4 : 2) + 16 * kCluster * kSortThreads - 1) / (16 * kCluster * kSortThreads);
+  const long long fill = (a->V * a->D * size + 16 * kCluster * kSortThreads - 1) / (16 * kCluster * kSortThreads);
   const unsigned clusters = 1 + (unsigned)std::min<long long>(fill, 14);
   const cudaError_t e = dfl_host::launch_early(embed_sort_kernel, clusters * kCluster, kSortThreads, 0, stream, *a, w);
-  if (e != cudaSuccess) return (int)e;
-  switch (a->dtype) {
-    case kDtypeF32: return launch_sum<kDtypeF32>(a, w, stream);
-    case kDtypeBf16: return launch_sum<kDtypeBf16>(a, w, stream);
-    case kDtypeF16: return launch_sum<kDtypeF16>(a, w, stream);
-    default: return -1;
-  }
+  return e != cudaSuccess ? (int)e : DFL_EMBED(launch_sum, a->dtype, bytes, a, w, stream);
 }

@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(256) glu_join_kernel(const __grid_constant__ G
   }
 }
 
-// dg, du: 8 columns a thread.  Bound by its bytes (14 M F): 4096 x 18944 see gated_train in the table.
+// dg, du: 8 columns a thread.  Bound by its bytes (14 M F): 4096 x 18944 169 us, 6.4 TB/s.
 template <bool F16, int ACT>
 __global__ void __launch_bounds__(256) glu_grad_kernel(GluGradArgs a) {
   griddep_wait();

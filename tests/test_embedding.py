@@ -99,6 +99,23 @@ def test_gradient(native, n, V, D, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FF])
+@pytest.mark.parametrize("D", [2, 6, 12, 255, 770, 772, 1030, 2052])
+def test_widths(native, D, dtype):
+    """Rows that pieces of 8, 4 or 2 bytes fit, and tables and gradients that start at any value."""
+    ids, w, dy = _make(333, 90, D, dtype, "cuda", "skewed")
+    want, grad = ops.embedding(ids, w, scale=0.7), F.embedding_grad(dy, ids, 90, 0.7)
+    assert torch.equal(want, (w[ids].float() * 0.7).to(dtype))
+    _check_grad(grad, ids, dy, 0.7)
+    for off in (1, 2, 4):
+        flat_w, flat_d = (torch.zeros(off + t.numel(), device="cuda", dtype=dtype)[off:].view(t.shape) for t in (w, dy))
+        flat_w.copy_(w)
+        flat_d.copy_(dy)
+        assert torch.equal(ops.embedding(ids, flat_w, scale=0.7), want)
+        assert torch.equal(F.embedding_grad(flat_d, ids, 90, 0.7), grad)
+
+
+@pytest.mark.gpu
 def test_gradient_of_many_tokens(native):
     """More tokens than one bitmap holds, of few ids: the order is found window by window."""
     n = 300_001
