@@ -86,7 +86,7 @@ def test_lookup(native, n, V, D, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, HF, FF])
 @pytest.mark.parametrize("kind", ["uniform", "one", "skewed", "runs"])
-@pytest.mark.parametrize("n,V,D", [(1, 1, 1), (5, 3, 8), (64, 2, 264), (65, 2, 33), (616, 5000, 771), (4097, 100, 512), (20000, 12, 72), (9000, 30000, 64)])
+@pytest.mark.parametrize("n,V,D", [(1, 1, 1), (5, 3, 8), (64, 2, 264), (65, 2, 33), (616, 5000, 771), (4097, 100, 512), (20000, 12, 72), (9000, 30000, 64), (30000, 60, 8), (70000, 150, 4)])
 def test_gradient(native, n, V, D, kind, dtype):
     ids, w, dy = _make(n, V, D, dtype, "cuda", kind)
     w.requires_grad_()
