@@ -20,7 +20,8 @@ def gated_linear(x, w_gate, w_up, *, act="silu"):
 
     ``act``: "silu", "gelu" / "gelu_tanh" (tanh form) or "gelu_erf".  Products are accumulated and the activation is
     evaluated in f32; the result is rounded to x's type once.  Differentiable in all three (once): the two projections are
-    kept in f32 for it (8 bytes a value of the result).  CUDA: bf16 and fp16 with K a multiple of 8; other types and sizes, tracing,
+    kept in f32 for it (8 bytes a value of the result), their gradients are
+    rounded to x's type.  CUDA: bf16 and fp16 with K a multiple of 8; other types and sizes, tracing,
     function transforms and forward-mode tangents run as torch operations."""
     if x.is_cuda and act in F.GATED_ACTS and type(x) in _PLAIN and not torch.compiler.is_compiling():
         try:  # the binding checks everything; what it refuses is looked at again below

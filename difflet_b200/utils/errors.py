@@ -8,7 +8,8 @@ _CODES = {
     3: "bounds guard tripped",
     4: "bad device-side argument",
 }
-_KERNELS = {1: "gemm", 2: "attention", 3: "comm", 4: "norm", 5: "mx", 6: "conv"}
+_KERNELS = {1: "gemm", 2: "attention", 3: "comm", 4: "norm", 5: "mx", 6: "conv", 7: "cross attention",
+            8: "adapters", 9: "gated projection", 10: "embedding"}
 
 
 class DeviceError(RuntimeError):

@@ -109,7 +109,7 @@ def test_shapes_and_refusals():
 
 # ----------------------------------------------------------------------------- kernels
 SHAPES = [(1, 8, 1), (1, 64, 8), (4, 512, 1000), (7, 136, 65), (16, 1024, 333), (17, 40, 128), (33, 96, 129), (127, 256, 511), (129, 72, 64),
-          (300, 1032, 257), (1000, 264, 1031), (2049, 64, 1280), (515, 2048, 2564)]
+          (300, 1032, 257), (1000, 264, 1031), (2049, 64, 1280), (515, 2048, 2564), (70, 4096, 333), (257, 1024, 4099), (600, 520, 1), (40, 8, 300)]
 
 
 @pytest.mark.gpu

@@ -89,6 +89,7 @@ CASES = [  # B, H, Hk, Sq, Sk, window, sinks
     (2, 8, 2, 5, 700, 130, 3), (1, 12, 12, 17, 1300, 1000, 100), (2, 2, 1, 40, 40, 7, 0), (2, 3, 3, 128, 128, 128, 0), (1, 4, 4, 129, 385, 1, 1),
     (3, 4, 1, 300, 300, 50, 3), (1, 2, 2, 700, 1500, 300, 200), (1, 40, 40, 513, 700, 129, 128), (2, 16, 4, 1021, 1021, 255, 1),
     (1, 24, 24, 900, 900, 10 ** 6, 0), (1, 3, 1, 257, 260, 128, 255), (5, 7, 7, 33, 64, 20, 70),
+    (1, 4, 4, 300, 6000, 4000, 200), (1, 6, 2, 200, 3000, 2500, 0), (2, 2, 1, 384, 2100, 2000, 1), (1, 1, 1, 1025, 1300, 700, 129),
 ]
 
 
