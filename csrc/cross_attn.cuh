@@ -411,8 +411,13 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
           if (q_issued[g]) mbar_wait(&q_full[g], 0, nullptr, 0, 0, nullptr, 200000000LL), mbar_wait(&q_full[g], 1, nullptr, 0, 0, nullptr, 200000000LL);
         for (int i = 0; i < R; ++i)
           if (issued[i]) {
-            if ((raw >> i) & 1u) mbar_wait(&v_raw[i], ((raw_par >> i) & 1u) ^ 1u, nullptr, 0, 0, nullptr, 200000000LL);
-            else mbar_wait(&kv_full[i], issued_par[i], nullptr, 0, 0, nullptr, 200000000LL);
+            if constexpr (MASK == kSlide) {
+              if ((raw >> i) & 1u) {
+                mbar_wait(&v_raw[i], ((raw_par >> i) & 1u) ^ 1u, nullptr, 0, 0, nullptr, 200000000LL);
+                continue;
+              }
+            }
+            mbar_wait(&kv_full[i], issued_par[i], nullptr, 0, 0, nullptr, 200000000LL);
           }
       }
     }
@@ -506,21 +511,6 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
     if constexpr (QT == 2) fewer_registers<MASK>();
     bool ok = true;
     int s = 0;
-    auto clean = [&](const Items& it, int k0, uint8_t* tile, const uint32_t (&w)[4]) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {  // key row 32 c + lane: 128 bytes in every chunk (the swizzle stays inside)
-        const int r = 32 * c + lane, key = k0 + r;
-        bool drop = key < it.lo || key >= it.hi || !((w[c] >> lane) & 1u);
-        if constexpr (MASK == kSlide) drop = key >= it.hi || (key < it.lo && key >= it.sinks);
-        if (drop) {
-#pragma unroll
-          for (int ch = 0; ch < C::kChunks; ++ch)
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4*>(tile + ch * kChunk + r * 128 + ((v + lane) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-    };
     if constexpr (MASK == kSlide) {
       // Only the tiles that hold keys which no query of the block sees pass here, a few at the window's ends: their copies are counted
       // on v_raw[slot], this warp's arrival completes kv_full[slot] in their place, and until it has the slot is not filled again, so
@@ -532,8 +522,18 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
           if (!cross_dirty<MASK>(p, it, k0)) continue;
           if (!mbar_wait_warp(&v_raw[slot], (par >> slot) & 1u, err, kKidCross, 141, abort_flag)) { ok = false; break; }
           par ^= 1u << slot;
-          const uint32_t all[4] = {~0u, ~0u, ~0u, ~0u};
-          clean(it, k0, smem + C::kKV + slot * C::kTile, all);
+          uint8_t* tile = smem + C::kKV + slot * C::kTile;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {  // as below
+            const int r = 32 * c + lane, key = k0 + r;
+            if (key >= it.hi || (key < it.lo && key >= it.sinks)) {
+#pragma unroll
+              for (int ch = 0; ch < C::kChunks; ++ch)
+#pragma unroll
+                for (int v = 0; v < 8; ++v)
+                  *reinterpret_cast<uint4*>(tile + ch * kChunk + r * 128 + ((v + lane) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) mbar_arrive(&kv_full[slot]);
@@ -553,7 +553,17 @@ __global__ void __launch_bounds__(CrossCfg<DH, QT>::kThreads, 1)
         }
         if (!mbar_wait_warp(&kv_full[L % R], (L / R) & 1, err, kKidCross, 140, abort_flag)) { ok = false; break; }
         uint8_t* tile = smem + C::kKV + (L % R) * C::kTile;
-        if (dirty) clean(it, k0, tile, w);
+#pragma unroll
+        for (int c = 0; c < 4 && dirty; ++c) {  // key row 32 c + lane: 128 bytes in every chunk (the swizzle stays inside)
+          const int r = 32 * c + lane, key = k0 + r;
+          if (key < it.lo || key >= it.hi || !((w[c] >> lane) & 1u)) {
+#pragma unroll
+            for (int ch = 0; ch < C::kChunks; ++ch)
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<uint4*>(tile + ch * kChunk + r * 128 + ((v + lane) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_clean[L % R]);
