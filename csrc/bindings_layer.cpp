@@ -1,4 +1,5 @@
 // torch bindings of the layer operators: gated projection, embedding lookup, windowed attention.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -31,9 +32,24 @@ variable_list once_differentiable(const char* name, Compute compute) {
   return grads;
 }
 
+// A pass captured into a CUDA graph cannot hand a gradient to a node of the default stream, and an eager graph that still
+// lives keeps such a node for each of its leaves. Refused before anything is recorded: the engine would meet it inside the
+// capture, where its failure ends the process.
+void check_capture(const char* name, std::initializer_list<const at::Tensor*> inputs) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const at::Tensor* t : inputs) {
+    if (!t->requires_grad()) continue;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::gradient_edge(*t).function;
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() != 0, name, ": an eager graph on the default stream still holds an input of this captured pass; "
+                "release it (or build it on a stream of its own) before the capture");
+  }
+}
+
 // Rows that the copy engine can address: unit inner stride, 16-byte aligned rows; anything else is laid out anew.
 at::Tensor rows16(const at::Tensor& t) {
-  const bool fits = t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) > 0)) &&
+  const bool fits = t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) &&
+                    (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&  // (rows that overlap do not fit)
                     reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
@@ -151,8 +167,10 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 
 at::Tensor gated_linear(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act) {
   TORCH_CHECK_VALUE(plain_tensors({&x, &wg, &wu}), "the kernel takes no wrapped tensors and no tangents");
-  if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad()))
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad())) {
+    check_capture("gated_linear", {&x, &wg, &wu});
     return GatedLinear::apply(x, wg, wu, act);
+  }
   return gated_forward(x, wg, wu, act, nullptr);
 }
 
@@ -237,7 +255,10 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale, c
     pad = *padding_idx + (*padding_idx < 0 ? w.size(0) : 0);
     TORCH_CHECK_VALUE(pad >= 0 && pad < w.size(0), "padding_idx ", *padding_idx, " is not a row of ", w.size(0));
   }
-  if (at::GradMode::is_enabled() && w.requires_grad()) return Embedding::apply(ids, w, scale, pad);
+  if (at::GradMode::is_enabled() && w.requires_grad()) {
+    check_capture("embedding", {&w});
+    return Embedding::apply(ids, w, scale, pad);
+  }
   return embedding_forward(ids, w, scale);
 }
 

@@ -261,3 +261,48 @@ def test_compiled(native):
     q = x.view(2, 90, H, DH).transpose(1, 2)
     want = F.gated_linear(ops.window_attention(q, q, q, window=7, scale=0.1).transpose(1, 2).reshape(2, 90, D), p["gate"], p["up"])
     assert torch.allclose(f(ids), want, atol=1e-4, rtol=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["gated_linear", "embedding"])
+def test_capture_beside_a_living_eager_graph(native, name):
+    """Gradients cannot be captured while an eager graph of the default stream holds the same leaves: refused before anything is
+    recorded, and both passes work afterwards."""
+    g = torch.Generator().manual_seed(0)
+    if name == "embedding":
+        leaves, ids = [torch.randn(50, 64, generator=g).to("cuda", BF)], torch.randint(0, 50, (70,), generator=g).cuda()
+        run = lambda: ops.embedding(ids, leaves[0], scale=2.0)  # noqa: E731
+    else:
+        leaves = [torch.randn(*s, generator=g).to("cuda", BF) for s in ((70, 64), (40, 64), (40, 64))]
+        run = lambda: ops.gated_linear(*leaves)  # noqa: E731
+    for t in leaves:
+        t.requires_grad_()
+    y = run()
+    dy = torch.ones_like(y)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            run()
+    with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        run()  # (nothing is recorded for gradients)
+    want = torch.autograd.grad(y, leaves, dy)
+    del y
+
+    def captured():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(run(), leaves, dy)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    captured()
+
+
+@pytest.mark.gpu
+def test_rows_that_overlap(native):
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(1024, generator=g).to("cuda", BF).as_strided((90, 64), (8, 1))  # windows of a signal
+    w = torch.randn(700, generator=g).to("cuda", BF).as_strided((40, 64), (16, 1))
+    assert torch.equal(ops.gated_linear(x, w, w), ops.gated_linear(x.contiguous(), w.contiguous(), w.contiguous()))
+    ids = torch.arange(40, device="cuda").flip(0)
+    assert torch.equal(ops.embedding(ids, w), w[ids])
